@@ -298,6 +298,67 @@ int pplb200_rope_kv_append_i8g8(const pplb200_rope_params* p, const pplb200_attn
                                 void* scale, void* stream);
 
 /*
+ * Accumulated attention weight.  For every cached position j of every sequence and every kv head g of layer
+ * layer_idx:  weight[layer_idx, g, row(j)] += sum over the query tokens i of the sequence and the query heads h of
+ * the group of softmax_j(q[i, h] . k[j] / sqrt(head_dim)),  where token i sees the positions <= start_pos[b] + i
+ * (all start_pos[b] + seqlen positions when is_causal is 0).  The K rows are those of the cache: the tokens of the
+ * call have been appended before.  No counterpart in the reference.
+ *   query   [total_tokens, num_heads, head_dim] fp16: one token per sequence (a decode step), or any number (the
+ *           observation window at the end of a prompt)
+ *   weight  [num_layer, num_kv_heads, max_tokens] fp32, indexed by cache row like the cache; rows of no sequence
+ *           of the call stay as they were.  Each position receives one addition per call and sequence, so the
+ *           result does not depend on the order of the kernel's work unless sequences share cache rows.
+ * Uses batch, max_seqlen, max_kvlen (>= start_pos[b] + seqlen), total_tokens, max_tokens, is_causal and the cache
+ * geometry of the params.  `workspace`: pplb200_attn_weight_workspace_size() bytes, 256-byte aligned; its first word
+ * is the status word that pplb200_mhca_device_status reads.
+ */
+int pplb200_attn_weight_workspace_size(const pplb200_attn_params* p, uint64_t* bytes);
+
+int pplb200_attn_weight_accumulate(const pplb200_attn_params* p, const void* query, const int64_t* seqstarts,
+                                   const int64_t* cachestarts, const int64_t* start_pos, const void* cache,
+                                   const void* scale, float* weight, void* workspace, uint64_t workspace_bytes,
+                                   void* stream);
+
+/*
+ * Eviction: which positions of a sequence to keep, per kv head.  With n = kvlens[b] cached positions and
+ * k = min(budgets[b], n): the last r = min(recent, k) positions, the first s = min(sink, k - r), and of the positions
+ * [s, n - r) the k - r - s with the highest weight (ties: the lowest position; a NaN is below every number).
+ *   weight   [num_layer, num_kv_heads, max_tokens] fp32 as above (layer layer_idx is read)
+ *   kvlens   [batch], budgets [batch] int64
+ *   kept     [batch, num_kv_heads, max_budget] int64: the kept positions in ascending order, then -1
+ * A budget above max_budget, or a length above max_kvlen, is cut to it (a cut length is reported as
+ * PPLB200_DEV_LENGTH_CLAMPED).  Uses batch, max_kvlen, max_tokens, num_kv_heads and the cache geometry.
+ * `workspace`: pplb200_kv_evict_workspace_size() bytes, 256-byte aligned (its first word is the status word).
+ * No counterpart in the reference.
+ */
+int pplb200_kv_evict_workspace_size(const pplb200_attn_params* p, uint64_t* bytes);
+
+int pplb200_kv_evict_select(const pplb200_attn_params* p, const float* weight, const int64_t* cachestarts,
+                            const int64_t* kvlens, const int64_t* budgets, int64_t sink, int64_t recent,
+                            int64_t max_budget, int64_t* kept, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/*
+ * Compaction in place: for every sequence b, layer in [layer_idx, layer_idx + layers) and kv head, the row of
+ * position base[b] + kept[i] moves to position base[b] + i, codes and scales of K and V, and the weight where `weight`
+ * is given.  A kept list is strictly ascending and ends at its first negative entry.
+ *   kept    [batch, kept_heads, max_kept] int64; kept_heads is num_kv_heads (a list per kv head: the survivors of
+ *           an eviction, base 0) or 1 (one list for all: the accepted path of a tree of drafts, base = start_pos)
+ *   kvlens  [batch]: the positions the sequence had; base[b] + kept[i] has to be below
+ *   weight  nullable; [num_layer, num_kv_heads, max_tokens] fp32.  The weights of the positions from
+ *           base[b] + (entries of the list) up to kvlens[b] are set to zero
+ * Positions behind the kept ones keep their codes and scales; the caller's lengths become base[b] + entries.  Two
+ * sequences of a call must not share rows that either of them moves.  An entry that breaks these rules is skipped
+ * and reported (PPLB200_DEV_KEPT_INVALID).  `workspace`: pplb200_kv_compact_workspace_size() bytes, 256-byte aligned
+ * (its first word is the status word).  No counterpart in the reference.
+ */
+int pplb200_kv_compact_workspace_size(const pplb200_attn_params* p, uint64_t* bytes);
+
+int pplb200_kv_compact(const pplb200_attn_params* p, const int64_t* kept, int64_t kept_heads, int64_t max_kept,
+                       const int64_t* base, const int64_t* kvlens, const int64_t* cachestarts, int64_t layers,
+                       void* cache, void* scale, float* weight, void* workspace, uint64_t workspace_bytes,
+                       void* stream);
+
+/*
  * Reads the device-side status word that the kernels of the last pplb200_mhca_forward on this
  * workspace left behind (0 = clean; non-zero = a bounded wait gave up, see PPLB200_DEV_*).
  * Synchronises `stream`.  Has no counterpart in the reference; it exists because every wait
@@ -312,8 +373,10 @@ enum {
     PPLB200_DEV_LENGTH_CLAMPED = 4,    /* a sequence exceeded max_kvlen / max_seqlen and was cut   */
     PPLB200_DEV_ROW_OUT_OF_RANGE = 8,  /* cachestarts/start_pos named a row outside [0, max_tokens):
                                           that row was neither read nor written                     */
-    PPLB200_DEV_MASK_OUT_OF_RANGE = 16 /* attn_mask has fewer columns than kvstarts needs: the missing
+    PPLB200_DEV_MASK_OUT_OF_RANGE = 16,/* attn_mask has fewer columns than kvstarts needs: the missing
                                           entries were read as 0                                    */
+    PPLB200_DEV_KEPT_INVALID = 32      /* a kept list is not strictly ascending or names a position outside
+                                          its sequence: that entry was skipped                      */
 };
 
 /* Name of a status code ("RC_SUCCESS", ...).  Never null. */

@@ -33,6 +33,7 @@ DEV_MMA_WAIT_TIMEOUT = 2
 DEV_LENGTH_CLAMPED = 4
 DEV_ROW_OUT_OF_RANGE = 8
 DEV_MASK_OUT_OF_RANGE = 16
+DEV_KEPT_INVALID = 32
 
 # every symbol include/ppl_nn_b200.h declares
 EXPORTS = (
@@ -53,6 +54,12 @@ EXPORTS = (
     "pplb200_rope_workspace_size",
     "pplb200_rope_forward",
     "pplb200_rope_kv_append_i8g8",
+    "pplb200_attn_weight_workspace_size",
+    "pplb200_attn_weight_accumulate",
+    "pplb200_kv_evict_workspace_size",
+    "pplb200_kv_evict_select",
+    "pplb200_kv_compact_workspace_size",
+    "pplb200_kv_compact",
     "pplb200_status_str",
     "pplb200_device_ready",
     "pplb200_launch_count",
@@ -183,6 +190,20 @@ class Library:
         d.pplb200_rope_kv_append_i8g8.restype = ctypes.c_int
         d.pplb200_rope_kv_append_i8g8.argtypes = [rp, pp, vp, vp, vp, i64p, i64p, i64p, vp, ctypes.c_uint64, vp, vp,
                                                   vp, vp, vp]
+        sizep = ctypes.POINTER(ctypes.c_uint64)
+        i64 = ctypes.c_int64
+        d.pplb200_attn_weight_workspace_size.restype = ctypes.c_int
+        d.pplb200_attn_weight_workspace_size.argtypes = [pp, sizep]
+        d.pplb200_attn_weight_accumulate.restype = ctypes.c_int
+        d.pplb200_attn_weight_accumulate.argtypes = [pp, vp, i64p, i64p, i64p, vp, vp, vp, vp, ctypes.c_uint64, vp]
+        d.pplb200_kv_evict_workspace_size.restype = ctypes.c_int
+        d.pplb200_kv_evict_workspace_size.argtypes = [pp, sizep]
+        d.pplb200_kv_evict_select.restype = ctypes.c_int
+        d.pplb200_kv_evict_select.argtypes = [pp, vp, i64p, i64p, i64p, i64, i64, i64, i64p, vp, ctypes.c_uint64, vp]
+        d.pplb200_kv_compact_workspace_size.restype = ctypes.c_int
+        d.pplb200_kv_compact_workspace_size.argtypes = [pp, sizep]
+        d.pplb200_kv_compact.restype = ctypes.c_int
+        d.pplb200_kv_compact.argtypes = [pp, i64p, i64, i64, i64p, i64p, i64p, i64, vp, vp, vp, vp, ctypes.c_uint64, vp]
         d.pplb200_status_str.restype = ctypes.c_char_p
         d.pplb200_status_str.argtypes = [ctypes.c_int]
         d.pplb200_device_ready.restype = ctypes.c_int
@@ -288,6 +309,37 @@ class Library:
         return self.dll.pplb200_rope_kv_append_i8g8(ctypes.byref(p), ctypes.byref(attn), q, k, v, seqstarts,
                                                     cachestarts, start_pos, workspace, int(workspace_bytes), rq, rk,
                                                     cache, scale, stream)
+
+    def _size(self, fn, p) -> tuple[int, int]:
+        n = ctypes.c_uint64(0)
+        rc = fn(ctypes.byref(p), ctypes.byref(n))
+        return rc, int(n.value)
+
+    def attn_weight_workspace_size(self, p) -> tuple[int, int]:
+        return self._size(self.dll.pplb200_attn_weight_workspace_size, p)
+
+    def attn_weight_accumulate(self, p, q, seqstarts, cachestarts, start_pos, cache, scale, weight, workspace,
+                               workspace_bytes, stream) -> int:
+        return self.dll.pplb200_attn_weight_accumulate(ctypes.byref(p), q, seqstarts, cachestarts, start_pos, cache,
+                                                       scale, weight, workspace, int(workspace_bytes), stream)
+
+    def kv_evict_workspace_size(self, p) -> tuple[int, int]:
+        return self._size(self.dll.pplb200_kv_evict_workspace_size, p)
+
+    def kv_evict_select(self, p, weight, cachestarts, kvlens, budgets, sink, recent, max_budget, kept, workspace,
+                        workspace_bytes, stream) -> int:
+        return self.dll.pplb200_kv_evict_select(ctypes.byref(p), weight, cachestarts, kvlens, budgets, int(sink),
+                                                int(recent), int(max_budget), kept, workspace, int(workspace_bytes),
+                                                stream)
+
+    def kv_compact_workspace_size(self, p) -> tuple[int, int]:
+        return self._size(self.dll.pplb200_kv_compact_workspace_size, p)
+
+    def kv_compact(self, p, kept, kept_heads, max_kept, base, kvlens, cachestarts, layers, cache, scale, weight,
+                   workspace, workspace_bytes, stream) -> int:
+        return self.dll.pplb200_kv_compact(ctypes.byref(p), kept, int(kept_heads), int(max_kept), base, kvlens,
+                                           cachestarts, int(layers), cache, scale, weight, workspace,
+                                           int(workspace_bytes), stream)
 
     def static_scratch_bytes(self) -> int:
         return int(self.dll.pplb200_static_scratch_bytes())

@@ -1,0 +1,464 @@
+// Accumulated attention weight: w[row(j)] += sum over the query heads of a kv group and over the query tokens of
+// softmax_j(q . k_j / sqrt(Dh)), for every cached position j of every sequence.  Only K is read.
+//
+// The normaliser of a row needs all its scores, so the scores are formed twice: attn_weight_stats_kernel leaves, per
+// query row and chunk of positions, the maximum and the sum of exponentials; attn_weight_merge_kernel joins the
+// chunks; attn_weight_apply_kernel forms the scores again and adds each position's normalised weights up.
+//
+// Both score kernels: a CTA takes a chunk of the positions of one (sequence, kv head), a warp 16 positions at a
+// time.  Positions are the M dimension of mma.m16n8k16, the query rows (token x head of the group) come in octets as
+// its N dimension.  A thread needs the channels 2t, 2t+1, 2t+8, 2t+9 of each block of 16 for rows g and g+8 of the
+// A operand; as the order of the channels does not matter as long as Q has the same, thread t takes 16 consecutive
+// code bytes per 64 channels straight from global memory.
+//
+// The weights are fp32 and proportional to exp(score), so a key rounded to fp16 would cost 1e-4 of their value;
+// k = code * scale is therefore split into fp16(k) and the exact remainder, and both enter the accumulator.
+#include "common.cuh"
+#include "launch.h"
+
+namespace pplb200 {
+
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
+constexpr int kChunk = 512;     // positions of a CTA
+constexpr int kRowBlock = 32;   // query rows whose fragments are held in registers at a time
+constexpr float kNegBig = -1.0e30f;
+
+struct WeightArgs {
+    const __half* q;
+    const int64_t* seqstarts;
+    const int64_t* cachestarts;
+    const int64_t* start_pos;
+    const int8_t* cache;
+    const __half* scale;
+    float* weight;   // [L, Hkv, MaxT]
+    float2* part;    // [chunks][T][Hq]: maximum (exp2 domain) and sum
+    float2* norm;    // [T][Hq]: maximum and reciprocal sum
+    uint32_t* status;
+    CacheGeom geom;
+    int64_t max_seqlen, max_kvlen, max_tokens, total_tokens;
+    int32_t num_heads, num_kv_heads, group, causal, chunks;
+    float scale_log2;
+};
+
+// Four codes with their group's scale -> the two half2 of fp16(code * scale) and of the exact remainders
+__device__ __forceinline__ void split_key_word(uint32_t w, __half2 s2, uint32_t& k0, uint32_t& k1, uint32_t& e0,
+                                               uint32_t& e1) {
+    const uint32_t x = w ^ 0x80808080u;
+    const __half2 c0 = biased_bytes_to_half2<0x5140u>(x), c1 = biased_bytes_to_half2<0x5342u>(x);
+    const __half2 p0 = __hmul2(c0, s2), p1 = __hmul2(c1, s2);
+    k0 = h2_as_u32(p0);
+    k1 = h2_as_u32(p1);
+    e0 = h2_as_u32(__hfma2(c0, s2, __hneg2(p0)));
+    e1 = h2_as_u32(__hfma2(c1, s2, __hneg2(p1)));
+}
+
+// What a CTA works on
+struct Span {
+    int64_t tok0;   // first query row of the sequence
+    int64_t start;  // positions before its first query token
+    int32_t rows;   // query rows: tokens * group
+    int32_t len;    // positions
+};
+
+__device__ __forceinline__ Span span_of(const WeightArgs& a, int64_t b) {
+    Span s;
+    s.tok0 = a.seqstarts[b];
+    int64_t n = a.seqstarts[b + 1] - s.tok0;
+    if (s.tok0 < 0 || s.tok0 + n > a.total_tokens) {
+        n = 0;
+    }
+    bool cut = n > a.max_seqlen;
+    n = cut ? a.max_seqlen : (n < 0 ? 0 : n);
+    s.start = a.start_pos[b];
+    int64_t len = s.start < 0 ? 0 : s.start + n;
+    if (len > a.max_kvlen) {
+        len = a.max_kvlen;
+        cut = true;
+    }
+    if (cut && threadIdx.x == 0) {
+        atomicOr(a.status, kDevLengthClamped);
+    }
+    s.rows = static_cast<int32_t>(n) * a.group;
+    s.len = n > 0 ? static_cast<int32_t>(len) : 0;
+    return s;
+}
+
+// Scores (unscaled) of the 16 positions from `tile0` on against NOCT octets of query rows whose fragments are in qf.
+// acc[o][0..1]: position g, rows 2t and 2t+1 of octet o; acc[o][2..3]: position g + 8.
+template <int DH, int NOCT>
+struct Tile {
+    static constexpr int kWords = DH / 16;
+    uint4 code[2][DH / 64];
+    uint32_t sc[2][DH / 64];
+
+    __device__ __forceinline__ void load(const WeightArgs& a, int64_t b, int head, int32_t tile0, int32_t len, int lane,
+                                         int64_t& row0) {
+        row0 = cache_row(a.geom, a.cachestarts, b, tile0);
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int i = g + 8 * r;
+            const bool ok = tile0 + i < len && row0 >= 0 && cache_row_ok(row0 + i, a.max_tokens);
+            if (tile0 + i < len && !ok) {
+                atomicOr(a.status, kDevRowOutOfRange);
+            }
+            const int64_t off = ok ? cache_offset(a.geom, row0 + i, 0, head) : 0;
+#pragma unroll
+            for (int h = 0; h < DH / 64; ++h) {
+                code[r][h] = make_uint4(0u, 0u, 0u, 0u);
+                sc[r][h] = 0u;
+                if (ok) {
+                    code[r][h] = *reinterpret_cast<const uint4*>(a.cache + off + h * 64 + t * 16);
+                    sc[r][h] = *reinterpret_cast<const uint32_t*>(a.scale + (off >> 3) + h * 8 + t * 2);
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void scores(const uint2 (&qf)[NOCT][kWords], float (&acc)[NOCT][4]) const {
+#pragma unroll
+        for (int o = 0; o < NOCT; ++o) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                acc[o][e] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+            uint32_t k[2][2], e[2][2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const uint4 c = code[r][w / 4];
+                const uint32_t word = (w & 3) == 0 ? c.x : ((w & 3) == 1 ? c.y : ((w & 3) == 2 ? c.z : c.w));
+                const uint32_t s = prmt(sc[r][w / 4], 0u, (w & 2) ? 0x3232u : 0x1010u);
+                split_key_word(word, u32_as_h2(s), k[r][0], k[r][1], e[r][0], e[r][1]);
+            }
+#pragma unroll
+            for (int o = 0; o < NOCT; ++o) {
+                mma_m16n8k16_f16f32(acc[o], k[0][0], k[1][0], k[0][1], k[1][1], qf[o][w].x, qf[o][w].y);
+                mma_m16n8k16_f16f32(acc[o], e[0][0], e[1][0], e[0][1], e[1][1], qf[o][w].x, qf[o][w].y);
+            }
+        }
+    }
+};
+
+// Query fragments of the rows [row0, row0 + 8 NOCT): rows behind the last read as zeros
+template <int DH, int NOCT>
+__device__ __forceinline__ void load_queries(const WeightArgs& a, const Span& s, int head, int32_t row0, int lane,
+                                             uint2 (&qf)[NOCT][DH / 16]) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int o = 0; o < NOCT; ++o) {
+        const int32_t r = row0 + o * 8 + g;
+        const int32_t i = r / a.group;
+        const __half* src = a.q + ((s.tok0 + i) * a.num_heads + head * a.group + (r - i * a.group)) * DH;
+#pragma unroll
+        for (int w = 0; w < DH / 16; ++w) {
+            qf[o][w] = make_uint2(0u, 0u);
+            if (r < s.rows) {
+                qf[o][w] = *reinterpret_cast<const uint2*>(src + (w / 4) * 64 + t * 16 + (w & 3) * 4);
+            }
+        }
+    }
+}
+
+// -inf in the places of `acc` that a query row may not see
+template <int NOCT>
+__device__ __forceinline__ void hide(const WeightArgs& a, const Span& s, int32_t row0, int32_t tile0, int lane,
+                                     float (&acc)[NOCT][4]) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int o = 0; o < NOCT; ++o) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int32_t r = row0 + o * 8 + 2 * t + c;
+            const int64_t last = a.causal ? s.start + r / a.group : s.len - 1;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int32_t j = tile0 + g + 8 * p;
+                if (j > last || j >= s.len) {
+                    acc[o][2 * p + c] = -INFINITY;
+                }
+            }
+        }
+    }
+}
+
+template <int DH, int NOCT>
+__global__ void __launch_bounds__(kThreads) attn_weight_stats_kernel(const WeightArgs a) {
+    __shared__ float2 red[kWarps][NOCT * 8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t b = blockIdx.z;
+    const int head = blockIdx.y, chunk = blockIdx.x;
+    const Span s = span_of(a, b);
+    const int32_t first = chunk * kChunk;
+    if (first >= s.len) {
+        return;
+    }
+    const int32_t end = first + kChunk < s.len ? first + kChunk : s.len;
+    for (int32_t row0 = 0; row0 < s.rows; row0 += NOCT * 8) {
+        uint2 qf[NOCT][DH / 16];
+        load_queries<DH, NOCT>(a, s, head, row0, lane, qf);
+        float m[NOCT][2], l[NOCT][2];
+#pragma unroll
+        for (int o = 0; o < NOCT; ++o) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                m[o][c] = kNegBig;
+                l[o][c] = 0.0f;
+            }
+        }
+        for (int32_t tile0 = first + warp * 16; tile0 < end; tile0 += kWarps * 16) {
+            Tile<DH, NOCT> tile;
+            int64_t row;
+            tile.load(a, b, head, tile0, s.len, lane, row);
+            float acc[NOCT][4];
+            tile.scores(qf, acc);
+            if (tile0 + 15 > s.start || tile0 + 15 >= s.len) {
+                hide<NOCT>(a, s, row0, tile0, lane, acc);
+            }
+#pragma unroll
+            for (int o = 0; o < NOCT; ++o) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float x = acc[o][c] * a.scale_log2, y = acc[o][2 + c] * a.scale_log2;
+                    const float top = fmaxf(m[o][c], fmaxf(x, y));
+                    l[o][c] = l[o][c] * ex2_approx(m[o][c] - top) + ex2_approx(x - top) + ex2_approx(y - top);
+                    m[o][c] = top;
+                }
+            }
+        }
+        // over the eight positions a column's values are spread over, then over the warps
+#pragma unroll
+        for (int o = 0; o < NOCT; ++o) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) {
+                    const float om = __shfl_xor_sync(0xffffffffu, m[o][c], x);
+                    const float ol = __shfl_xor_sync(0xffffffffu, l[o][c], x);
+                    const float top = fmaxf(m[o][c], om);
+                    l[o][c] = l[o][c] * ex2_approx(m[o][c] - top) + ol * ex2_approx(om - top);
+                    m[o][c] = top;
+                }
+                if (lane < 4) {
+                    red[warp][o * 8 + 2 * lane + c] = make_float2(m[o][c], l[o][c]);
+                }
+            }
+        }
+        __syncthreads();
+        const int32_t r = row0 + threadIdx.x;
+        if (threadIdx.x < NOCT * 8 && r < s.rows) {
+            float2 v = red[0][threadIdx.x];
+#pragma unroll
+            for (int k = 1; k < kWarps; ++k) {
+                const float2 u = red[k][threadIdx.x];
+                const float top = fmaxf(v.x, u.x);
+                v.y = v.y * ex2_approx(v.x - top) + u.y * ex2_approx(u.x - top);
+                v.x = top;
+            }
+            const int32_t i = r / a.group;
+            const int64_t at = (s.tok0 + i) * a.num_heads + head * a.group + (r - i * a.group);
+            a.part[chunk * a.total_tokens * a.num_heads + at] = v;
+        }
+        __syncthreads();
+    }
+}
+
+// One warp per (query token, head): joins the chunks of its sequence.
+__global__ void __launch_bounds__(256) attn_weight_merge_kernel(const WeightArgs a, int32_t batch) {
+    const int lane = threadIdx.x & 31;
+    const int64_t id = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
+    const int64_t tok = id / a.num_heads;
+    if (tok >= a.total_tokens) {
+        return;
+    }
+    int32_t lo = 0, hi = batch;  // sequence of the token
+    while (hi - lo > 1) {
+        const int32_t mid = (lo + hi) >> 1;
+        if (a.seqstarts[mid] <= tok) {
+            lo = mid;
+        } else {
+            hi = mid;
+        }
+    }
+    const int64_t i = tok - a.seqstarts[lo], start = a.start_pos[lo];
+    int64_t n = a.seqstarts[lo + 1] - a.seqstarts[lo];
+    n = n > a.max_seqlen ? a.max_seqlen : n;
+    int64_t len = start < 0 ? 0 : start + n;
+    len = len > a.max_kvlen ? a.max_kvlen : len;
+    if (i < 0 || i >= n) {
+        return;
+    }
+    const int32_t chunks = static_cast<int32_t>((len + kChunk - 1) / kChunk);
+    float m = kNegBig, l = 0.0f;
+    for (int32_t c = lane; c < chunks; c += 32) {
+        const float2 v = a.part[c * a.total_tokens * a.num_heads + id];
+        const float top = fmaxf(m, v.x);
+        l = l * ex2_approx(m - top) + v.y * ex2_approx(v.x - top);
+        m = top;
+    }
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const float om = __shfl_xor_sync(0xffffffffu, m, x), ol = __shfl_xor_sync(0xffffffffu, l, x);
+        const float top = fmaxf(m, om);
+        l = l * ex2_approx(m - top) + ol * ex2_approx(om - top);
+        m = top;
+    }
+    if (lane == 0) {
+        a.norm[id] = make_float2(m, l > 0.0f ? 1.0f / l : 0.0f);
+    }
+}
+
+template <int DH, int NOCT>
+__global__ void __launch_bounds__(kThreads) attn_weight_apply_kernel(const WeightArgs a) {
+    __shared__ float sum[kChunk];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int64_t b = blockIdx.z;
+    const int head = blockIdx.y, chunk = blockIdx.x;
+    const Span s = span_of(a, b);
+    const int32_t first = chunk * kChunk;
+    if (first >= s.len) {
+        return;
+    }
+    const int32_t end = first + kChunk < s.len ? first + kChunk : s.len;
+    float* w = a.weight + (a.geom.layer_idx * a.num_kv_heads + head) * a.max_tokens;
+    for (int32_t row0 = 0; row0 < s.rows; row0 += NOCT * 8) {
+        uint2 qf[NOCT][DH / 16];
+        load_queries<DH, NOCT>(a, s, head, row0, lane, qf);
+        float neg_m[NOCT][2], inv[NOCT][2];
+#pragma unroll
+        for (int o = 0; o < NOCT; ++o) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int32_t r = row0 + o * 8 + 2 * t + c;
+                neg_m[o][c] = -INFINITY;  // rows behind the last: no weight
+                inv[o][c] = 0.0f;
+                if (r < s.rows) {
+                    const int32_t i = r / a.group;
+                    const float2 v = a.norm[(s.tok0 + i) * a.num_heads + head * a.group + (r - i * a.group)];
+                    neg_m[o][c] = -v.x;
+                    inv[o][c] = v.y;
+                }
+            }
+        }
+        const bool last_rows = row0 + NOCT * 8 >= s.rows;
+        for (int32_t tile0 = first + warp * 16; tile0 < end; tile0 += kWarps * 16) {
+            Tile<DH, NOCT> tile;
+            int64_t row;
+            tile.load(a, b, head, tile0, s.len, lane, row);
+            float acc[NOCT][4];
+            tile.scores(qf, acc);
+            if (tile0 + 15 > s.start || tile0 + 15 >= s.len) {
+                hide<NOCT>(a, s, row0, tile0, lane, acc);
+            }
+            float part[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int o = 0; o < NOCT; ++o) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        part[p] = fmaf(ex2_approx(fmaf(acc[o][2 * p + c], a.scale_log2, neg_m[o][c])), inv[o][c], part[p]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                part[p] += __shfl_xor_sync(0xffffffffu, part[p], 1);
+                part[p] += __shfl_xor_sync(0xffffffffu, part[p], 2);
+            }
+            // lane t = 0 of a quad owns position g, t = 1 position g + 8: one addition per position and call
+            if (t < 2) {
+                const int i = g + 8 * t;
+                float x = t == 0 ? part[0] : part[1];
+                float* acc_row = &sum[tile0 - first + i];
+                if (row0 > 0) {
+                    x += *acc_row;
+                }
+                if (!last_rows) {
+                    *acc_row = x;
+                } else if (tile0 + i < s.len && row >= 0 && cache_row_ok(row + i, a.max_tokens)) {
+                    atomicAdd(w + row + i, x);
+                }
+            }
+        }
+    }
+}
+
+template <int DH>
+int launch_dh(const pplb200_attn_params& p, const WeightArgs& a, cudaStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(a.chunks), static_cast<unsigned>(p.num_kv_heads), static_cast<unsigned>(p.batch));
+    const int64_t rows = p.max_seqlen * a.group;
+    int rc;
+    if (rows <= 8) {
+        attn_weight_stats_kernel<DH, 1><<<grid, kThreads, 0, stream>>>(a);
+    } else {
+        attn_weight_stats_kernel<DH, kRowBlock / 8><<<grid, kThreads, 0, stream>>>(a);
+    }
+    rc = check_launch("attn_weight_stats_kernel");
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    const int64_t warps = p.total_tokens * p.num_heads;
+    attn_weight_merge_kernel<<<static_cast<unsigned>((warps * 32 + 255) / 256), 256, 0, stream>>>(
+        a, static_cast<int32_t>(p.batch));
+    rc = check_launch("attn_weight_merge_kernel");
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    if (rows <= 8) {
+        attn_weight_apply_kernel<DH, 1><<<grid, kThreads, 0, stream>>>(a);
+    } else {
+        attn_weight_apply_kernel<DH, kRowBlock / 8><<<grid, kThreads, 0, stream>>>(a);
+    }
+    return check_launch("attn_weight_apply_kernel");
+}
+
+}  // namespace
+
+int make_weight_plan(const pplb200_attn_params& p, WeightPlan* plan) {
+    plan->chunks = (p.max_kvlen + kChunk - 1) / kChunk;
+    const uint64_t rows = static_cast<uint64_t>(p.total_tokens) * p.num_heads;
+    plan->off_norm = 256;  // behind the status word
+    plan->off_part = plan->off_norm + (rows * 8 + 255) / 256 * 256;
+    plan->bytes = plan->off_part + (rows * plan->chunks * 8 + 255) / 256 * 256;
+    return plan->chunks > 0x7fffffff / kChunk ? PPLB200_UNSUPPORTED : PPLB200_SUCCESS;
+}
+
+int launch_attn_weight(const pplb200_attn_params& p, const CacheGeom& geom, const WeightPlan& plan, const void* query,
+                       const int64_t* seqstarts, const int64_t* cachestarts, const int64_t* start_pos,
+                       const void* cache, const void* scale, float* weight, void* workspace, cudaStream_t stream) {
+    if (plan.chunks <= 0 || p.max_seqlen <= 0) {
+        return PPLB200_SUCCESS;
+    }
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    WeightArgs a = {};
+    a.q = static_cast<const __half*>(query);
+    a.seqstarts = seqstarts;
+    a.cachestarts = cachestarts;
+    a.start_pos = start_pos;
+    a.cache = static_cast<const int8_t*>(cache);
+    a.scale = static_cast<const __half*>(scale);
+    a.weight = weight;
+    a.norm = reinterpret_cast<float2*>(ws + plan.off_norm);
+    a.part = reinterpret_cast<float2*>(ws + plan.off_part);
+    a.status = reinterpret_cast<uint32_t*>(ws);
+    a.geom = geom;
+    a.max_seqlen = p.max_seqlen;
+    a.max_kvlen = p.max_kvlen;
+    a.max_tokens = p.max_tokens;
+    a.total_tokens = p.total_tokens;
+    a.num_heads = p.num_heads;
+    a.num_kv_heads = p.num_kv_heads;
+    a.group = p.num_heads / p.num_kv_heads;
+    a.causal = p.is_causal ? 1 : 0;
+    a.chunks = static_cast<int32_t>(plan.chunks);
+    a.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(p.head_dim));
+    return p.head_dim == 128 ? launch_dh<128>(p, a, stream) : launch_dh<64>(p, a, stream);
+}
+
+}  // namespace pplb200

@@ -662,6 +662,210 @@ int pplb200_rope_kv_append_i8g8(const pplb200_rope_params* p, const pplb200_attn
                        rotated_key, cache, scale, di.sm_count, st);
 }
 
+// Checks shared by the operators around the cache that take a workspace; `bytes` is what they need.
+static int check_workspace(const void* workspace, uint64_t workspace_bytes, uint64_t bytes, const char* too_small) {
+    if (!workspace) {
+        return fail(PPLB200_NOT_FOUND, "workspace is null");
+    }
+    if (workspace_bytes < bytes) {
+        return fail(PPLB200_OUT_OF_MEMORY, too_small);
+    }
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) {
+        return fail(PPLB200_INVALID_VALUE, "workspace must be 256-byte aligned");
+    }
+    return PPLB200_SUCCESS;
+}
+
+static int clear_status(void* workspace, cudaStream_t stream) {
+    if (cudaMemsetAsync(workspace, 0, 4, stream) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return fail(PPLB200_DEVICE_RUNTIME_ERROR, "cudaMemsetAsync(status) failed");
+    }
+    return PPLB200_SUCCESS;
+}
+
+// validate() and what these operators need beyond it: positions and grid indices that fit their kernels
+static int validate_cache_op(const pplb200_attn_params* p) {
+    const int rc = validate(p);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    if (p->max_kvlen > 0x7fff0000) {
+        return fail(PPLB200_UNSUPPORTED, "max_kvlen above 2^31 - 2^16");
+    }
+    if (p->batch > 65535 || p->num_kv_heads > 65535) {
+        return fail(PPLB200_UNSUPPORTED, "more than 65535 sequences or kv heads");
+    }
+    return PPLB200_SUCCESS;
+}
+
+int pplb200_attn_weight_workspace_size(const pplb200_attn_params* p, uint64_t* bytes) {
+    int rc = validate_cache_op(p);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    if (!bytes) {
+        return fail(PPLB200_NOT_FOUND, "bytes is null");
+    }
+    WeightPlan plan;
+    rc = make_weight_plan(*p, &plan);
+    *bytes = plan.bytes;
+    return rc;
+}
+
+int pplb200_attn_weight_accumulate(const pplb200_attn_params* p, const void* query, const int64_t* seqstarts,
+                                   const int64_t* cachestarts, const int64_t* start_pos, const void* cache,
+                                   const void* scale, float* weight, void* workspace, uint64_t workspace_bytes,
+                                   void* stream_v) {
+    int rc = validate_cache_op(p);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    if (!scale) {
+        return fail(PPLB200_UNSUPPORTED, "only a quantised cache is supported but scale is null");
+    }
+    // an empty batch is a no-op whatever the pointers are (empty tensors have none)
+    if (p->batch == 0 || p->total_tokens == 0) {
+        return PPLB200_SUCCESS;
+    }
+    if (!query || !seqstarts || !cachestarts || !start_pos || !cache || !weight) {
+        return fail(PPLB200_NOT_FOUND, "a required tensor pointer is null");
+    }
+    if (misaligned({query, cache, scale, weight}, {seqstarts, cachestarts, start_pos})) {
+        return fail(PPLB200_INVALID_VALUE, "tensor pointers must be 16-byte aligned (index tensors 8-byte)");
+    }
+    DeviceInfo di;
+    rc = require_device(&di);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    WeightPlan plan;
+    rc = make_weight_plan(*p, &plan);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    rc = check_workspace(workspace, workspace_bytes, plan.bytes, "workspace is smaller than pplb200_attn_weight_workspace_size()");
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+    rc = clear_status(workspace, stream);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    return launch_attn_weight(*p, make_geom(*p), plan, query, seqstarts, cachestarts, start_pos, cache, scale, weight,
+                              workspace, stream);
+}
+
+int pplb200_kv_evict_workspace_size(const pplb200_attn_params* p, uint64_t* bytes) {
+    const int rc = validate_cache_op(p);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    if (!bytes) {
+        return fail(PPLB200_NOT_FOUND, "bytes is null");
+    }
+    *bytes = 256;  // the device status word
+    return PPLB200_SUCCESS;
+}
+
+int pplb200_kv_evict_select(const pplb200_attn_params* p, const float* weight, const int64_t* cachestarts,
+                            const int64_t* kvlens, const int64_t* budgets, int64_t sink, int64_t recent,
+                            int64_t max_budget, int64_t* kept, void* workspace, uint64_t workspace_bytes,
+                            void* stream_v) {
+    int rc = validate_cache_op(p);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    if (sink < 0 || recent < 0 || max_budget < 0) {
+        return fail(PPLB200_INVALID_VALUE, "sink, recent and max_budget must not be negative");
+    }
+    if (p->batch == 0 || max_budget == 0) {
+        return PPLB200_SUCCESS;
+    }
+    if (!weight || !cachestarts || !kvlens || !budgets || !kept) {
+        return fail(PPLB200_NOT_FOUND, "a required tensor pointer is null");
+    }
+    if (misaligned({weight}, {cachestarts, kvlens, budgets, kept})) {
+        return fail(PPLB200_INVALID_VALUE, "tensor pointers must be 16-byte aligned (index tensors 8-byte)");
+    }
+    DeviceInfo di;
+    rc = require_device(&di);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    rc = check_workspace(workspace, workspace_bytes, 256, "workspace is smaller than pplb200_kv_evict_workspace_size()");
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+    rc = clear_status(workspace, stream);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    return launch_kv_evict_select(*p, make_geom(*p), weight, cachestarts, kvlens, budgets, sink, recent, max_budget,
+                                  static_cast<uint32_t*>(workspace), kept, stream);
+}
+
+int pplb200_kv_compact_workspace_size(const pplb200_attn_params* p, uint64_t* bytes) {
+    const int rc = validate_cache_op(p);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    if (!bytes) {
+        return fail(PPLB200_NOT_FOUND, "bytes is null");
+    }
+    *bytes = 256;  // the device status word
+    return PPLB200_SUCCESS;
+}
+
+int pplb200_kv_compact(const pplb200_attn_params* p, const int64_t* kept, int64_t kept_heads, int64_t max_kept,
+                       const int64_t* base, const int64_t* kvlens, const int64_t* cachestarts, int64_t layers,
+                       void* cache, void* scale, float* weight, void* workspace, uint64_t workspace_bytes,
+                       void* stream_v) {
+    int rc = validate_cache_op(p);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    if (!scale) {
+        return fail(PPLB200_UNSUPPORTED, "only a quantised cache is supported but scale is null");
+    }
+    if (kept_heads != 1 && kept_heads != p->num_kv_heads) {
+        return fail(PPLB200_INVALID_VALUE, "kept_heads must be 1 or num_kv_heads");
+    }
+    if (layers <= 0 || layers > p->num_layer - p->layer_idx) {
+        return fail(PPLB200_INVALID_VALUE, "layers must be positive and end within num_layer");
+    }
+    if (max_kept < 0 || max_kept > 0x7fff0000) {
+        return fail(PPLB200_INVALID_VALUE, "max_kept out of range");
+    }
+    if (p->batch == 0 || (max_kept == 0 && !weight)) {
+        return PPLB200_SUCCESS;
+    }
+    if ((!kept && max_kept > 0) || !base || !kvlens || !cachestarts || !cache) {
+        return fail(PPLB200_NOT_FOUND, "a required tensor pointer is null");
+    }
+    if (misaligned({cache, scale, weight}, {kept, base, kvlens, cachestarts})) {
+        return fail(PPLB200_INVALID_VALUE, "tensor pointers must be 16-byte aligned (index tensors 8-byte)");
+    }
+    DeviceInfo di;
+    rc = require_device(&di);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    rc = check_workspace(workspace, workspace_bytes, 256, "workspace is smaller than pplb200_kv_compact_workspace_size()");
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+    rc = clear_status(workspace, stream);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    return launch_kv_compact(*p, make_geom(*p), kept, kept_heads, max_kept, base, kvlens, cachestarts, layers, cache,
+                             scale, weight, static_cast<uint32_t*>(workspace), stream);
+}
+
 int pplb200_mhca_device_status(const void* workspace, void* stream, uint32_t* status) {
     if (!workspace || !status) {
         return PPLB200_NOT_FOUND;

@@ -119,6 +119,24 @@ int launch_mha(int num_heads, int num_kv_heads, int head_dim, int is_causal, int
                const void* value, const int64_t* seqstarts, const int64_t* kvstarts, const MaskDev& mask,
                uint32_t* status_word, void* attn_output, cudaStream_t stream);
 
+// ---- accumulated attention weight, eviction, compaction --------------------------------------------
+struct WeightPlan {
+    int64_t chunks;  // chunks of positions per sequence
+    uint64_t off_norm, off_part, bytes;
+};
+int make_weight_plan(const pplb200_attn_params& p, WeightPlan* plan);
+int launch_attn_weight(const pplb200_attn_params& p, const CacheGeom& geom, const WeightPlan& plan, const void* query,
+                       const int64_t* seqstarts, const int64_t* cachestarts, const int64_t* start_pos,
+                       const void* cache, const void* scale, float* weight, void* workspace, cudaStream_t stream);
+
+int launch_kv_evict_select(const pplb200_attn_params& p, const CacheGeom& geom, const float* weight,
+                           const int64_t* cachestarts, const int64_t* kvlens, const int64_t* budgets, int64_t sink,
+                           int64_t recent, int64_t max_budget, uint32_t* status, int64_t* kept, cudaStream_t stream);
+
+int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const int64_t* kept, int64_t kept_heads,
+                      int64_t max_kept, const int64_t* base, const int64_t* kvlens, const int64_t* cachestarts,
+                      int64_t layers, void* cache, void* scale, float* weight, uint32_t* status, cudaStream_t stream);
+
 // Rotary position embedding, alone (append == nullptr) or fused with the cache append.
 uint64_t rope_workspace_bytes(const pplb200_rope_params& p);
 int launch_rope(const pplb200_rope_params& p, const pplb200_attn_params* append, const CacheGeom* geom,

@@ -383,3 +383,195 @@ class RotaryPositionEmbedding(_Base):
                                      _ptr(cache), _ptr(scale), _stream())
         self._raise("pplb200_rope_kv_append_i8g8", rc)
         return rotated_query, rotated_key
+
+
+def _require_index(device, **tensors):
+    """CUDA tensors of one device, int64, as the kernels read them."""
+    _require_cuda(**tensors)
+    for name, t in tensors.items():
+        if t.dtype != torch.int64:
+            raise OpError("RC_INVALID_VALUE", f"{name} must be int64")
+    _require_device(device, **tensors)
+
+
+def _require_device(device, **tensors):
+    for name, t in tensors.items():
+        if t.device != device:
+            raise OpError("RC_INVALID_VALUE", f"{name} is on {t.device}, not on {device}")
+
+
+def _require_cache(cache, scale, layout):
+    """Checks an INT8 cache and its scales against one another; returns (layers, kv heads, head_dim)."""
+    _require_cuda(cache=cache)
+    if scale is None or scale.numel() == 0:
+        raise OpError("RC_UNSUPPORTED", "currently only support qunatized cache but scale not found")
+    _require_cuda(scale=scale)
+    if cache.dtype != torch.int8 or scale.dtype != torch.float16:
+        raise OpError("RC_UNSUPPORTED", "the cache must be int8 with fp16 scales")
+    if layout not in (0, 3):
+        raise OpError("RC_UNSUPPORTED", "currently only support cache_layout == 0 or cache_layout == 3")
+    _require_device(cache.device, scale=scale)
+    if cache.dim() != 5 or cache.shape[:4] != scale.shape[:4] or cache.shape[4] != 8 * scale.shape[4]:
+        raise OpError("RC_INVALID_VALUE", "cache and scale do not belong together")
+    layers, heads = (cache.shape[1], cache.shape[3]) if layout == 0 else (cache.shape[0], cache.shape[2])
+    return layers, heads, cache.shape[4]
+
+
+def _require_weight(weight, num_layer):
+    _require_cuda(weight=weight)
+    if weight.dtype != torch.float32:
+        raise OpError("RC_UNSUPPORTED", "weight must be fp32")
+    if weight.dim() != 3 or weight.shape[0] != num_layer:
+        raise OpError("RC_INVALID_VALUE", "weight must be [num_layer, num_kv_heads, max_tokens]")
+
+
+class _CacheOp(_Base):
+    """What the operators around the cache share: parameters from the cache's geometry, and a workspace whose first
+    word is the device status word.  The workspace is allocated per call, so that calls of one object on two streams,
+    or in two captured graphs, never share one; the last call's is kept for device_status()."""
+
+    def __init__(self, param):
+        super().__init__()
+        self.param = param
+        self._workspace: torch.Tensor | None = None
+
+    def _params(self, *, num_heads, num_kv_heads, head_dim, batch, max_kvlen, max_tokens, cachestarts, max_seqlen=0,
+                total_tokens=0, is_causal=True) -> capi.AttnParams:
+        a = self.param
+        if a.cache_mode == 1 and cachestarts.dim() != 2:
+            raise OpError("RC_INVALID_VALUE", "cachestarts must be a 2d tensor in cache_mode 1")
+        if cachestarts.shape[0] != batch or (a.cache_mode == 0 and cachestarts.dim() != 1):
+            raise OpError("RC_INVALID_VALUE", "cachestarts must have an entry (cache_mode 1: a row) per sequence")
+        p = capi.AttnParams()
+        p.num_heads, p.num_kv_heads, p.head_dim = num_heads, num_kv_heads, head_dim
+        p.is_causal = int(is_causal)
+        p.num_layer, p.layer_idx = a.num_layer, a.layer_idx
+        p.quant_bit, p.quant_group = a.quant_bit, a.quant_group
+        p.cache_mode, p.cache_layout, p.page_size = a.cache_mode, a.cache_layout, a.page_size
+        p.batch, p.total_tokens, p.max_tokens = batch, total_tokens, max_tokens
+        p.max_seqlen, p.max_kvlen = int(max_seqlen), int(max_kvlen)
+        p.cachestart_stride_b = cachestarts.shape[1] if a.cache_mode == 1 else 0
+        self._raise("pplb200_fill_cache_strides", self.lib.fill_cache_strides(p))
+        return p
+
+    def _call(self, name, size_fn, fn, p, device, *args) -> None:
+        """Runs fn(p, *args, workspace, bytes, stream) on the tensors' device and its current stream."""
+        rc, nbytes = size_fn(p)
+        self._raise(name, rc)
+        with torch.cuda.device(device):
+            self._workspace = ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            rc = fn(p, *args, _ptr(ws), nbytes, _stream())
+        self._raise(name, rc)
+
+    def device_status(self) -> int:
+        """Status word left by the kernels of the last forward (synchronises the stream)."""
+        if self._workspace is None:
+            return 0
+        with torch.cuda.device(self._workspace.device):
+            rc, s = self.lib.mhca_device_status(_ptr(self._workspace), _stream())
+        self._raise("pplb200_mhca_device_status", rc)
+        return s
+
+
+class AttentionWeight(_CacheOp):
+    """Adds to ``weight`` [num_layer, num_kv_heads, max_tokens] (fp32, by cache row) the softmax weights that this
+    call's query tokens give each cached position, summed over the tokens and the query heads of a kv group.  The
+    tokens themselves have been appended already."""
+
+    def __init__(self, param: MultiHeadCacheAttentionParam):
+        super().__init__(param)
+
+    def forward(self, query, seqstarts, cachestarts, start_pos, max_seqlen: int, max_kvlen: int, cache, scale,
+                weight) -> torch.Tensor:
+        a = self.param
+        layers, kv_heads, dim = _require_cache(cache, scale, a.cache_layout)
+        _require_cuda(query=query)
+        _require_weight(weight, a.num_layer)
+        _require_device(cache.device, query=query, weight=weight)
+        _require_index(cache.device, seqstarts=seqstarts, cachestarts=cachestarts, start_pos=start_pos)
+        if a.is_alibi:
+            raise OpError("RC_UNSUPPORTED", "currently only support is_alibi == false")
+        if query.dtype != torch.float16:
+            raise OpError("RC_UNSUPPORTED", "currently only support fp16")
+        max_tokens = _max_tokens(cache, a.cache_layout)
+        if query.shape[1:] != (a.num_heads, a.head_dim) or (layers, kv_heads, dim) != (a.num_layer, a.num_kv_heads,
+                                                                                      a.head_dim):
+            raise OpError("RC_INVALID_VALUE", "query or cache does not have the shape of the attributes")
+        if weight.shape[1:] != (kv_heads, max_tokens) or seqstarts.shape[0] != start_pos.shape[0] + 1:
+            raise OpError("RC_INVALID_VALUE", "weight or seqstarts does not have the shape of the cache and batch")
+        p = self._params(num_heads=a.num_heads, num_kv_heads=kv_heads, head_dim=dim, batch=start_pos.shape[0],
+                         max_kvlen=max_kvlen, max_tokens=max_tokens, cachestarts=cachestarts, max_seqlen=max_seqlen,
+                         total_tokens=query.shape[0], is_causal=a.is_causal)
+        self._call("pplb200_attn_weight_accumulate", self.lib.attn_weight_workspace_size,
+                   self.lib.attn_weight_accumulate, p, cache.device, _ptr(query), _ptr(seqstarts), _ptr(cachestarts),
+                   _ptr(start_pos), _ptr(cache), _ptr(scale), _ptr(weight))
+        return weight
+
+
+@dataclass
+class KeyValueCacheEvictParam(KeyValueCacheParam):
+    """Cache geometry, and the positions that stay whatever their weight: the first ``sink``, the last ``recent``."""
+    sink: int = 0
+    recent: int = 0
+
+
+class KeyValueCacheEvict(_CacheOp):
+    """Which cached positions to keep, per kv head: the last ``recent``, the first ``sink``, and the highest
+    accumulated weights (ties: the lowest position) up to the sequence's budget.  Returns the kept positions
+    [batch, num_kv_heads, max_budget] in ascending order, -1 behind them; KeyValueCacheCompact moves their rows."""
+
+    def __init__(self, param: KeyValueCacheEvictParam):
+        super().__init__(param)
+
+    def forward(self, weight, cachestarts, kvlens, budgets, max_kvlen: int, max_budget: int,
+                kept: torch.Tensor | None = None) -> torch.Tensor:
+        a = self.param
+        _require_weight(weight, a.num_layer)
+        _require_index(weight.device, cachestarts=cachestarts, kvlens=kvlens, budgets=budgets)
+        batch, heads = kvlens.shape[0], weight.shape[1]
+        if budgets.shape != kvlens.shape or max_budget < 0:
+            raise OpError("RC_INVALID_VALUE", "budgets must have an entry per sequence and max_budget not be negative")
+        if kept is None:
+            kept = torch.empty((batch, heads, int(max_budget)), dtype=torch.int64, device=weight.device)
+        _require_index(weight.device, kept=kept)
+        if kept.shape != (batch, heads, int(max_budget)):
+            raise OpError("RC_INVALID_VALUE", "kept must be [batch, num_kv_heads, max_budget]")
+        # the choice does not depend on the head size; any supported one describes the rows
+        p = self._params(num_heads=heads, num_kv_heads=heads, head_dim=128, batch=batch, max_kvlen=max_kvlen,
+                         max_tokens=weight.shape[2], cachestarts=cachestarts)
+        self._call("pplb200_kv_evict_select", self.lib.kv_evict_workspace_size, self.lib.kv_evict_select, p,
+                   weight.device, _ptr(weight), _ptr(cachestarts), _ptr(kvlens), _ptr(budgets), a.sink, a.recent,
+                   max_budget, _ptr(kept))
+        return kept
+
+
+class KeyValueCacheCompact(_CacheOp):
+    """Moves the cache rows of the kept positions to the front, in place: position base + kept[i] to base + i, of
+    ``num_layers`` layers from layer_idx on.  ``kept`` [batch, num_kv_heads or 1, K] is strictly ascending and ends at
+    its first negative entry; ``kvlens`` are the positions the sequences had.  ``weight`` (as of AttentionWeight)
+    moves along and is zeroed behind the kept positions."""
+
+    def __init__(self, param: KeyValueCacheParam):
+        super().__init__(param)
+
+    def forward(self, kept, cachestarts, base, kvlens, max_kvlen: int, cache, scale, weight=None,
+                num_layers: int = 1) -> None:
+        a = self.param
+        layers, heads, dim = _require_cache(cache, scale, a.cache_layout)
+        _require_index(cache.device, kept=kept, cachestarts=cachestarts, base=base, kvlens=kvlens)
+        max_tokens = _max_tokens(cache, a.cache_layout)
+        if layers != a.num_layer:
+            raise OpError("RC_INVALID_VALUE", "cache does not have num_layer layers")
+        batch = kvlens.shape[0]
+        if kept.dim() != 3 or kept.shape[0] != batch or kept.shape[1] not in (1, heads) or base.shape != kvlens.shape:
+            raise OpError("RC_INVALID_VALUE", "kept must be [batch, num_kv_heads or 1, K], base and kvlens [batch]")
+        if weight is not None:
+            _require_weight(weight, a.num_layer)
+            _require_device(cache.device, weight=weight)
+            if weight.shape[1:] != (heads, max_tokens):
+                raise OpError("RC_INVALID_VALUE", "weight does not have the shape of the cache")
+        p = self._params(num_heads=heads, num_kv_heads=heads, head_dim=dim, batch=batch, max_kvlen=max_kvlen,
+                         max_tokens=max_tokens, cachestarts=cachestarts)
+        self._call("pplb200_kv_compact", self.lib.kv_compact_workspace_size, self.lib.kv_compact, p, cache.device,
+                   _ptr(kept), kept.shape[1], kept.shape[2], _ptr(base), _ptr(kvlens), _ptr(cachestarts), num_layers,
+                   _ptr(cache), _ptr(scale), _ptr(weight))
