@@ -298,6 +298,28 @@ int pplb200_rope_kv_append_i8g8(const pplb200_rope_params* p, const pplb200_attn
                                 void* scale, void* stream);
 
 /*
+ * Attention of a tree of drafted tokens over the cache: the verification step of speculative decoding.  Sequence b has
+ * start_pos[b] tokens of history and seqlen drafted tokens behind them, at positions start_pos[b] + i; their K and V
+ * have been appended before (pplb200_kv_append_i8g8 with the same seqstarts and start_pos).  Drafted token i sees the
+ * history, itself and its ancestors:
+ *   parents [total_tokens] int64: the index within the sequence's drafted tokens of token i's parent, which comes
+ *           before it (parent < i); -1: a child of the history.  Null: every token is the child of the one before it
+ *           (a single drafted chain).  A parent that breaks the rule counts as -1 (PPLB200_DEV_PARENT_INVALID).
+ *   query, attn_output [total_tokens, num_heads, head_dim] fp16; keys and values are the cache's codes times scales,
+ *           scores scaled by 1 / sqrt(head_dim).  The accepted path is kept with pplb200_kv_compact.
+ * Uses batch, max_seqlen (<= 1024), max_kvlen (>= start_pos[b] + seqlen), total_tokens, max_tokens and the cache
+ * geometry of the params; is_causal, decoding_batches and phase_mask are not used.  `workspace`:
+ * pplb200_tree_attn_workspace_size() bytes, 256-byte aligned (its first word is the status word); attn_output is
+ * 32-byte aligned.  No counterpart in the reference.
+ */
+int pplb200_tree_attn_workspace_size(const pplb200_attn_params* p, uint64_t* bytes);
+
+int pplb200_tree_attn_forward(const pplb200_attn_params* p, const void* query, const int64_t* parents,
+                              const int64_t* seqstarts, const int64_t* cachestarts, const int64_t* start_pos,
+                              const void* cache, const void* scale, void* workspace, uint64_t workspace_bytes,
+                              void* attn_output, void* stream);
+
+/*
  * Accumulated attention weight.  For every cached position j of every sequence and every kv head g of layer
  * layer_idx:  weight[layer_idx, g, row(j)] += sum over the query tokens i of the sequence and the query heads h of
  * the group of softmax_j(q[i, h] . k[j] / sqrt(head_dim)),  where token i sees the positions <= start_pos[b] + i
@@ -375,8 +397,10 @@ enum {
                                           that row was neither read nor written                     */
     PPLB200_DEV_MASK_OUT_OF_RANGE = 16,/* attn_mask has fewer columns than kvstarts needs: the missing
                                           entries were read as 0                                    */
-    PPLB200_DEV_KEPT_INVALID = 32      /* a kept list is not strictly ascending or names a position outside
+    PPLB200_DEV_KEPT_INVALID = 32,     /* a kept list is not strictly ascending or names a position outside
                                           its sequence: that entry was skipped                      */
+    PPLB200_DEV_PARENT_INVALID = 64    /* a drafted token's parent does not come before it: it was taken as a
+                                          child of the history                                      */
 };
 
 /* Name of a status code ("RC_SUCCESS", ...).  Never null. */

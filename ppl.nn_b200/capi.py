@@ -34,6 +34,7 @@ DEV_LENGTH_CLAMPED = 4
 DEV_ROW_OUT_OF_RANGE = 8
 DEV_MASK_OUT_OF_RANGE = 16
 DEV_KEPT_INVALID = 32
+DEV_PARENT_INVALID = 64
 
 # every symbol include/ppl_nn_b200.h declares
 EXPORTS = (
@@ -54,6 +55,8 @@ EXPORTS = (
     "pplb200_rope_workspace_size",
     "pplb200_rope_forward",
     "pplb200_rope_kv_append_i8g8",
+    "pplb200_tree_attn_workspace_size",
+    "pplb200_tree_attn_forward",
     "pplb200_attn_weight_workspace_size",
     "pplb200_attn_weight_accumulate",
     "pplb200_kv_evict_workspace_size",
@@ -192,6 +195,10 @@ class Library:
                                                   vp, vp, vp]
         sizep = ctypes.POINTER(ctypes.c_uint64)
         i64 = ctypes.c_int64
+        d.pplb200_tree_attn_workspace_size.restype = ctypes.c_int
+        d.pplb200_tree_attn_workspace_size.argtypes = [pp, sizep]
+        d.pplb200_tree_attn_forward.restype = ctypes.c_int
+        d.pplb200_tree_attn_forward.argtypes = [pp, vp, i64p, i64p, i64p, i64p, vp, vp, vp, ctypes.c_uint64, vp, vp]
         d.pplb200_attn_weight_workspace_size.restype = ctypes.c_int
         d.pplb200_attn_weight_workspace_size.argtypes = [pp, sizep]
         d.pplb200_attn_weight_accumulate.restype = ctypes.c_int
@@ -314,6 +321,14 @@ class Library:
         n = ctypes.c_uint64(0)
         rc = fn(ctypes.byref(p), ctypes.byref(n))
         return rc, int(n.value)
+
+    def tree_attn_workspace_size(self, p) -> tuple[int, int]:
+        return self._size(self.dll.pplb200_tree_attn_workspace_size, p)
+
+    def tree_attn_forward(self, p, q, parents, seqstarts, cachestarts, start_pos, cache, scale, out, workspace,
+                          workspace_bytes, stream) -> int:
+        return self.dll.pplb200_tree_attn_forward(ctypes.byref(p), q, parents, seqstarts, cachestarts, start_pos, cache,
+                                                  scale, workspace, int(workspace_bytes), out, stream)
 
     def attn_weight_workspace_size(self, p) -> tuple[int, int]:
         return self._size(self.dll.pplb200_attn_weight_workspace_size, p)

@@ -699,6 +699,79 @@ static int validate_cache_op(const pplb200_attn_params* p) {
     return PPLB200_SUCCESS;
 }
 
+static int validate_tree(const pplb200_attn_params* p) {
+    const int rc = validate_cache_op(p);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    if (p->max_seqlen > kTreeMaxTokens) {
+        return fail(PPLB200_UNSUPPORTED, "more than 1024 drafted tokens in a sequence");
+    }
+    if (p->max_seqlen * (p->num_heads / p->num_kv_heads) > 0x7fffff) {
+        return fail(PPLB200_UNSUPPORTED, "more than 2^23 query rows of a kv head in a sequence");
+    }
+    return PPLB200_SUCCESS;
+}
+
+int pplb200_tree_attn_workspace_size(const pplb200_attn_params* p, uint64_t* bytes) {
+    int rc = validate_tree(p);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    if (!bytes) {
+        return fail(PPLB200_NOT_FOUND, "bytes is null");
+    }
+    TreePlan plan;
+    rc = make_tree_plan(*p, planning_sm_count(), &plan);
+    *bytes = plan.bytes;
+    return rc;
+}
+
+int pplb200_tree_attn_forward(const pplb200_attn_params* p, const void* query, const int64_t* parents,
+                              const int64_t* seqstarts, const int64_t* cachestarts, const int64_t* start_pos,
+                              const void* cache, const void* scale, void* workspace, uint64_t workspace_bytes,
+                              void* attn_output, void* stream_v) {
+    int rc = validate_tree(p);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    if (!scale) {
+        return fail(PPLB200_UNSUPPORTED, "only a quantised cache is supported but scale is null");
+    }
+    // an empty batch is a no-op whatever the pointers are (empty tensors have none)
+    if (p->batch == 0 || p->total_tokens == 0) {
+        return PPLB200_SUCCESS;
+    }
+    if (!query || !seqstarts || !cachestarts || !start_pos || !cache || !attn_output) {
+        return fail(PPLB200_NOT_FOUND, "a required tensor pointer is null");
+    }
+    if (misaligned({query, cache, scale, attn_output}, {parents, seqstarts, cachestarts, start_pos}) ||
+        (reinterpret_cast<uintptr_t>(attn_output) & 31u) != 0) {
+        return fail(PPLB200_INVALID_VALUE, "tensor pointers must be 16-byte aligned (index tensors 8-byte, attn_output 32-byte)");
+    }
+    DeviceInfo di;
+    rc = require_device(&di);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    TreePlan plan;
+    rc = make_tree_plan(*p, di.sm_count, &plan);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    rc = check_workspace(workspace, workspace_bytes, plan.bytes, "workspace is smaller than pplb200_tree_attn_workspace_size()");
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+    rc = clear_status(workspace, stream);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    return launch_tree_attn(*p, make_geom(*p), plan, query, parents, seqstarts, cachestarts, start_pos, cache, scale,
+                            workspace, attn_output, stream);
+}
+
 int pplb200_attn_weight_workspace_size(const pplb200_attn_params* p, uint64_t* bytes) {
     int rc = validate_cache_op(p);
     if (rc != PPLB200_SUCCESS) {

@@ -20,6 +20,7 @@ constexpr uint32_t kDevRowOutOfRange = 8;   // an index tensor named a cache row
 
 constexpr uint32_t kDevMaskOutOfRange = 16;  // attn_mask is narrower than kvstarts needs: the missing entries read as 0
 constexpr uint32_t kDevKeptInvalid = 32;     // a kept list is not ascending or leaves its sequence: entry skipped
+constexpr uint32_t kDevParentInvalid = 64;   // a drafted token's parent does not come before it: taken as a root
 
 // Time budget of ONE bounded wait in every kernel of the library, in SM clock cycles: about 100 ms at
 // 2 GHz, four orders of magnitude beyond any legitimate copy or MMA latency.  A wait that exhausts it

@@ -119,6 +119,19 @@ int launch_mha(int num_heads, int num_kv_heads, int head_dim, int is_causal, int
                const void* value, const int64_t* seqstarts, const int64_t* kvstarts, const MaskDev& mask,
                uint32_t* status_word, void* attn_output, cudaStream_t stream);
 
+// ---- attention of drafted token trees -----------------------------------------------------------------
+constexpr int kTreeMaxTokens = 1024;  // drafted tokens of one sequence
+struct TreePlan {
+    int64_t ranges;  // persistent CTAs, one range of blocks each
+    int64_t words;   // 64-bit words of a token's ancestor mask
+    uint64_t off_prefix, off_ancestor, off_part_ml, off_part_o, bytes;
+};
+int make_tree_plan(const pplb200_attn_params& p, int sm_count, TreePlan* plan);
+int launch_tree_attn(const pplb200_attn_params& p, const CacheGeom& geom, const TreePlan& plan, const void* query,
+                     const int64_t* parents, const int64_t* seqstarts, const int64_t* cachestarts,
+                     const int64_t* start_pos, const void* cache, const void* scale, void* workspace,
+                     void* attn_output, cudaStream_t stream);
+
 // ---- accumulated attention weight, eviction, compaction --------------------------------------------
 struct WeightPlan {
     int64_t chunks;  // chunks of positions per sequence

@@ -38,11 +38,8 @@
 #include "common.cuh"
 #include "launch.h"
 #include "ragged.cuh"
+#include "tcgen05.cuh"
 #include "tensor_map.h"
-
-#ifndef PPLB200_PREFILL_WAIT
-#define PPLB200_PREFILL_WAIT mbar_test_wait
-#endif
 
 namespace pplb200 {
 
@@ -134,203 +131,6 @@ struct Barriers {
     int abort_word;
 };
 static_assert(sizeof(Barriers) <= 512, "barrier block");
-
-// ---- tcgen05 wrappers ---------------------------------------------------------------------------
-__device__ __forceinline__ void tmem_alloc(uint32_t* smem_slot, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_slot)),
-                 "r"(cols)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish() {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() {
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-// D[tmem] (+)= A[smem] * B[smem], M = 128, K = 16, fp16 inputs, fp32 accumulate
-__device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                           uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
-        "}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// D[tmem] (+)= A[tmem] * B[smem]: the A operand (128 rows x 16 halves, two per column) read from TMEM
-__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                              uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
-        "}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-// l += lo(ph) + hi(ph), the two fp16 values widened exactly
-__device__ __forceinline__ void add_half2_to_float(float& l, uint32_t ph) {
-    asm("{\n"
-        ".reg .b16 h0, h1;\n"
-        "mov.b32 {h0, h1}, %1;\n"
-        "add.rn.f32.f16 %0, h0, %0;\n"
-        "add.rn.f32.f16 %0, h1, %0;\n"
-        "}\n"
-        : "+f"(l)
-        : "r"(ph));
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-// 256-bit store (32-byte aligned address)
-__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&r)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
-}
-
-__device__ __forceinline__ void tmem_wait_ld() {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() {
-    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
-// Shared-memory matrix descriptors (descriptor version 1, sm_100).
-//   K-major operand, 128-byte swizzle ([rows][64 halves] blocks): lbo is unused (16), sbo = 1024 (8 rows
-//   of 128 bytes).
-//   MN-major operand, 128-byte swizzle (V as [kv rows][64 channels]): lbo = bytes between 64-channel
-//   blocks, sbo = 1024 (8 kv rows of 128 bytes).
-//   No swizzle: 8 x 8-half core matrices of 128 contiguous bytes, lbo / sbo apart along K / along N.
-// Descriptors are built once as (low word, high word); stepping through a tile only adds to the low word
-// (the start address in 16-byte units), which stays in uniform registers in warp-uniform code.
-__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo_bytes) {
-    return ((saddr & 0x3ffffu) >> 4) | (((lbo_bytes >> 4) & 0x3fffu) << 16);
-}
-__device__ __forceinline__ constexpr uint32_t desc_hi(uint32_t sbo_bytes, uint32_t layout) {
-    return ((sbo_bytes >> 4) & 0x3fffu) | (1u << 14) | (layout << 29);
-}
-__device__ __forceinline__ uint64_t desc_join(uint32_t lo, uint32_t hi) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
-    return d;
-}
-// One lane of a converged warp; the code around it stays warp-uniform.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t pred;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "elect.sync _|p, 0xffffffff;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(pred));
-    return pred != 0;
-}
-
-// Instruction descriptor for kind::f16: fp16 A and B, fp32 D, M = 128.
-__host__ __device__ constexpr uint32_t instr_desc_f16(int n, bool b_mn_major) {
-    return (1u << 4) |                                 // D format: F32
-           (0u << 7) | (0u << 10) |                    // A, B format: F16
-           (0u << 15) | ((b_mn_major ? 1u : 0u) << 16) |  // A K-major; B K- or MN-major
-           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kBlockM >> 4) << 24);
-}
-
-// Non-blocking test of an mbarrier phase.  The waits below poll with it: the blocking form
-// (mbarrier.try_wait) parks the thread, and a parked thread was measured to resume a few hundred cycles
-// after the phase had completed, which is as long as some of the pipeline stages here.
-__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-
-// Bounded wait that also gives up as soon as another thread of the CTA has given up.  The common case,
-// a phase that has completed already, costs one test; the polling loop is kept out of line.
-__device__ __noinline__ bool wait_or_abort_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                                uint32_t* status, uint32_t code) {
-    const long long t0 = clock64();
-    for (uint32_t i = 0;; i += 4) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (PPLB200_PREFILL_WAIT(bar, parity)) {
-                return true;
-            }
-        }
-        if ((i & 255u) == 252u) {
-            if (*abort_flag) {
-                return false;
-            }
-            if (clock64() - t0 > kWaitBudgetCycles) {
-                break;
-            }
-        }
-    }
-    *abort_flag = 1;
-    atomicOr(status, code);
-    return false;
-}
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                              uint32_t* status, uint32_t code) {
-    if (PPLB200_PREFILL_WAIT(bar, parity)) {
-        return true;
-    }
-    return wait_or_abort_slow(bar, parity, abort_flag, status, code);
-}
 
 template <int DH, bool MASK>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)

@@ -1,0 +1,835 @@
+// Attention of a tree of drafted tokens over the INT8 KV cache (speculative decoding's verification step).
+//
+// Sequence b has start_pos[b] tokens of history and n_b drafted tokens behind them, all in the cache.  Drafted token i
+// sees the history, itself and its ancestors.  The query rows that share a kv head -- n_b tokens x the heads of the
+// group -- are the M dimension of tcgen05.mma, so that each cached byte is read once per 128 rows:
+//   bytes per (position, kv head)  2 (Dh + Dh/4) = 320 at Dh 128; flops 4 Dh per query row, so with the measured
+//   rates 160 rows per kv head balance HBM and the tensor cores; below that the cache's bytes are the bound.
+//
+// Shape of the computation
+//   * The unit of work is a BLOCK of 64 positions of one segment = (sequence, kv head, tile of 128 query rows).  All
+//     blocks of the batch form one sequence, cut into equal ranges, one per resident CTA (two per SM).  A range that
+//     holds part of a segment leaves an fp32 partial (at most two per range), which tree_merge_kernel joins.
+//   * tree_plan_kernel turns the device-side lengths into the prefix sum of blocks, and the parents into one bit mask
+//     of ancestors per token.  Only blocks that reach behind the history look at the masks, 64 bits a row and block.
+//   * Roles of a CTA: warps 0..3 are 128 softmax threads, one query row each; warps 4..7 load codes and scales from
+//     global memory (the next block's while this one is worked on), dequantise them to fp16 and write the swizzled
+//     K and V tiles; warp 8 issues the MMAs.  S = Q K^T goes to a 64-column TMEM buffer, P returns to TMEM as the A
+//     operand of O += P V (two buffers), as in the prefill kernel.
+//
+// Waits on mbarriers are bounded and give up together (see tcgen05.cuh).
+#include <cub/block/block_scan.cuh>
+
+#include "common.cuh"
+#include "launch.h"
+#include "ragged.cuh"
+#include "tcgen05.cuh"
+
+namespace pplb200 {
+
+namespace {
+
+constexpr int kBlockM = 128;
+constexpr int kBlockN = 64;
+constexpr int kThreads = 288;
+constexpr int kStages = 2;
+constexpr int kCtasPerSm = 2;
+constexpr int kMinRange = 4;  // blocks: no range is cut finer
+constexpr float kNegBig = -1.0e30f;
+constexpr float kRescaleSlack = 8.0f;
+
+template <int DH>
+struct TTraits {
+    static constexpr int kColBlocks = DH / 64;
+    static constexpr int kQBlockBytes = kBlockM * 128;
+    static constexpr int kKVBlockBytes = kBlockN * 128;
+    static constexpr int kQBytes = kColBlocks * kQBlockBytes;
+    static constexpr int kKVBytes = kColBlocks * kKVBlockBytes;
+    // the same for every head size, so that never more than two CTAs share an SM and both TMEM allocations fit
+    static constexpr int kSmemBytes = 32768 + 2 * kStages * (kBlockN * 256) + 512;
+    static constexpr uint32_t kPCols = kBlockN / 2;
+    static constexpr uint32_t kColS = 0, kColP = kBlockN, kColO = kColP + 2 * kPCols;
+    static constexpr uint32_t kTmemCols = 256;
+};
+
+struct TreeHeader {
+    uint32_t status;  // first word of the workspace
+    uint32_t reserved;
+    int64_t total;  // blocks
+    int64_t range;  // blocks per range
+};
+
+struct TreeArgs {
+    const __half* q;
+    const int64_t* parents;
+    const int64_t* seqstarts;
+    const int64_t* cachestarts;
+    const int64_t* start_pos;
+    const int8_t* cache;
+    const __half* scale;
+    __half* out;
+    TreeHeader* hdr;
+    int64_t* prefix;     // [batch + 1] blocks before each sequence
+    uint64_t* ancestor;  // [total_tokens][words]
+    float* part_o;       // [slots][128][Dh]
+    float2* part_ml;     // [slots][128]
+    CacheGeom geom;
+    int64_t max_kvlen, max_tokens, total_tokens;
+    int32_t max_seqlen;
+    int32_t words;
+    int32_t batch;
+    int32_t num_heads, num_kv_heads, group;
+    int32_t ranges;
+    float scale_log2;
+};
+
+// What a sequence is made of; every kernel goes by this
+struct Seq {
+    int64_t tok0;
+    int32_t n, len, start, blocks, row_tiles;
+};
+
+__device__ __forceinline__ Seq seq_of(const TreeArgs& a, int64_t b) {
+    Seq s;
+    s.tok0 = a.seqstarts[b];
+    int64_t n = a.seqstarts[b + 1] - s.tok0;
+    if (s.tok0 < 0 || s.tok0 + n > a.total_tokens || n < 0) {
+        n = 0;
+    }
+    n = n > a.max_seqlen ? a.max_seqlen : n;
+    int64_t start = a.start_pos[b];
+    start = start < 0 ? 0 : start;
+    start = start > a.max_kvlen ? a.max_kvlen : start;
+    const int64_t len = start + n > a.max_kvlen ? a.max_kvlen : start + n;
+    s.n = static_cast<int32_t>(n);
+    s.start = static_cast<int32_t>(start);
+    s.len = static_cast<int32_t>(len);
+    s.blocks = n > 0 ? (s.len + kBlockN - 1) / kBlockN : 0;
+    s.row_tiles = (s.n * a.group + kBlockM - 1) / kBlockM;
+    return s;
+}
+
+// ---- planning: prefix sum of blocks (CTA 0), ancestor masks (a CTA per sequence) --------------------
+constexpr int kPlanThreads = 256;
+
+__global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(const TreeArgs a) {
+    using Scan = cub::BlockScan<int64_t, kPlanThreads>;
+    __shared__ typename Scan::TempStorage tmp;
+    __shared__ int64_t carry;
+    __shared__ int32_t up[kTreeMaxTokens];
+    const int tid = threadIdx.x;
+    if (blockIdx.x == 0) {
+        if (tid == 0) {
+            carry = 0;
+        }
+        __syncthreads();
+        for (int32_t base = 0; base < a.batch; base += kPlanThreads) {
+            const int32_t b = base + tid;
+            int64_t units = 0;
+            if (b < a.batch) {
+                const Seq s = seq_of(a, b);
+                units = static_cast<int64_t>(s.blocks) * s.row_tiles * a.num_kv_heads;
+            }
+            int64_t excl, total;
+            Scan(tmp).ExclusiveSum(units, excl, total);
+            const int64_t c = carry;
+            if (b < a.batch) {
+                a.prefix[b] = c + excl;
+            }
+            __syncthreads();
+            if (tid == 0) {
+                carry = c + total;
+            }
+            __syncthreads();
+        }
+        if (tid == 0) {
+            a.prefix[a.batch] = carry;
+            int64_t r = (carry + a.ranges - 1) / a.ranges;
+            a.hdr->total = carry;
+            a.hdr->range = r < kMinRange ? kMinRange : r;
+        }
+        return;
+    }
+    const int32_t b = blockIdx.x - 1;
+    const Seq s = seq_of(a, b);
+    if (tid == 0) {
+        const int64_t n = a.seqstarts[b + 1] - s.tok0;
+        if (n != s.n || a.start_pos[b] != s.start || s.start + n > a.max_kvlen) {
+            atomicOr(&a.hdr->status, kDevLengthClamped);
+        }
+    }
+    for (int32_t i = tid; i < s.n; i += kPlanThreads) {
+        int64_t p = a.parents != nullptr ? a.parents[s.tok0 + i] : i - 1;
+        if (p < -1 || p >= i) {
+            atomicOr(&a.hdr->status, kDevParentInvalid);
+            p = -1;
+        }
+        up[i] = static_cast<int32_t>(p);
+    }
+    __syncthreads();
+    for (int32_t i = tid; i < s.n; i += kPlanThreads) {
+        uint64_t* row = a.ancestor + (s.tok0 + i) * a.words;
+        int32_t at = i;  // ancestors have strictly smaller indices: the words fill from the highest down
+        for (int32_t w = a.words - 1; w >= 0; --w) {
+            uint64_t bits = 0;
+            while (at >= w * 64) {
+                bits |= 1ull << (at & 63);
+                at = up[at];
+            }
+            row[w] = bits;
+        }
+    }
+}
+
+// ---- main kernel -----------------------------------------------------------------------------------
+
+// Part of a segment that lies in the CTA's range
+struct Piece {
+    Seq seq;
+    int32_t b, kvh, rows_valid, row0;  // row0: first query row (token x head of the group) of the tile
+    int32_t blk0, blk1;                // blocks [blk0, blk1) of the segment's seq.blocks
+};
+
+// The piece that starts at unit u of [.., end); all lanes of a warp call it together.
+__device__ __forceinline__ void piece_at(const TreeArgs& a, int64_t u, int64_t end, int lane, Piece& p) {
+    p.b = warp_find_segment(a.prefix, a.batch, u, lane);
+    p.seq = seq_of(a, p.b);
+    const int32_t per_head = p.seq.blocks * p.seq.row_tiles;
+    const int64_t q = u - a.prefix[p.b];
+    p.kvh = static_cast<int32_t>(q / per_head);
+    const int32_t rem = static_cast<int32_t>(q - static_cast<int64_t>(p.kvh) * per_head);
+    const int32_t rt = rem / p.seq.blocks;
+    p.blk0 = rem - rt * p.seq.blocks;
+    const int64_t stop = p.blk0 + (end - u);
+    p.blk1 = stop < p.seq.blocks ? static_cast<int32_t>(stop) : p.seq.blocks;
+    p.row0 = rt * kBlockM;
+    const int32_t rows = p.seq.n * a.group - p.row0;
+    p.rows_valid = rows < kBlockM ? rows : kBlockM;
+}
+
+struct Barriers {
+    uint64_t q_full, q_empty, o_free;
+    uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+    uint64_t s_full, s_free;
+    uint64_t p_full[2], pv_done[2];
+    uint32_t tmem_slot;
+    int abort_word;
+};
+static_assert(sizeof(Barriers) <= 512, "barrier block");
+
+// 16 codes -> 16 halves of value, scaled by two groups' scales (s = scale of channels 0..7 | 8..15 << 16)
+__device__ __forceinline__ void dequant16(const uint4& c, uint32_t s, uint4& lo, uint4& hi) {
+    const __half2 s0 = u32_as_h2(prmt(s, 0u, 0x1010u)), s1 = u32_as_h2(prmt(s, 0u, 0x3232u));
+    const uint32_t x0 = c.x ^ 0x80808080u, x1 = c.y ^ 0x80808080u, x2 = c.z ^ 0x80808080u, x3 = c.w ^ 0x80808080u;
+    lo.x = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5140u>(x0), s0));
+    lo.y = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5342u>(x0), s0));
+    lo.z = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5140u>(x1), s0));
+    lo.w = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5342u>(x1), s0));
+    hi.x = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5140u>(x2), s1));
+    hi.y = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5342u>(x2), s1));
+    hi.z = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5140u>(x3), s1));
+    hi.w = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5342u>(x3), s1));
+}
+
+__device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// One thread's share of a K or V block: 16-byte piece `piece` of kRows rows
+template <int DH>
+struct Raw {
+    static constexpr int kPieces = DH / 16;             // 16-byte pieces of a row
+    static constexpr int kRowsPerStep = 32 / kPieces;   // rows a warp loads at once
+    static constexpr int kRows = 16 / kRowsPerStep;     // steps over the warp's 16 rows
+    uint4 code[kRows];
+    uint32_t sc[kRows];
+
+    // `off`: element offset of the thread's piece in the first of its rows; `rows`: how many of the warp's 16 rows exist
+    __device__ __forceinline__ void load(const TreeArgs& a, int64_t off, int32_t r, int32_t rows) {
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            code[k] = make_uint4(0u, 0u, 0u, 0u);
+            sc[k] = 0u;
+            if (r + k * kRowsPerStep < rows) {
+                code[k] = *reinterpret_cast<const uint4*>(a.cache + off);
+                sc[k] = *reinterpret_cast<const uint32_t*>(a.scale + (off >> 3));
+            }
+            off += a.geom.stride_s * kRowsPerStep;
+        }
+    }
+
+    // -> the swizzled fp16 tile at `tile`: [64 rows][64 halves] blocks, 16-byte chunk c of row r at chunk c ^ (r & 7)
+    __device__ __forceinline__ void store(uint32_t tile, int32_t row, int32_t piece) const {
+        const int32_t cb = piece >> 2, c = (piece & 3) * 2;
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            const int32_t r = row + k * kRowsPerStep;
+            const uint32_t at = tile + cb * (kBlockN * 128) + r * 128;
+            uint4 lo, hi;
+            dequant16(code[k], sc[k], lo, hi);
+            const uint32_t c0 = at + ((c ^ (r & 7)) << 4), c1 = at + (((c + 1) ^ (r & 7)) << 4);
+            // the two column blocks start with different chunks: eight lanes then fill all banks once
+            const bool odd = cb != 0;
+            sts128(odd ? c1 : c0, odd ? hi : lo);
+            sts128(odd ? c0 : c1, odd ? lo : hi);
+        }
+    }
+};
+
+template <int DH>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attn_kernel(const TreeArgs a) {
+    using T = TTraits<DH>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* sQ = smem;
+    uint8_t* sK = sQ + T::kQBytes;
+    uint8_t* sV = sK + kStages * T::kKVBytes;
+    Barriers& bars = *reinterpret_cast<Barriers*>(sV + kStages * T::kKVBytes);
+    volatile int* abort_flag = &bars.abort_word;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t* status = &a.hdr->status;
+
+    if ((smem_u32(smem) & 1023u) != 0u) {  // no static shared memory: the window starts on a 1 KB boundary
+        if (threadIdx.x == 0) {
+            atomicOr(status, kDevMmaTimeout);
+        }
+        return;
+    }
+    const int64_t begin = blockIdx.x * a.hdr->range;
+    const int64_t total = a.hdr->total;
+    const int64_t end = begin + a.hdr->range < total ? begin + a.hdr->range : total;
+    if (begin >= end) {
+        return;  // uniform for the CTA, before any barrier or TMEM allocation
+    }
+    if (threadIdx.x == 0) {
+        bars.abort_word = 0;
+        mbar_init(&bars.q_full, 128);
+        mbar_init(&bars.q_empty, 1);
+        mbar_init(&bars.o_free, 128);
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&bars.k_full[s], 128);
+            mbar_init(&bars.v_full[s], 128);
+            mbar_init(&bars.k_empty[s], 1);
+            mbar_init(&bars.v_empty[s], 1);
+        }
+        mbar_init(&bars.s_full, 1);
+        mbar_init(&bars.s_free, 128);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.p_full[i], 128);
+            mbar_init(&bars.pv_done[i], 1);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 8) {
+        tmem_alloc(&bars.tmem_slot, T::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = bars.tmem_slot;
+
+    if (warp >= 4 && warp < 8) {
+        // =========================== converters ===========================
+        const int ct = threadIdx.x - 128;
+        const int cw = warp - 4;  // this warp's 16 rows of a block
+        constexpr int kPieces = Raw<DH>::kPieces;
+        const int piece = lane % kPieces, rr = lane / kPieces;
+        const uint32_t k_tile = smem_u32(sK), v_tile = smem_u32(sV);
+        bool ok = true;
+        int pieces = 0, n = 0;  // pieces and blocks converted so far
+        for (int64_t u = begin; ok && u < end;) {
+            Piece p;
+            piece_at(a, u, end, lane, p);
+            const int64_t head_off = a.geom.layer_idx * a.geom.stride_l + p.kvh * a.geom.stride_h + piece * 16;
+            Raw<DH> kr, vr;
+            // position of a block's rows of this warp: element offset of the thread's piece, rows that exist
+            auto locate = [&](int32_t blk, int64_t& off) -> int32_t {
+                const int32_t pos = blk * kBlockN + cw * 16;
+                int32_t rows = p.seq.len - pos;
+                rows = rows > 16 ? 16 : rows;
+                off = 0;
+                if (rows > 0) {
+                    const int64_t row = cache_row(a.geom, a.cachestarts, p.b, pos);
+                    if (row < 0 || row + rows > a.max_tokens) {  // a wrong index tensor: flagged, those rows read as zeros
+                        if (lane == 0) {
+                            atomicOr(status, kDevRowOutOfRange);
+                        }
+                        rows = row < 0 || row >= a.max_tokens ? 0 : static_cast<int32_t>(a.max_tokens - row);
+                    }
+                    off = (row + rr) * a.geom.stride_s + head_off;
+                }
+                return rows;
+            };
+            int64_t off, next_off = 0;
+            int32_t rows = locate(p.blk0, off);
+            kr.load(a, off, rr, rows);
+            vr.load(a, off + a.geom.stride_kv, rr, rows);
+            // Q: row r of the tile is query row row0 + r = token x head of the group
+            if (pieces > 0) {
+                ok = wait_or_abort(&bars.q_empty, (pieces - 1) & 1, abort_flag, status, kDevMmaTimeout);
+                if (!ok) {
+                    break;
+                }
+            }
+            constexpr int kQPieces = DH / 8;  // 16-byte pieces of a query row
+            for (int i = ct; i < p.rows_valid * kQPieces; i += 128) {
+                const int r = i / kQPieces, c = i - r * kQPieces;
+                const int32_t row = p.row0 + r;
+                const int32_t tok = row / a.group;
+                const uint4 v = *reinterpret_cast<const uint4*>(
+                    a.q + ((p.seq.tok0 + tok) * a.num_heads + p.kvh * a.group + (row - tok * a.group)) * DH + c * 8);
+                sts128(smem_u32(sQ) + (c >> 3) * T::kQBlockBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4), v);
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&bars.q_full);
+            ++pieces;
+            for (int32_t blk = p.blk0; blk < p.blk1; ++blk, ++n) {
+                const int s = n % kStages;
+                const bool more = blk + 1 < p.blk1;
+                int32_t next_rows = 0;
+                if (more) {
+                    next_rows = locate(blk + 1, next_off);
+                }
+                if (n >= kStages) {
+                    ok = wait_or_abort(&bars.k_empty[s], ((n / kStages) - 1) & 1, abort_flag, status, kDevMmaTimeout);
+                    if (!ok) {
+                        break;
+                    }
+                }
+                kr.store(k_tile + s * T::kKVBytes, cw * 16 + rr, piece);
+                fence_proxy_async_smem();
+                mbar_arrive(&bars.k_full[s]);
+                if (more) {
+                    kr.load(a, next_off, rr, next_rows);
+                }
+                if (n >= kStages) {
+                    ok = wait_or_abort(&bars.v_empty[s], ((n / kStages) - 1) & 1, abort_flag, status, kDevMmaTimeout);
+                    if (!ok) {
+                        break;
+                    }
+                }
+                vr.store(v_tile + s * T::kKVBytes, cw * 16 + rr, piece);
+                fence_proxy_async_smem();
+                mbar_arrive(&bars.v_full[s]);
+                if (more) {
+                    vr.load(a, next_off + a.geom.stride_kv, rr, next_rows);
+                }
+            }
+            u += p.blk1 - p.blk0;
+        }
+    } else if (warp == 8) {
+        // =========================== MMA issuer ===========================
+        constexpr uint32_t idesc_qk = instr_desc_f16(kBlockN, false);
+        constexpr uint32_t idesc_pv = instr_desc_f16(DH, true);
+        constexpr uint32_t hi_sw128 = desc_hi(1024, 2);
+        const uint32_t q_lo = desc_lo(smem_u32(sQ), 16);
+        const uint32_t k_lo = desc_lo(smem_u32(sK), 16);
+        const uint32_t v_lo = desc_lo(smem_u32(sV), T::kKVBlockBytes);
+        const uint32_t d_s = tmem_base + T::kColS, d_o = tmem_base + T::kColO, a_p = tmem_base + T::kColP;
+        bool ok = true;
+        int pieces = 0, kc = 0, vc = 0;
+        for (int64_t u = begin; ok && u < end;) {
+            Piece p;
+            piece_at(a, u, end, lane, p);
+            const int32_t blocks = p.blk1 - p.blk0;
+            ok = wait_or_abort(&bars.q_full, pieces & 1, abort_flag, status, kDevMmaTimeout);
+            for (int32_t j = 0; ok && j <= blocks; ++j) {
+                if (j < blocks) {
+                    const int s = kc % kStages;
+                    ok = wait_or_abort(&bars.k_full[s], (kc / kStages) & 1, abort_flag, status, kDevMmaTimeout) &&
+                         (kc == 0 || wait_or_abort(&bars.s_free, (kc - 1) & 1, abort_flag, status, kDevMmaTimeout));
+                    if (!ok) {
+                        break;
+                    }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t ks_lo = k_lo + s * (T::kKVBytes >> 4);
+#pragma unroll
+                        for (int cb = 0; cb < T::kColBlocks; ++cb) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                tc_mma_f16(d_s, desc_join(q_lo + cb * (T::kQBlockBytes >> 4) + 2 * k, hi_sw128),
+                                           desc_join(ks_lo + cb * (T::kKVBlockBytes >> 4) + 2 * k, hi_sw128), idesc_qk,
+                                           (cb | k) ? 1u : 0u);
+                            }
+                        }
+                        tc_commit(&bars.s_full);
+                        tc_commit(&bars.k_empty[s]);
+                        if (j == blocks - 1) {
+                            tc_commit(&bars.q_empty);
+                        }
+                    }
+                    __syncwarp();
+                    ++kc;
+                }
+                if (j > 0) {
+                    const int s = vc % kStages;
+                    ok = wait_or_abort(&bars.v_full[s], (vc / kStages) & 1, abort_flag, status, kDevMmaTimeout) &&
+                         wait_or_abort(&bars.p_full[vc & 1], (vc >> 1) & 1, abort_flag, status, kDevMmaTimeout);
+                    if (ok && j == 1 && pieces > 0) {
+                        ok = wait_or_abort(&bars.o_free, (pieces - 1) & 1, abort_flag, status, kDevMmaTimeout);
+                    }
+                    if (!ok) {
+                        break;
+                    }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t vs_lo = v_lo + s * (T::kKVBytes >> 4);
+                        const uint32_t pa = a_p + (vc & 1) * T::kPCols;
+#pragma unroll
+                        for (int ks = 0; ks < kBlockN / 16; ++ks) {
+                            tc_mma_f16_ts(d_o, pa + 8 * ks, desc_join(vs_lo + ks * (2048 >> 4), hi_sw128), idesc_pv,
+                                          ((j - 1) | ks) ? 1u : 0u);
+                        }
+                        tc_commit(&bars.v_empty[s]);
+                        tc_commit(&bars.pv_done[vc & 1]);
+                    }
+                    __syncwarp();
+                    ++vc;
+                }
+            }
+            ++pieces;
+            u += blocks;
+        }
+    } else if (warp < 4) {
+        // =========================== softmax / epilogue ===========================
+        const int r = warp * 32 + lane;  // row of the tile = TMEM lane
+        const uint32_t t_lane = static_cast<uint32_t>(warp * 32) << 16;
+        const uint32_t t_s = tmem_base + t_lane + T::kColS;
+        const uint32_t t_o = tmem_base + t_lane + T::kColO;
+        const uint32_t t_p = tmem_base + t_lane + T::kColP;
+        const float sc = a.scale_log2;
+        bool ok = true;
+        int pc = 0;
+        for (int64_t u = begin; ok && u < end;) {
+            Piece p;
+            piece_at(a, u, end, lane, p);
+            const bool warp_live = warp * 32 < p.rows_valid;  // rows behind the last are carried along unread
+            const bool live = r < p.rows_valid;
+            const int32_t row = p.row0 + r;
+            const int32_t tok = live ? row / a.group : 0;
+            const uint64_t* anc = a.ancestor + (p.seq.tok0 + tok) * a.words;
+            float m_ref = kNegBig, l_sum = 0.0f;
+            for (int32_t blk = p.blk0; ok && blk < p.blk1; ++blk, ++pc) {
+                if (pc >= 2) {
+                    ok = wait_or_abort(&bars.pv_done[pc & 1], ((pc - 2) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
+                    if (!ok) {
+                        break;
+                    }
+                }
+                // 64 positions of this row: bit e = position blk * 64 + e is visible
+                const int32_t a0 = blk * kBlockN - p.seq.start;  // index of the block's first position among the drafts
+                const bool masked = a0 + kBlockN > 0;
+                uint64_t seen = ~0ull;
+                if (masked && live) {
+                    if (a0 <= 0) {
+                        seen = (a0 == 0 ? 0ull : ~0ull >> (64 + a0)) | (anc[0] << -a0);
+                    } else {
+                        const int32_t w = a0 >> 6, sh = a0 & 63;
+                        seen = w < a.words ? anc[w] >> sh : 0ull;
+                        if (sh > 0 && w + 1 < a.words) {
+                            seen |= anc[w + 1] << (64 - sh);
+                        }
+                    }
+                    const int32_t room = p.seq.len - blk * kBlockN;  // positions that exist
+                    if (room < kBlockN) {
+                        seen &= ~0ull >> (64 - room);
+                    }
+                }
+                ok = wait_or_abort(&bars.s_full, pc & 1, abort_flag, status, kDevMmaTimeout);
+                if (!ok) {
+                    break;
+                }
+                tc_fence_after();
+                if (!warp_live) {
+                    tc_fence_before();
+                    mbar_arrive(&bars.s_free);
+                    mbar_arrive(&bars.p_full[pc & 1]);
+                    continue;
+                }
+                float sv[kBlockN];
+                {
+                    uint32_t v[kBlockN / 32][32];
+#pragma unroll
+                    for (int c = 0; c < kBlockN / 32; ++c) {
+                        tmem_ld32(t_s + 32 * c, v[c]);
+                    }
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < kBlockN / 32; ++c) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            sv[32 * c + e] = __uint_as_float(v[c][e]);
+                        }
+                    }
+                }
+                tc_fence_before();
+                mbar_arrive(&bars.s_free);
+                if (masked) {
+                    const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
+#pragma unroll
+                    for (int e = 0; e < kBlockN; ++e) {
+                        sv[e] = ((e < 32 ? lo : hi) >> (e & 31)) & 1u ? sv[e] : -INFINITY;
+                    }
+                }
+                float mx0 = fmax3(sv[0], sv[1], sv[2]), mx1 = fmax3(sv[3], sv[4], sv[5]);
+#pragma unroll
+                for (int e = 6; e + 3 < kBlockN; e += 4) {
+                    mx0 = fmax3(mx0, sv[e], sv[e + 1]);
+                    mx1 = fmax3(mx1, sv[e + 2], sv[e + 3]);
+                }
+                float mx = fmax3(mx0, mx1, fmaxf(sv[kBlockN - 2], sv[kBlockN - 1]));
+                mx *= sc;
+                const bool grow = mx > m_ref + kRescaleSlack;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float m_new = grow ? mx : m_ref;
+                    const float f = ex2_approx(m_ref - m_new);
+                    m_ref = m_new;
+                    l_sum *= f;
+                    if (blk > p.blk0) {
+                        ok = wait_or_abort(&bars.pv_done[(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
+                        if (!ok) {
+                            break;
+                        }
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < DH / 8; ++c) {  // eight columns at a time: the scores stay in registers
+                            uint32_t v[8];
+                            tmem_ld8(t_o + c * 8, v);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                            }
+                            tmem_st8(t_o + c * 8, v);
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                // P = exp2(s * scale - m_ref) as packed fp16; the row sum adds the rounded values that P V uses
+                const uint32_t t_pb = t_p + (pc & 1) * T::kPCols;
+#pragma unroll
+                for (int q = 0; q < kBlockN / 32; ++q) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float2 x = __ffma2_rn(make_float2(sv[32 * q + 2 * e], sv[32 * q + 2 * e + 1]),
+                                                    make_float2(sc, sc), make_float2(-m_ref, -m_ref));
+                        pk[e] = h2_as_u32(__floats2half2_rn(ex2_approx(x.x), ex2_approx(x.y)));
+                        add_half2_to_float(l_sum, pk[e]);
+                    }
+                    tmem_st16(t_pb + 16 * q, pk);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&bars.p_full[pc & 1]);
+            }
+            // ---- epilogue: the whole segment -> fp16 rows; a part of one -> fp32 partial ----
+            if (ok) {
+                ok = wait_or_abort(&bars.pv_done[(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
+            }
+            if (ok) {
+                tc_fence_after();
+                const bool whole = p.blk0 == 0 && p.blk1 == p.seq.blocks;
+                const float inv = l_sum > 0.0f ? 1.0f / l_sum : 0.0f;
+                __half* dst = a.out + ((p.seq.tok0 + tok) * a.num_heads + p.kvh * a.group + (row - tok * a.group)) * DH;
+                const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (p.blk0 == 0 ? 1 : 0);
+                float* part = a.part_o + (slot * kBlockM + r) * DH;
+                if (!whole && live) {
+                    a.part_ml[slot * kBlockM + r] = make_float2(m_ref, l_sum);
+                }
+#pragma unroll
+                for (int c = 0; c < DH / 32; ++c) {
+                    uint32_t v[32];
+                    tmem_ld32(t_o + c * 32, v);
+                    tmem_wait_ld();
+                    if (c == DH / 32 - 1) {
+                        tc_fence_before();
+                        mbar_arrive(&bars.o_free);
+                    }
+                    if (live && whole) {
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            uint32_t o[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                o[e] = h2_as_u32(__floats2half2_rn(__uint_as_float(v[16 * q + 2 * e]) * inv,
+                                                                   __uint_as_float(v[16 * q + 2 * e + 1]) * inv));
+                            }
+                            st_global_v8(dst + c * 32 + q * 16, o);
+                        }
+                    } else if (live) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            uint32_t o[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                o[e] = v[8 * q + e];
+                            }
+                            st_global_v8(part + c * 32 + q * 8, o);
+                        }
+                    }
+                }
+            }
+            u += p.blk1 - p.blk0;
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, T::kTmemCols);
+    }
+}
+
+// ---- joining the parts of a segment that several ranges hold -----------------------------------------
+
+// One warp per (query token, head).
+template <int DH>
+__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a) {
+    constexpr int kPer = DH / 32;  // channels of a lane
+    const int lane = threadIdx.x & 31;
+    const int64_t id = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
+    const int64_t tok = id / a.num_heads;
+    if (tok >= a.total_tokens) {
+        return;
+    }
+    const int32_t head = static_cast<int32_t>(id - tok * a.num_heads);
+    const int32_t b = warp_find_segment(a.seqstarts, a.batch, tok, lane);
+    const Seq s = seq_of(a, b);
+    const int64_t i = tok - s.tok0;
+    if (i < 0 || i >= s.n) {
+        return;
+    }
+    const int32_t kvh = head / a.group;
+    const int32_t row = static_cast<int32_t>(i) * a.group + (head - kvh * a.group);
+    const int32_t rt = row / kBlockM, r = row - rt * kBlockM;
+    const int64_t u0 = a.prefix[b] + (static_cast<int64_t>(kvh) * s.row_tiles + rt) * s.blocks;
+    const int64_t range = a.hdr->range;
+    const int64_t first = u0 / range, last = (u0 + s.blocks - 1) / range;
+    if (first == last) {
+        return;  // one range held all of it and wrote the output
+    }
+    float m = kNegBig;
+    for (int64_t w = first; w <= last; ++w) {
+        const int64_t slot = 2 * w + (u0 >= w * range ? 1 : 0);
+        m = fmaxf(m, a.part_ml[slot * kBlockM + r].x);
+    }
+    float l = 0.0f, o[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        o[e] = 0.0f;
+    }
+    for (int64_t w = first; w <= last; ++w) {
+        const int64_t slot = 2 * w + (u0 >= w * range ? 1 : 0);
+        const float2 ml = a.part_ml[slot * kBlockM + r];
+        const float f = ex2_approx(ml.x - m);
+        const float* part = a.part_o + (slot * kBlockM + r) * DH + lane * kPer;
+        l += ml.y * f;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            o[e] += part[e] * f;
+        }
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    __half2* dst = reinterpret_cast<__half2*>(a.out + (tok * a.num_heads + head) * DH + lane * kPer);
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) {
+        dst[e / 2] = __floats2half2_rn(o[e] * inv, o[e + 1] * inv);
+    }
+}
+
+uint64_t align256(uint64_t x) {
+    return (x + 255) / 256 * 256;
+}
+
+template <int DH>
+int launch_dh(const TreeArgs& a, const TreePlan& plan, cudaStream_t stream) {
+    using T = TTraits<DH>;
+    // the attribute belongs to the (kernel, device) pair
+    static bool attr_set[kMaxDevices] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
+        (void)cudaGetLastError();
+        return PPLB200_DEVICE_RUNTIME_ERROR;
+    }
+    if (!attr_set[dev]) {
+        if (cudaFuncSetAttribute(tree_attn_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmemBytes) !=
+            cudaSuccess) {
+            (void)cudaGetLastError();
+            return PPLB200_DEVICE_RUNTIME_ERROR;
+        }
+        attr_set[dev] = true;
+    }
+    tree_plan_kernel<<<static_cast<unsigned>(a.batch + 1), kPlanThreads, 0, stream>>>(a);
+    int rc = check_launch("tree_plan_kernel");
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    tree_attn_kernel<DH><<<static_cast<unsigned>(plan.ranges), kThreads, T::kSmemBytes, stream>>>(a);
+    rc = check_launch("tree_attn_kernel");
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    const int64_t warps = a.total_tokens * a.num_heads;
+    tree_merge_kernel<DH><<<static_cast<unsigned>((warps * 32 + 255) / 256), 256, 0, stream>>>(a);
+    return check_launch("tree_merge_kernel");
+}
+
+}  // namespace
+
+int make_tree_plan(const pplb200_attn_params& p, int sm_count, TreePlan* plan) {
+    // no more ranges than there can be work for
+    const int64_t row_tiles = (p.max_seqlen * (p.num_heads / p.num_kv_heads) + kBlockM - 1) / kBlockM;
+    const int64_t blocks = (p.max_kvlen + kBlockN - 1) / kBlockN;
+    int64_t ranges = (p.batch * p.num_kv_heads * row_tiles * blocks + kMinRange - 1) / kMinRange;
+    const int64_t resident = static_cast<int64_t>(sm_count) * kCtasPerSm;
+    plan->ranges = ranges > resident ? resident : ranges;
+    plan->words = (p.max_seqlen + 63) / 64;
+    plan->off_prefix = 256;
+    plan->off_ancestor = plan->off_prefix + align256(static_cast<uint64_t>(p.batch + 1) * 8);
+    plan->off_part_ml = plan->off_ancestor + align256(static_cast<uint64_t>(p.total_tokens) * plan->words * 8);
+    plan->off_part_o = plan->off_part_ml + static_cast<uint64_t>(plan->ranges) * 2 * kBlockM * 8;
+    plan->bytes = plan->off_part_o + static_cast<uint64_t>(plan->ranges) * 2 * kBlockM * p.head_dim * 4;
+    return PPLB200_SUCCESS;
+}
+
+int launch_tree_attn(const pplb200_attn_params& p, const CacheGeom& geom, const TreePlan& plan, const void* query,
+                     const int64_t* parents, const int64_t* seqstarts, const int64_t* cachestarts,
+                     const int64_t* start_pos, const void* cache, const void* scale, void* workspace,
+                     void* attn_output, cudaStream_t stream) {
+    if (plan.ranges <= 0) {
+        return PPLB200_SUCCESS;
+    }
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    TreeArgs a = {};
+    a.q = static_cast<const __half*>(query);
+    a.parents = parents;
+    a.seqstarts = seqstarts;
+    a.cachestarts = cachestarts;
+    a.start_pos = start_pos;
+    a.cache = static_cast<const int8_t*>(cache);
+    a.scale = static_cast<const __half*>(scale);
+    a.out = static_cast<__half*>(attn_output);
+    a.hdr = reinterpret_cast<TreeHeader*>(ws);
+    a.prefix = reinterpret_cast<int64_t*>(ws + plan.off_prefix);
+    a.ancestor = reinterpret_cast<uint64_t*>(ws + plan.off_ancestor);
+    a.part_ml = reinterpret_cast<float2*>(ws + plan.off_part_ml);
+    a.part_o = reinterpret_cast<float*>(ws + plan.off_part_o);
+    a.geom = geom;
+    a.max_kvlen = p.max_kvlen;
+    a.max_tokens = p.max_tokens;
+    a.total_tokens = p.total_tokens;
+    a.max_seqlen = static_cast<int32_t>(p.max_seqlen);
+    a.words = static_cast<int32_t>(plan.words);
+    a.batch = static_cast<int32_t>(p.batch);
+    a.num_heads = p.num_heads;
+    a.num_kv_heads = p.num_kv_heads;
+    a.group = p.num_heads / p.num_kv_heads;
+    a.ranges = static_cast<int32_t>(plan.ranges);
+    a.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(p.head_dim));
+    return p.head_dim == 128 ? launch_dh<128>(a, plan, stream) : launch_dh<64>(a, plan, stream);
+}
+
+}  // namespace pplb200

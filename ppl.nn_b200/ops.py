@@ -454,6 +454,26 @@ class _CacheOp(_Base):
         self._raise("pplb200_fill_cache_strides", self.lib.fill_cache_strides(p))
         return p
 
+    def _query_params(self, query, seqstarts, cachestarts, start_pos, max_seqlen, max_kvlen, cache, scale):
+        """Checks and parameters of the operators whose query tokens attend to the cache."""
+        a = self.param
+        layers, kv_heads, dim = _require_cache(cache, scale, a.cache_layout)
+        _require_cuda(query=query)
+        _require_device(cache.device, query=query)
+        _require_index(cache.device, seqstarts=seqstarts, cachestarts=cachestarts, start_pos=start_pos)
+        if a.is_alibi:
+            raise OpError("RC_UNSUPPORTED", "currently only support is_alibi == false")
+        if query.dtype != torch.float16:
+            raise OpError("RC_UNSUPPORTED", "currently only support fp16")
+        if query.shape[1:] != (a.num_heads, a.head_dim) or (layers, kv_heads, dim) != (a.num_layer, a.num_kv_heads,
+                                                                                      a.head_dim):
+            raise OpError("RC_INVALID_VALUE", "query or cache does not have the shape of the attributes")
+        if seqstarts.shape[0] != start_pos.shape[0] + 1:
+            raise OpError("RC_INVALID_VALUE", "seqstarts must have one entry more than start_pos")
+        return self._params(num_heads=a.num_heads, num_kv_heads=kv_heads, head_dim=dim, batch=start_pos.shape[0],
+                            max_kvlen=max_kvlen, max_tokens=_max_tokens(cache, a.cache_layout), cachestarts=cachestarts,
+                            max_seqlen=max_seqlen, total_tokens=query.shape[0], is_causal=a.is_causal)
+
     def _call(self, name, size_fn, fn, p, device, *args) -> None:
         """Runs fn(p, *args, workspace, bytes, stream) on the tensors' device and its current stream."""
         rc, nbytes = size_fn(p)
@@ -473,6 +493,34 @@ class _CacheOp(_Base):
         return s
 
 
+class TreeAttention(_CacheOp):
+    """Attention of a tree of drafted tokens over the cache, in which they already are (positions start_pos[b] + i):
+    drafted token i sees the history, itself and its ancestors.  ``parents`` [tokens] holds the index, among its
+    sequence's drafted tokens, of each one's parent (before it), -1 for a child of the history; None for a chain."""
+
+    def __init__(self, param: MultiHeadCacheAttentionParam):
+        super().__init__(param)
+
+    def forward(self, query, parents, seqstarts, cachestarts, start_pos, max_seqlen: int, max_kvlen: int, cache, scale,
+                attn_output: torch.Tensor | None = None) -> torch.Tensor:
+        a = self.param
+        p = self._query_params(query, seqstarts, cachestarts, start_pos, max_seqlen, max_kvlen, cache, scale)
+        if parents is not None:
+            _require_index(cache.device, parents=parents)
+            if parents.shape != query.shape[:1]:
+                raise OpError("RC_INVALID_VALUE", "parents must have an entry per query token")
+        if attn_output is None:
+            attn_output = torch.empty_like(query)
+        _require_cuda(attn_output=attn_output)
+        _require_device(cache.device, attn_output=attn_output)
+        if attn_output.shape != query.shape or attn_output.dtype != query.dtype:
+            raise OpError("RC_INVALID_VALUE", "attn_output must be like query")
+        self._call("pplb200_tree_attn_forward", self.lib.tree_attn_workspace_size, self.lib.tree_attn_forward, p,
+                   cache.device, _ptr(query), _ptr(parents), _ptr(seqstarts), _ptr(cachestarts), _ptr(start_pos),
+                   _ptr(cache), _ptr(scale), _ptr(attn_output))
+        return attn_output
+
+
 class AttentionWeight(_CacheOp):
     """Adds to ``weight`` [num_layer, num_kv_heads, max_tokens] (fp32, by cache row) the softmax weights that this
     call's query tokens give each cached position, summed over the tokens and the query heads of a kv group.  The
@@ -483,25 +531,11 @@ class AttentionWeight(_CacheOp):
 
     def forward(self, query, seqstarts, cachestarts, start_pos, max_seqlen: int, max_kvlen: int, cache, scale,
                 weight) -> torch.Tensor:
-        a = self.param
-        layers, kv_heads, dim = _require_cache(cache, scale, a.cache_layout)
-        _require_cuda(query=query)
-        _require_weight(weight, a.num_layer)
-        _require_device(cache.device, query=query, weight=weight)
-        _require_index(cache.device, seqstarts=seqstarts, cachestarts=cachestarts, start_pos=start_pos)
-        if a.is_alibi:
-            raise OpError("RC_UNSUPPORTED", "currently only support is_alibi == false")
-        if query.dtype != torch.float16:
-            raise OpError("RC_UNSUPPORTED", "currently only support fp16")
-        max_tokens = _max_tokens(cache, a.cache_layout)
-        if query.shape[1:] != (a.num_heads, a.head_dim) or (layers, kv_heads, dim) != (a.num_layer, a.num_kv_heads,
-                                                                                      a.head_dim):
-            raise OpError("RC_INVALID_VALUE", "query or cache does not have the shape of the attributes")
-        if weight.shape[1:] != (kv_heads, max_tokens) or seqstarts.shape[0] != start_pos.shape[0] + 1:
-            raise OpError("RC_INVALID_VALUE", "weight or seqstarts does not have the shape of the cache and batch")
-        p = self._params(num_heads=a.num_heads, num_kv_heads=kv_heads, head_dim=dim, batch=start_pos.shape[0],
-                         max_kvlen=max_kvlen, max_tokens=max_tokens, cachestarts=cachestarts, max_seqlen=max_seqlen,
-                         total_tokens=query.shape[0], is_causal=a.is_causal)
+        p = self._query_params(query, seqstarts, cachestarts, start_pos, max_seqlen, max_kvlen, cache, scale)
+        _require_weight(weight, self.param.num_layer)
+        _require_device(cache.device, weight=weight)
+        if weight.shape[1:] != (p.num_kv_heads, p.max_tokens):
+            raise OpError("RC_INVALID_VALUE", "weight does not have the shape of the cache")
         self._call("pplb200_attn_weight_accumulate", self.lib.attn_weight_workspace_size,
                    self.lib.attn_weight_accumulate, p, cache.device, _ptr(query), _ptr(seqstarts), _ptr(cachestarts),
                    _ptr(start_pos), _ptr(cache), _ptr(scale), _ptr(weight))
