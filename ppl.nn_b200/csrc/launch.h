@@ -122,7 +122,9 @@ int launch_mha(int num_heads, int num_kv_heads, int head_dim, int is_causal, int
 // ---- attention of drafted token trees -----------------------------------------------------------------
 constexpr int kTreeMaxTokens = 1024;  // drafted tokens of one sequence
 struct TreePlan {
-    int64_t ranges;  // persistent CTAs, one range of blocks each
+    int32_t tiles;   // 128-row MMA tiles of a CTA: 1 or 2
+    int32_t lanes;   // classes of kv heads
+    int64_t ranges;  // ranges of blocks per class, one for each of ranges * lanes persistent CTAs
     int64_t words;   // 64-bit words of a token's ancestor mask
     uint64_t off_prefix, off_ancestor, off_part_ml, off_part_o, bytes;
 };

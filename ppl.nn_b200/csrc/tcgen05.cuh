@@ -218,4 +218,26 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, vo
     return wait_or_abort_slow(bar, parity, abort_flag, status, code);
 }
 
+// The same for a thread that is in no hurry: parked by the hardware instead of polling, so that it leaves the issue
+// slots to the others.
+__device__ __forceinline__ bool wait_or_abort_parked(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                                     uint32_t* status, uint32_t code) {
+    const uint32_t addr = smem_u32(bar);
+    if (mbar_try_wait_hint(addr, parity, PPLB200_WAIT_HINT_NS)) {
+        return true;
+    }
+    const long long t0 = clock64();
+    while (!mbar_try_wait_hint(addr, parity, PPLB200_WAIT_HINT_NS)) {
+        if (*abort_flag) {
+            return false;
+        }
+        if (clock64() - t0 > kWaitBudgetCycles) {
+            *abort_flag = 1;
+            atomicOr(status, code);
+            return false;
+        }
+    }
+    return true;
+}
+
 }  // namespace pplb200

@@ -64,48 +64,70 @@ int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t rank
     return PPLB200_SUCCESS;
 }
 
-int make_cache_tensor_map(const pplb200_attn_params& p, const void* cache, int tile_tokens, CUtensorMap* codes,
-                          CacheMapOrder* order) {
-    // logical outer dimensions: 0 row, 1 kv head, 2 k|v, 3 layer
-    const uint64_t extent[4] = {static_cast<uint64_t>(p.max_tokens), static_cast<uint64_t>(p.num_kv_heads), 2,
-                                static_cast<uint64_t>(p.num_layer)};
-    const uint64_t stride[4] = {static_cast<uint64_t>(p.cache_stride_s), static_cast<uint64_t>(p.cache_stride_h),
-                                static_cast<uint64_t>(p.cache_stride_kv), static_cast<uint64_t>(p.cache_stride_l)};
-    int idx[4] = {0, 1, 2, 3};
-    // Insertion sort by stride; among equal strides the row dimension goes last, so that a one-layer
-    // token-major cache (row and layer strides tie) gets the same order as a multi-layer one.
-    auto before = [&](int x, int y) {
-        return stride[x] < stride[y] || (stride[x] == stride[y] && y == 0 && x != 0);
-    };
-    for (int i = 1; i < 4; ++i) {
-        for (int j = i; j > 0 && before(idx[j], idx[j - 1]); --j) {
-            const int tmp = idx[j];
-            idx[j] = idx[j - 1];
-            idx[j - 1] = tmp;
+namespace {
+
+// The logical outer dimensions of a cache -- 0 row, 1 kv head, 2 k|v, 3 layer -- sorted by stride.
+struct CacheDims {
+    uint64_t extent[4], stride[4];
+    int idx[4];
+
+    explicit CacheDims(const pplb200_attn_params& p)
+        : extent{static_cast<uint64_t>(p.max_tokens), static_cast<uint64_t>(p.num_kv_heads), 2,
+                 static_cast<uint64_t>(p.num_layer)},
+          stride{static_cast<uint64_t>(p.cache_stride_s), static_cast<uint64_t>(p.cache_stride_h),
+                 static_cast<uint64_t>(p.cache_stride_kv), static_cast<uint64_t>(p.cache_stride_l)},
+          idx{0, 1, 2, 3} {
+        // Insertion sort by stride; among equal strides the row dimension goes last, so that a one-layer
+        // token-major cache (row and layer strides tie) gets the same order as a multi-layer one.
+        auto before = [&](int x, int y) {
+            return stride[x] < stride[y] || (stride[x] == stride[y] && y == 0 && x != 0);
+        };
+        for (int i = 1; i < 4; ++i) {
+            for (int j = i; j > 0 && before(idx[j], idx[j - 1]); --j) {
+                const int tmp = idx[j];
+                idx[j] = idx[j - 1];
+                idx[j - 1] = tmp;
+            }
         }
     }
+
+    // `inner` elements per row of one head; strides are those of the codes divided by `divisor`
+    int encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t divisor,
+               uint64_t elem_bytes, int tile_tokens, CUtensorMapSwizzle swizzle) const {
+        uint64_t dims[5], str[4];
+        uint32_t box[5];
+        dims[0] = inner;
+        box[0] = static_cast<uint32_t>(inner);
+        for (int i = 0; i < 4; ++i) {
+            const int d = idx[i];
+            dims[i + 1] = extent[d];
+            str[i] = stride[d] / divisor * elem_bytes;
+            box[i + 1] = (d == 0) ? static_cast<uint32_t>(tile_tokens) : 1u;
+        }
+        return encode_tensor_map(map, type, 5, base, dims, str, box, swizzle);
+    }
+};
+
+}  // namespace
+
+int make_cache_tensor_map(const pplb200_attn_params& p, const void* cache, int tile_tokens, CUtensorMap* codes,
+                          CacheMapOrder* order) {
+    const CacheDims d(p);
     int pos[4];
     for (int i = 0; i < 4; ++i) {
-        pos[idx[i]] = i + 1;
+        pos[d.idx[i]] = i + 1;
     }
     order->pos_row = pos[0];
     order->pos_head = pos[1];
     order->pos_kv = pos[2];
     order->pos_layer = pos[3];
+    return d.encode(codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, cache, static_cast<uint64_t>(p.head_dim), 1, 1, tile_tokens,
+                    p.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
+}
 
-    const uint64_t dh = static_cast<uint64_t>(p.head_dim);
-    uint64_t dims_c[5], str_c[4];
-    uint32_t box_c[5];
-    dims_c[0] = dh;
-    box_c[0] = static_cast<uint32_t>(dh);
-    for (int i = 0; i < 4; ++i) {
-        const int d = idx[i];
-        dims_c[i + 1] = extent[d];
-        str_c[i] = stride[d];  // int8: elements == bytes
-        box_c[i + 1] = (d == 0) ? static_cast<uint32_t>(tile_tokens) : 1u;
-    }
-    return encode_tensor_map(codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, cache, dims_c, str_c, box_c,
-                             p.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
+int make_scale_tensor_map(const pplb200_attn_params& p, const void* scale, int tile_tokens, CUtensorMap* scales) {
+    return CacheDims(p).encode(scales, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, scale, static_cast<uint64_t>(p.head_dim / 8), 8, 2,
+                               tile_tokens, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 }  // namespace pplb200

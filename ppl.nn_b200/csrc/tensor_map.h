@@ -28,4 +28,7 @@ struct CacheMapOrder {
 int make_cache_tensor_map(const pplb200_attn_params& p, const void* cache, int tile_tokens, CUtensorMap* codes,
                           CacheMapOrder* order);
 
+// The same for the scale tensor (head_dim / 8 halves per row of a head, not swizzled); same dimension order.
+int make_scale_tensor_map(const pplb200_attn_params& p, const void* scale, int tile_tokens, CUtensorMap* scales);
+
 }  // namespace pplb200

@@ -7,15 +7,19 @@
 //   rates 160 rows per kv head balance HBM and the tensor cores; below that the cache's bytes are the bound.
 //
 // Shape of the computation
-//   * The unit of work is a BLOCK of 64 positions of one segment = (sequence, kv head, tile of 128 query rows).  All
-//     blocks of the batch form one sequence, cut into equal ranges, one per resident CTA (two per SM).  A range that
-//     holds part of a segment leaves an fp32 partial (at most two per range), which tree_merge_kernel joins.
+//   * The unit of work is a BLOCK of 64 positions of one segment = (sequence, kv head, tile of 128 MT query rows).  The
+//     kv heads are dealt round-robin into `lanes` classes; neighbouring CTAs take the same range of different classes,
+//     i.e. neighbouring heads of the same rows at the same time.  All blocks of a class form one sequence, cut into
+//     equal ranges, one per resident CTA.  A range that holds part of a segment leaves an fp32 partial (at most two
+//     per range), which tree_merge_kernel joins.
 //   * tree_plan_kernel turns the device-side lengths into the prefix sum of blocks, and the parents into one bit mask
 //     of ancestors per token.  Only blocks that reach behind the history look at the masks, 64 bits a row and block.
-//   * Roles of a CTA: warps 0..3 are 128 softmax threads, one query row each; warps 4..7 load codes and scales from
-//     global memory (the next block's while this one is worked on), dequantise them to fp16 and write the swizzled
-//     K and V tiles; warp 8 issues the MMAs.  S = Q K^T goes to a 64-column TMEM buffer, P returns to TMEM as the A
-//     operand of O += P V (two buffers), as in the prefill kernel.
+//   * Roles of a CTA: 4 MT softmax warps, one thread per query row; four converter warps, which turn the raw codes and
+//     scales of a block into the swizzled fp16 K and V tiles; MT warps that issue the MMAs of a 128-row tile each; one
+//     warp that fetches the raw blocks by TMA into a ring of two, K and V apart.  S = Q K^T goes to a 64-column TMEM
+//     buffer, P returns to TMEM as the A operand of O += P V (two buffers), as in the prefill kernel.
+//   * MT = 1: two CTAs per SM.  MT = 2, for more than 128 rows per kv head: one CTA per SM, whose two tiles share the
+//     fetched and converted K and V.
 //
 // Waits on mbarriers are bounded and give up together (see tcgen05.cuh).
 #include <cub/block/block_scan.cuh>
@@ -24,32 +28,38 @@
 #include "launch.h"
 #include "ragged.cuh"
 #include "tcgen05.cuh"
+#include "tensor_map.h"
 
 namespace pplb200 {
 
 namespace {
 
-constexpr int kBlockM = 128;
+constexpr int kTileM = 128;  // rows of an MMA
 constexpr int kBlockN = 64;
-constexpr int kThreads = 288;
-constexpr int kStages = 2;
-constexpr int kCtasPerSm = 2;
+constexpr int kRawStages = 2;
 constexpr int kMinRange = 4;  // blocks: no range is cut finer
 constexpr float kNegBig = -1.0e30f;
 constexpr float kRescaleSlack = 8.0f;
 
-template <int DH>
+template <int DH, int MT>
 struct TTraits {
+    static constexpr int kBlockM = kTileM * MT;
+    static constexpr int kThreads = 32 * (4 * MT + 4 + MT + 1);
+    static constexpr int kCtasPerSm = MT == 1 ? 2 : 1;
+    static constexpr int kConvWarp = 4 * MT, kMmaWarp = kConvWarp + 4, kLoadWarp = kMmaWarp + MT;
     static constexpr int kColBlocks = DH / 64;
-    static constexpr int kQBlockBytes = kBlockM * 128;
+    static constexpr int kQBlockBytes = kTileM * 128;
     static constexpr int kKVBlockBytes = kBlockN * 128;
-    static constexpr int kQBytes = kColBlocks * kQBlockBytes;
+    static constexpr int kQBytes = kColBlocks * kQBlockBytes;  // one 128-row tile
     static constexpr int kKVBytes = kColBlocks * kKVBlockBytes;
-    // the same for every head size, so that never more than two CTAs share an SM and both TMEM allocations fit
-    static constexpr int kSmemBytes = 32768 + 2 * kStages * (kBlockN * 256) + 512;
+    static constexpr int kCodeBytes = kBlockN * DH;
+    static constexpr int kRawBytes = kCodeBytes + kBlockN * (DH / 8) * 2;  // codes and scales of K or V of a block
+    // The same for every head size, so that never more CTAs share an SM than its TMEM holds; MT = 2 asks for more
+    // than half of the SM's.
+    static constexpr int kSmemBytes = MT * 32768 + 2 * (kBlockN * 256) + 2 * kRawStages * (kBlockN * 160) + 512;
     static constexpr uint32_t kPCols = kBlockN / 2;
     static constexpr uint32_t kColS = 0, kColP = kBlockN, kColO = kColP + 2 * kPCols;
-    static constexpr uint32_t kTmemCols = 256;
+    static constexpr uint32_t kTileCols = 256;  // TMEM columns of a tile: S 64 | P 2 x 32 | O 128
 };
 
 struct TreeHeader {
@@ -79,7 +89,11 @@ struct TreeArgs {
     int32_t words;
     int32_t batch;
     int32_t num_heads, num_kv_heads, group;
-    int32_t ranges;
+    int32_t ranges;   // of a class
+    int32_t lanes;    // classes of kv heads
+    int32_t tile_rows;  // query rows of a segment: 128 MT
+    int32_t box_rows;  // rows of a copy: 64, or 16 where pages may end inside a block
+    CacheMapOrder order;
     float scale_log2;
 };
 
@@ -105,7 +119,7 @@ __device__ __forceinline__ Seq seq_of(const TreeArgs& a, int64_t b) {
     s.start = static_cast<int32_t>(start);
     s.len = static_cast<int32_t>(len);
     s.blocks = n > 0 ? (s.len + kBlockN - 1) / kBlockN : 0;
-    s.row_tiles = (s.n * a.group + kBlockM - 1) / kBlockM;
+    s.row_tiles = (s.n * a.group + a.tile_rows - 1) / a.tile_rows;
     return s;
 }
 
@@ -128,7 +142,7 @@ __global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(const TreeArgs 
             int64_t units = 0;
             if (b < a.batch) {
                 const Seq s = seq_of(a, b);
-                units = static_cast<int64_t>(s.blocks) * s.row_tiles * a.num_kv_heads;
+                units = static_cast<int64_t>(s.blocks) * s.row_tiles * (a.num_kv_heads / a.lanes);
             }
             int64_t excl, total;
             Scan(tmp).ExclusiveSum(units, excl, total);
@@ -186,36 +200,39 @@ __global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(const TreeArgs 
 // Part of a segment that lies in the CTA's range
 struct Piece {
     Seq seq;
-    int32_t b, kvh, rows_valid, row0;  // row0: first query row (token x head of the group) of the tile
+    int32_t b, kvh, rows_valid, row0;  // row0: first query row (token x head of the group) of the segment
     int32_t blk0, blk1;                // blocks [blk0, blk1) of the segment's seq.blocks
 };
 
-// The piece that starts at unit u of [.., end); all lanes of a warp call it together.
-__device__ __forceinline__ void piece_at(const TreeArgs& a, int64_t u, int64_t end, int lane, Piece& p) {
+// The piece that starts at unit u of [.., end) of class `lane_class`; all lanes of a warp call it together.
+__device__ __forceinline__ void piece_at(const TreeArgs& a, int64_t u, int64_t end, int lane_class, int lane, Piece& p) {
     p.b = warp_find_segment(a.prefix, a.batch, u, lane);
     p.seq = seq_of(a, p.b);
     const int32_t per_head = p.seq.blocks * p.seq.row_tiles;
     const int64_t q = u - a.prefix[p.b];
-    p.kvh = static_cast<int32_t>(q / per_head);
-    const int32_t rem = static_cast<int32_t>(q - static_cast<int64_t>(p.kvh) * per_head);
+    const int32_t vc = static_cast<int32_t>(q / per_head);
+    p.kvh = vc * a.lanes + lane_class;
+    const int32_t rem = static_cast<int32_t>(q - static_cast<int64_t>(vc) * per_head);
     const int32_t rt = rem / p.seq.blocks;
     p.blk0 = rem - rt * p.seq.blocks;
     const int64_t stop = p.blk0 + (end - u);
     p.blk1 = stop < p.seq.blocks ? static_cast<int32_t>(stop) : p.seq.blocks;
-    p.row0 = rt * kBlockM;
+    p.row0 = rt * a.tile_rows;
     const int32_t rows = p.seq.n * a.group - p.row0;
-    p.rows_valid = rows < kBlockM ? rows : kBlockM;
+    p.rows_valid = rows < a.tile_rows ? rows : a.tile_rows;
 }
 
+template <int MT>
 struct Barriers {
-    uint64_t q_full, q_empty, o_free;
-    uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-    uint64_t s_full, s_free;
-    uint64_t p_full[2], pv_done[2];
+    uint64_t q_full, q_empty;
+    uint64_t raw_full[2][kRawStages], raw_empty[2][kRawStages];  // [K | V]
+    uint64_t k_full, k_empty, v_full, v_empty;
+    uint64_t o_free[MT], s_full[MT], s_free[MT];
+    uint64_t p_full[MT][2], pv_done[MT][2];
     uint32_t tmem_slot;
     int abort_word;
 };
-static_assert(sizeof(Barriers) <= 512, "barrier block");
+static_assert(sizeof(Barriers<2>) <= 512, "barrier block");
 
 // 16 codes -> 16 halves of value, scaled by two groups' scales (s = scale of channels 0..7 | 8..15 << 16)
 __device__ __forceinline__ void dequant16(const uint4& c, uint32_t s, uint4& lo, uint4& hi) {
@@ -234,27 +251,37 @@ __device__ __forceinline__ void dequant16(const uint4& c, uint32_t s, uint4& lo,
 __device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
 
-// One thread's share of a K or V block: 16-byte piece `piece` of kRows rows
+// One thread's share of a raw K or V block: 16-byte piece `piece` of the rows row, row + kRowsPerStep, ..
 template <int DH>
 struct Raw {
-    static constexpr int kPieces = DH / 16;             // 16-byte pieces of a row
-    static constexpr int kRowsPerStep = 32 / kPieces;   // rows a warp loads at once
-    static constexpr int kRows = 16 / kRowsPerStep;     // steps over the warp's 16 rows
+    static constexpr int kPieces = DH / 16;            // 16-byte pieces of a row
+    static constexpr int kRowsPerStep = 32 / kPieces;  // rows of a warp at once
+    static constexpr int kRows = 16 / kRowsPerStep;    // steps over the warp's 16 rows
     uint4 code[kRows];
     uint32_t sc[kRows];
 
-    // `off`: element offset of the thread's piece in the first of its rows; `rows`: how many of the warp's 16 rows exist
-    __device__ __forceinline__ void load(const TreeArgs& a, int64_t off, int32_t r, int32_t rows) {
+    __device__ __forceinline__ void load(uint32_t raw, int32_t row, int32_t piece, int32_t rows) {
 #pragma unroll
         for (int k = 0; k < kRows; ++k) {
-            code[k] = make_uint4(0u, 0u, 0u, 0u);
-            sc[k] = 0u;
-            if (r + k * kRowsPerStep < rows) {
-                code[k] = *reinterpret_cast<const uint4*>(a.cache + off);
-                sc[k] = *reinterpret_cast<const uint32_t*>(a.scale + (off >> 3));
+            const int32_t r = row + k * kRowsPerStep;
+            const int32_t chunk = DH == 128 ? piece ^ (r & 7) : piece;  // as the 128-byte swizzle of the copy left it
+            code[k] = lds128(raw + r * DH + chunk * 16);
+            sc[k] = lds32(raw + kBlockN * DH + r * (DH / 4) + piece * 4);
+            if (r >= rows) {  // rows behind the sequence's end may hold anything
+                code[k] = make_uint4(0u, 0u, 0u, 0u);
+                sc[k] = 0u;
             }
-            off += a.geom.stride_s * kRowsPerStep;
         }
     }
 
@@ -276,14 +303,29 @@ struct Raw {
     }
 };
 
-template <int DH>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attn_kernel(const TreeArgs a) {
-    using T = TTraits<DH>;
+// `rows` rows of one head, K (0) or V (1), from cache row `row` on
+__device__ __forceinline__ void load_rows(const TreeArgs& a, void* dst, const CUtensorMap* map, uint64_t* bar, int row,
+                                          int head, int kv) {
+    int c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int pos = i + 1;
+        c[i] = a.order.pos_row == pos ? row
+                                      : (a.order.pos_head == pos ? head : (a.order.pos_kv == pos ? kv : static_cast<int>(a.geom.layer_idx)));
+    }
+    tma_load_5d(dst, map, bar, 0, c[0], c[1], c[2], c[3]);
+}
+
+template <int DH, int MT>
+__global__ void __launch_bounds__(TTraits<DH, MT>::kThreads, TTraits<DH, MT>::kCtasPerSm)
+tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_constant__ CUtensorMap tm_scale, const TreeArgs a) {
+    using T = TTraits<DH, MT>;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sQ = smem;
-    uint8_t* sK = sQ + T::kQBytes;
-    uint8_t* sV = sK + kStages * T::kKVBytes;
-    Barriers& bars = *reinterpret_cast<Barriers*>(sV + kStages * T::kKVBytes);
+    uint8_t* sK = sQ + MT * T::kQBytes;
+    uint8_t* sV = sK + T::kKVBytes;
+    uint8_t* sRaw = sV + T::kKVBytes;  // [stage][K | V]
+    Barriers<MT>& bars = *reinterpret_cast<Barriers<MT>*>(sRaw + 2 * kRawStages * T::kRawBytes);
     volatile int* abort_flag = &bars.abort_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t* status = &a.hdr->status;
@@ -294,7 +336,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attn_kernel(const T
         }
         return;
     }
-    const int64_t begin = blockIdx.x * a.hdr->range;
+    const int lane_class = blockIdx.x % a.lanes;
+    const int64_t begin = blockIdx.x / a.lanes * a.hdr->range;
     const int64_t total = a.hdr->total;
     const int64_t end = begin + a.hdr->range < total ? begin + a.hdr->range : total;
     if (begin >= end) {
@@ -303,24 +346,32 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attn_kernel(const T
     if (threadIdx.x == 0) {
         bars.abort_word = 0;
         mbar_init(&bars.q_full, 128);
-        mbar_init(&bars.q_empty, 1);
-        mbar_init(&bars.o_free, 128);
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(&bars.k_full[s], 128);
-            mbar_init(&bars.v_full[s], 128);
-            mbar_init(&bars.k_empty[s], 1);
-            mbar_init(&bars.v_empty[s], 1);
+        mbar_init(&bars.q_empty, MT);
+        for (int s = 0; s < kRawStages; ++s) {
+            for (int kv = 0; kv < 2; ++kv) {
+                mbar_init(&bars.raw_full[kv][s], 1);
+                mbar_init(&bars.raw_empty[kv][s], 128);
+            }
         }
-        mbar_init(&bars.s_full, 1);
-        mbar_init(&bars.s_free, 128);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&bars.p_full[i], 128);
-            mbar_init(&bars.pv_done[i], 1);
+        mbar_init(&bars.k_full, 128);
+        mbar_init(&bars.v_full, 128);
+        mbar_init(&bars.k_empty, MT);
+        mbar_init(&bars.v_empty, MT);
+        for (int t = 0; t < MT; ++t) {
+            mbar_init(&bars.o_free[t], 128);
+            mbar_init(&bars.s_full[t], 1);
+            mbar_init(&bars.s_free[t], 128);
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&bars.p_full[t][i], 128);
+                mbar_init(&bars.pv_done[t][i], 1);
+            }
         }
         mbar_fence_init();
+        tma_prefetch_desc(&tm_code);
+        tma_prefetch_desc(&tm_scale);
     }
-    if (warp == 8) {
-        tmem_alloc(&bars.tmem_slot, T::kTmemCols);
+    if (warp == T::kMmaWarp) {
+        tmem_alloc(&bars.tmem_slot, MT * T::kTileCols);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -328,42 +379,168 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attn_kernel(const T
     tc_fence_after();
     const uint32_t tmem_base = bars.tmem_slot;
 
-    if (warp >= 4 && warp < 8) {
-        // =========================== converters ===========================
-        const int ct = threadIdx.x - 128;
-        const int cw = warp - 4;  // this warp's 16 rows of a block
-        constexpr int kPieces = Raw<DH>::kPieces;
-        const int piece = lane % kPieces, rr = lane / kPieces;
-        const uint32_t k_tile = smem_u32(sK), v_tile = smem_u32(sV);
+    if (warp == T::kLoadWarp) {
+        // =========================== TMA producer ===========================
         bool ok = true;
-        int pieces = 0, n = 0;  // pieces and blocks converted so far
+        int n = 0;  // blocks requested so far
         for (int64_t u = begin; ok && u < end;) {
             Piece p;
-            piece_at(a, u, end, lane, p);
-            const int64_t head_off = a.geom.layer_idx * a.geom.stride_l + p.kvh * a.geom.stride_h + piece * 16;
-            Raw<DH> kr, vr;
-            // position of a block's rows of this warp: element offset of the thread's piece, rows that exist
-            auto locate = [&](int32_t blk, int64_t& off) -> int32_t {
-                const int32_t pos = blk * kBlockN + cw * 16;
-                int32_t rows = p.seq.len - pos;
-                rows = rows > 16 ? 16 : rows;
-                off = 0;
-                if (rows > 0) {
-                    const int64_t row = cache_row(a.geom, a.cachestarts, p.b, pos);
-                    if (row < 0 || row + rows > a.max_tokens) {  // a wrong index tensor: flagged, those rows read as zeros
-                        if (lane == 0) {
+            piece_at(a, u, end, lane_class, lane, p);
+            const int boxes = kBlockN / a.box_rows;
+            for (int32_t blk = p.blk0; ok && blk < p.blk1; ++blk, ++n) {
+                const int s = n % kRawStages;
+                // lane i < boxes: cache row of the i-th copy; rows outside the cache are flagged and read as zeros
+                int row = static_cast<int>(a.max_tokens);
+                if (lane < boxes) {
+                    const int32_t pos = blk * kBlockN + lane * a.box_rows;
+                    const int32_t rows = p.seq.len - pos < a.box_rows ? p.seq.len - pos : a.box_rows;
+                    if (rows > 0) {
+                        const int64_t first = cache_row(a.geom, a.cachestarts, p.b, pos);
+                        if (first < 0 || first + rows > a.max_tokens) {
                             atomicOr(status, kDevRowOutOfRange);
                         }
-                        rows = row < 0 || row >= a.max_tokens ? 0 : static_cast<int32_t>(a.max_tokens - row);
+                        if (first >= 0 && first < a.max_tokens) {
+                            row = static_cast<int>(first);
+                        }
                     }
-                    off = (row + rr) * a.geom.stride_s + head_off;
                 }
-                return rows;
-            };
-            int64_t off, next_off = 0;
-            int32_t rows = locate(p.blk0, off);
-            kr.load(a, off, rr, rows);
-            vr.load(a, off + a.geom.stride_kv, rr, rows);
+                for (int kv = 0; ok && kv < 2; ++kv) {
+                    if (n >= kRawStages) {
+                        ok = wait_or_abort_parked(&bars.raw_empty[kv][s], ((n / kRawStages) - 1) & 1, abort_flag, status,
+                                                  kDevMmaTimeout);
+                        if (!ok) {
+                            break;
+                        }
+                    }
+                    uint8_t* dst = sRaw + (2 * s + kv) * T::kRawBytes;
+                    uint64_t* bar = &bars.raw_full[kv][s];
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(bar, T::kRawBytes);
+                    }
+                    __syncwarp();
+                    if (lane < boxes) {
+                        load_rows(a, dst + lane * a.box_rows * DH, &tm_code, bar, row, p.kvh, kv);
+                        load_rows(a, dst + T::kCodeBytes + lane * a.box_rows * (DH / 4), &tm_scale, bar, row, p.kvh, kv);
+                    }
+                    __syncwarp();
+                }
+            }
+            u += p.blk1 - p.blk0;
+        }
+        if (*abort_flag) {
+            // every copy this warp issued must have landed before the CTA may exit; a stage whose copies were issued
+            // is complete at the latest parity it was armed with (a stage that was never armed is left alone)
+            for (int j = n > kRawStages ? n - kRawStages : 0; j < n; ++j) {
+                for (int kv = 0; kv < 2; ++kv) {
+                    mbar_wait_bounded(&bars.raw_full[kv][j % kRawStages], (j / kRawStages) & 1);
+                }
+            }
+        }
+    } else if (warp >= T::kMmaWarp) {
+        // =========================== MMA issuer of one 128-row tile ===========================
+        constexpr uint32_t idesc_qk = instr_desc_f16(kBlockN, false);
+        constexpr uint32_t idesc_pv = instr_desc_f16(DH, true);
+        constexpr uint32_t hi_sw128 = desc_hi(1024, 2);
+        const int t = warp - T::kMmaWarp;
+        const uint32_t q_lo = desc_lo(smem_u32(sQ) + t * T::kQBytes, 16);
+        const uint32_t k_lo = desc_lo(smem_u32(sK), 16);
+        const uint32_t v_lo = desc_lo(smem_u32(sV), T::kKVBlockBytes);
+        const uint32_t tm = tmem_base + t * T::kTileCols;
+        const uint32_t d_s = tm + T::kColS, d_o = tm + T::kColO, a_p = tm + T::kColP;
+        bool ok = true;
+        int pieces = 0, blocks_done = 0;    // of the CTA
+        int mine = 0, kc = 0, vc = 0;       // pieces, Q K^T and P V of this tile
+        for (int64_t u = begin; ok && u < end; ++pieces) {
+            Piece p;
+            piece_at(a, u, end, lane_class, lane, p);
+            const int32_t blocks = p.blk1 - p.blk0;
+            u += blocks;
+            ok = wait_or_abort(&bars.q_full, pieces & 1, abort_flag, status, kDevMmaTimeout);
+            if (t * kTileM >= p.rows_valid) {
+                // no rows for this tile: only hand the operands back
+                for (int32_t j = 0; ok && j < blocks; ++j, ++blocks_done) {
+                    ok = wait_or_abort_parked(&bars.k_full, blocks_done & 1, abort_flag, status, kDevMmaTimeout);
+                    if (ok && lane == 0) {
+                        mbar_arrive(&bars.k_empty);
+                        if (j == blocks - 1) {
+                            mbar_arrive(&bars.q_empty);
+                        }
+                    }
+                    ok = ok && wait_or_abort_parked(&bars.v_full, blocks_done & 1, abort_flag, status, kDevMmaTimeout);
+                    if (ok && lane == 0) {
+                        mbar_arrive(&bars.v_empty);
+                    }
+                    __syncwarp();
+                }
+                continue;
+            }
+            for (int32_t j = 0; ok && j <= blocks; ++j) {
+                if (j < blocks) {
+                    ok = wait_or_abort(&bars.k_full, (blocks_done + j) & 1, abort_flag, status, kDevMmaTimeout) &&
+                         (kc == 0 || wait_or_abort(&bars.s_free[t], (kc - 1) & 1, abort_flag, status, kDevMmaTimeout));
+                    if (!ok) {
+                        break;
+                    }
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int cb = 0; cb < T::kColBlocks; ++cb) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                tc_mma_f16(d_s, desc_join(q_lo + cb * (T::kQBlockBytes >> 4) + 2 * k, hi_sw128),
+                                           desc_join(k_lo + cb * (T::kKVBlockBytes >> 4) + 2 * k, hi_sw128), idesc_qk,
+                                           (cb | k) ? 1u : 0u);
+                            }
+                        }
+                        tc_commit(&bars.s_full[t]);
+                        tc_commit(&bars.k_empty);
+                        if (j == blocks - 1) {
+                            tc_commit(&bars.q_empty);
+                        }
+                    }
+                    __syncwarp();
+                    ++kc;
+                }
+                if (j > 0) {
+                    ok = wait_or_abort(&bars.v_full, (blocks_done + j - 1) & 1, abort_flag, status, kDevMmaTimeout) &&
+                         wait_or_abort(&bars.p_full[t][vc & 1], (vc >> 1) & 1, abort_flag, status, kDevMmaTimeout);
+                    if (ok && j == 1 && mine > 0) {
+                        ok = wait_or_abort(&bars.o_free[t], (mine - 1) & 1, abort_flag, status, kDevMmaTimeout);
+                    }
+                    if (!ok) {
+                        break;
+                    }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t pa = a_p + (vc & 1) * T::kPCols;
+#pragma unroll
+                        for (int ks = 0; ks < kBlockN / 16; ++ks) {
+                            tc_mma_f16_ts(d_o, pa + 8 * ks, desc_join(v_lo + ks * (2048 >> 4), hi_sw128), idesc_pv,
+                                          ((j - 1) | ks) ? 1u : 0u);
+                        }
+                        tc_commit(&bars.v_empty);
+                        tc_commit(&bars.pv_done[t][vc & 1]);
+                    }
+                    __syncwarp();
+                    ++vc;
+                }
+            }
+            blocks_done += blocks;
+            ++mine;
+        }
+    } else if (warp >= T::kConvWarp) {
+        // =========================== converters ===========================
+        const int ct = threadIdx.x - 32 * T::kConvWarp;
+        constexpr int kPieces = Raw<DH>::kPieces;
+        const int piece = lane % kPieces;
+        const int row = (warp - T::kConvWarp) * 16 + lane / kPieces;  // first of the thread's rows of a block
+        const uint32_t k_tile = smem_u32(sK), v_tile = smem_u32(sV), raw0 = smem_u32(sRaw), q_tile = smem_u32(sQ);
+        bool ok = true;
+        int pieces = 0, n = 0;  // pieces and blocks so far
+        for (int64_t u = begin; ok && u < end; ++pieces) {
+            Piece p;
+            piece_at(a, u, end, lane_class, lane, p);
+            u += p.blk1 - p.blk0;
             // Q: row r of the tile is query row row0 + r = token x head of the group
             if (pieces > 0) {
                 ok = wait_or_abort(&bars.q_empty, (pieces - 1) & 1, abort_flag, status, kDevMmaTimeout);
@@ -374,127 +551,52 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attn_kernel(const T
             constexpr int kQPieces = DH / 8;  // 16-byte pieces of a query row
             for (int i = ct; i < p.rows_valid * kQPieces; i += 128) {
                 const int r = i / kQPieces, c = i - r * kQPieces;
-                const int32_t row = p.row0 + r;
-                const int32_t tok = row / a.group;
+                const int32_t qrow = p.row0 + r;
+                const int32_t tok = qrow / a.group;
                 const uint4 v = *reinterpret_cast<const uint4*>(
-                    a.q + ((p.seq.tok0 + tok) * a.num_heads + p.kvh * a.group + (row - tok * a.group)) * DH + c * 8);
-                sts128(smem_u32(sQ) + (c >> 3) * T::kQBlockBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4), v);
+                    a.q + ((p.seq.tok0 + tok) * a.num_heads + p.kvh * a.group + (qrow - tok * a.group)) * DH + c * 8);
+                sts128(q_tile + (r / kTileM) * T::kQBytes + (c >> 3) * T::kQBlockBytes + (r % kTileM) * 128 +
+                           (((c & 7) ^ (r & 7)) << 4), v);
             }
             fence_proxy_async_smem();
             mbar_arrive(&bars.q_full);
-            ++pieces;
             for (int32_t blk = p.blk0; blk < p.blk1; ++blk, ++n) {
-                const int s = n % kStages;
-                const bool more = blk + 1 < p.blk1;
-                int32_t next_rows = 0;
-                if (more) {
-                    next_rows = locate(blk + 1, next_off);
+                const int s = n % kRawStages;
+                const int32_t rows = p.seq.len - blk * kBlockN;  // rows of the block that exist
+                Raw<DH> raw;
+                ok = wait_or_abort(&bars.raw_full[0][s], (n / kRawStages) & 1, abort_flag, status, kDevTmaTimeout);
+                if (!ok) {
+                    break;
                 }
-                if (n >= kStages) {
-                    ok = wait_or_abort(&bars.k_empty[s], ((n / kStages) - 1) & 1, abort_flag, status, kDevMmaTimeout);
-                    if (!ok) {
-                        break;
-                    }
+                raw.load(raw0 + 2 * s * T::kRawBytes, row, piece, rows);
+                mbar_arrive(&bars.raw_empty[0][s]);
+                ok = n == 0 || wait_or_abort(&bars.k_empty, (n - 1) & 1, abort_flag, status, kDevMmaTimeout);
+                if (!ok) {
+                    break;
                 }
-                kr.store(k_tile + s * T::kKVBytes, cw * 16 + rr, piece);
+                raw.store(k_tile, row, piece);
                 fence_proxy_async_smem();
-                mbar_arrive(&bars.k_full[s]);
-                if (more) {
-                    kr.load(a, next_off, rr, next_rows);
+                mbar_arrive(&bars.k_full);
+                ok = wait_or_abort(&bars.raw_full[1][s], (n / kRawStages) & 1, abort_flag, status, kDevTmaTimeout);
+                if (!ok) {
+                    break;
                 }
-                if (n >= kStages) {
-                    ok = wait_or_abort(&bars.v_empty[s], ((n / kStages) - 1) & 1, abort_flag, status, kDevMmaTimeout);
-                    if (!ok) {
-                        break;
-                    }
+                raw.load(raw0 + (2 * s + 1) * T::kRawBytes, row, piece, rows);
+                mbar_arrive(&bars.raw_empty[1][s]);
+                ok = n == 0 || wait_or_abort(&bars.v_empty, (n - 1) & 1, abort_flag, status, kDevMmaTimeout);
+                if (!ok) {
+                    break;
                 }
-                vr.store(v_tile + s * T::kKVBytes, cw * 16 + rr, piece);
+                raw.store(v_tile, row, piece);
                 fence_proxy_async_smem();
-                mbar_arrive(&bars.v_full[s]);
-                if (more) {
-                    vr.load(a, next_off + a.geom.stride_kv, rr, next_rows);
-                }
+                mbar_arrive(&bars.v_full);
             }
-            u += p.blk1 - p.blk0;
         }
-    } else if (warp == 8) {
-        // =========================== MMA issuer ===========================
-        constexpr uint32_t idesc_qk = instr_desc_f16(kBlockN, false);
-        constexpr uint32_t idesc_pv = instr_desc_f16(DH, true);
-        constexpr uint32_t hi_sw128 = desc_hi(1024, 2);
-        const uint32_t q_lo = desc_lo(smem_u32(sQ), 16);
-        const uint32_t k_lo = desc_lo(smem_u32(sK), 16);
-        const uint32_t v_lo = desc_lo(smem_u32(sV), T::kKVBlockBytes);
-        const uint32_t d_s = tmem_base + T::kColS, d_o = tmem_base + T::kColO, a_p = tmem_base + T::kColP;
-        bool ok = true;
-        int pieces = 0, kc = 0, vc = 0;
-        for (int64_t u = begin; ok && u < end;) {
-            Piece p;
-            piece_at(a, u, end, lane, p);
-            const int32_t blocks = p.blk1 - p.blk0;
-            ok = wait_or_abort(&bars.q_full, pieces & 1, abort_flag, status, kDevMmaTimeout);
-            for (int32_t j = 0; ok && j <= blocks; ++j) {
-                if (j < blocks) {
-                    const int s = kc % kStages;
-                    ok = wait_or_abort(&bars.k_full[s], (kc / kStages) & 1, abort_flag, status, kDevMmaTimeout) &&
-                         (kc == 0 || wait_or_abort(&bars.s_free, (kc - 1) & 1, abort_flag, status, kDevMmaTimeout));
-                    if (!ok) {
-                        break;
-                    }
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint32_t ks_lo = k_lo + s * (T::kKVBytes >> 4);
-#pragma unroll
-                        for (int cb = 0; cb < T::kColBlocks; ++cb) {
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                tc_mma_f16(d_s, desc_join(q_lo + cb * (T::kQBlockBytes >> 4) + 2 * k, hi_sw128),
-                                           desc_join(ks_lo + cb * (T::kKVBlockBytes >> 4) + 2 * k, hi_sw128), idesc_qk,
-                                           (cb | k) ? 1u : 0u);
-                            }
-                        }
-                        tc_commit(&bars.s_full);
-                        tc_commit(&bars.k_empty[s]);
-                        if (j == blocks - 1) {
-                            tc_commit(&bars.q_empty);
-                        }
-                    }
-                    __syncwarp();
-                    ++kc;
-                }
-                if (j > 0) {
-                    const int s = vc % kStages;
-                    ok = wait_or_abort(&bars.v_full[s], (vc / kStages) & 1, abort_flag, status, kDevMmaTimeout) &&
-                         wait_or_abort(&bars.p_full[vc & 1], (vc >> 1) & 1, abort_flag, status, kDevMmaTimeout);
-                    if (ok && j == 1 && pieces > 0) {
-                        ok = wait_or_abort(&bars.o_free, (pieces - 1) & 1, abort_flag, status, kDevMmaTimeout);
-                    }
-                    if (!ok) {
-                        break;
-                    }
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint32_t vs_lo = v_lo + s * (T::kKVBytes >> 4);
-                        const uint32_t pa = a_p + (vc & 1) * T::kPCols;
-#pragma unroll
-                        for (int ks = 0; ks < kBlockN / 16; ++ks) {
-                            tc_mma_f16_ts(d_o, pa + 8 * ks, desc_join(vs_lo + ks * (2048 >> 4), hi_sw128), idesc_pv,
-                                          ((j - 1) | ks) ? 1u : 0u);
-                        }
-                        tc_commit(&bars.v_empty[s]);
-                        tc_commit(&bars.pv_done[vc & 1]);
-                    }
-                    __syncwarp();
-                    ++vc;
-                }
-            }
-            ++pieces;
-            u += blocks;
-        }
-    } else if (warp < 4) {
+    } else {
         // =========================== softmax / epilogue ===========================
-        const int r = warp * 32 + lane;  // row of the tile = TMEM lane
-        const uint32_t t_lane = static_cast<uint32_t>(warp * 32) << 16;
+        const int t = warp >> 2, quarter = warp & 3;
+        const int r = quarter * 32 + lane;  // row of the tile = TMEM lane
+        const uint32_t t_lane = (static_cast<uint32_t>(quarter * 32) << 16) + t * T::kTileCols;
         const uint32_t t_s = tmem_base + t_lane + T::kColS;
         const uint32_t t_o = tmem_base + t_lane + T::kColO;
         const uint32_t t_p = tmem_base + t_lane + T::kColP;
@@ -503,50 +605,45 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attn_kernel(const T
         int pc = 0;
         for (int64_t u = begin; ok && u < end;) {
             Piece p;
-            piece_at(a, u, end, lane, p);
-            const bool warp_live = warp * 32 < p.rows_valid;  // rows behind the last are carried along unread
-            const bool live = r < p.rows_valid;
-            const int32_t row = p.row0 + r;
+            piece_at(a, u, end, lane_class, lane, p);
+            u += p.blk1 - p.blk0;
+            const int32_t rows_valid = p.rows_valid - t * kTileM;  // of this tile
+            if (rows_valid <= 0) {
+                continue;
+            }
+            if (quarter * 32 >= rows_valid) {
+                // the rows of this warp are behind the last one: its lanes only keep the barriers going
+                for (int32_t blk = p.blk0; ok && blk < p.blk1; ++blk, ++pc) {
+                    ok = wait_or_abort_parked(&bars.s_full[t], pc & 1, abort_flag, status, kDevMmaTimeout);
+                    if (ok) {
+                        mbar_arrive(&bars.s_free[t]);
+                        mbar_arrive(&bars.p_full[t][pc & 1]);
+                    }
+                }
+                ok = ok && wait_or_abort_parked(&bars.pv_done[t][(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status,
+                                                kDevMmaTimeout);
+                if (ok) {
+                    mbar_arrive(&bars.o_free[t]);
+                }
+                continue;
+            }
+            const bool live = r < rows_valid;
+            const int32_t row = p.row0 + t * kTileM + r;
             const int32_t tok = live ? row / a.group : 0;
             const uint64_t* anc = a.ancestor + (p.seq.tok0 + tok) * a.words;
             float m_ref = kNegBig, l_sum = 0.0f;
             for (int32_t blk = p.blk0; ok && blk < p.blk1; ++blk, ++pc) {
                 if (pc >= 2) {
-                    ok = wait_or_abort(&bars.pv_done[pc & 1], ((pc - 2) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
+                    ok = wait_or_abort(&bars.pv_done[t][pc & 1], ((pc - 2) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
                     if (!ok) {
                         break;
                     }
                 }
-                // 64 positions of this row: bit e = position blk * 64 + e is visible
-                const int32_t a0 = blk * kBlockN - p.seq.start;  // index of the block's first position among the drafts
-                const bool masked = a0 + kBlockN > 0;
-                uint64_t seen = ~0ull;
-                if (masked && live) {
-                    if (a0 <= 0) {
-                        seen = (a0 == 0 ? 0ull : ~0ull >> (64 + a0)) | (anc[0] << -a0);
-                    } else {
-                        const int32_t w = a0 >> 6, sh = a0 & 63;
-                        seen = w < a.words ? anc[w] >> sh : 0ull;
-                        if (sh > 0 && w + 1 < a.words) {
-                            seen |= anc[w + 1] << (64 - sh);
-                        }
-                    }
-                    const int32_t room = p.seq.len - blk * kBlockN;  // positions that exist
-                    if (room < kBlockN) {
-                        seen &= ~0ull >> (64 - room);
-                    }
-                }
-                ok = wait_or_abort(&bars.s_full, pc & 1, abort_flag, status, kDevMmaTimeout);
+                ok = wait_or_abort(&bars.s_full[t], pc & 1, abort_flag, status, kDevMmaTimeout);
                 if (!ok) {
                     break;
                 }
                 tc_fence_after();
-                if (!warp_live) {
-                    tc_fence_before();
-                    mbar_arrive(&bars.s_free);
-                    mbar_arrive(&bars.p_full[pc & 1]);
-                    continue;
-                }
                 float sv[kBlockN];
                 {
                     uint32_t v[kBlockN / 32][32];
@@ -564,8 +661,26 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attn_kernel(const T
                     }
                 }
                 tc_fence_before();
-                mbar_arrive(&bars.s_free);
-                if (masked) {
+                mbar_arrive(&bars.s_free[t]);
+                const int32_t a0 = blk * kBlockN - p.seq.start;  // index of the block's first position among the drafts
+                if (a0 + kBlockN > 0) {
+                    // 64 positions of this row: bit e = position blk * 64 + e is visible
+                    uint64_t seen = ~0ull;
+                    if (live) {
+                        if (a0 <= 0) {
+                            seen = (a0 == 0 ? 0ull : ~0ull >> (64 + a0)) | (anc[0] << -a0);
+                        } else {
+                            const int32_t w = a0 >> 6, sh = a0 & 63;
+                            seen = w < a.words ? anc[w] >> sh : 0ull;
+                            if (sh > 0 && w + 1 < a.words) {
+                                seen |= anc[w + 1] << (64 - sh);
+                            }
+                        }
+                        const int32_t room = p.seq.len - blk * kBlockN;  // positions that exist
+                        if (room < kBlockN) {
+                            seen &= ~0ull >> (64 - room);
+                        }
+                    }
                     const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
 #pragma unroll
                     for (int e = 0; e < kBlockN; ++e) {
@@ -587,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attn_kernel(const T
                     m_ref = m_new;
                     l_sum *= f;
                     if (blk > p.blk0) {
-                        ok = wait_or_abort(&bars.pv_done[(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
+                        ok = wait_or_abort(&bars.pv_done[t][(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
                         if (!ok) {
                             break;
                         }
@@ -606,8 +721,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attn_kernel(const T
                         tmem_wait_st();
                     }
                 }
-                // P = exp2(s * scale - m_ref) as packed fp16; the row sum adds the rounded values that P V uses
+                // P = exp2(s * scale - m_ref) as packed fp16; the row sum adds the rounded values that P V uses, in
+                // four chains (one chain of 64 dependent additions would be as long as the exponentials)
                 const uint32_t t_pb = t_p + (pc & 1) * T::kPCols;
+                float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int q = 0; q < kBlockN / 32; ++q) {
                     uint32_t pk[16];
@@ -616,27 +733,28 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attn_kernel(const T
                         const float2 x = __ffma2_rn(make_float2(sv[32 * q + 2 * e], sv[32 * q + 2 * e + 1]),
                                                     make_float2(sc, sc), make_float2(-m_ref, -m_ref));
                         pk[e] = h2_as_u32(__floats2half2_rn(ex2_approx(x.x), ex2_approx(x.y)));
-                        add_half2_to_float(l_sum, pk[e]);
+                        add_half2_to_float(l4[e & 3], pk[e]);
                     }
                     tmem_st16(t_pb + 16 * q, pk);
                 }
+                l_sum += (l4[0] + l4[1]) + (l4[2] + l4[3]);
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&bars.p_full[pc & 1]);
+                mbar_arrive(&bars.p_full[t][pc & 1]);
             }
             // ---- epilogue: the whole segment -> fp16 rows; a part of one -> fp32 partial ----
             if (ok) {
-                ok = wait_or_abort(&bars.pv_done[(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
+                ok = wait_or_abort(&bars.pv_done[t][(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
             }
             if (ok) {
                 tc_fence_after();
                 const bool whole = p.blk0 == 0 && p.blk1 == p.seq.blocks;
                 const float inv = l_sum > 0.0f ? 1.0f / l_sum : 0.0f;
                 __half* dst = a.out + ((p.seq.tok0 + tok) * a.num_heads + p.kvh * a.group + (row - tok * a.group)) * DH;
-                const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (p.blk0 == 0 ? 1 : 0);
-                float* part = a.part_o + (slot * kBlockM + r) * DH;
+                const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (p.blk0 == 0 ? 1 : 0)) * T::kBlockM + t * kTileM + r;
+                float* part = a.part_o + slot * DH;
                 if (!whole && live) {
-                    a.part_ml[slot * kBlockM + r] = make_float2(m_ref, l_sum);
+                    a.part_ml[slot] = make_float2(m_ref, l_sum);
                 }
 #pragma unroll
                 for (int c = 0; c < DH / 32; ++c) {
@@ -645,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attn_kernel(const T
                     tmem_wait_ld();
                     if (c == DH / 32 - 1) {
                         tc_fence_before();
-                        mbar_arrive(&bars.o_free);
+                        mbar_arrive(&bars.o_free[t]);
                     }
                     if (live && whole) {
 #pragma unroll
@@ -671,15 +789,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) tree_attn_kernel(const T
                     }
                 }
             }
-            u += p.blk1 - p.blk0;
         }
     }
 
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == T::kMmaWarp) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, T::kTmemCols);
+        tmem_dealloc(tmem_base, MT * T::kTileCols);
     }
 }
 
@@ -704,17 +821,20 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a) {
     }
     const int32_t kvh = head / a.group;
     const int32_t row = static_cast<int32_t>(i) * a.group + (head - kvh * a.group);
-    const int32_t rt = row / kBlockM, r = row - rt * kBlockM;
-    const int64_t u0 = a.prefix[b] + (static_cast<int64_t>(kvh) * s.row_tiles + rt) * s.blocks;
+    const int32_t rt = row / a.tile_rows, r = row - rt * a.tile_rows;
+    const int32_t vc = kvh / a.lanes, lane_class = kvh - vc * a.lanes;
+    const int64_t u0 = a.prefix[b] + (static_cast<int64_t>(vc) * s.row_tiles + rt) * s.blocks;
     const int64_t range = a.hdr->range;
     const int64_t first = u0 / range, last = (u0 + s.blocks - 1) / range;
     if (first == last) {
         return;  // one range held all of it and wrote the output
     }
+    auto slot_of = [&](int64_t w) -> int64_t {
+        return (2 * (w * a.lanes + lane_class) + (u0 >= w * range ? 1 : 0)) * a.tile_rows + r;
+    };
     float m = kNegBig;
     for (int64_t w = first; w <= last; ++w) {
-        const int64_t slot = 2 * w + (u0 >= w * range ? 1 : 0);
-        m = fmaxf(m, a.part_ml[slot * kBlockM + r].x);
+        m = fmaxf(m, a.part_ml[slot_of(w)].x);
     }
     float l = 0.0f, o[kPer];
 #pragma unroll
@@ -722,10 +842,10 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a) {
         o[e] = 0.0f;
     }
     for (int64_t w = first; w <= last; ++w) {
-        const int64_t slot = 2 * w + (u0 >= w * range ? 1 : 0);
-        const float2 ml = a.part_ml[slot * kBlockM + r];
+        const int64_t slot = slot_of(w);
+        const float2 ml = a.part_ml[slot];
         const float f = ex2_approx(ml.x - m);
-        const float* part = a.part_o + (slot * kBlockM + r) * DH + lane * kPer;
+        const float* part = a.part_o + slot * DH + lane * kPer;
         l += ml.y * f;
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
@@ -744,9 +864,10 @@ uint64_t align256(uint64_t x) {
     return (x + 255) / 256 * 256;
 }
 
-template <int DH>
-int launch_dh(const TreeArgs& a, const TreePlan& plan, cudaStream_t stream) {
-    using T = TTraits<DH>;
+template <int DH, int MT>
+int launch_dh(const pplb200_attn_params& p, TreeArgs a, cudaStream_t stream) {
+    using T = TTraits<DH, MT>;
+    auto kernel = tree_attn_kernel<DH, MT>;
     // the attribute belongs to the (kernel, device) pair
     static bool attr_set[kMaxDevices] = {};
     int dev = 0;
@@ -755,19 +876,29 @@ int launch_dh(const TreeArgs& a, const TreePlan& plan, cudaStream_t stream) {
         return PPLB200_DEVICE_RUNTIME_ERROR;
     }
     if (!attr_set[dev]) {
-        if (cudaFuncSetAttribute(tree_attn_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmemBytes) !=
-            cudaSuccess) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmemBytes) != cudaSuccess) {
             (void)cudaGetLastError();
             return PPLB200_DEVICE_RUNTIME_ERROR;
         }
         attr_set[dev] = true;
     }
-    tree_plan_kernel<<<static_cast<unsigned>(a.batch + 1), kPlanThreads, 0, stream>>>(a);
-    int rc = check_launch("tree_plan_kernel");
+    a.tile_rows = T::kBlockM;
+    a.box_rows = a.geom.cache_mode == 0 || a.geom.page_size % kBlockN == 0 ? kBlockN : 16;
+    CUtensorMap tm_code, tm_scale;
+    int rc = make_cache_tensor_map(p, a.cache, a.box_rows, &tm_code, &a.order);
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    tree_attn_kernel<DH><<<static_cast<unsigned>(plan.ranges), kThreads, T::kSmemBytes, stream>>>(a);
+    rc = make_scale_tensor_map(p, a.scale, a.box_rows, &tm_scale);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    tree_plan_kernel<<<static_cast<unsigned>(a.batch + 1), kPlanThreads, 0, stream>>>(a);
+    rc = check_launch("tree_plan_kernel");
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    kernel<<<static_cast<unsigned>(a.ranges * a.lanes), T::kThreads, T::kSmemBytes, stream>>>(tm_code, tm_scale, a);
     rc = check_launch("tree_attn_kernel");
     if (rc != PPLB200_SUCCESS) {
         return rc;
@@ -780,18 +911,26 @@ int launch_dh(const TreeArgs& a, const TreePlan& plan, cudaStream_t stream) {
 }  // namespace
 
 int make_tree_plan(const pplb200_attn_params& p, int sm_count, TreePlan* plan) {
+    // query rows per kv head beyond one MMA tile: two tiles of a CTA share K and V
+    plan->tiles = p.max_seqlen * (p.num_heads / p.num_kv_heads) > kTileM ? 2 : 1;
+    const int64_t tile_rows = plan->tiles * kTileM;
+    const int64_t resident = plan->tiles == 1 ? 2 * static_cast<int64_t>(sm_count) : sm_count;
+    plan->lanes = 8;
+    while (p.num_kv_heads % plan->lanes != 0 || resident % plan->lanes != 0) {
+        plan->lanes >>= 1;
+    }
     // no more ranges than there can be work for
-    const int64_t row_tiles = (p.max_seqlen * (p.num_heads / p.num_kv_heads) + kBlockM - 1) / kBlockM;
+    const int64_t row_tiles = (p.max_seqlen * (p.num_heads / p.num_kv_heads) + tile_rows - 1) / tile_rows;
     const int64_t blocks = (p.max_kvlen + kBlockN - 1) / kBlockN;
-    int64_t ranges = (p.batch * p.num_kv_heads * row_tiles * blocks + kMinRange - 1) / kMinRange;
-    const int64_t resident = static_cast<int64_t>(sm_count) * kCtasPerSm;
-    plan->ranges = ranges > resident ? resident : ranges;
+    const int64_t most = (p.batch * (p.num_kv_heads / plan->lanes) * row_tiles * blocks + kMinRange - 1) / kMinRange;
+    plan->ranges = most > resident / plan->lanes ? resident / plan->lanes : most;
     plan->words = (p.max_seqlen + 63) / 64;
+    const uint64_t slot_rows = static_cast<uint64_t>(plan->ranges) * plan->lanes * 2 * tile_rows;
     plan->off_prefix = 256;
     plan->off_ancestor = plan->off_prefix + align256(static_cast<uint64_t>(p.batch + 1) * 8);
     plan->off_part_ml = plan->off_ancestor + align256(static_cast<uint64_t>(p.total_tokens) * plan->words * 8);
-    plan->off_part_o = plan->off_part_ml + static_cast<uint64_t>(plan->ranges) * 2 * kBlockM * 8;
-    plan->bytes = plan->off_part_o + static_cast<uint64_t>(plan->ranges) * 2 * kBlockM * p.head_dim * 4;
+    plan->off_part_o = plan->off_part_ml + slot_rows * 8;
+    plan->bytes = plan->off_part_o + slot_rows * p.head_dim * 4;
     return PPLB200_SUCCESS;
 }
 
@@ -828,8 +967,12 @@ int launch_tree_attn(const pplb200_attn_params& p, const CacheGeom& geom, const 
     a.num_kv_heads = p.num_kv_heads;
     a.group = p.num_heads / p.num_kv_heads;
     a.ranges = static_cast<int32_t>(plan.ranges);
+    a.lanes = static_cast<int32_t>(plan.lanes);
     a.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(p.head_dim));
-    return p.head_dim == 128 ? launch_dh<128>(a, plan, stream) : launch_dh<64>(a, plan, stream);
+    if (plan.tiles == 2) {
+        return p.head_dim == 128 ? launch_dh<128, 2>(p, a, stream) : launch_dh<64, 2>(p, a, stream);
+    }
+    return p.head_dim == 128 ? launch_dh<128, 1>(p, a, stream) : launch_dh<64, 1>(p, a, stream);
 }
 
 }  // namespace pplb200
