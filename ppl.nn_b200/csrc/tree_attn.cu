@@ -537,6 +537,24 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
         const uint32_t k_tile = smem_u32(sK), v_tile = smem_u32(sV), raw0 = smem_u32(sRaw), q_tile = smem_u32(sQ);
         bool ok = true;
         int pieces = 0, n = 0;  // pieces and blocks so far
+        // K (0) or V (1) of the CTA's block number `blk_no`, of which `rows` rows exist
+        auto convert = [&](int kv, int blk_no, int32_t rows) -> bool {
+            const int s = blk_no % kRawStages;
+            if (!wait_or_abort(&bars.raw_full[kv][s], (blk_no / kRawStages) & 1, abort_flag, status, kDevTmaTimeout)) {
+                return false;
+            }
+            Raw<DH> raw;
+            raw.load(raw0 + (2 * s + kv) * T::kRawBytes, row, piece, rows);
+            mbar_arrive(&bars.raw_empty[kv][s]);
+            if (blk_no > 0 && !wait_or_abort(kv ? &bars.v_empty : &bars.k_empty, (blk_no - 1) & 1, abort_flag, status,
+                                             kDevMmaTimeout)) {
+                return false;
+            }
+            raw.store(kv ? v_tile : k_tile, row, piece);
+            fence_proxy_async_smem();
+            mbar_arrive(kv ? &bars.v_full : &bars.k_full);
+            return true;
+        };
         for (int64_t u = begin; ok && u < end; ++pieces) {
             Piece p;
             piece_at(a, u, end, lane_class, lane, p);
@@ -560,36 +578,14 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
             }
             fence_proxy_async_smem();
             mbar_arrive(&bars.q_full);
-            for (int32_t blk = p.blk0; blk < p.blk1; ++blk, ++n) {
-                const int s = n % kRawStages;
-                const int32_t rows = p.seq.len - blk * kBlockN;  // rows of the block that exist
-                Raw<DH> raw;
-                ok = wait_or_abort(&bars.raw_full[0][s], (n / kRawStages) & 1, abort_flag, status, kDevTmaTimeout);
-                if (!ok) {
-                    break;
+            // K runs one block ahead of V: V(j) has to wait for P V(j - 1), i.e. for a softmax, and the scores of block
+            // j + 1 should not wait with it
+            ok = convert(0, n, p.seq.len - p.blk0 * kBlockN);
+            for (int32_t blk = p.blk0; ok && blk < p.blk1; ++blk, ++n) {
+                if (blk + 1 < p.blk1) {
+                    ok = convert(0, n + 1, p.seq.len - (blk + 1) * kBlockN);
                 }
-                raw.load(raw0 + 2 * s * T::kRawBytes, row, piece, rows);
-                mbar_arrive(&bars.raw_empty[0][s]);
-                ok = n == 0 || wait_or_abort(&bars.k_empty, (n - 1) & 1, abort_flag, status, kDevMmaTimeout);
-                if (!ok) {
-                    break;
-                }
-                raw.store(k_tile, row, piece);
-                fence_proxy_async_smem();
-                mbar_arrive(&bars.k_full);
-                ok = wait_or_abort(&bars.raw_full[1][s], (n / kRawStages) & 1, abort_flag, status, kDevTmaTimeout);
-                if (!ok) {
-                    break;
-                }
-                raw.load(raw0 + (2 * s + 1) * T::kRawBytes, row, piece, rows);
-                mbar_arrive(&bars.raw_empty[1][s]);
-                ok = n == 0 || wait_or_abort(&bars.v_empty, (n - 1) & 1, abort_flag, status, kDevMmaTimeout);
-                if (!ok) {
-                    break;
-                }
-                raw.store(v_tile, row, piece);
-                fence_proxy_async_smem();
-                mbar_arrive(&bars.v_full);
+                ok = ok && convert(1, n, p.seq.len - blk * kBlockN);
             }
         }
     } else {
