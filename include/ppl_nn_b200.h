@@ -373,7 +373,8 @@ int pplb200_kv_evict_select(const pplb200_attn_params* p, const float* weight, c
  * and reported (PPLB200_DEV_KEPT_INVALID).  `workspace`: pplb200_kv_compact_workspace_size() bytes, 256-byte aligned
  * (its first word is the status word).  No counterpart in the reference.
  */
-int pplb200_kv_compact_workspace_size(const pplb200_attn_params* p, uint64_t* bytes);
+int pplb200_kv_compact_workspace_size(const pplb200_attn_params* p, int64_t kept_heads, int64_t max_kept,
+                                      int64_t layers, uint64_t* bytes);
 
 int pplb200_kv_compact(const pplb200_attn_params* p, const int64_t* kept, int64_t kept_heads, int64_t max_kept,
                        const int64_t* base, const int64_t* kvlens, const int64_t* cachestarts, int64_t layers,

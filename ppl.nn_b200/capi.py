@@ -208,7 +208,7 @@ class Library:
         d.pplb200_kv_evict_select.restype = ctypes.c_int
         d.pplb200_kv_evict_select.argtypes = [pp, vp, i64p, i64p, i64p, i64, i64, i64, i64p, vp, ctypes.c_uint64, vp]
         d.pplb200_kv_compact_workspace_size.restype = ctypes.c_int
-        d.pplb200_kv_compact_workspace_size.argtypes = [pp, sizep]
+        d.pplb200_kv_compact_workspace_size.argtypes = [pp, i64, i64, i64, sizep]
         d.pplb200_kv_compact.restype = ctypes.c_int
         d.pplb200_kv_compact.argtypes = [pp, i64p, i64, i64, i64p, i64p, i64p, i64, vp, vp, vp, vp, ctypes.c_uint64, vp]
         d.pplb200_status_str.restype = ctypes.c_char_p
@@ -317,9 +317,9 @@ class Library:
                                                     cachestarts, start_pos, workspace, int(workspace_bytes), rq, rk,
                                                     cache, scale, stream)
 
-    def _size(self, fn, p) -> tuple[int, int]:
+    def _size(self, fn, p, *args) -> tuple[int, int]:
         n = ctypes.c_uint64(0)
-        rc = fn(ctypes.byref(p), ctypes.byref(n))
+        rc = fn(ctypes.byref(p), *args, ctypes.byref(n))
         return rc, int(n.value)
 
     def tree_attn_workspace_size(self, p) -> tuple[int, int]:
@@ -347,8 +347,8 @@ class Library:
                                                 int(recent), int(max_budget), kept, workspace, int(workspace_bytes),
                                                 stream)
 
-    def kv_compact_workspace_size(self, p) -> tuple[int, int]:
-        return self._size(self.dll.pplb200_kv_compact_workspace_size, p)
+    def kv_compact_workspace_size(self, p, kept_heads, max_kept, layers) -> tuple[int, int]:
+        return self._size(self.dll.pplb200_kv_compact_workspace_size, p, int(kept_heads), int(max_kept), int(layers))
 
     def kv_compact(self, p, kept, kept_heads, max_kept, base, kvlens, cachestarts, layers, cache, scale, weight,
                    workspace, workspace_bytes, stream) -> int:

@@ -880,28 +880,11 @@ int pplb200_kv_evict_select(const pplb200_attn_params* p, const float* weight, c
                                   static_cast<uint32_t*>(workspace), kept, stream);
 }
 
-int pplb200_kv_compact_workspace_size(const pplb200_attn_params* p, uint64_t* bytes) {
+static int validate_compact(const pplb200_attn_params* p, int64_t kept_heads, int64_t max_kept, int64_t layers,
+                            CompactPlan* plan) {
     const int rc = validate_cache_op(p);
     if (rc != PPLB200_SUCCESS) {
         return rc;
-    }
-    if (!bytes) {
-        return fail(PPLB200_NOT_FOUND, "bytes is null");
-    }
-    *bytes = 256;  // the device status word
-    return PPLB200_SUCCESS;
-}
-
-int pplb200_kv_compact(const pplb200_attn_params* p, const int64_t* kept, int64_t kept_heads, int64_t max_kept,
-                       const int64_t* base, const int64_t* kvlens, const int64_t* cachestarts, int64_t layers,
-                       void* cache, void* scale, float* weight, void* workspace, uint64_t workspace_bytes,
-                       void* stream_v) {
-    int rc = validate_cache_op(p);
-    if (rc != PPLB200_SUCCESS) {
-        return rc;
-    }
-    if (!scale) {
-        return fail(PPLB200_UNSUPPORTED, "only a quantised cache is supported but scale is null");
     }
     if (kept_heads != 1 && kept_heads != p->num_kv_heads) {
         return fail(PPLB200_INVALID_VALUE, "kept_heads must be 1 or num_kv_heads");
@@ -911,6 +894,38 @@ int pplb200_kv_compact(const pplb200_attn_params* p, const int64_t* kept, int64_
     }
     if (max_kept < 0 || max_kept > 0x7fff0000) {
         return fail(PPLB200_INVALID_VALUE, "max_kept out of range");
+    }
+    if (make_compact_plan(*p, kept_heads, max_kept, layers, plan) != PPLB200_SUCCESS) {
+        return fail(PPLB200_UNSUPPORTED, "more segments than a grid holds");
+    }
+    return PPLB200_SUCCESS;
+}
+
+int pplb200_kv_compact_workspace_size(const pplb200_attn_params* p, int64_t kept_heads, int64_t max_kept,
+                                      int64_t layers, uint64_t* bytes) {
+    CompactPlan plan;
+    const int rc = validate_compact(p, kept_heads, max_kept, layers, &plan);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    if (!bytes) {
+        return fail(PPLB200_NOT_FOUND, "bytes is null");
+    }
+    *bytes = plan.bytes;
+    return PPLB200_SUCCESS;
+}
+
+int pplb200_kv_compact(const pplb200_attn_params* p, const int64_t* kept, int64_t kept_heads, int64_t max_kept,
+                       const int64_t* base, const int64_t* kvlens, const int64_t* cachestarts, int64_t layers,
+                       void* cache, void* scale, float* weight, void* workspace, uint64_t workspace_bytes,
+                       void* stream_v) {
+    CompactPlan plan;
+    int rc = validate_compact(p, kept_heads, max_kept, layers, &plan);
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
+    }
+    if (!scale) {
+        return fail(PPLB200_UNSUPPORTED, "only a quantised cache is supported but scale is null");
     }
     if (p->batch == 0 || (max_kept == 0 && !weight)) {
         return PPLB200_SUCCESS;
@@ -926,17 +941,12 @@ int pplb200_kv_compact(const pplb200_attn_params* p, const int64_t* kept, int64_
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    rc = check_workspace(workspace, workspace_bytes, 256, "workspace is smaller than pplb200_kv_compact_workspace_size()");
+    rc = check_workspace(workspace, workspace_bytes, plan.bytes, "workspace is smaller than pplb200_kv_compact_workspace_size()");
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-    rc = clear_status(workspace, stream);
-    if (rc != PPLB200_SUCCESS) {
-        return rc;
-    }
-    return launch_kv_compact(*p, make_geom(*p), kept, kept_heads, max_kept, base, kvlens, cachestarts, layers, cache,
-                             scale, weight, static_cast<uint32_t*>(workspace), stream);
+    return launch_kv_compact(*p, make_geom(*p), plan, kept, kept_heads, max_kept, base, kvlens, cachestarts, layers, cache,
+                             scale, weight, workspace, static_cast<cudaStream_t>(stream_v));
 }
 
 int pplb200_mhca_device_status(const void* workspace, void* stream, uint32_t* status) {

@@ -2,15 +2,24 @@
 //
 // Select.  For one (sequence, kv head) with n cached positions and a budget of k, the last r = min(recent, k)
 // positions stay, then the first s = min(sink, k - r), and of the positions [s, n - r) the k - r - s of highest
-// accumulated weight, ties going to the lowest position.  The order of fp32 weights is the order of a 32-bit
-// key (order_key below), so the weight of the last one taken is found exactly by a radix descent: four rounds
-// of 8 bits, each a histogram of the keys that share the digits found so far.  A last pass over the positions
-// writes the kept ones in ascending order.
+// accumulated weight, ties going to the lowest position.  The order of fp32 weights is the order of a 32-bit key
+// (order_key below).  One CTA per list, and one read of the weights:
+//   1. A sample of 4096 keys brackets the key of the last candidate taken: [low, high] around the sample's quantile,
+//      four standard deviations wide on either side.  (Up to kListCap candidates need no sample: all go to the list.)
+//   2. Every weight is read once.  A key above the bracket sets its position's bit in a mask in shared memory, a key
+//      inside it joins a list in shared memory.
+//   3. A radix descent over that list (four rounds of 8 bits) gives the exact key of the last one taken; the list's
+//      keys above it set their bits, the equal ones theirs in a second mask.
+//   4. The masks are walked in order of position: bits of the first mask, and the first so many of the second.
+// Should the bracket miss (too many keys above, or too few down to its end) or the list overflow (many equal weights),
+// the radix descent runs over the weights themselves, and so it does for lists too long for the masks.
 //
-// Compact.  Row base + kept[i] moves to row base + i.  kept is strictly ascending, so kept[i] >= i, and a list
-// can be worked through in place in ascending blocks: a later block's sources lie at or behind its own
-// destinations, hence behind every destination of the earlier blocks; only the writes of a block have to wait
-// until the sources of that block (and of those before it) have been read.
+// Compact.  Row base + kept[i] moves to row base + i.  kept is strictly ascending, so kept[i] >= i.  A list is cut into
+// segments; a segment reads all its sources before it writes.  Its destinations may still be the sources of EARLIER
+// segments (kept[i'] = i with i' < i), never of later ones, so a segment raises a flag once it has read, and writes
+// once the flags of the earlier segments of its list are up.  The CTAs draw their segments from a counter in an order
+// in which a list's earlier segments come first: whoever waits, waits for CTAs that are running and that do not wait
+// before they raise their flag.
 #include "common.cuh"
 #include "launch.h"
 
@@ -18,7 +27,14 @@ namespace pplb200 {
 
 namespace {
 
+// Threads of a CTA: 1024 for long lists, one CTA per SM; for lists of up to kShortList positions, which come in large
+// numbers, four times as many CTAs of a quarter of the threads.
 constexpr int kSelectThreads = 1024;
+constexpr int kShortThreads = 256;
+constexpr int kShortList = 4096;
+constexpr int kListCap = 12288;    // keys inside the bracket
+constexpr int kSample = 4096;
+constexpr int kMaskWords = 8192;   // 262144 positions
 
 // Unsigned key with the order of the weights: -0 counts as +0, NaN as the lowest.
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -39,121 +55,317 @@ struct SelectArgs {
     CacheGeom geom;
     int64_t sink, recent, max_budget, max_kvlen, max_tokens;
     int32_t num_kv_heads;
+    int32_t mask_words;  // 32-bit words of a mask, and keys of the list: the shared memory the launch asked for
+    int32_t list_cap;
 };
 
-__global__ void __launch_bounds__(kSelectThreads) kv_evict_select_kernel(const SelectArgs a) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t warp_sum[2][32];
-    __shared__ uint32_t s_digit, s_below;
+struct SelectShared {
+    uint32_t hist[256];
+    uint32_t warp_sum[32];
+    uint32_t digit, left, listed, above;
+};
+
+// The key of rank `rank` (1: the highest) among the keys that for_each(f) passes to f, and how many of that key belong
+// to the `rank` highest.  Four rounds: a histogram of the next 8 bits of the keys that share the digits found so far.
+template <typename ForEach>
+__device__ __forceinline__ uint32_t radix_rank(SelectShared& sh, uint32_t rank, uint32_t& equal, ForEach for_each) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    uint32_t prefix = 0, left = rank;
+#pragma unroll 1
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (tid < 256) {
+            sh.hist[tid] = 0;
+        }
+        __syncthreads();
+        for_each([&](uint32_t key) {
+            if (shift == 24 || (key >> (shift + 8)) == prefix) {
+                atomicAdd(&sh.hist[(key >> shift) & 255u], 1u);
+            }
+        });
+        __syncthreads();
+        if (tid < 32) {
+            // lane l holds digits 255 - 8 l .. 248 - 8 l, from the highest down
+            uint32_t c[8], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                c[i] = sh.hist[255 - 8 * lane - i];
+                sum += c[i];
+            }
+            uint32_t before = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t x = __shfl_up_sync(0xffffffffu, before, o);
+                before += lane >= o ? x : 0u;
+            }
+            before -= sum;  // keys with a higher digit than this lane's
+            if (before < left && left <= before + sum) {
+                uint32_t d = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (before < left) {
+                        d = 255 - 8 * lane - i;
+                        sh.left = left - before;
+                    }
+                    before += c[i];
+                }
+                sh.digit = d;
+            }
+        }
+        __syncthreads();
+        prefix = (prefix << 8) | sh.digit;
+        left = sh.left;
+    }
+    equal = left;
+    return prefix;
+}
+
+// Exclusive sum over the CTA's warps of a warp-uniform value; `total` is the sum over all of them.
+__device__ __forceinline__ uint32_t sum_before(SelectShared& sh, uint32_t v, uint32_t& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __syncthreads();
+    if (lane == 0) {
+        sh.warp_sum[warp] = v;
+    }
+    __syncthreads();
+    const uint32_t x = lane < static_cast<int>(blockDim.x >> 5) ? sh.warp_sum[lane] : 0u;
+    uint32_t incl = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        incl += lane >= o ? y : 0u;
+    }
+    total = __shfl_sync(0xffffffffu, incl, 31);
+    return __shfl_sync(0xffffffffu, incl - x, warp);
+}
+
+__device__ __forceinline__ uint32_t warp_total(uint32_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    return v;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(NT) kv_evict_select_kernel(const SelectArgs a) {
+    __shared__ SelectShared sh;
+    extern __shared__ __align__(16) uint32_t dyn[];
+    uint32_t* mask = dyn;                      // kept for sure
+    uint32_t* tie = mask + a.mask_words;       // has the key of the last one taken
+    uint32_t* list_key = tie + a.mask_words;
+    int32_t* list_pos = reinterpret_cast<int32_t*>(list_key + a.list_cap);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t b = blockIdx.y;
     const int head = blockIdx.x;
-    int64_t n = a.kvlens[b], k = a.budgets[b];
-    if (n > a.max_kvlen || k > a.max_budget) {
+    int64_t n64 = a.kvlens[b], k64 = a.budgets[b];
+    if (n64 > a.max_kvlen) {
         if (tid == 0) {
             atomicOr(a.status, kDevLengthClamped);
         }
-        n = n > a.max_kvlen ? a.max_kvlen : n;
+        n64 = a.max_kvlen;
     }
-    n = n < 0 ? 0 : n;
-    k = k > a.max_budget ? a.max_budget : k;
-    k = k > n ? n : (k < 0 ? 0 : k);
-    const int64_t r = a.recent < k ? a.recent : k;
-    const int64_t s = a.sink < k - r ? a.sink : k - r;
-    const int32_t lo = static_cast<int32_t>(s), hi = static_cast<int32_t>(n - r);  // candidates [lo, hi)
-    const uint32_t want = static_cast<uint32_t>(k - r - s);
+    n64 = n64 < 0 ? 0 : n64;
+    k64 = k64 > a.max_budget ? a.max_budget : k64;
+    k64 = k64 > n64 ? n64 : (k64 < 0 ? 0 : k64);
+    const int64_t r = a.recent < k64 ? a.recent : k64;
+    const int64_t s = a.sink < k64 - r ? a.sink : k64 - r;
+    const int32_t n = static_cast<int32_t>(n64), k = static_cast<int32_t>(k64);
+    const int32_t lo = static_cast<int32_t>(s), hi = static_cast<int32_t>(n64 - r);  // candidates [lo, hi)
+    const uint32_t want = static_cast<uint32_t>(k64 - r - s), have = static_cast<uint32_t>(hi - lo);
     const float* w = a.weight + (a.geom.layer_idx * a.num_kv_heads + head) * a.max_tokens;
     int64_t* out = a.kept + (b * a.num_kv_heads + head) * a.max_budget;
 
+    const int64_t first_row = a.geom.cache_mode == 0 ? a.cachestarts[b] : 0;
     auto key_at = [&](int32_t pos) -> uint32_t {
-        const int64_t row = cache_row(a.geom, a.cachestarts, b, pos);
+        int64_t row = first_row < 0 ? -1 : first_row + pos;
+        if (a.geom.cache_mode != 0) {
+            row = cache_row(a.geom, a.cachestarts, b, pos);
+        }
         if (!cache_row_ok(row, a.max_tokens)) {
             atomicOr(a.status, kDevRowOutOfRange);
             return 0u;
         }
-        return order_key(w[row]);
+        return order_key(__ldg(w + row));
+    };
+    auto all_keys = [&](auto f) {
+        for (int32_t pos = lo + tid; pos < hi; pos += NT) {
+            f(key_at(pos));
+        }
     };
 
-    // the key of the last candidate taken, and how many candidates with exactly that key are taken
-    uint32_t cut = 0, equal_left = want;
-    if (want > 0 && static_cast<int64_t>(want) < hi - lo) {
-        uint32_t prefix = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += kSelectThreads) {
-                hist[i] = 0;
+    // cut: the key of the last candidate taken; equal: how many candidates with that key are taken
+    const bool choose = want > 0 && want < have;
+    uint32_t cut = 0, equal = 0;
+    const int32_t words = (n + 31) / 32;
+    const bool fits = words <= a.mask_words;
+    bool done = !choose;
+    if (fits) {
+        for (int32_t i = tid; i < words; i += NT) {
+            // sinks and recent positions; all of them, or nothing else, where there is no choice to make
+            uint32_t m = 0;
+#pragma unroll 4
+            for (int e = 0; e < 32; ++e) {
+                const int32_t pos = i * 32 + e;
+                m |= (pos < n && (pos < lo || pos >= hi || (!choose && want > 0))) ? 1u << e : 0u;
             }
-            __syncthreads();
-            for (int32_t pos = lo + tid; pos < hi; pos += kSelectThreads) {
-                const uint32_t key = key_at(pos);
-                if (shift == 24 || (key >> (shift + 8)) == prefix) {
-                    atomicAdd(&hist[(key >> shift) & 255u], 1u);
-                }
-            }
-            __syncthreads();
-            if (tid == 0) {  // from the highest digit down
-                uint32_t above = 0;
-                int d = 255;
-                while (d > 0 && above + hist[d] < equal_left) {
-                    above += hist[d];
-                    --d;
-                }
-                s_digit = static_cast<uint32_t>(d);
-                s_below = equal_left - above;
-            }
-            __syncthreads();
-            prefix = (prefix << 8) | s_digit;
-            equal_left = s_below;
+            mask[i] = m;
+            tie[i] = 0;
         }
-        cut = prefix;
     }
-    const bool all = static_cast<int64_t>(want) >= hi - lo;
+    if (choose && fits) {
+        uint32_t low = 0, high = 0xffffffffu;
+        if (have > static_cast<uint32_t>(a.list_cap)) {
+            const double step = static_cast<double>(have) / kSample;
+            const float q = static_cast<float>(want) / static_cast<float>(have) * kSample;
+            const float wide = 4.0f * sqrtf(q * (1.0f - q / kSample)) + 8.0f;
+            uint32_t keys[kSample / NT];
+#pragma unroll
+            for (int i = 0; i < kSample / NT; ++i) {
+                keys[i] = key_at(lo + static_cast<int32_t>((i * NT + tid) * step));
+            }
+            auto sample = [&](auto f) {
+#pragma unroll
+                for (int i = 0; i < kSample / NT; ++i) {
+                    f(keys[i]);
+                }
+            };
+            uint32_t unused;
+            if (q - wide >= 1.0f) {
+                high = radix_rank(sh, static_cast<uint32_t>(q - wide), unused, sample);
+            }
+            if (q + wide < kSample) {
+                low = radix_rank(sh, static_cast<uint32_t>(q + wide) + 1u, unused, sample);
+            }
+        }
+        if (tid == 0) {
+            sh.listed = 0;
+            sh.above = 0;
+        }
+        __syncthreads();
+        constexpr int kAhead = 4;
+        uint32_t above = 0;
+        for (int32_t base = (lo & ~31) + warp * 32; base < hi; base += NT * kAhead) {
+            uint32_t key[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int32_t pos = base + i * NT + lane;
+                key[i] = pos >= lo && pos < hi ? key_at(pos) : 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int32_t pos = base + i * NT + lane;
+                const bool in = pos >= lo && pos < hi;
+                const uint32_t up = __ballot_sync(0xffffffffu, in && key[i] > high);
+                const bool listed = in && key[i] >= low && key[i] <= high;
+                const uint32_t mid = __ballot_sync(0xffffffffu, listed);
+                if (up != 0u && lane == 0) {
+                    mask[pos >> 5] |= up;  // this warp alone owns the word
+                }
+                above += __popc(up);
+                if (mid != 0u) {
+                    uint32_t at = 0;
+                    if (lane == 0) {
+                        at = atomicAdd(&sh.listed, __popc(mid));
+                    }
+                    at = __shfl_sync(0xffffffffu, at, 0) + __popc(mid & ((1u << lane) - 1u));
+                    if (listed && at < static_cast<uint32_t>(a.list_cap)) {
+                        list_key[at] = key[i];
+                        list_pos[at] = pos;
+                    }
+                }
+            }
+        }
+        if (lane == 0) {
+            atomicAdd(&sh.above, above);
+        }
+        __syncthreads();
+        above = sh.above;
+        const uint32_t listed = sh.listed;
+        done = listed <= static_cast<uint32_t>(a.list_cap) && above < want && want <= above + listed;
+        if (done) {
+            cut = radix_rank(sh, want - above, equal, [&](auto f) {
+                for (uint32_t i = tid; i < listed; i += NT) {
+                    f(list_key[i]);
+                }
+            });
+            for (uint32_t i = tid; i < listed; i += NT) {
+                if (list_key[i] >= cut) {
+                    uint32_t* m = list_key[i] > cut ? mask : tie;
+                    atomicOr(&m[list_pos[i] >> 5], 1u << (list_pos[i] & 31));
+                }
+            }
+        }
+    }
+    if (!done) {
+        cut = radix_rank(sh, want, equal, all_keys);
+        if (fits) {
+            __syncthreads();
+            for (int32_t base = (lo & ~31) + warp * 32; base < hi; base += NT) {
+                const int32_t pos = base + lane;
+                const bool in = pos >= lo && pos < hi;
+                const uint32_t key = in ? key_at(pos) : 0u;
+                const uint32_t up = __ballot_sync(0xffffffffu, in && key > cut);
+                const uint32_t mid = __ballot_sync(0xffffffffu, in && key == cut);
+                const uint32_t forced = __ballot_sync(0xffffffffu, !in && pos < n);
+                if (lane == 0) {
+                    mask[pos >> 5] = forced | up;
+                    tie[pos >> 5] = mid;
+                }
+            }
+        }
+    }
+    __syncthreads();
 
-    // kept positions in ascending order
-    uint32_t taken = 0, equal_seen = 0;
-    for (int32_t base = 0; base < n; base += kSelectThreads) {
-        const int32_t pos = base + tid;
-        bool forced = false, above = false, equal = false;
-        if (pos < n) {
-            forced = pos < lo || pos >= hi;
-            if (!forced && want > 0) {
-                const uint32_t key = all ? 1u : key_at(pos);
-                above = key > cut;
-                equal = key == cut;
-            }
+    // kept positions in ascending order: a warp takes a run of words, after the counts of the runs before it
+    const int32_t total_words = fits ? words : (n + 31) / 32;
+    const int32_t run = (total_words + (NT / 32) - 1) / (NT / 32);
+    const int32_t w0 = warp * run, w1 = w0 + run < total_words ? w0 + run : total_words;
+    auto word_at = [&](int32_t i, uint32_t& ties) -> uint32_t {  // the words of 32 positions; all lanes call it
+        if (fits) {
+            ties = tie[i];
+            return mask[i];
         }
-        const uint32_t eq_mask = __ballot_sync(0xffffffffu, equal);
-        if (lane == 0) {
-            warp_sum[0][warp] = __popc(eq_mask);
+        const int32_t pos = i * 32 + lane;
+        const bool forced = pos < n && (pos < lo || pos >= hi || (!choose && want > 0));
+        const uint32_t key = choose && pos >= lo && pos < hi ? key_at(pos) : 0u;
+        ties = __ballot_sync(0xffffffffu, choose && pos >= lo && pos < hi && key == cut);
+        return __ballot_sync(0xffffffffu, forced || (choose && pos >= lo && pos < hi && key > cut));
+    };
+    uint32_t sure = 0, ties = 0;
+    if (fits) {
+        for (int32_t i = w0 + lane; i < w1; i += 32) {
+            sure += __popc(mask[i]);
+            ties += __popc(tie[i]);
         }
-        __syncthreads();
-        uint32_t v = warp_sum[0][lane], before = 0, total = 0;
-        for (int o = 0; o < 32; ++o) {
-            const uint32_t x = __shfl_sync(0xffffffffu, v, o);
-            before += o < warp ? x : 0u;
-            total += x;
-        }
-        const uint32_t eq_rank = equal_seen + before + __popc(eq_mask & ((1u << lane) - 1u));
-        equal_seen += total;
-        const bool keep = forced || above || (equal && eq_rank < equal_left);
-        const uint32_t mask = __ballot_sync(0xffffffffu, keep);
-        if (lane == 0) {
-            warp_sum[1][warp] = __popc(mask);
-        }
-        __syncthreads();
-        v = warp_sum[1][lane];
-        before = total = 0;
-        for (int o = 0; o < 32; ++o) {
-            const uint32_t x = __shfl_sync(0xffffffffu, v, o);
-            before += o < warp ? x : 0u;
-            total += x;
-        }
-        const uint32_t rank = taken + before + __popc(mask & ((1u << lane) - 1u));
-        taken += total;
-        if (keep && rank < k) {
-            out[rank] = pos;
+        sure = warp_total(sure);
+        ties = warp_total(ties);
+    } else {
+        for (int32_t i = w0; i < w1; ++i) {
+            uint32_t t;
+            sure += __popc(word_at(i, t));
+            ties += __popc(t);
         }
     }
-    for (int64_t i = k + tid; i < a.max_budget; i += kSelectThreads) {
+    uint32_t total;
+    uint32_t ties_before = sum_before(sh, ties, total);
+    const uint32_t ties_taken = ties_before >= equal ? 0u : (equal - ties_before < ties ? equal - ties_before : ties);
+    uint32_t rank = sum_before(sh, sure + ties_taken, total);
+    for (int32_t i = w0; i < w1; ++i) {
+        uint32_t t;
+        uint32_t m = word_at(i, t);
+        if (t != 0u) {
+            const uint32_t mine = __popc(t & ((1u << lane) - 1u));
+            const bool take = ((t >> lane) & 1u) != 0u && ties_before + mine < equal;
+            m |= __ballot_sync(0xffffffffu, take);
+            ties_before += __popc(t);
+        }
+        const uint32_t at = rank + __popc(m & ((1u << lane) - 1u));
+        if (((m >> lane) & 1u) != 0u && at < static_cast<uint32_t>(k)) {
+            out[at] = i * 32 + lane;
+        }
+        rank += __popc(m);
+    }
+    for (int64_t i = k + tid; i < a.max_budget; i += NT) {
         out[i] = -1;
     }
 }
@@ -169,30 +381,55 @@ struct CompactArgs {
     __half* scale;
     float* weight;  // [L, Hkv, MaxT] or null
     uint32_t* status;
+    uint32_t* ticket;
+    uint32_t* flags;  // [segments][lists]
     CacheGeom geom;
     int64_t max_kept, max_kvlen, max_tokens;
+    int64_t lists;       // batch * layers * head groups
+    int64_t move_tasks;  // segments * lists
     int32_t kept_heads, num_kv_heads, layers;
+    int32_t heads_per_cta, head_groups, rows_per_seg, segments;
 };
 
 constexpr int kCompactThreads = 256;
-constexpr int kUnits = 4;  // 16-byte pieces a thread has in flight
+constexpr int kSegmentRows = 64;      // rows x heads of a segment
+constexpr int kClearRows = 8192;      // weights zeroed by a CTA
 
-// One CTA per (sequence, layer, kv head, K | V | weight).
+// Up to this many clock cycles a segment waits for the ones before it
+__device__ __forceinline__ bool wait_flag(const uint32_t* flag) {
+    const long long t0 = clock64();
+    for (;;) {
+        uint32_t v;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
+        if (v != 0u) {
+            return true;
+        }
+        if (clock64() - t0 > kWaitBudgetCycles) {
+            return false;
+        }
+    }
+}
+
 template <int DH>
 __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const CompactArgs a) {
-    constexpr int kCodeUnits = DH / 16;            // 16-byte pieces of a row's codes
+    constexpr int kCodeUnits = DH / 16;              // 16-byte pieces of a row's codes
     constexpr int kRowUnits = kCodeUnits + DH / 64;  // and of its scales
-    constexpr int kRows = kCompactThreads * kUnits / kRowUnits;  // rows of a block
+    constexpr int kUnits = (kSegmentRows * 2 * kRowUnits + kCompactThreads - 1) / kCompactThreads;
+    __shared__ uint32_t s_ticket;
+    __shared__ int64_t s_src[kSegmentRows], s_dst[kSegmentRows];
     const int tid = threadIdx.x;
-    const int parts = a.weight != nullptr ? 3 : 2;
-    int64_t id = blockIdx.x;
-    const int part = static_cast<int>(id % parts);
-    id /= parts;
-    const int head = static_cast<int>(id % a.num_kv_heads);
-    id /= a.num_kv_heads;
-    const int layer = static_cast<int>(id % a.layers);
-    const int64_t b = id / a.layers;
-    const int64_t* kept = a.kept + (b * a.kept_heads + (a.kept_heads > 1 ? head : 0)) * a.max_kept;
+    if (tid == 0) {
+        s_ticket = atomicAdd(a.ticket, 1u);
+    }
+    __syncthreads();
+    const int64_t task = s_ticket;
+    const bool clear = task >= a.move_tasks;
+    const int64_t list = (clear ? task - a.move_tasks : task) % a.lists;
+    const int32_t seg = static_cast<int32_t>((clear ? task - a.move_tasks : task) / a.lists);
+    const int head0 = static_cast<int>(list % a.head_groups) * a.heads_per_cta;
+    const int layer = static_cast<int>(list / a.head_groups % a.layers);
+    const int64_t b = list / a.head_groups / a.layers;
+    const int64_t* kept = a.kept + (b * a.kept_heads + (a.kept_heads > 1 ? head0 : 0)) * a.max_kept;
     const int64_t base = a.base[b];
     int64_t n = a.kvlens[b];
     if (n > a.max_kvlen) {
@@ -203,104 +440,96 @@ __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const Compa
     }
     CacheGeom geom = a.geom;
     geom.layer_idx += layer;
+    float* weight = a.weight == nullptr ? nullptr : a.weight + (geom.layer_idx * a.num_kv_heads + head0) * a.max_tokens;
 
-    // cache rows of entry i: destination, and source (or -1: not to be moved)
-    auto rows_of = [&](int64_t i, int64_t& dst) -> int64_t {
-        const int64_t p = kept[i];
-        const int64_t before = i > 0 ? kept[i - 1] : -1;
-        if (p < 0) {
-            return -1;
-        }
-        if (base < 0 || p < i || (i > 0 && (before < 0 || p <= before)) || base + p >= n) {
-            atomicOr(a.status, kDevKeptInvalid);
-            return -1;
-        }
-        if (p == i) {
-            return -1;
-        }
-        const int64_t src = cache_row(geom, a.cachestarts, b, base + p);
-        dst = cache_row(geom, a.cachestarts, b, base + i);
-        if (!cache_row_ok(src, a.max_tokens) || !cache_row_ok(dst, a.max_tokens)) {
-            atomicOr(a.status, kDevRowOutOfRange);
-            return -1;
-        }
-        return src;
-    };
-
-    if (part < 2) {
-        const int64_t fixed = cache_offset(geom, 0, part, head);
-        for (int64_t first = 0; first < a.max_kept; first += kRows) {
-            uint4 v[kUnits];
-            uint8_t* to[kUnits];
-#pragma unroll
-            for (int u = 0; u < kUnits; ++u) {
-                const int unit = u * kCompactThreads + tid;
-                const int rr = unit / kRowUnits, piece = unit - rr * kRowUnits;
-                to[u] = nullptr;
-                if (rr < kRows && first + rr < a.max_kept) {
-                    int64_t dst = 0;
-                    const int64_t src = rows_of(first + rr, dst);
-                    if (src >= 0) {
-                        const int64_t so = fixed + src * geom.stride_s, d_o = fixed + dst * geom.stride_s;
-                        const uint8_t* from;
-                        if (piece < kCodeUnits) {
-                            from = reinterpret_cast<const uint8_t*>(a.cache + so) + piece * 16;
-                            to[u] = reinterpret_cast<uint8_t*>(a.cache + d_o) + piece * 16;
-                        } else {
-                            from = reinterpret_cast<const uint8_t*>(a.scale + (so >> 3)) + (piece - kCodeUnits) * 16;
-                            to[u] = reinterpret_cast<uint8_t*>(a.scale + (d_o >> 3)) + (piece - kCodeUnits) * 16;
-                        }
-                        v[u] = *reinterpret_cast<const uint4*>(from);
+    if (!clear) {
+        // cache rows of the segment's entries: source and destination, or -1: not to be moved
+        if (tid < a.rows_per_seg) {
+            const int64_t i = static_cast<int64_t>(seg) * a.rows_per_seg + tid;
+            int64_t src = -1, dst = -1;
+            const int64_t p = i < a.max_kept ? kept[i] : -1;
+            if (p >= 0) {
+                const int64_t before = i > 0 ? kept[i - 1] : -1;
+                if (base < 0 || p < i || (i > 0 && (before < 0 || p <= before)) || base + p >= n) {
+                    atomicOr(a.status, kDevKeptInvalid);
+                } else if (p != i) {
+                    src = cache_row(geom, a.cachestarts, b, base + p);
+                    dst = cache_row(geom, a.cachestarts, b, base + i);
+                    if (!cache_row_ok(src, a.max_tokens) || !cache_row_ok(dst, a.max_tokens)) {
+                        atomicOr(a.status, kDevRowOutOfRange);
+                        src = -1;
                     }
                 }
             }
-            const bool end = kept[first] < 0;
-            __syncthreads();  // every source of the block has been read
+            s_src[tid] = src;
+            s_dst[tid] = dst;
+        }
+        __syncthreads();
+        // unit = ((row * 2 + K | V) * heads + head) * pieces + piece: neighbouring threads, neighbouring bytes
+        uint4 v[kUnits];
+        int64_t to[kUnits];
+        const int units = a.rows_per_seg * 2 * a.heads_per_cta * kRowUnits;
 #pragma unroll
-            for (int u = 0; u < kUnits; ++u) {
-                if (to[u] != nullptr) {
-                    *reinterpret_cast<uint4*>(to[u]) = v[u];
+        for (int u = 0; u < kUnits; ++u) {
+            const int unit = u * kCompactThreads + tid;
+            to[u] = -1;
+            if (unit < units) {
+                const int piece = unit % kRowUnits, x = unit / kRowUnits;
+                const int head = x % a.heads_per_cta, y = x / a.heads_per_cta;
+                const int64_t src = s_src[y >> 1];
+                if (src >= 0) {
+                    const int64_t fixed = cache_offset(geom, 0, y & 1, head0 + head);
+                    const int64_t so = fixed + src * geom.stride_s, d_o = fixed + s_dst[y >> 1] * geom.stride_s;
+                    const bool code = piece < kCodeUnits;
+                    const uint8_t* from = code ? reinterpret_cast<const uint8_t*>(a.cache + so) + piece * 16
+                                               : reinterpret_cast<const uint8_t*>(a.scale + (so >> 3)) + (piece - kCodeUnits) * 16;
+                    to[u] = code ? d_o + piece * 16 : (d_o >> 3) * 2 + (piece - kCodeUnits) * 16;
+                    v[u] = *reinterpret_cast<const uint4*>(from);
                 }
             }
-            if (end) {
-                break;
+        }
+        float wv = 0.0f;
+        int64_t wto = -1;
+        if (weight != nullptr && tid < a.rows_per_seg * a.heads_per_cta) {
+            const int rr = tid % a.rows_per_seg, head = tid / a.rows_per_seg;
+            if (s_src[rr] >= 0) {
+                wv = weight[head * a.max_tokens + s_src[rr]];
+                wto = head * a.max_tokens + s_dst[rr];
             }
+        }
+        __syncthreads();  // every source of the segment has been read
+        if (tid == 0) {
+            __threadfence();
+            asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(a.flags + seg * a.lists + list), "r"(1u) : "memory");
+        }
+        bool ok = true;
+        for (int32_t e = tid; e < seg; e += kCompactThreads) {
+            ok = wait_flag(a.flags + e * a.lists + list) && ok;
+        }
+        if (!__syncthreads_and(ok)) {
+            if (tid == 0) {
+                atomicOr(a.status, kDevTmaTimeout);
+            }
+            return;
+        }
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            const int piece = (u * kCompactThreads + tid) % kRowUnits;
+            if (to[u] >= 0) {
+                uint8_t* dst = piece < kCodeUnits ? reinterpret_cast<uint8_t*>(a.cache) : reinterpret_cast<uint8_t*>(a.scale);
+                *reinterpret_cast<uint4*>(dst + to[u]) = v[u];
+            }
+        }
+        if (wto >= 0) {
+            weight[wto] = wv;
         }
         return;
     }
 
-    float* w = a.weight + ((a.geom.layer_idx + layer) * a.num_kv_heads + head) * a.max_tokens;
-    for (int64_t first = 0; first < a.max_kept; first += kCompactThreads * kUnits) {
-        float v[kUnits];
-        int64_t to[kUnits];
-#pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-            const int64_t i = first + u * kCompactThreads + tid;
-            to[u] = -1;
-            v[u] = 0.0f;
-            if (i < a.max_kept) {
-                int64_t dst = 0;
-                const int64_t src = rows_of(i, dst);
-                if (src >= 0) {
-                    v[u] = w[src];
-                    to[u] = dst;
-                }
-            }
-        }
-        const bool end = kept[first] < 0;
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-            if (to[u] >= 0) {
-                w[to[u]] = v[u];
-            }
-        }
-        if (end) {
-            break;
-        }
+    // the positions behind the kept ones hold no token any more: the next ones start from zero weight
+    if (base < 0) {
+        return;
     }
-    __syncthreads();
-    // the positions behind the kept ones hold no token any more: the next ones start from zero
     int64_t count = 0, top = a.max_kept;  // first negative entry
     while (count < top) {
         const int64_t mid = (count + top) >> 1;
@@ -310,15 +539,29 @@ __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const Compa
             top = mid;
         }
     }
-    if (base < 0) {
+    const int64_t from = base + count + static_cast<int64_t>(seg) * kClearRows;
+    const int64_t end = from + kClearRows < n ? from + kClearRows : n;
+    if (from >= end) {
         return;
     }
-    for (int64_t pos = base + count + tid; pos < n; pos += kCompactThreads) {
+    bool ok = true;
+    for (int32_t e = tid; e < a.segments; e += kCompactThreads) {
+        ok = wait_flag(a.flags + e * a.lists + list) && ok;
+    }
+    if (!__syncthreads_and(ok)) {
+        if (tid == 0) {
+            atomicOr(a.status, kDevTmaTimeout);
+        }
+        return;
+    }
+    for (int64_t pos = from + tid; pos < end; pos += kCompactThreads) {
         const int64_t row = cache_row(geom, a.cachestarts, b, pos);
-        if (cache_row_ok(row, a.max_tokens)) {
-            w[row] = 0.0f;
-        } else {
+        if (!cache_row_ok(row, a.max_tokens)) {
             atomicOr(a.status, kDevRowOutOfRange);
+            continue;
+        }
+        for (int head = 0; head < a.heads_per_cta; ++head) {
+            weight[head * a.max_tokens + row] = 0.0f;
         }
     }
 }
@@ -342,14 +585,60 @@ int launch_kv_evict_select(const pplb200_attn_params& p, const CacheGeom& geom, 
     a.max_kvlen = p.max_kvlen;
     a.max_tokens = p.max_tokens;
     a.num_kv_heads = p.num_kv_heads;
+    const int64_t words = (p.max_kvlen + 31) / 32;
+    a.mask_words = static_cast<int32_t>(words > kMaskWords ? kMaskWords : words);
+    a.list_cap = static_cast<int32_t>(p.max_kvlen > kListCap ? kListCap : p.max_kvlen);
     const dim3 grid(static_cast<unsigned>(p.num_kv_heads), static_cast<unsigned>(p.batch));
-    kv_evict_select_kernel<<<grid, kSelectThreads, 0, stream>>>(a);
+    const size_t bytes = 2 * (static_cast<size_t>(a.mask_words) + a.list_cap) * 4;
+    if (p.max_kvlen <= kShortList) {  // at most 33 KB of dynamic shared memory
+        kv_evict_select_kernel<kShortThreads><<<grid, kShortThreads, bytes, stream>>>(a);
+        return check_launch("kv_evict_select_kernel");
+    }
+    // the attribute belongs to the (kernel, device) pair
+    static bool attr_set[kMaxDevices] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
+        (void)cudaGetLastError();
+        return PPLB200_DEVICE_RUNTIME_ERROR;
+    }
+    if (!attr_set[dev]) {
+        if (cudaFuncSetAttribute(kv_evict_select_kernel<kSelectThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 2 * (kMaskWords + kListCap) * 4) != cudaSuccess) {
+            (void)cudaGetLastError();
+            return PPLB200_DEVICE_RUNTIME_ERROR;
+        }
+        attr_set[dev] = true;
+    }
+    kv_evict_select_kernel<kSelectThreads><<<grid, kSelectThreads, bytes, stream>>>(a);
     return check_launch("kv_evict_select_kernel");
 }
 
-int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const int64_t* kept, int64_t kept_heads,
-                      int64_t max_kept, const int64_t* base, const int64_t* kvlens, const int64_t* cachestarts,
-                      int64_t layers, void* cache, void* scale, float* weight, uint32_t* status, cudaStream_t stream) {
+int make_compact_plan(const pplb200_attn_params& p, int64_t kept_heads, int64_t max_kept, int64_t layers,
+                      CompactPlan* plan) {
+    // One list per kv head: a CTA takes 64 rows of it.  One list for all heads: as many rows times up to 8 heads, whose
+    // rows lie next to one another in the token-major layout, and short lists fill a CTA.
+    plan->heads_per_cta = 1;
+    if (kept_heads == 1) {
+        for (int h = 8; h > 1; h >>= 1) {
+            if (p.num_kv_heads % h == 0) {
+                plan->heads_per_cta = h;
+                break;
+            }
+        }
+    }
+    plan->rows_per_seg = kSegmentRows / plan->heads_per_cta;
+    plan->lists = p.batch * layers * (p.num_kv_heads / plan->heads_per_cta);
+    plan->segments = (max_kept + plan->rows_per_seg - 1) / plan->rows_per_seg;
+    plan->off_flags = 256;  // behind the status word and the ticket counter
+    plan->bytes = plan->off_flags + (static_cast<uint64_t>(plan->segments) * plan->lists * 4 + 255) / 256 * 256;
+    const int64_t clears = (p.max_kvlen + kClearRows - 1) / kClearRows;
+    return (plan->segments + clears) * plan->lists > 0x7fffffff ? PPLB200_UNSUPPORTED : PPLB200_SUCCESS;
+}
+
+int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const CompactPlan& plan, const int64_t* kept,
+                      int64_t kept_heads, int64_t max_kept, const int64_t* base, const int64_t* kvlens,
+                      const int64_t* cachestarts, int64_t layers, void* cache, void* scale, float* weight,
+                      void* workspace, cudaStream_t stream) {
     CompactArgs a = {};
     a.kept = kept;
     a.base = base;
@@ -358,17 +647,30 @@ int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const
     a.cache = static_cast<int8_t*>(cache);
     a.scale = static_cast<__half*>(scale);
     a.weight = weight;
-    a.status = status;
+    a.status = static_cast<uint32_t*>(workspace);
+    a.ticket = a.status + 1;
+    a.flags = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + plan.off_flags);
     a.geom = geom;
     a.max_kept = max_kept;
     a.max_kvlen = p.max_kvlen;
     a.max_tokens = p.max_tokens;
+    a.lists = plan.lists;
+    a.move_tasks = plan.segments * plan.lists;
     a.kept_heads = static_cast<int32_t>(kept_heads);
     a.num_kv_heads = p.num_kv_heads;
     a.layers = static_cast<int32_t>(layers);
-    const int64_t ctas = p.batch * layers * p.num_kv_heads * (weight != nullptr ? 3 : 2);
-    if (ctas > 0x7fffffff) {
-        return PPLB200_UNSUPPORTED;
+    a.heads_per_cta = plan.heads_per_cta;
+    a.head_groups = p.num_kv_heads / plan.heads_per_cta;
+    a.rows_per_seg = plan.rows_per_seg;
+    a.segments = static_cast<int32_t>(plan.segments);
+    if (cudaMemsetAsync(workspace, 0, plan.bytes, stream) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return PPLB200_DEVICE_RUNTIME_ERROR;
+    }
+    const int64_t clears = weight == nullptr ? 0 : (p.max_kvlen + kClearRows - 1) / kClearRows;
+    const int64_t ctas = (plan.segments + clears) * plan.lists;
+    if (ctas <= 0) {
+        return PPLB200_SUCCESS;
     }
     auto kernel = p.head_dim == 128 ? kv_compact_kernel<128> : kv_compact_kernel<64>;
     kernel<<<static_cast<unsigned>(ctas), kCompactThreads, 0, stream>>>(a);

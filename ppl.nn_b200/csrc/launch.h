@@ -148,9 +148,17 @@ int launch_kv_evict_select(const pplb200_attn_params& p, const CacheGeom& geom, 
                            const int64_t* cachestarts, const int64_t* kvlens, const int64_t* budgets, int64_t sink,
                            int64_t recent, int64_t max_budget, uint32_t* status, int64_t* kept, cudaStream_t stream);
 
-int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const int64_t* kept, int64_t kept_heads,
-                      int64_t max_kept, const int64_t* base, const int64_t* kvlens, const int64_t* cachestarts,
-                      int64_t layers, void* cache, void* scale, float* weight, uint32_t* status, cudaStream_t stream);
+struct CompactPlan {
+    int32_t heads_per_cta, rows_per_seg;
+    int64_t lists, segments;
+    uint64_t off_flags, bytes;
+};
+int make_compact_plan(const pplb200_attn_params& p, int64_t kept_heads, int64_t max_kept, int64_t layers,
+                      CompactPlan* plan);
+int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const CompactPlan& plan, const int64_t* kept,
+                      int64_t kept_heads, int64_t max_kept, const int64_t* base, const int64_t* kvlens,
+                      const int64_t* cachestarts, int64_t layers, void* cache, void* scale, float* weight,
+                      void* workspace, cudaStream_t stream);
 
 // Rotary position embedding, alone (append == nullptr) or fused with the cache append.
 uint64_t rope_workspace_bytes(const pplb200_rope_params& p);

@@ -606,6 +606,7 @@ class KeyValueCacheCompact(_CacheOp):
                 raise OpError("RC_INVALID_VALUE", "weight does not have the shape of the cache")
         p = self._params(num_heads=heads, num_kv_heads=heads, head_dim=dim, batch=batch, max_kvlen=max_kvlen,
                          max_tokens=max_tokens, cachestarts=cachestarts)
-        self._call("pplb200_kv_compact", self.lib.kv_compact_workspace_size, self.lib.kv_compact, p, cache.device,
+        size = lambda q: self.lib.kv_compact_workspace_size(q, kept.shape[1], kept.shape[2], num_layers)  # noqa: E731
+        self._call("pplb200_kv_compact", size, self.lib.kv_compact, p, cache.device,
                    _ptr(kept), kept.shape[1], kept.shape[2], _ptr(base), _ptr(kvlens), _ptr(cachestarts), num_layers,
                    _ptr(cache), _ptr(scale), _ptr(weight))

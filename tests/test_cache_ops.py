@@ -152,8 +152,13 @@ def test_empty_calls_and_missing_device(built_lib, pkg):
 
 def test_workspace_sizes(built_lib, pkg):
     from ppl_nn_b200 import capi
-    for size in (built_lib.kv_evict_workspace_size, built_lib.kv_compact_workspace_size):
-        assert size(_params(built_lib, capi)) == (capi.SUCCESS, 256)
+    assert built_lib.kv_evict_workspace_size(_params(built_lib, capi)) == (capi.SUCCESS, 256)
+    sizes = [built_lib.kv_compact_workspace_size(_params(built_lib, capi), heads, most, layers)
+             for heads, most, layers in ((1, 0, 1), (1, 8, 1), (8, 64, 1), (8, 640, 3))]
+    assert all(rc == capi.SUCCESS and n % 256 == 0 for rc, n in sizes)
+    assert [n for _, n in sizes] == sorted(n for _, n in sizes)
+    rc, _ = built_lib.kv_compact_workspace_size(_params(built_lib, capi), 3, 8, 1)
+    assert built_lib.status_str(rc) == "RC_INVALID_VALUE"
     rc, n = built_lib.attn_weight_workspace_size(_params(built_lib, capi))
     assert rc == capi.SUCCESS and n % 256 == 0 and n > 8 * 8 * 32
     rc, more = built_lib.attn_weight_workspace_size(_params(built_lib, capi, max_kvlen=60000))
