@@ -31,10 +31,11 @@ namespace {
 // numbers, four times as many CTAs of a quarter of the threads.
 constexpr int kSelectThreads = 1024;
 constexpr int kShortThreads = 256;
-constexpr int kShortList = 4096;
+constexpr int kShortList = 2048;
 constexpr int kListCap = 12288;    // keys inside the bracket
 constexpr int kSample = 4096;
 constexpr int kMaskWords = 8192;   // 262144 positions
+constexpr int kAhead = 8;          // weights per thread of a stage, of which two are on their way
 
 // Unsigned key with the order of the weights: -0 counts as +0, NaN as the lowest.
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -43,6 +44,26 @@ __device__ __forceinline__ uint32_t order_key(float w) {
     }
     const uint32_t u = __float_as_uint(w + 0.0f);  // -0 + 0 = +0
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// The weight of a key (of a number, not of the NaN key 0)
+__device__ __forceinline__ float key_weight(uint32_t key) {
+    return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
+}
+
+// 4-byte asynchronous copy global -> shared
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int PENDING>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
 struct SelectArgs {
@@ -154,6 +175,7 @@ __global__ void __launch_bounds__(NT) kv_evict_select_kernel(const SelectArgs a)
     uint32_t* tie = mask + a.mask_words;       // has the key of the last one taken
     uint32_t* list_key = tie + a.mask_words;
     int32_t* list_pos = reinterpret_cast<int32_t*>(list_key + a.list_cap);
+    float* ring = reinterpret_cast<float*>(list_pos + a.list_cap);  // [2][kAhead][NT]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t b = blockIdx.y;
     const int head = blockIdx.x;
@@ -176,11 +198,14 @@ __global__ void __launch_bounds__(NT) kv_evict_select_kernel(const SelectArgs a)
     int64_t* out = a.kept + (b * a.num_kv_heads + head) * a.max_budget;
 
     const int64_t first_row = a.geom.cache_mode == 0 ? a.cachestarts[b] : 0;
-    auto key_at = [&](int32_t pos) -> uint32_t {
-        int64_t row = first_row < 0 ? -1 : first_row + pos;
+    auto row_at = [&](int32_t pos) -> int64_t {
         if (a.geom.cache_mode != 0) {
-            row = cache_row(a.geom, a.cachestarts, b, pos);
+            return cache_row(a.geom, a.cachestarts, b, pos);
         }
+        return first_row < 0 ? -1 : first_row + pos;
+    };
+    auto key_at = [&](int32_t pos) -> uint32_t {
+        const int64_t row = row_at(pos);
         if (!cache_row_ok(row, a.max_tokens)) {
             atomicOr(a.status, kDevRowOutOfRange);
             return 0u;
@@ -201,13 +226,12 @@ __global__ void __launch_bounds__(NT) kv_evict_select_kernel(const SelectArgs a)
     bool done = !choose;
     if (fits) {
         for (int32_t i = tid; i < words; i += NT) {
-            // sinks and recent positions; all of them, or nothing else, where there is no choice to make
-            uint32_t m = 0;
-#pragma unroll 4
-            for (int e = 0; e < 32; ++e) {
-                const int32_t pos = i * 32 + e;
-                m |= (pos < n && (pos < lo || pos >= hi || (!choose && want > 0))) ? 1u << e : 0u;
-            }
+            // sinks and recent positions; all of them where there is no choice to make
+            const int32_t p0 = i * 32;
+            const uint32_t exist = n - p0 >= 32 ? ~0u : (1u << (n - p0)) - 1u;
+            const int32_t c0 = lo - p0 < 0 ? 0 : (lo - p0 > 32 ? 32 : lo - p0), c1 = hi - p0 < c0 ? c0 : (hi - p0 > 32 ? 32 : hi - p0);
+            const uint32_t from = c0 == 32 ? 0u : ~0u << c0, to = c1 == 32 ? ~0u : (1u << c1) - 1u;  // candidates: both
+            const uint32_t m = !choose && want > 0 ? exist : exist & ~(from & to);
             mask[i] = m;
             tie[i] = 0;
         }
@@ -242,39 +266,85 @@ __global__ void __launch_bounds__(NT) kv_evict_select_kernel(const SelectArgs a)
             sh.above = 0;
         }
         __syncthreads();
-        constexpr int kAhead = 4;
+        // A warp takes 32 consecutive positions at a time; each thread copies its own weights, kAhead a stage, and no
+        // one else reads them, so the stages need no barrier.
+        const float high_w = high == 0xffffffffu ? INFINITY : key_weight(high);
+        const float low_w = low == 0u ? -INFINITY : key_weight(low);
+        const bool list_all = low == 0u;
         uint32_t above = 0;
-        for (int32_t base = (lo & ~31) + warp * 32; base < hi; base += NT * kAhead) {
-            uint32_t key[kAhead];
+        const int32_t first = (lo & ~31) + tid, step = NT * kAhead;
+        const uint32_t mine = smem_u32(ring + tid);
+        const bool plain = a.geom.cache_mode == 0 && first_row >= 0 && first_row + hi <= a.max_tokens;
+        const float* src = w + first_row;  // used where plain
+        auto fetch = [&](int stage, int32_t pos0) {
+            if (plain && pos0 - lane >= lo && pos0 - lane + (kAhead - 1) * NT + 32 <= hi) {
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const int32_t pos = base + i * NT + lane;
-                key[i] = pos >= lo && pos < hi ? key_at(pos) : 0u;
+                for (int i = 0; i < kAhead; ++i) {
+                    cp_async4(mine + static_cast<uint32_t>(stage * kAhead + i) * (NT * 4), src + pos0 + i * NT);
+                }
+                cp_async_commit();
+                return;
             }
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-                const int32_t pos = base + i * NT + lane;
-                const bool in = pos >= lo && pos < hi;
-                const uint32_t up = __ballot_sync(0xffffffffu, in && key[i] > high);
-                const bool listed = in && key[i] >= low && key[i] <= high;
-                const uint32_t mid = __ballot_sync(0xffffffffu, listed);
-                if (up != 0u && lane == 0) {
-                    mask[pos >> 5] |= up;  // this warp alone owns the word
+                const int32_t pos = pos0 + i * NT;
+                if (pos >= lo && pos < hi) {
+                    const int64_t row = row_at(pos);
+                    const uint32_t at = mine + static_cast<uint32_t>(stage * kAhead + i) * (NT * 4);
+                    if (cache_row_ok(row, a.max_tokens)) {
+                        cp_async4(at, w + row);
+                    } else {
+                        atomicOr(a.status, kDevRowOutOfRange);
+                        ring[(stage * kAhead + i) * NT + tid] = __uint_as_float(0x7fffffffu);  // counts as a NaN
+                    }
                 }
-                above += __popc(up);
-                if (mid != 0u) {
-                    uint32_t at = 0;
-                    if (lane == 0) {
-                        at = atomicAdd(&sh.listed, __popc(mid));
+            }
+            cp_async_commit();
+        };
+        fetch(0, first);
+        int stage = 0;
+        for (int32_t pos0 = first; pos0 - lane < hi; pos0 += step, stage ^= 1) {
+            fetch(stage ^ 1, pos0 + step);
+            cp_async_wait<1>();
+            uint32_t mid[kAhead], count = 0, in_list = 0, my_up = 0;
+            float x[kAhead];
+            const bool inner = pos0 - lane >= lo && pos0 - lane + (kAhead - 1) * NT + 32 <= hi;  // all of the stage
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int32_t pos = pos0 + i * NT;
+                const bool in = inner || (pos >= lo && pos < hi);
+                x[i] = in ? ring[(stage * kAhead + i) * NT + tid] : 0.0f;
+                const bool up_here = in && x[i] > high_w;
+                const bool listed = in && !up_here && (list_all || x[i] >= low_w);
+                const uint32_t up = __ballot_sync(0xffffffffu, up_here);
+                mid[i] = __ballot_sync(0xffffffffu, listed);
+                my_up = lane == i ? up : my_up;
+                count += __popc(mid[i]);
+                in_list |= (listed ? 1u : 0u) << i;
+            }
+            if (my_up != 0u) {  // lanes 0 .. kAhead - 1 hold a word each; this warp alone owns them
+                mask[(pos0 >> 5) + lane * (NT / 32)] |= my_up;
+                above += __popc(my_up);
+            }
+            if (count != 0u) {
+                uint32_t at = 0;
+                if (lane == 0) {
+                    at = atomicAdd(&sh.listed, count);
+                }
+                at = __shfl_sync(0xffffffffu, at, 0);
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    const uint32_t slot = at + __popc(mid[i] & ((1u << lane) - 1u));
+                    if (((in_list >> i) & 1u) != 0u && slot < static_cast<uint32_t>(a.list_cap)) {
+                        list_key[slot] = order_key(x[i]);
+                        list_pos[slot] = pos0 + i * NT;
                     }
-                    at = __shfl_sync(0xffffffffu, at, 0) + __popc(mid & ((1u << lane) - 1u));
-                    if (listed && at < static_cast<uint32_t>(a.list_cap)) {
-                        list_key[at] = key[i];
-                        list_pos[at] = pos;
-                    }
+                    at += __popc(mid[i]);
                 }
             }
         }
+        cp_async_wait<0>();
+        above = warp_total(above);
         if (lane == 0) {
             atomicAdd(&sh.above, above);
         }
@@ -350,20 +420,60 @@ __global__ void __launch_bounds__(NT) kv_evict_select_kernel(const SelectArgs a)
     uint32_t ties_before = sum_before(sh, ties, total);
     const uint32_t ties_taken = ties_before >= equal ? 0u : (equal - ties_before < ties ? equal - ties_before : ties);
     uint32_t rank = sum_before(sh, sure + ties_taken, total);
-    for (int32_t i = w0; i < w1; ++i) {
-        uint32_t t;
-        uint32_t m = word_at(i, t);
-        if (t != 0u) {
-            const uint32_t mine = __popc(t & ((1u << lane) - 1u));
-            const bool take = ((t >> lane) & 1u) != 0u && ties_before + mine < equal;
-            m |= __ballot_sync(0xffffffffu, take);
-            ties_before += __popc(t);
+    // the word of the positions kept among 32: the sure ones and the first of the ties, up to `equal` in the list
+    auto with_ties = [&](uint32_t m, uint32_t t) -> uint32_t {
+        while (t != 0u && ties_before < equal) {
+            m |= t & (0u - t);
+            t &= t - 1u;
+            ++ties_before;
         }
-        const uint32_t at = rank + __popc(m & ((1u << lane) - 1u));
-        if (((m >> lane) & 1u) != 0u && at < static_cast<uint32_t>(k)) {
-            out[at] = i * 32 + lane;
+        return m;
+    };
+    if (fits && k < n / 8) {
+        // few bits a word: a lane takes a word and writes its positions one after the other
+        for (int32_t i0 = w0; i0 < w1; i0 += 32) {
+            const int32_t i = i0 + lane;
+            uint32_t m = i < w1 ? mask[i] : 0u;
+            const uint32_t t = i < w1 ? tie[i] : 0u;
+            if (__any_sync(0xffffffffu, t != 0u)) {
+                uint32_t incl = __popc(t);
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+                    incl += lane >= o ? y : 0u;
+                }
+                const uint32_t all = __shfl_sync(0xffffffffu, incl, 31), before = ties_before;
+                ties_before = before + incl - __popc(t);
+                m = with_ties(m, t);
+                ties_before = before + all;
+            }
+            uint32_t incl = __popc(m);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+                incl += lane >= o ? y : 0u;
+            }
+            uint32_t at = rank + incl - __popc(m);
+            rank += __shfl_sync(0xffffffffu, incl, 31);
+            while (m != 0u) {
+                if (at < static_cast<uint32_t>(k)) {
+                    out[at] = i * 32 + __ffs(m) - 1;
+                }
+                m &= m - 1u;
+                ++at;
+            }
         }
-        rank += __popc(m);
+    } else {
+        for (int32_t i = w0; i < w1; ++i) {
+            uint32_t t;
+            uint32_t m = word_at(i, t);
+            m = with_ties(m, t);
+            const uint32_t at = rank + __popc(m & ((1u << lane) - 1u));
+            if (((m >> lane) & 1u) != 0u && at < static_cast<uint32_t>(k)) {
+                out[at] = i * 32 + lane;
+            }
+            rank += __popc(m);
+        }
     }
     for (int64_t i = k + tid; i < a.max_budget; i += NT) {
         out[i] = -1;
@@ -385,10 +495,11 @@ struct CompactArgs {
     uint32_t* flags;  // [segments][lists]
     CacheGeom geom;
     int64_t max_kept, max_kvlen, max_tokens;
-    int64_t lists;       // batch * layers * head groups
-    int64_t move_tasks;  // segments * lists
-    int32_t kept_heads, num_kv_heads, layers;
-    int32_t heads_per_cta, head_groups, rows_per_seg, segments;
+    uint32_t lists;       // batch * layers * head groups
+    uint32_t move_tasks;  // segments * lists
+    int32_t kept_heads, num_kv_heads;
+    uint32_t layers, head_groups;
+    int32_t heads_shift, rows_per_seg, segments;  // 1 << heads_shift heads per CTA
 };
 
 constexpr int kCompactThreads = 256;
@@ -411,23 +522,26 @@ __device__ __forceinline__ bool wait_flag(const uint32_t* flag) {
 }
 
 template <int DH>
-__global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const CompactArgs a) {
-    constexpr int kCodeUnits = DH / 16;              // 16-byte pieces of a row's codes
-    constexpr int kRowUnits = kCodeUnits + DH / 64;  // and of its scales
-    constexpr int kUnits = (kSegmentRows * 2 * kRowUnits + kCompactThreads - 1) / kCompactThreads;
+__global__ void __launch_bounds__(kCompactThreads, 8) kv_compact_kernel(const CompactArgs a) {
+    constexpr int kCodePieces = DH / 16;   // 16-byte pieces of a row's codes
+    constexpr int kScalePieces = DH / 64;  // and of its scales
+    constexpr int kCodeStep = kCompactThreads / kCodePieces;  // rows (of K or V of a head) the CTA moves at once
+    constexpr int kCodeSteps = 2 * kSegmentRows / kCodeStep;
     __shared__ uint32_t s_ticket;
     __shared__ int64_t s_src[kSegmentRows], s_dst[kSegmentRows];
+    __shared__ int2 s_row[kSegmentRows];
+    __shared__ uint4 stage[(kCodeSteps + 1) * kCompactThreads];
     const int tid = threadIdx.x;
     if (tid == 0) {
         s_ticket = atomicAdd(a.ticket, 1u);
     }
     __syncthreads();
-    const int64_t task = s_ticket;
-    const bool clear = task >= a.move_tasks;
-    const int64_t list = (clear ? task - a.move_tasks : task) % a.lists;
-    const int32_t seg = static_cast<int32_t>((clear ? task - a.move_tasks : task) / a.lists);
-    const int head0 = static_cast<int>(list % a.head_groups) * a.heads_per_cta;
-    const int layer = static_cast<int>(list / a.head_groups % a.layers);
+    const bool clear = s_ticket >= a.move_tasks;  // tasks and lists fit 31 bits
+    const uint32_t task = clear ? s_ticket - a.move_tasks : s_ticket;
+    const uint32_t lists = a.lists, list = task % lists;
+    const int32_t seg = task / lists;
+    const int head0 = static_cast<int>(list % a.head_groups) << a.heads_shift;
+    const int layer = list / a.head_groups % a.layers;
     const int64_t b = list / a.head_groups / a.layers;
     const int64_t* kept = a.kept + (b * a.kept_heads + (a.kept_heads > 1 ? head0 : 0)) * a.max_kept;
     const int64_t base = a.base[b];
@@ -461,50 +575,53 @@ __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const Compa
                     }
                 }
             }
-            s_src[tid] = src;
-            s_dst[tid] = dst;
+            // element offsets of K of the first head
+            const int64_t fixed = geom.layer_idx * geom.stride_l + head0 * geom.stride_h;
+            s_src[tid] = src < 0 ? -1 : src * geom.stride_s + fixed;
+            s_dst[tid] = dst * geom.stride_s + fixed;
+            s_row[tid] = make_int2(static_cast<int>(src), static_cast<int>(dst));
         }
         __syncthreads();
-        // unit = ((row * 2 + K | V) * heads + head) * pieces + piece: neighbouring threads, neighbouring bytes
-        uint4 v[kUnits];
-        int64_t to[kUnits];
-        const int units = a.rows_per_seg * 2 * a.heads_per_cta * kRowUnits;
+        // x = (row * 2 + K | V) * heads + head, and pieces of it by neighbouring threads: neighbouring bytes.  A thread
+        // stages its own pieces in shared memory, which keeps the bytes in flight out of the registers.
+        const int shift = a.heads_shift, count = a.rows_per_seg * 2 << shift;
+        auto offset = [&](const int64_t* rows, int x) -> int64_t {  // of a row of K or V of a head, or negative
+            const int y = x >> shift;
+            const int64_t row = rows[y >> 1];
+            return row < 0 ? -1 : row + (y & 1) * geom.stride_kv + (x & ((1 << shift) - 1)) * geom.stride_h;
+        };
+        const int cx = tid / kCodePieces, cp = tid % kCodePieces * 16, sx = tid / kScalePieces, sp = tid % kScalePieces * 8;
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-            const int unit = u * kCompactThreads + tid;
-            to[u] = -1;
-            if (unit < units) {
-                const int piece = unit % kRowUnits, x = unit / kRowUnits;
-                const int head = x % a.heads_per_cta, y = x / a.heads_per_cta;
-                const int64_t src = s_src[y >> 1];
-                if (src >= 0) {
-                    const int64_t fixed = cache_offset(geom, 0, y & 1, head0 + head);
-                    const int64_t so = fixed + src * geom.stride_s, d_o = fixed + s_dst[y >> 1] * geom.stride_s;
-                    const bool code = piece < kCodeUnits;
-                    const uint8_t* from = code ? reinterpret_cast<const uint8_t*>(a.cache + so) + piece * 16
-                                               : reinterpret_cast<const uint8_t*>(a.scale + (so >> 3)) + (piece - kCodeUnits) * 16;
-                    to[u] = code ? d_o + piece * 16 : (d_o >> 3) * 2 + (piece - kCodeUnits) * 16;
-                    v[u] = *reinterpret_cast<const uint4*>(from);
-                }
+        for (int u = 0; u < kCodeSteps; ++u) {
+            const int x = u * kCodeStep + cx;
+            const int64_t off = x < count ? offset(s_src, x) : -1;
+            if (off >= 0) {
+                cp_async16(smem_u32(&stage[u * kCompactThreads + tid]), a.cache + off + cp);
             }
+        }
+        const int64_t scale_off = sx < count ? offset(s_src, sx) : -1;
+        if (scale_off >= 0) {
+            cp_async16(smem_u32(&stage[kCodeSteps * kCompactThreads + tid]), a.scale + (scale_off >> 3) + sp);
         }
         float wv = 0.0f;
         int64_t wto = -1;
-        if (weight != nullptr && tid < a.rows_per_seg * a.heads_per_cta) {
-            const int rr = tid % a.rows_per_seg, head = tid / a.rows_per_seg;
+        if (weight != nullptr && tid < a.rows_per_seg << shift) {
+            const int rr = tid >> shift, head = tid & ((1 << shift) - 1);
             if (s_src[rr] >= 0) {
-                wv = weight[head * a.max_tokens + s_src[rr]];
-                wto = head * a.max_tokens + s_dst[rr];
+                wv = weight[head * a.max_tokens + s_row[rr].x];
+                wto = head * a.max_tokens + s_row[rr].y;
             }
         }
+        cp_async_commit();
+        cp_async_wait<0>();
         __syncthreads();  // every source of the segment has been read
         if (tid == 0) {
             __threadfence();
-            asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(a.flags + seg * a.lists + list), "r"(1u) : "memory");
+            asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(a.flags + static_cast<int64_t>(seg) * lists + list), "r"(1u) : "memory");
         }
         bool ok = true;
         for (int32_t e = tid; e < seg; e += kCompactThreads) {
-            ok = wait_flag(a.flags + e * a.lists + list) && ok;
+            ok = wait_flag(a.flags + static_cast<int64_t>(e) * lists + list) && ok;
         }
         if (!__syncthreads_and(ok)) {
             if (tid == 0) {
@@ -513,12 +630,14 @@ __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const Compa
             return;
         }
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-            const int piece = (u * kCompactThreads + tid) % kRowUnits;
-            if (to[u] >= 0) {
-                uint8_t* dst = piece < kCodeUnits ? reinterpret_cast<uint8_t*>(a.cache) : reinterpret_cast<uint8_t*>(a.scale);
-                *reinterpret_cast<uint4*>(dst + to[u]) = v[u];
+        for (int u = 0; u < kCodeSteps; ++u) {
+            const int x = u * kCodeStep + cx;
+            if (x < count && s_src[x >> shift >> 1] >= 0) {
+                *reinterpret_cast<uint4*>(a.cache + offset(s_dst, x) + cp) = stage[u * kCompactThreads + tid];
             }
+        }
+        if (scale_off >= 0) {
+            *reinterpret_cast<uint4*>(a.scale + (offset(s_dst, sx) >> 3) + sp) = stage[kCodeSteps * kCompactThreads + tid];
         }
         if (wto >= 0) {
             weight[wto] = wv;
@@ -546,7 +665,7 @@ __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const Compa
     }
     bool ok = true;
     for (int32_t e = tid; e < a.segments; e += kCompactThreads) {
-        ok = wait_flag(a.flags + e * a.lists + list) && ok;
+        ok = wait_flag(a.flags + static_cast<int64_t>(e) * lists + list) && ok;
     }
     if (!__syncthreads_and(ok)) {
         if (tid == 0) {
@@ -560,7 +679,7 @@ __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const Compa
             atomicOr(a.status, kDevRowOutOfRange);
             continue;
         }
-        for (int head = 0; head < a.heads_per_cta; ++head) {
+        for (int head = 0; head < 1 << a.heads_shift; ++head) {
             weight[head * a.max_tokens + row] = 0.0f;
         }
     }
@@ -589,9 +708,12 @@ int launch_kv_evict_select(const pplb200_attn_params& p, const CacheGeom& geom, 
     a.mask_words = static_cast<int32_t>(words > kMaskWords ? kMaskWords : words);
     a.list_cap = static_cast<int32_t>(p.max_kvlen > kListCap ? kListCap : p.max_kvlen);
     const dim3 grid(static_cast<unsigned>(p.num_kv_heads), static_cast<unsigned>(p.batch));
-    const size_t bytes = 2 * (static_cast<size_t>(a.mask_words) + a.list_cap) * 4;
-    if (p.max_kvlen <= kShortList) {  // at most 33 KB of dynamic shared memory
-        kv_evict_select_kernel<kShortThreads><<<grid, kShortThreads, bytes, stream>>>(a);
+    const size_t fixed = 2 * (static_cast<size_t>(a.mask_words) + a.list_cap) * 4;
+    const size_t bytes = fixed + 2 * kAhead * kSelectThreads * 4;
+    if (p.max_kvlen <= kShortList) {
+        // at most 48 KB of dynamic shared memory, what a kernel may have without asking
+        static_assert(2 * (kShortList / 32 + kShortList) * 4 + 2 * kAhead * kShortThreads * 4 <= 47104, "short lists");
+        kv_evict_select_kernel<kShortThreads><<<grid, kShortThreads, fixed + 2 * kAhead * kShortThreads * 4, stream>>>(a);
         return check_launch("kv_evict_select_kernel");
     }
     // the attribute belongs to the (kernel, device) pair
@@ -603,7 +725,7 @@ int launch_kv_evict_select(const pplb200_attn_params& p, const CacheGeom& geom, 
     }
     if (!attr_set[dev]) {
         if (cudaFuncSetAttribute(kv_evict_select_kernel<kSelectThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 2 * (kMaskWords + kListCap) * 4) != cudaSuccess) {
+                                 2 * (kMaskWords + kListCap) * 4 + 2 * kAhead * kSelectThreads * 4) != cudaSuccess) {
             (void)cudaGetLastError();
             return PPLB200_DEVICE_RUNTIME_ERROR;
         }
@@ -654,12 +776,14 @@ int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const
     a.max_kept = max_kept;
     a.max_kvlen = p.max_kvlen;
     a.max_tokens = p.max_tokens;
-    a.lists = plan.lists;
-    a.move_tasks = plan.segments * plan.lists;
+    a.lists = static_cast<uint32_t>(plan.lists);
+    a.move_tasks = static_cast<uint32_t>(plan.segments * plan.lists);
     a.kept_heads = static_cast<int32_t>(kept_heads);
     a.num_kv_heads = p.num_kv_heads;
-    a.layers = static_cast<int32_t>(layers);
-    a.heads_per_cta = plan.heads_per_cta;
+    a.layers = static_cast<uint32_t>(layers);
+    while (1 << a.heads_shift < plan.heads_per_cta) {
+        ++a.heads_shift;
+    }
     a.head_groups = p.num_kv_heads / plan.heads_per_cta;
     a.rows_per_seg = plan.rows_per_seg;
     a.segments = static_cast<int32_t>(plan.segments);
