@@ -1,9 +1,11 @@
 // Accumulated attention weight: w[row(j)] += sum over the query heads of a kv group and over the query tokens of
 // softmax_j(q . k_j / sqrt(Dh)), for every cached position j of every sequence.  Only K is read.
 //
-// The normaliser of a row needs all its scores, so the scores are formed twice: attn_weight_stats_kernel leaves, per
-// query row and chunk of positions, the maximum and the sum of exponentials; attn_weight_merge_kernel joins the
-// chunks; attn_weight_apply_kernel forms the scores again and adds each position's normalised weights up.
+// The normaliser of a row needs all its scores before any weight is known.  attn_weight_stats_kernel leaves, per query
+// row and chunk of positions, the maximum and the sum of exponentials, and attn_weight_merge_kernel joins the chunks.
+// Then, with up to 8 query rows per kv head (decode steps), the scores themselves have been written to the workspace
+// (4 bytes a row against the 160 of a K row at Dh 128) and attn_weight_spread_kernel only reads those; with more rows
+// attn_weight_apply_kernel forms them again and adds each position's normalised weights up.
 //
 // Both score kernels: a CTA takes a chunk of the positions of one (sequence, kv head), a warp 16 positions at a
 // time.  Positions are the M dimension of mma.m16n8k16, the query rows (token x head of the group) come in octets as
@@ -24,6 +26,7 @@ constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kChunk = 512;     // positions of a CTA
 constexpr int kRowBlock = 32;   // query rows whose fragments are held in registers at a time
+constexpr int kScoreRows = 8;   // up to so many query rows per kv head the scores are kept
 constexpr float kNegBig = -1.0e30f;
 
 struct WeightArgs {
@@ -36,6 +39,8 @@ struct WeightArgs {
     float* weight;   // [L, Hkv, MaxT]
     float2* part;    // [chunks][T][Hq]: maximum (exp2 domain) and sum
     float2* norm;    // [T][Hq]: maximum and reciprocal sum
+    float* score;    // [batch][Hkv][max_kvlen][kScoreRows or fewer]: raw scores, -inf where hidden, or null
+    int32_t score_rows;
     uint32_t* status;
     CacheGeom geom;
     int64_t max_seqlen, max_kvlen, max_tokens, total_tokens;
@@ -192,7 +197,7 @@ __global__ void __launch_bounds__(kThreads) attn_weight_stats_kernel(const Weigh
     __shared__ float2 red[kWarps][NOCT * 8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t b = blockIdx.z;
-    const int head = blockIdx.y, chunk = blockIdx.x;
+    const int head = blockIdx.x, chunk = blockIdx.y;  // neighbouring CTAs read neighbouring heads of the same rows
     const Span s = span_of(a, b);
     const int32_t first = chunk * kChunk;
     if (first >= s.len) {
@@ -211,14 +216,31 @@ __global__ void __launch_bounds__(kThreads) attn_weight_stats_kernel(const Weigh
                 l[o][c] = 0.0f;
             }
         }
+        Tile<DH, NOCT> next;
+        int64_t row;
+        next.load(a, b, head, first + warp * 16, s.len, lane, row);
         for (int32_t tile0 = first + warp * 16; tile0 < end; tile0 += kWarps * 16) {
-            Tile<DH, NOCT> tile;
-            int64_t row;
-            tile.load(a, b, head, tile0, s.len, lane, row);
+            const Tile<DH, NOCT> tile = next;
+            if (tile0 + kWarps * 16 < end) {
+                next.load(a, b, head, tile0 + kWarps * 16, s.len, lane, row);
+            }
             float acc[NOCT][4];
             tile.scores(qf, acc);
             if (tile0 + 15 > s.start || tile0 + 15 >= s.len) {
                 hide<NOCT>(a, s, row0, tile0, lane, acc);
+            }
+            if constexpr (NOCT == 1) {
+                const int g = lane >> 2, t = lane & 3;
+                float* dst = a.score + ((b * a.num_kv_heads + head) * a.max_kvlen + tile0 + g) * a.score_rows + 2 * t;
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        if (2 * t + c < s.rows && tile0 + g + 8 * p < s.len) {
+                            dst[p * 8 * a.score_rows + c] = acc[0][2 * p + c];
+                        }
+                    }
+                }
             }
 #pragma unroll
             for (int o = 0; o < NOCT; ++o) {
@@ -318,7 +340,7 @@ __global__ void __launch_bounds__(kThreads) attn_weight_apply_kernel(const Weigh
     __shared__ float sum[kChunk];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int64_t b = blockIdx.z;
-    const int head = blockIdx.y, chunk = blockIdx.x;
+    const int head = blockIdx.x, chunk = blockIdx.y;  // neighbouring CTAs read neighbouring heads of the same rows
     const Span s = span_of(a, b);
     const int32_t first = chunk * kChunk;
     if (first >= s.len) {
@@ -389,12 +411,47 @@ __global__ void __launch_bounds__(kThreads) attn_weight_apply_kernel(const Weigh
     }
 }
 
+// One thread per position: the weights of the kept scores.
+__global__ void __launch_bounds__(256) attn_weight_spread_kernel(const WeightArgs a) {
+    __shared__ float2 norm[kScoreRows];
+    const int64_t b = blockIdx.z;
+    const int head = blockIdx.x;
+    const Span s = span_of(a, b);
+    const int32_t first = blockIdx.y * kChunk;
+    if (first >= s.len) {
+        return;
+    }
+    if (static_cast<int32_t>(threadIdx.x) < s.rows) {
+        const int32_t i = threadIdx.x / a.group;
+        norm[threadIdx.x] = a.norm[(s.tok0 + i) * a.num_heads + head * a.group + (threadIdx.x - i * a.group)];
+    }
+    __syncthreads();
+    float* w = a.weight + (a.geom.layer_idx * a.num_kv_heads + head) * a.max_tokens;
+    const float* score = a.score + (b * a.num_kv_heads + head) * a.max_kvlen * a.score_rows;
+#pragma unroll
+    for (int k = 0; k < kChunk / 256; ++k) {
+        const int32_t pos = first + k * 256 + threadIdx.x;
+        if (pos >= s.len) {
+            break;
+        }
+        float sum = 0.0f;
+        for (int32_t r = 0; r < s.rows; ++r) {
+            const float2 v = norm[r];
+            sum = fmaf(ex2_approx(fmaf(score[static_cast<int64_t>(pos) * a.score_rows + r], a.scale_log2, -v.x)), v.y, sum);
+        }
+        const int64_t row = cache_row(a.geom, a.cachestarts, b, pos);
+        if (cache_row_ok(row, a.max_tokens)) {
+            atomicAdd(w + row, sum);  // one addition per position and call
+        }
+    }
+}
+
 template <int DH>
 int launch_dh(const pplb200_attn_params& p, const WeightArgs& a, cudaStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(a.chunks), static_cast<unsigned>(p.num_kv_heads), static_cast<unsigned>(p.batch));
+    const dim3 grid(static_cast<unsigned>(p.num_kv_heads), static_cast<unsigned>(a.chunks), static_cast<unsigned>(p.batch));
     const int64_t rows = p.max_seqlen * a.group;
     int rc;
-    if (rows <= 8) {
+    if (rows <= kScoreRows) {
         attn_weight_stats_kernel<DH, 1><<<grid, kThreads, 0, stream>>>(a);
     } else {
         attn_weight_stats_kernel<DH, kRowBlock / 8><<<grid, kThreads, 0, stream>>>(a);
@@ -410,11 +467,11 @@ int launch_dh(const pplb200_attn_params& p, const WeightArgs& a, cudaStream_t st
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    if (rows <= 8) {
-        attn_weight_apply_kernel<DH, 1><<<grid, kThreads, 0, stream>>>(a);
-    } else {
-        attn_weight_apply_kernel<DH, kRowBlock / 8><<<grid, kThreads, 0, stream>>>(a);
+    if (rows <= kScoreRows) {
+        attn_weight_spread_kernel<<<grid, 256, 0, stream>>>(a);
+        return check_launch("attn_weight_spread_kernel");
     }
+    attn_weight_apply_kernel<DH, kRowBlock / 8><<<grid, kThreads, 0, stream>>>(a);
     return check_launch("attn_weight_apply_kernel");
 }
 
@@ -425,8 +482,12 @@ int make_weight_plan(const pplb200_attn_params& p, WeightPlan* plan) {
     const uint64_t rows = static_cast<uint64_t>(p.total_tokens) * p.num_heads;
     plan->off_norm = 256;  // behind the status word
     plan->off_part = plan->off_norm + (rows * 8 + 255) / 256 * 256;
-    plan->bytes = plan->off_part + (rows * plan->chunks * 8 + 255) / 256 * 256;
-    return plan->chunks > 0x7fffffff / kChunk ? PPLB200_UNSUPPORTED : PPLB200_SUCCESS;
+    plan->off_score = plan->off_part + (rows * plan->chunks * 8 + 255) / 256 * 256;
+    plan->score_rows = static_cast<int32_t>(p.max_seqlen * (p.num_heads / p.num_kv_heads));
+    const bool kept = p.max_seqlen > 0 && p.max_seqlen * (p.num_heads / p.num_kv_heads) <= kScoreRows;
+    const uint64_t positions = static_cast<uint64_t>(p.batch) * p.num_kv_heads * p.max_kvlen;
+    plan->bytes = plan->off_score + (kept ? (positions * plan->score_rows * 4 + 255) / 256 * 256 : 0);
+    return plan->chunks > 65535 ? PPLB200_UNSUPPORTED : PPLB200_SUCCESS;  // a grid dimension
 }
 
 int launch_attn_weight(const pplb200_attn_params& p, const CacheGeom& geom, const WeightPlan& plan, const void* query,
@@ -446,6 +507,8 @@ int launch_attn_weight(const pplb200_attn_params& p, const CacheGeom& geom, cons
     a.weight = weight;
     a.norm = reinterpret_cast<float2*>(ws + plan.off_norm);
     a.part = reinterpret_cast<float2*>(ws + plan.off_part);
+    a.score = reinterpret_cast<float*>(ws + plan.off_score);
+    a.score_rows = plan.score_rows;
     a.status = reinterpret_cast<uint32_t*>(ws);
     a.geom = geom;
     a.max_seqlen = p.max_seqlen;

@@ -946,7 +946,7 @@ int pplb200_kv_compact(const pplb200_attn_params* p, const int64_t* kept, int64_
         return rc;
     }
     return launch_kv_compact(*p, make_geom(*p), plan, kept, kept_heads, max_kept, base, kvlens, cachestarts, layers, cache,
-                             scale, weight, workspace, static_cast<cudaStream_t>(stream_v));
+                             scale, weight, workspace, di.sm_count, static_cast<cudaStream_t>(stream_v));
 }
 
 int pplb200_mhca_device_status(const void* workspace, void* stream, uint32_t* status) {

@@ -16,10 +16,11 @@
 //
 // Compact.  Row base + kept[i] moves to row base + i.  kept is strictly ascending, so kept[i] >= i.  A list is cut into
 // segments; a segment reads all its sources before it writes.  Its destinations may still be the sources of EARLIER
-// segments (kept[i'] = i with i' < i), never of later ones, so a segment raises a flag once it has read, and writes
-// once the flags of the earlier segments of its list are up.  The CTAs draw their segments from a counter in an order
-// in which a list's earlier segments come first: whoever waits, waits for CTAs that are running and that do not wait
-// before they raise their flag.
+// segments (kept[i'] = i with i' < i), never of later ones, so a segment raises a flag once it has read, and before it
+// writes waits for the flags of those earlier segments whose sources lie among its destinations -- few, and long done
+// where many positions were dropped.  Persistent CTAs draw their segments from a counter in an order in which a list's
+// earlier segments come first.  Nobody waits before it has raised the flags of the segments it has begun, so the lowest
+// flag not yet up always belongs to a CTA that can go on.
 #include "common.cuh"
 #include "launch.h"
 
@@ -497,131 +498,259 @@ struct CompactArgs {
     int64_t max_kept, max_kvlen, max_tokens;
     uint32_t lists;       // batch * layers * head groups
     uint32_t move_tasks;  // segments * lists
+    uint32_t tasks;       // and the clearing of weights
     int32_t kept_heads, num_kv_heads;
     uint32_t layers, head_groups;
     int32_t heads_shift, rows_per_seg, segments;  // 1 << heads_shift heads per CTA
 };
 
 constexpr int kCompactThreads = 256;
+constexpr int kCompactCtas = 8;       // per SM: 160 KB on their way
 constexpr int kSegmentRows = 64;      // rows x heads of a segment
 constexpr int kClearRows = 8192;      // weights zeroed by a CTA
 
-// Up to this many clock cycles a segment waits for the ones before it
+// Flags order reads before other CTAs' writes, and nothing else.  When a segment raises its flag its sources have
+// arrived in its shared memory (the asynchronous copies have completed and the CTA has met at a barrier), so no later
+// write can reach them, and nothing it wrote is read by whoever sees the flag.  A relaxed store and relaxed loads do: a
+// fence ahead of the store would wait for the stores of every CTA on the SM (measured 4 to 7 us per segment).
+__device__ __forceinline__ void raise_flag(uint32_t* flag) {
+    asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(flag), "r"(1u) : "memory");
+}
 __device__ __forceinline__ bool wait_flag(const uint32_t* flag) {
-    const long long t0 = clock64();
+    long long t0 = 0;
     for (;;) {
         uint32_t v;
-        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
+        asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
         if (v != 0u) {
             return true;
         }
-        if (clock64() - t0 > kWaitBudgetCycles) {
+        const long long t = clock64();
+        t0 = t0 == 0 ? t : t0;
+        if (t - t0 > kWaitBudgetCycles) {
             return false;
         }
     }
 }
 
+// What a task works on
+struct Task {
+    int64_t b, base, n;   // sequence, its base, the positions it had
+    const int64_t* kept;
+    int32_t seg, head0;
+    int64_t layer_idx;
+    uint32_t list;
+    bool clear;
+};
+
+// Rows of a segment, worked out while the segment before it is on its way
+struct SegmentRows {
+    int64_t src[kSegmentRows], dst[kSegmentRows];  // element offsets of K of the first head; src < 0: not to be moved
+    int2 row[kSegmentRows];                        // cache rows
+    int32_t wait_from, wait_to;                    // earlier segments whose sources may be among the destinations
+    uint32_t ticket;
+};
+
+__device__ __forceinline__ Task task_of(const CompactArgs& a, uint32_t ticket) {
+    Task t;
+    t.clear = ticket >= a.move_tasks;
+    const uint32_t task = t.clear ? ticket - a.move_tasks : ticket;
+    t.list = task % a.lists;
+    t.seg = task / a.lists;
+    t.head0 = static_cast<int>(t.list % a.head_groups) << a.heads_shift;
+    t.layer_idx = a.geom.layer_idx + t.list / a.head_groups % a.layers;
+    t.b = t.list / a.head_groups / a.layers;
+    t.kept = a.kept + (t.b * a.kept_heads + (a.kept_heads > 1 ? t.head0 : 0)) * a.max_kept;
+    t.base = a.base[t.b];
+    t.n = a.kvlens[t.b];
+    if (t.n > a.max_kvlen) {
+        t.n = a.max_kvlen;
+        atomicOr(a.status, kDevLengthClamped);
+    }
+    return t;
+}
+
+// The last segment in [0, seg] whose first entry is at most `pos` (0 if none is); all lanes of a warp call it.
+__device__ __forceinline__ int32_t segment_of(const CompactArgs& a, const int64_t* kept, int32_t seg, int64_t pos,
+                                              int lane) {
+    int32_t lo = 0, hi = seg + 1;  // answer in [lo, hi)
+    while (hi - lo > 1) {
+        const int32_t step = (hi - lo + 31) >> 5;
+        const int32_t pivot = lo + (lane + 1) * step;
+        // entries behind the end of the list are negative: above every position when read as unsigned
+        const bool le = pivot < hi && static_cast<uint64_t>(kept[static_cast<int64_t>(pivot) * a.rows_per_seg]) <=
+                                          static_cast<uint64_t>(pos);
+        const int32_t next = lo + __popc(__ballot_sync(0xffffffffu, le)) * step;
+        hi = next + step < hi ? next + step : hi;
+        lo = next;
+    }
+    return lo;
+}
+
+// Warps 0 and 1 look up the rows of the segment that `ticket` names, warps 2 and 3 the segments it has to wait for.
+__device__ __forceinline__ void prepare_segment(const CompactArgs& a, uint32_t ticket, SegmentRows& rows) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (tid >= 128 || ticket >= a.move_tasks) {
+        return;
+    }
+    const Task t = task_of(a, ticket);
+    const int64_t first = static_cast<int64_t>(t.seg) * a.rows_per_seg;
+    if (tid >= kSegmentRows) {
+        const int32_t e = segment_of(a, t.kept, t.seg, tid < 96 ? first : first + a.rows_per_seg - 1, lane);
+        if (lane == 0) {
+            *(tid < 96 ? &rows.wait_from : &rows.wait_to) = e;
+        }
+        return;
+    }
+    if (tid >= a.rows_per_seg) {
+        return;
+    }
+    const int64_t i = first + tid;
+    const int64_t p = i < a.max_kept ? t.kept[i] : -1;
+    const int64_t before = i > 0 && i < a.max_kept ? t.kept[i - 1] : -1;
+    CacheGeom geom = a.geom;
+    int64_t src = -1, dst = 0;
+    if (p >= 0) {
+        if (t.base < 0 || p < i || (i > 0 && (before < 0 || p <= before)) || t.base + p >= t.n) {
+            atomicOr(a.status, kDevKeptInvalid);
+        } else if (p != i) {
+            src = cache_row(geom, a.cachestarts, t.b, t.base + p);
+            dst = cache_row(geom, a.cachestarts, t.b, t.base + i);
+            if (!cache_row_ok(src, a.max_tokens) || !cache_row_ok(dst, a.max_tokens)) {
+                atomicOr(a.status, kDevRowOutOfRange);
+                src = -1;
+            }
+        }
+    }
+    const int64_t fixed = t.layer_idx * geom.stride_l + t.head0 * geom.stride_h;
+    rows.src[tid] = src < 0 ? -1 : src * geom.stride_s + fixed;
+    rows.dst[tid] = dst * geom.stride_s + fixed;
+    rows.row[tid] = make_int2(static_cast<int>(src), static_cast<int>(dst));
+}
+
+// The positions behind the kept ones hold no token any more: the next ones start from zero weight.
+__device__ __forceinline__ bool clear_weights(const CompactArgs& a, uint32_t ticket) {
+    const Task t = task_of(a, ticket);
+    if (t.base < 0) {
+        return true;
+    }
+    int64_t count = 0, top = a.max_kept;  // first negative entry
+    while (count < top) {
+        const int64_t mid = (count + top) >> 1;
+        if (t.kept[mid] >= 0) {
+            count = mid + 1;
+        } else {
+            top = mid;
+        }
+    }
+    const int64_t from = t.base + count + static_cast<int64_t>(t.seg) * kClearRows;
+    const int64_t end = from + kClearRows < t.n ? from + kClearRows : t.n;
+    if (from >= end) {
+        return true;
+    }
+    bool ok = true;
+    for (int32_t e = threadIdx.x; e < a.segments; e += kCompactThreads) {
+        ok = wait_flag(a.flags + static_cast<int64_t>(e) * a.lists + t.list) && ok;
+    }
+    if (!__syncthreads_and(ok)) {
+        return false;
+    }
+    float* weight = a.weight + (t.layer_idx * a.num_kv_heads + t.head0) * a.max_tokens;
+    for (int64_t pos = from + threadIdx.x; pos < end; pos += kCompactThreads) {
+        const int64_t row = cache_row(a.geom, a.cachestarts, t.b, pos);
+        if (!cache_row_ok(row, a.max_tokens)) {
+            atomicOr(a.status, kDevRowOutOfRange);
+            continue;
+        }
+        for (int head = 0; head < 1 << a.heads_shift; ++head) {
+            weight[head * a.max_tokens + row] = 0.0f;
+        }
+    }
+    return true;
+}
+
 template <int DH>
-__global__ void __launch_bounds__(kCompactThreads, 8) kv_compact_kernel(const CompactArgs a) {
+__global__ void __launch_bounds__(kCompactThreads, kCompactCtas) kv_compact_kernel(const CompactArgs a) {
     constexpr int kCodePieces = DH / 16;   // 16-byte pieces of a row's codes
     constexpr int kScalePieces = DH / 64;  // and of its scales
     constexpr int kCodeStep = kCompactThreads / kCodePieces;  // rows (of K or V of a head) the CTA moves at once
     constexpr int kCodeSteps = 2 * kSegmentRows / kCodeStep;
-    __shared__ uint32_t s_ticket;
-    __shared__ int64_t s_src[kSegmentRows], s_dst[kSegmentRows];
-    __shared__ int2 s_row[kSegmentRows];
+    __shared__ SegmentRows s_rows[2];
     __shared__ uint4 stage[(kCodeSteps + 1) * kCompactThreads];
+    __shared__ float stage_w[kSegmentRows];
     const int tid = threadIdx.x;
     if (tid == 0) {
-        s_ticket = atomicAdd(a.ticket, 1u);
+        s_rows[0].ticket = atomicAdd(a.ticket, 1u);
     }
     __syncthreads();
-    const bool clear = s_ticket >= a.move_tasks;  // tasks and lists fit 31 bits
-    const uint32_t task = clear ? s_ticket - a.move_tasks : s_ticket;
-    const uint32_t lists = a.lists, list = task % lists;
-    const int32_t seg = task / lists;
-    const int head0 = static_cast<int>(list % a.head_groups) << a.heads_shift;
-    const int layer = list / a.head_groups % a.layers;
-    const int64_t b = list / a.head_groups / a.layers;
-    const int64_t* kept = a.kept + (b * a.kept_heads + (a.kept_heads > 1 ? head0 : 0)) * a.max_kept;
-    const int64_t base = a.base[b];
-    int64_t n = a.kvlens[b];
-    if (n > a.max_kvlen) {
-        n = a.max_kvlen;
-        if (tid == 0) {
-            atomicOr(a.status, kDevLengthClamped);
+    prepare_segment(a, s_rows[0].ticket, s_rows[0]);
+    __syncthreads();
+    for (int buf = 0;; buf ^= 1) {
+        const SegmentRows& rows = s_rows[buf];
+        SegmentRows& next = s_rows[buf ^ 1];
+        const uint32_t ticket = rows.ticket;
+        if (ticket >= a.tasks) {
+            return;
         }
-    }
-    CacheGeom geom = a.geom;
-    geom.layer_idx += layer;
-    float* weight = a.weight == nullptr ? nullptr : a.weight + (geom.layer_idx * a.num_kv_heads + head0) * a.max_tokens;
-
-    if (!clear) {
-        // cache rows of the segment's entries: source and destination, or -1: not to be moved
-        if (tid < a.rows_per_seg) {
-            const int64_t i = static_cast<int64_t>(seg) * a.rows_per_seg + tid;
-            int64_t src = -1, dst = -1;
-            const int64_t p = i < a.max_kept ? kept[i] : -1;
-            if (p >= 0) {
-                const int64_t before = i > 0 ? kept[i - 1] : -1;
-                if (base < 0 || p < i || (i > 0 && (before < 0 || p <= before)) || base + p >= n) {
-                    atomicOr(a.status, kDevKeptInvalid);
-                } else if (p != i) {
-                    src = cache_row(geom, a.cachestarts, b, base + p);
-                    dst = cache_row(geom, a.cachestarts, b, base + i);
-                    if (!cache_row_ok(src, a.max_tokens) || !cache_row_ok(dst, a.max_tokens)) {
-                        atomicOr(a.status, kDevRowOutOfRange);
-                        src = -1;
-                    }
-                }
-            }
-            // element offsets of K of the first head
-            const int64_t fixed = geom.layer_idx * geom.stride_l + head0 * geom.stride_h;
-            s_src[tid] = src < 0 ? -1 : src * geom.stride_s + fixed;
-            s_dst[tid] = dst * geom.stride_s + fixed;
-            s_row[tid] = make_int2(static_cast<int>(src), static_cast<int>(dst));
-        }
-        __syncthreads();
+        const bool move = ticket < a.move_tasks;
         // x = (row * 2 + K | V) * heads + head, and pieces of it by neighbouring threads: neighbouring bytes.  A thread
         // stages its own pieces in shared memory, which keeps the bytes in flight out of the registers.
         const int shift = a.heads_shift, count = a.rows_per_seg * 2 << shift;
-        auto offset = [&](const int64_t* rows, int x) -> int64_t {  // of a row of K or V of a head, or negative
+        auto offset = [&](const int64_t* of, int x) -> int64_t {  // of a row of K or V of a head, or negative
             const int y = x >> shift;
-            const int64_t row = rows[y >> 1];
-            return row < 0 ? -1 : row + (y & 1) * geom.stride_kv + (x & ((1 << shift) - 1)) * geom.stride_h;
+            const int64_t row = of[y >> 1];
+            return row < 0 ? -1 : row + (y & 1) * a.geom.stride_kv + (x & ((1 << shift) - 1)) * a.geom.stride_h;
         };
         const int cx = tid / kCodePieces, cp = tid % kCodePieces * 16, sx = tid / kScalePieces, sp = tid % kScalePieces * 8;
+        if (move) {
 #pragma unroll
-        for (int u = 0; u < kCodeSteps; ++u) {
-            const int x = u * kCodeStep + cx;
-            const int64_t off = x < count ? offset(s_src, x) : -1;
+            for (int u = 0; u < kCodeSteps; ++u) {
+                const int x = u * kCodeStep + cx;
+                const int64_t off = x < count ? offset(rows.src, x) : -1;
+                if (off >= 0) {
+                    cp_async16(smem_u32(&stage[u * kCompactThreads + tid]), a.cache + off + cp);
+                }
+            }
+            const int64_t off = sx < count ? offset(rows.src, sx) : -1;
             if (off >= 0) {
-                cp_async16(smem_u32(&stage[u * kCompactThreads + tid]), a.cache + off + cp);
+                cp_async16(smem_u32(&stage[kCodeSteps * kCompactThreads + tid]), a.scale + (off >> 3) + sp);
             }
         }
-        const int64_t scale_off = sx < count ? offset(s_src, sx) : -1;
-        if (scale_off >= 0) {
-            cp_async16(smem_u32(&stage[kCodeSteps * kCompactThreads + tid]), a.scale + (scale_off >> 3) + sp);
-        }
-        float wv = 0.0f;
-        int64_t wto = -1;
-        if (weight != nullptr && tid < a.rows_per_seg << shift) {
-            const int rr = tid >> shift, head = tid & ((1 << shift) - 1);
-            if (s_src[rr] >= 0) {
-                wv = weight[head * a.max_tokens + s_row[rr].x];
-                wto = head * a.max_tokens + s_row[rr].y;
-            }
+        const bool has_weight = move && a.weight != nullptr && tid < a.rows_per_seg << shift && rows.src[tid >> shift] >= 0;
+        float* weight = nullptr;
+        if (has_weight) {
+            const uint32_t list = ticket % a.lists;
+            const int64_t head = (static_cast<int64_t>(list % a.head_groups) << shift) + (tid & ((1 << shift) - 1));
+            weight = a.weight + ((a.geom.layer_idx + list / a.head_groups % a.layers) * a.num_kv_heads + head) * a.max_tokens;
+            cp_async4(smem_u32(&stage_w[tid]), weight + rows.row[tid >> shift].x);
         }
         cp_async_commit();
+        // the next task's rows, while the copies are on their way
+        if (tid == 0) {
+            next.ticket = atomicAdd(a.ticket, 1u);
+        }
+        __syncthreads();
+        prepare_segment(a, next.ticket, next);
+        if (!move) {
+            if (!clear_weights(a, ticket)) {
+                if (tid == 0) {
+                    atomicOr(a.status, kDevTmaTimeout);
+                }
+                return;
+            }
+            __syncthreads();
+            continue;
+        }
         cp_async_wait<0>();
         __syncthreads();  // every source of the segment has been read
+        const uint32_t list = ticket % a.lists;
+        const int32_t seg = ticket / a.lists;
         if (tid == 0) {
-            __threadfence();
-            asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(a.flags + static_cast<int64_t>(seg) * lists + list), "r"(1u) : "memory");
+            raise_flag(a.flags + static_cast<int64_t>(seg) * a.lists + list);
         }
         bool ok = true;
-        for (int32_t e = tid; e < seg; e += kCompactThreads) {
-            ok = wait_flag(a.flags + static_cast<int64_t>(e) * lists + list) && ok;
+        const int32_t wait_to = rows.wait_to < seg ? rows.wait_to : seg - 1;
+        for (int32_t e = rows.wait_from + tid; e <= wait_to; e += kCompactThreads) {
+            ok = wait_flag(a.flags + static_cast<int64_t>(e) * a.lists + list) && ok;
         }
         if (!__syncthreads_and(ok)) {
             if (tid == 0) {
@@ -632,55 +761,15 @@ __global__ void __launch_bounds__(kCompactThreads, 8) kv_compact_kernel(const Co
 #pragma unroll
         for (int u = 0; u < kCodeSteps; ++u) {
             const int x = u * kCodeStep + cx;
-            if (x < count && s_src[x >> shift >> 1] >= 0) {
-                *reinterpret_cast<uint4*>(a.cache + offset(s_dst, x) + cp) = stage[u * kCompactThreads + tid];
+            if (x < count && rows.src[x >> shift >> 1] >= 0) {
+                *reinterpret_cast<uint4*>(a.cache + offset(rows.dst, x) + cp) = stage[u * kCompactThreads + tid];
             }
         }
-        if (scale_off >= 0) {
-            *reinterpret_cast<uint4*>(a.scale + (offset(s_dst, sx) >> 3) + sp) = stage[kCodeSteps * kCompactThreads + tid];
+        if (sx < count && rows.src[sx >> shift >> 1] >= 0) {
+            *reinterpret_cast<uint4*>(a.scale + (offset(rows.dst, sx) >> 3) + sp) = stage[kCodeSteps * kCompactThreads + tid];
         }
-        if (wto >= 0) {
-            weight[wto] = wv;
-        }
-        return;
-    }
-
-    // the positions behind the kept ones hold no token any more: the next ones start from zero weight
-    if (base < 0) {
-        return;
-    }
-    int64_t count = 0, top = a.max_kept;  // first negative entry
-    while (count < top) {
-        const int64_t mid = (count + top) >> 1;
-        if (kept[mid] >= 0) {
-            count = mid + 1;
-        } else {
-            top = mid;
-        }
-    }
-    const int64_t from = base + count + static_cast<int64_t>(seg) * kClearRows;
-    const int64_t end = from + kClearRows < n ? from + kClearRows : n;
-    if (from >= end) {
-        return;
-    }
-    bool ok = true;
-    for (int32_t e = tid; e < a.segments; e += kCompactThreads) {
-        ok = wait_flag(a.flags + static_cast<int64_t>(e) * lists + list) && ok;
-    }
-    if (!__syncthreads_and(ok)) {
-        if (tid == 0) {
-            atomicOr(a.status, kDevTmaTimeout);
-        }
-        return;
-    }
-    for (int64_t pos = from + tid; pos < end; pos += kCompactThreads) {
-        const int64_t row = cache_row(geom, a.cachestarts, b, pos);
-        if (!cache_row_ok(row, a.max_tokens)) {
-            atomicOr(a.status, kDevRowOutOfRange);
-            continue;
-        }
-        for (int head = 0; head < 1 << a.heads_shift; ++head) {
-            weight[head * a.max_tokens + row] = 0.0f;
+        if (has_weight) {
+            weight[rows.row[tid >> shift].y] = stage_w[tid];
         }
     }
 }
@@ -760,7 +849,7 @@ int make_compact_plan(const pplb200_attn_params& p, int64_t kept_heads, int64_t 
 int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const CompactPlan& plan, const int64_t* kept,
                       int64_t kept_heads, int64_t max_kept, const int64_t* base, const int64_t* kvlens,
                       const int64_t* cachestarts, int64_t layers, void* cache, void* scale, float* weight,
-                      void* workspace, cudaStream_t stream) {
+                      void* workspace, int sm_count, cudaStream_t stream) {
     CompactArgs a = {};
     a.kept = kept;
     a.base = base;
@@ -792,10 +881,13 @@ int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const
         return PPLB200_DEVICE_RUNTIME_ERROR;
     }
     const int64_t clears = weight == nullptr ? 0 : (p.max_kvlen + kClearRows - 1) / kClearRows;
-    const int64_t ctas = (plan.segments + clears) * plan.lists;
-    if (ctas <= 0) {
+    const int64_t tasks = (plan.segments + clears) * plan.lists;
+    if (tasks <= 0) {
         return PPLB200_SUCCESS;
     }
+    a.tasks = static_cast<uint32_t>(tasks);
+    const int64_t resident = static_cast<int64_t>(sm_count) * kCompactCtas;
+    const int64_t ctas = tasks < resident ? tasks : resident;
     auto kernel = p.head_dim == 128 ? kv_compact_kernel<128> : kv_compact_kernel<64>;
     kernel<<<static_cast<unsigned>(ctas), kCompactThreads, 0, stream>>>(a);
     return check_launch("kv_compact_kernel");

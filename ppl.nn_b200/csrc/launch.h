@@ -137,7 +137,8 @@ int launch_tree_attn(const pplb200_attn_params& p, const CacheGeom& geom, const 
 // ---- accumulated attention weight, eviction, compaction --------------------------------------------
 struct WeightPlan {
     int64_t chunks;  // chunks of positions per sequence
-    uint64_t off_norm, off_part, bytes;
+    int32_t score_rows;  // query rows per kv head
+    uint64_t off_norm, off_part, off_score, bytes;
 };
 int make_weight_plan(const pplb200_attn_params& p, WeightPlan* plan);
 int launch_attn_weight(const pplb200_attn_params& p, const CacheGeom& geom, const WeightPlan& plan, const void* query,
@@ -158,7 +159,7 @@ int make_compact_plan(const pplb200_attn_params& p, int64_t kept_heads, int64_t 
 int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const CompactPlan& plan, const int64_t* kept,
                       int64_t kept_heads, int64_t max_kept, const int64_t* base, const int64_t* kvlens,
                       const int64_t* cachestarts, int64_t layers, void* cache, void* scale, float* weight,
-                      void* workspace, cudaStream_t stream);
+                      void* workspace, int sm_count, cudaStream_t stream);
 
 // Rotary position embedding, alone (append == nullptr) or fused with the cache append.
 uint64_t rope_workspace_bytes(const pplb200_rope_params& p);

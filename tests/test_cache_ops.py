@@ -400,3 +400,30 @@ def test_compact_reports_bad_lists(gpu, pkg):
         keep = np.ones(hc.max_tokens, dtype=bool)
         keep[hc.starts[0]:hc.starts[0] + 4] = False
         assert np.array_equal(got[keep], hc.cache[keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drop", [1, 3, 64, 200])
+@pytest.mark.parametrize("per_head", [True, False])
+def test_compact_shifts_by_a_few_rows(gpu, pkg, drop, per_head):
+    """Only the first few positions go, so that every row's destination is another row's source: all the segments of a
+    list depend on one another."""
+    from ppl_nn_b200 import ops
+    rng = np.random.default_rng(drop)
+    lens = [5000, 4111, 700, 4999, 2048, 201]
+    hc = HostCache(rng, lens, 4, 64, 0, 0, 2)
+    kept = np.full((len(lens), 4 if per_head else 1, max(lens)), -1, dtype=np.int64)
+    for b, n in enumerate(lens):
+        for g in range(kept.shape[1]):
+            cut = min(drop + (g if per_head else 0), n)
+            kept[b, g, :n - cut] = np.arange(cut, n)
+    base = np.zeros(len(lens), dtype=np.int64)
+    want = compact_reference(hc, kept, base, 0, 2, True)
+    op = ops.KeyValueCacheCompact(ops.KeyValueCacheParam(**hc.param()))
+    for _ in range(5):
+        got = [dev(hc.cache), dev(hc.scale), dev(hc.weight)]
+        op.forward(dev(kept), dev(hc.starts), dev(base), dev(np.array(lens)), hc.max_len, *got[:2], weight=got[2],
+                   num_layers=2)
+        assert op.device_status() == 0
+        for g, x in zip(got, want):
+            assert np.array_equal(g.cpu().numpy(), x)
