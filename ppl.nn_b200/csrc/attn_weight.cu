@@ -24,9 +24,11 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kChunk = 512;     // positions of a CTA
+constexpr int kChunk = 512;     // positions of a CTA where the scores are formed twice
+constexpr int kSpread = 2048;   // positions of a CTA of attn_weight_spread_kernel
 constexpr int kRowBlock = 32;   // query rows whose fragments are held in registers at a time
 constexpr int kScoreRows = 8;   // up to so many query rows per kv head the scores are kept
+constexpr int kStages = 3;      // tiles of a warp's ring
 constexpr float kNegBig = -1.0e30f;
 
 struct WeightArgs {
@@ -45,8 +47,18 @@ struct WeightArgs {
     CacheGeom geom;
     int64_t max_seqlen, max_kvlen, max_tokens, total_tokens;
     int32_t num_heads, num_kv_heads, group, causal, chunks;
+    int32_t chunk;   // positions of a chunk
     float scale_log2;
 };
+
+// D = A B, without an accumulator to start from
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 
 // Four codes with their group's scale -> the two half2 of fp16(code * scale) and of the exact remainders
 __device__ __forceinline__ void split_key_word(uint32_t w, __half2 s2, uint32_t& k0, uint32_t& k1, uint32_t& e0,
@@ -91,7 +103,85 @@ __device__ __forceinline__ Span span_of(const WeightArgs& a, int64_t b) {
     return s;
 }
 
-// Scores (unscaled) of the 16 positions from `tile0` on against NOCT octets of query rows whose fragments are in qf.
+// A warp's ring of tiles in shared memory: 16 K rows of one (sequence, kv head), codes and scales, copied
+// asynchronously, so that kStages - 1 tiles are on their way while one is worked on.
+template <int DH>
+struct Ring {
+    static constexpr int kCodeBytes = 16 * DH;
+    static constexpr int kTileBytes = kCodeBytes + 2 * DH * 2;
+    static constexpr int kWarpBytes = kStages * kTileBytes;
+    static constexpr int kPieces = DH / 16;           // 16-byte pieces of a row's codes
+    static constexpr int kRowStep = 32 / kPieces;     // rows the warp copies at once
+    static constexpr int kScalePieces = DH / 64;
+    const int8_t* code;    // this lane's piece of cache row 0
+    const __half* scale;
+    int64_t first;         // cache row of position 0 (contiguous cache)
+    int32_t safe;          // contiguous cache: tiles below this position are whole and inside the cache
+    uint32_t base;         // the ring, in shared memory
+    uint32_t code_at, scale_at;  // where in a tile this lane's first copies go
+
+    __device__ __forceinline__ Ring(const WeightArgs& a, const Span& s, int64_t b, int head, int warp, int lane, void* smem) {
+        const int64_t off = a.geom.layer_idx * a.geom.stride_l + head * a.geom.stride_h;
+        const int i = lane / kPieces, c = lane % kPieces;
+        code = a.cache + off + i * a.geom.stride_s + c * 16;
+        scale = a.scale + ((off + lane / kScalePieces * a.geom.stride_s) >> 3) + lane % kScalePieces * 8;
+        // Dh 128: neighbouring rows swap halves, so that the eight lanes of a read fill all banks
+        code_at = i * DH + (DH == 128 ? c ^ ((i & 1) << 2) : c) * 16;
+        scale_at = kCodeBytes + lane * 16;
+        first = a.geom.cache_mode == 0 ? a.cachestarts[b] : 0;
+        safe = s.len & ~15;
+        if (a.geom.cache_mode != 0 || first < 0 || first + s.len > a.max_tokens) {
+            safe = 0;
+        }
+        base = smem_u32(smem) + warp * kWarpBytes;
+    }
+
+    __device__ __forceinline__ int64_t row_of(const WeightArgs& a, int64_t b, int32_t tile0) const {
+        return tile0 < safe ? first + tile0 : cache_row(a.geom, a.cachestarts, b, tile0);
+    }
+
+    // The copies of the tile at position tile0 into stage `stage`; every call is one group
+    __device__ __forceinline__ void issue(const WeightArgs& a, int64_t b, int32_t tile0, int32_t end, int32_t len, int stage,
+                                          int lane) const {
+        const uint32_t dst = base + stage * kTileBytes;
+        const int64_t row_step = kRowStep * a.geom.stride_s;
+        if (tile0 < end && tile0 < safe) {
+            const int64_t off = (first + tile0) * a.geom.stride_s;
+            const int8_t* src = code + off;
+#pragma unroll
+            for (int k = 0; k < 16 / kRowStep; ++k) {
+                cp_async16(dst + code_at + k * kRowStep * DH, src);
+                src += row_step;
+            }
+            if (lane < 16 * kScalePieces) {
+                cp_async16(dst + scale_at, scale + (off >> 3));
+            }
+        } else if (tile0 < end) {
+            // a page, or the last tile: rows that do not exist read as zeros
+            const int64_t row0 = cache_row(a.geom, a.cachestarts, b, tile0);
+            auto there = [&](int i) -> bool {
+                const bool ok = row0 >= 0 && cache_row_ok(row0 + i, a.max_tokens);
+                if (tile0 + i < len && !ok) {
+                    atomicOr(a.status, kDevRowOutOfRange);
+                }
+                return tile0 + i < len && ok;
+            };
+            const int64_t off = row0 * a.geom.stride_s;
+#pragma unroll
+            for (int k = 0; k < 16 / kRowStep; ++k) {
+                const bool ok = there(k * kRowStep + lane / kPieces);
+                cp_async16(dst + code_at + k * kRowStep * DH, ok ? code + off + k * row_step : a.cache, ok ? 16u : 0u);
+            }
+            if (lane < 16 * kScalePieces) {
+                const bool ok = there(lane / kScalePieces);
+                cp_async16(dst + scale_at, ok ? scale + (off >> 3) : a.scale, ok ? 16u : 0u);
+            }
+        }
+        cp_async_commit();
+    }
+};
+
+// Scores (unscaled) of 16 positions against NOCT octets of query rows whose fragments are in qf.
 // acc[o][0..1]: position g, rows 2t and 2t+1 of octet o; acc[o][2..3]: position g + 8.
 template <int DH, int NOCT>
 struct Tile {
@@ -99,38 +189,34 @@ struct Tile {
     uint4 code[2][DH / 64];
     uint32_t sc[2][DH / 64];
 
-    __device__ __forceinline__ void load(const WeightArgs& a, int64_t b, int head, int32_t tile0, int32_t len, int lane,
-                                         int64_t& row0) {
-        row0 = cache_row(a.geom, a.cachestarts, b, tile0);
+    // Where in a tile a lane reads its 16 code bytes of row g (Dh 128: of the first 64 channels; the others are 64
+    // bytes up or down, as the copy left them) and its scales
+    static __device__ __forceinline__ uint32_t code_offset(int lane) {
         const int g = lane >> 2, t = lane & 3;
+        return g * DH + (DH == 128 ? t ^ ((g & 1) << 2) : t) * 16;
+    }
+    static __device__ __forceinline__ uint32_t scale_offset(int lane) {
+        return Ring<DH>::kCodeBytes + (lane >> 2) * (DH / 4) + (lane & 3) * 4;
+    }
+
+    __device__ __forceinline__ void read(uint32_t code_addr, uint32_t scale_addr) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const int i = g + 8 * r;
-            const bool ok = tile0 + i < len && row0 >= 0 && cache_row_ok(row0 + i, a.max_tokens);
-            if (tile0 + i < len && !ok) {
-                atomicOr(a.status, kDevRowOutOfRange);
-            }
-            const int64_t off = ok ? cache_offset(a.geom, row0 + i, 0, head) : 0;
 #pragma unroll
             for (int h = 0; h < DH / 64; ++h) {
-                code[r][h] = make_uint4(0u, 0u, 0u, 0u);
-                sc[r][h] = 0u;
-                if (ok) {
-                    code[r][h] = *reinterpret_cast<const uint4*>(a.cache + off + h * 64 + t * 16);
-                    sc[r][h] = *reinterpret_cast<const uint32_t*>(a.scale + (off >> 3) + h * 8 + t * 2);
-                }
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(code[r][h].x), "=r"(code[r][h].y), "=r"(code[r][h].z), "=r"(code[r][h].w)
+                             : "r"((h == 0 ? code_addr : code_addr ^ 64u) + r * 8 * DH));
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sc[r][h]) : "r"(scale_addr + r * 8 * (DH / 4) + h * 16));
             }
         }
     }
 
+    // The keys and their remainders have accumulators of their own, and with one octet there are two of each: shorter
+    // chains of dependent instructions, and of roundings.
     __device__ __forceinline__ void scores(const uint2 (&qf)[NOCT][kWords], float (&acc)[NOCT][4]) const {
-#pragma unroll
-        for (int o = 0; o < NOCT; ++o) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                acc[o][e] = 0.0f;
-            }
-        }
+        constexpr int kChains = NOCT == 1 ? 2 : 1;
+        float key[kChains][NOCT][4], rest[kChains][NOCT][4];
 #pragma unroll
         for (int w = 0; w < kWords; ++w) {
             uint32_t k[2][2], e[2][2];
@@ -143,8 +229,29 @@ struct Tile {
             }
 #pragma unroll
             for (int o = 0; o < NOCT; ++o) {
-                mma_m16n8k16_f16f32(acc[o], k[0][0], k[1][0], k[0][1], k[1][1], qf[o][w].x, qf[o][w].y);
-                mma_m16n8k16_f16f32(acc[o], e[0][0], e[1][0], e[0][1], e[1][1], qf[o][w].x, qf[o][w].y);
+                if (w < kChains) {
+                    mma_first(key[w % kChains][o], k[0][0], k[1][0], k[0][1], k[1][1], qf[o][w].x, qf[o][w].y);
+                } else {
+                    mma_m16n8k16_f16f32(key[w % kChains][o], k[0][0], k[1][0], k[0][1], k[1][1], qf[o][w].x, qf[o][w].y);
+                }
+            }
+#pragma unroll
+            for (int o = 0; o < NOCT; ++o) {
+                if (w < kChains) {
+                    mma_first(rest[w % kChains][o], e[0][0], e[1][0], e[0][1], e[1][1], qf[o][w].x, qf[o][w].y);
+                } else {
+                    mma_m16n8k16_f16f32(rest[w % kChains][o], e[0][0], e[1][0], e[0][1], e[1][1], qf[o][w].x, qf[o][w].y);
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 0; o < NOCT; ++o) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                acc[o][e] = key[0][o][e] + rest[0][o][e];
+                if constexpr (kChains == 2) {
+                    acc[o][e] = (key[0][o][e] + key[1][o][e]) + (rest[0][o][e] + rest[1][o][e]);
+                }
             }
         }
     }
@@ -192,18 +299,48 @@ __device__ __forceinline__ void hide(const WeightArgs& a, const Span& s, int32_t
     }
 }
 
+// work(tile, position) for this warp's tiles of [tile0, end)
+template <int DH, int NOCT, typename Work>
+__device__ __forceinline__ void for_tiles(const WeightArgs& a, const Ring<DH>& ring, int64_t b, int32_t tile0, int32_t end,
+                                          int32_t len, int lane, Work work) {
+    constexpr int kStep = kWarps * 16;
+    __syncwarp();  // the ring may still be read for the rows before
+#pragma unroll
+    for (int k = 0; k < kStages - 1; ++k) {
+        ring.issue(a, b, tile0 + k * kStep, end, len, k, lane);
+    }
+    const uint32_t code_addr = ring.base + Tile<DH, NOCT>::code_offset(lane);
+    const uint32_t scale_addr = ring.base + Tile<DH, NOCT>::scale_offset(lane);
+    int stage = 0, ahead = kStages - 1;
+    for (; tile0 < end; tile0 += kStep) {
+        ring.issue(a, b, tile0 + (kStages - 1) * kStep, end, len, ahead, lane);
+        cp_async_wait<kStages - 1>();
+        __syncwarp();
+        Tile<DH, NOCT> tile;
+        tile.read(code_addr + stage * Ring<DH>::kTileBytes, scale_addr + stage * Ring<DH>::kTileBytes);
+        __syncwarp();  // everyone has read: the next round may overwrite the stage
+        work(tile, tile0);
+        ahead = stage;
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    cp_async_wait<0>();
+}
+
 template <int DH, int NOCT>
-__global__ void __launch_bounds__(kThreads) attn_weight_stats_kernel(const WeightArgs a) {
+__global__ void __launch_bounds__(kThreads, NOCT == 1 ? 6 : 3) attn_weight_stats_kernel(const WeightArgs a) {
     __shared__ float2 red[kWarps][NOCT * 8];
+    __shared__ __align__(128) uint8_t smem[kWarps * Ring<DH>::kWarpBytes];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t b = blockIdx.z;
     const int head = blockIdx.x, chunk = blockIdx.y;  // neighbouring CTAs read neighbouring heads of the same rows
     const Span s = span_of(a, b);
-    const int32_t first = chunk * kChunk;
+    const int32_t first = chunk * a.chunk;
     if (first >= s.len) {
         return;
     }
-    const int32_t end = first + kChunk < s.len ? first + kChunk : s.len;
+    const int32_t end = first + a.chunk < s.len ? first + a.chunk : s.len;
+    const Ring<DH> ring(a, s, b, head, warp, lane, smem);
+    float* score = a.score + (b * a.num_kv_heads + head) * a.max_kvlen * a.score_rows;  // NOCT == 1
     for (int32_t row0 = 0; row0 < s.rows; row0 += NOCT * 8) {
         uint2 qf[NOCT][DH / 16];
         load_queries<DH, NOCT>(a, s, head, row0, lane, qf);
@@ -216,14 +353,7 @@ __global__ void __launch_bounds__(kThreads) attn_weight_stats_kernel(const Weigh
                 l[o][c] = 0.0f;
             }
         }
-        Tile<DH, NOCT> next;
-        int64_t row;
-        next.load(a, b, head, first + warp * 16, s.len, lane, row);
-        for (int32_t tile0 = first + warp * 16; tile0 < end; tile0 += kWarps * 16) {
-            const Tile<DH, NOCT> tile = next;
-            if (tile0 + kWarps * 16 < end) {
-                next.load(a, b, head, tile0 + kWarps * 16, s.len, lane, row);
-            }
+        auto work = [&](const Tile<DH, NOCT>& tile, int32_t tile0) {
             float acc[NOCT][4];
             tile.scores(qf, acc);
             if (tile0 + 15 > s.start || tile0 + 15 >= s.len) {
@@ -231,13 +361,15 @@ __global__ void __launch_bounds__(kThreads) attn_weight_stats_kernel(const Weigh
             }
             if constexpr (NOCT == 1) {
                 const int g = lane >> 2, t = lane & 3;
-                float* dst = a.score + ((b * a.num_kv_heads + head) * a.max_kvlen + tile0 + g) * a.score_rows + 2 * t;
+                if (2 * t < s.rows) {
+                    float* dst = score + (tile0 + g) * a.score_rows + 2 * t;
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        if (2 * t + c < s.rows && tile0 + g + 8 * p < s.len) {
-                            dst[p * 8 * a.score_rows + c] = acc[0][2 * p + c];
+                    for (int p = 0; p < 2; ++p) {
+                        if (tile0 + g + 8 * p < s.len) {
+                            dst[p * 8 * a.score_rows] = acc[0][2 * p];
+                            if (2 * t + 1 < s.rows) {
+                                dst[p * 8 * a.score_rows + 1] = acc[0][2 * p + 1];
+                            }
                         }
                     }
                 }
@@ -252,7 +384,8 @@ __global__ void __launch_bounds__(kThreads) attn_weight_stats_kernel(const Weigh
                     m[o][c] = top;
                 }
             }
-        }
+        };
+        for_tiles<DH, NOCT>(a, ring, b, first + warp * 16, end, s.len, lane, work);
         // over the eight positions a column's values are spread over, then over the warps
 #pragma unroll
         for (int o = 0; o < NOCT; ++o) {
@@ -315,7 +448,7 @@ __global__ void __launch_bounds__(256) attn_weight_merge_kernel(const WeightArgs
     if (i < 0 || i >= n) {
         return;
     }
-    const int32_t chunks = static_cast<int32_t>((len + kChunk - 1) / kChunk);
+    const int32_t chunks = static_cast<int32_t>((len + a.chunk - 1) / a.chunk);
     float m = kNegBig, l = 0.0f;
     for (int32_t c = lane; c < chunks; c += 32) {
         const float2 v = a.part[c * a.total_tokens * a.num_heads + id];
@@ -336,8 +469,9 @@ __global__ void __launch_bounds__(256) attn_weight_merge_kernel(const WeightArgs
 }
 
 template <int DH, int NOCT>
-__global__ void __launch_bounds__(kThreads) attn_weight_apply_kernel(const WeightArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) attn_weight_apply_kernel(const WeightArgs a) {
     __shared__ float sum[kChunk];
+    __shared__ __align__(128) uint8_t smem[kWarps * Ring<DH>::kWarpBytes];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int64_t b = blockIdx.z;
     const int head = blockIdx.x, chunk = blockIdx.y;  // neighbouring CTAs read neighbouring heads of the same rows
@@ -347,6 +481,7 @@ __global__ void __launch_bounds__(kThreads) attn_weight_apply_kernel(const Weigh
         return;
     }
     const int32_t end = first + kChunk < s.len ? first + kChunk : s.len;
+    const Ring<DH> ring(a, s, b, head, warp, lane, smem);
     float* w = a.weight + (a.geom.layer_idx * a.num_kv_heads + head) * a.max_tokens;
     for (int32_t row0 = 0; row0 < s.rows; row0 += NOCT * 8) {
         uint2 qf[NOCT][DH / 16];
@@ -368,10 +503,7 @@ __global__ void __launch_bounds__(kThreads) attn_weight_apply_kernel(const Weigh
             }
         }
         const bool last_rows = row0 + NOCT * 8 >= s.rows;
-        for (int32_t tile0 = first + warp * 16; tile0 < end; tile0 += kWarps * 16) {
-            Tile<DH, NOCT> tile;
-            int64_t row;
-            tile.load(a, b, head, tile0, s.len, lane, row);
+        auto work = [&](const Tile<DH, NOCT>& tile, int32_t tile0) {
             float acc[NOCT][4];
             tile.scores(qf, acc);
             if (tile0 + 15 > s.start || tile0 + 15 >= s.len) {
@@ -403,11 +535,15 @@ __global__ void __launch_bounds__(kThreads) attn_weight_apply_kernel(const Weigh
                 }
                 if (!last_rows) {
                     *acc_row = x;
-                } else if (tile0 + i < s.len && row >= 0 && cache_row_ok(row + i, a.max_tokens)) {
-                    atomicAdd(w + row + i, x);
+                } else if (tile0 + i < s.len) {
+                    const int64_t row = ring.row_of(a, b, tile0);
+                    if (row >= 0 && cache_row_ok(row + i, a.max_tokens)) {
+                        atomicAdd(w + row + i, x);
+                    }
                 }
             }
-        }
+        };
+        for_tiles<DH, NOCT>(a, ring, b, first + warp * 16, end, s.len, lane, work);
     }
 }
 
@@ -417,7 +553,7 @@ __global__ void __launch_bounds__(256) attn_weight_spread_kernel(const WeightArg
     const int64_t b = blockIdx.z;
     const int head = blockIdx.x;
     const Span s = span_of(a, b);
-    const int32_t first = blockIdx.y * kChunk;
+    const int32_t first = blockIdx.y * kSpread;
     if (first >= s.len) {
         return;
     }
@@ -428,20 +564,35 @@ __global__ void __launch_bounds__(256) attn_weight_spread_kernel(const WeightArg
     __syncthreads();
     float* w = a.weight + (a.geom.layer_idx * a.num_kv_heads + head) * a.max_tokens;
     const float* score = a.score + (b * a.num_kv_heads + head) * a.max_kvlen * a.score_rows;
+    const int64_t start_row = a.geom.cache_mode == 0 ? a.cachestarts[b] : 0;
+    constexpr int kPer = kSpread / 256;  // positions of a thread: their loads go out together
+    const int32_t pos0 = first + threadIdx.x;
+    float sum[kPer];
 #pragma unroll
-    for (int k = 0; k < kChunk / 256; ++k) {
-        const int32_t pos = first + k * 256 + threadIdx.x;
-        if (pos >= s.len) {
-            break;
+    for (int k = 0; k < kPer; ++k) {
+        sum[k] = 0.0f;
+    }
+    for (int32_t r = 0; r < s.rows; ++r) {
+        const float2 v = norm[r];
+        float x[kPer];
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            x[k] = pos0 + k * 256 < s.len ? score[static_cast<int64_t>(pos0 + k * 256) * a.score_rows + r] : -INFINITY;
         }
-        float sum = 0.0f;
-        for (int32_t r = 0; r < s.rows; ++r) {
-            const float2 v = norm[r];
-            sum = fmaf(ex2_approx(fmaf(score[static_cast<int64_t>(pos) * a.score_rows + r], a.scale_log2, -v.x)), v.y, sum);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            sum[k] = fmaf(ex2_approx(fmaf(x[k], a.scale_log2, -v.x)), v.y, sum[k]);
         }
-        const int64_t row = cache_row(a.geom, a.cachestarts, b, pos);
-        if (cache_row_ok(row, a.max_tokens)) {
-            atomicAdd(w + row, sum);  // one addition per position and call
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int32_t pos = pos0 + k * 256;
+        if (pos < s.len) {
+            const int64_t row = a.geom.cache_mode == 0 ? (start_row < 0 ? -1 : start_row + pos)
+                                                       : cache_row(a.geom, a.cachestarts, b, pos);
+            if (cache_row_ok(row, a.max_tokens)) {
+                atomicAdd(w + row, sum[k]);  // one addition per position and call
+            }
         }
     }
 }
@@ -468,7 +619,8 @@ int launch_dh(const pplb200_attn_params& p, const WeightArgs& a, cudaStream_t st
         return rc;
     }
     if (rows <= kScoreRows) {
-        attn_weight_spread_kernel<<<grid, 256, 0, stream>>>(a);
+        const dim3 spread(grid.x, static_cast<unsigned>((p.max_kvlen + kSpread - 1) / kSpread), grid.z);
+        attn_weight_spread_kernel<<<spread, 256, 0, stream>>>(a);
         return check_launch("attn_weight_spread_kernel");
     }
     attn_weight_apply_kernel<DH, kRowBlock / 8><<<grid, kThreads, 0, stream>>>(a);
@@ -478,13 +630,20 @@ int launch_dh(const pplb200_attn_params& p, const WeightArgs& a, cudaStream_t st
 }  // namespace
 
 int make_weight_plan(const pplb200_attn_params& p, WeightPlan* plan) {
-    plan->chunks = (p.max_kvlen + kChunk - 1) / kChunk;
+    // With kept scores a CTA's start (lengths, rows and queries, each waiting for the one before) is worth longer chunks
+    // as long as there are some 8 CTAs for each place on the chip.
+    const bool kept = p.max_seqlen > 0 && p.max_seqlen * (p.num_heads / p.num_kv_heads) <= kScoreRows;
+    plan->chunk = kChunk;
+    while (kept && plan->chunk < 8 * kChunk &&
+           p.batch * p.num_kv_heads * ((p.max_kvlen + 2 * plan->chunk - 1) / (2 * plan->chunk)) >= 148 * 4 * 8) {
+        plan->chunk *= 2;
+    }
+    plan->chunks = (p.max_kvlen + plan->chunk - 1) / plan->chunk;
     const uint64_t rows = static_cast<uint64_t>(p.total_tokens) * p.num_heads;
     plan->off_norm = 256;  // behind the status word
     plan->off_part = plan->off_norm + (rows * 8 + 255) / 256 * 256;
     plan->off_score = plan->off_part + (rows * plan->chunks * 8 + 255) / 256 * 256;
     plan->score_rows = static_cast<int32_t>(p.max_seqlen * (p.num_heads / p.num_kv_heads));
-    const bool kept = p.max_seqlen > 0 && p.max_seqlen * (p.num_heads / p.num_kv_heads) <= kScoreRows;
     const uint64_t positions = static_cast<uint64_t>(p.batch) * p.num_kv_heads * p.max_kvlen;
     plan->bytes = plan->off_score + (kept ? (positions * plan->score_rows * 4 + 255) / 256 * 256 : 0);
     return plan->chunks > 65535 ? PPLB200_UNSUPPORTED : PPLB200_SUCCESS;  // a grid dimension
@@ -520,6 +679,7 @@ int launch_attn_weight(const pplb200_attn_params& p, const CacheGeom& geom, cons
     a.group = p.num_heads / p.num_kv_heads;
     a.causal = p.is_causal ? 1 : 0;
     a.chunks = static_cast<int32_t>(plan.chunks);
+    a.chunk = plan.chunk;
     a.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(p.head_dim));
     return p.head_dim == 128 ? launch_dh<128>(p, a, stream) : launch_dh<64>(p, a, stream);
 }

@@ -136,7 +136,8 @@ int launch_tree_attn(const pplb200_attn_params& p, const CacheGeom& geom, const 
 
 // ---- accumulated attention weight, eviction, compaction --------------------------------------------
 struct WeightPlan {
-    int64_t chunks;  // chunks of positions per sequence
+    int32_t chunk;   // positions of a chunk
+    int64_t chunks;  // chunks per sequence
     int32_t score_rows;  // query rows per kv head
     uint64_t off_norm, off_part, off_score, bytes;
 };
