@@ -3,9 +3,9 @@
 //
 // The normaliser of a row needs all its scores before any weight is known.  attn_weight_stats_kernel leaves, per query
 // row and chunk of positions, the maximum and the sum of exponentials, and attn_weight_merge_kernel joins the chunks.
-// Then, with up to 8 query rows per kv head (decode steps), the scores themselves have been written to the workspace
-// (4 bytes a row against the 160 of a K row at Dh 128) and attn_weight_spread_kernel only reads those; with more rows
-// attn_weight_apply_kernel forms them again and adds each position's normalised weights up.
+// With up to 8 query rows per kv head (decode steps) the scores themselves go to the workspace as well (4 bytes a row
+// against the 160 of a K row at Dh 128), and attn_weight_spread_kernel joins the chunks and reads the scores; with more
+// rows attn_weight_apply_kernel forms them again and adds each position's normalised weights up.
 //
 // Both score kernels: a CTA takes a chunk of the positions of one (sequence, kv head), a warp 16 positions at a
 // time.  Positions are the M dimension of mma.m16n8k16, the query rows (token x head of the group) come in octets as
@@ -206,8 +206,12 @@ struct Tile {
             for (int h = 0; h < DH / 64; ++h) {
                 asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                              : "=r"(code[r][h].x), "=r"(code[r][h].y), "=r"(code[r][h].z), "=r"(code[r][h].w)
-                             : "r"((h == 0 ? code_addr : code_addr ^ 64u) + r * 8 * DH));
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sc[r][h]) : "r"(scale_addr + r * 8 * (DH / 4) + h * 16));
+                             : "r"((h == 0 ? code_addr : code_addr ^ 64u) + r * 8 * DH)
+                             : "memory");
+                asm volatile("ld.shared.u32 %0, [%1];"
+                             : "=r"(sc[r][h])
+                             : "r"(scale_addr + r * 8 * (DH / 4) + h * 16)
+                             : "memory");
             }
         }
     }
@@ -328,6 +332,8 @@ __device__ __forceinline__ void for_tiles(const WeightArgs& a, const Ring<DH>& r
 
 template <int DH, int NOCT>
 __global__ void __launch_bounds__(kThreads, NOCT == 1 ? 6 : 3) attn_weight_stats_kernel(const WeightArgs a) {
+    grid_launch_dependents();
+    grid_dependency_wait();
     __shared__ float2 red[kWarps][NOCT * 8];
     __shared__ __align__(128) uint8_t smem[kWarps * Ring<DH>::kWarpBytes];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -423,8 +429,29 @@ __global__ void __launch_bounds__(kThreads, NOCT == 1 ? 6 : 3) attn_weight_stats
     }
 }
 
+// Maximum and reciprocal sum of row `at` over its chunks; all lanes of a warp call it.
+__device__ __forceinline__ float2 join_chunks(const WeightArgs& a, int64_t at, int32_t chunks, int lane) {
+    float m = kNegBig, l = 0.0f;
+    for (int32_t c = lane; c < chunks; c += 32) {
+        const float2 v = a.part[c * a.total_tokens * a.num_heads + at];
+        const float top = fmaxf(m, v.x);
+        l = l * ex2_approx(m - top) + v.y * ex2_approx(v.x - top);
+        m = top;
+    }
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const float om = __shfl_xor_sync(0xffffffffu, m, x), ol = __shfl_xor_sync(0xffffffffu, l, x);
+        const float top = fmaxf(m, om);
+        l = l * ex2_approx(m - top) + ol * ex2_approx(om - top);
+        m = top;
+    }
+    return make_float2(m, l > 0.0f ? 1.0f / l : 0.0f);
+}
+
 // One warp per (query token, head): joins the chunks of its sequence.
 __global__ void __launch_bounds__(256) attn_weight_merge_kernel(const WeightArgs a, int32_t batch) {
+    grid_launch_dependents();
+    grid_dependency_wait();
     const int lane = threadIdx.x & 31;
     const int64_t id = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
     const int64_t tok = id / a.num_heads;
@@ -448,28 +475,16 @@ __global__ void __launch_bounds__(256) attn_weight_merge_kernel(const WeightArgs
     if (i < 0 || i >= n) {
         return;
     }
-    const int32_t chunks = static_cast<int32_t>((len + a.chunk - 1) / a.chunk);
-    float m = kNegBig, l = 0.0f;
-    for (int32_t c = lane; c < chunks; c += 32) {
-        const float2 v = a.part[c * a.total_tokens * a.num_heads + id];
-        const float top = fmaxf(m, v.x);
-        l = l * ex2_approx(m - top) + v.y * ex2_approx(v.x - top);
-        m = top;
-    }
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, x), ol = __shfl_xor_sync(0xffffffffu, l, x);
-        const float top = fmaxf(m, om);
-        l = l * ex2_approx(m - top) + ol * ex2_approx(om - top);
-        m = top;
-    }
+    const float2 v = join_chunks(a, id, static_cast<int32_t>((len + a.chunk - 1) / a.chunk), lane);
     if (lane == 0) {
-        a.norm[id] = make_float2(m, l > 0.0f ? 1.0f / l : 0.0f);
+        a.norm[id] = v;
     }
 }
 
 template <int DH, int NOCT>
 __global__ void __launch_bounds__(kThreads, 3) attn_weight_apply_kernel(const WeightArgs a) {
+    grid_launch_dependents();
+    grid_dependency_wait();
     __shared__ float sum[kChunk];
     __shared__ __align__(128) uint8_t smem[kWarps * Ring<DH>::kWarpBytes];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -549,6 +564,8 @@ __global__ void __launch_bounds__(kThreads, 3) attn_weight_apply_kernel(const We
 
 // One thread per position: the weights of the kept scores.
 __global__ void __launch_bounds__(256) attn_weight_spread_kernel(const WeightArgs a) {
+    grid_launch_dependents();
+    grid_dependency_wait();
     __shared__ float2 norm[kScoreRows];
     const int64_t b = blockIdx.z;
     const int head = blockIdx.x;
@@ -557,9 +574,15 @@ __global__ void __launch_bounds__(256) attn_weight_spread_kernel(const WeightArg
     if (first >= s.len) {
         return;
     }
-    if (static_cast<int32_t>(threadIdx.x) < s.rows) {
-        const int32_t i = threadIdx.x / a.group;
-        norm[threadIdx.x] = a.norm[(s.tok0 + i) * a.num_heads + head * a.group + (threadIdx.x - i * a.group)];
+    // a warp per query row joins its chunks
+    const int32_t my_row = threadIdx.x >> 5;
+    if (my_row < s.rows) {
+        const int32_t i = my_row / a.group;
+        const int64_t at = (s.tok0 + i) * a.num_heads + head * a.group + (my_row - i * a.group);
+        const float2 v = join_chunks(a, at, (s.len + a.chunk - 1) / a.chunk, threadIdx.x & 31);
+        if ((threadIdx.x & 31) == 0) {
+            norm[my_row] = v;
+        }
     }
     __syncthreads();
     float* w = a.weight + (a.geom.layer_idx * a.num_kv_heads + head) * a.max_tokens;
@@ -600,30 +623,30 @@ __global__ void __launch_bounds__(256) attn_weight_spread_kernel(const WeightArg
 template <int DH>
 int launch_dh(const pplb200_attn_params& p, const WeightArgs& a, cudaStream_t stream) {
     const dim3 grid(static_cast<unsigned>(p.num_kv_heads), static_cast<unsigned>(a.chunks), static_cast<unsigned>(p.batch));
-    const int64_t rows = p.max_seqlen * a.group;
-    int rc;
-    if (rows <= kScoreRows) {
-        attn_weight_stats_kernel<DH, 1><<<grid, kThreads, 0, stream>>>(a);
-    } else {
-        attn_weight_stats_kernel<DH, kRowBlock / 8><<<grid, kThreads, 0, stream>>>(a);
+    // each kernel starts while the one before it drains, and waits for it before it reads anything
+    if (p.max_seqlen * a.group <= kScoreRows) {
+        launch_dependent(attn_weight_stats_kernel<DH, 1>, grid, dim3(kThreads), 0, stream, a);
+        const int rc = check_launch("attn_weight_stats_kernel");
+        if (rc != PPLB200_SUCCESS) {
+            return rc;
+        }
+        const dim3 spread(grid.x, static_cast<unsigned>((p.max_kvlen + kSpread - 1) / kSpread), grid.z);
+        launch_dependent(attn_weight_spread_kernel, spread, dim3(256), 0, stream, a);
+        return check_launch("attn_weight_spread_kernel");
     }
-    rc = check_launch("attn_weight_stats_kernel");
+    launch_dependent(attn_weight_stats_kernel<DH, kRowBlock / 8>, grid, dim3(kThreads), 0, stream, a);
+    int rc = check_launch("attn_weight_stats_kernel");
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
     const int64_t warps = p.total_tokens * p.num_heads;
-    attn_weight_merge_kernel<<<static_cast<unsigned>((warps * 32 + 255) / 256), 256, 0, stream>>>(
-        a, static_cast<int32_t>(p.batch));
+    launch_dependent(attn_weight_merge_kernel, dim3(static_cast<unsigned>((warps * 32 + 255) / 256)), dim3(256), 0, stream, a,
+                     static_cast<int32_t>(p.batch));
     rc = check_launch("attn_weight_merge_kernel");
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    if (rows <= kScoreRows) {
-        const dim3 spread(grid.x, static_cast<unsigned>((p.max_kvlen + kSpread - 1) / kSpread), grid.z);
-        attn_weight_spread_kernel<<<spread, 256, 0, stream>>>(a);
-        return check_launch("attn_weight_spread_kernel");
-    }
-    attn_weight_apply_kernel<DH, kRowBlock / 8><<<grid, kThreads, 0, stream>>>(a);
+    launch_dependent(attn_weight_apply_kernel<DH, kRowBlock / 8>, grid, dim3(kThreads), 0, stream, a);
     return check_launch("attn_weight_apply_kernel");
 }
 

@@ -126,7 +126,7 @@ struct TreePlan {
     int32_t lanes;   // classes of kv heads
     int64_t ranges;  // ranges of blocks per class, one for each of ranges * lanes persistent CTAs
     int64_t words;   // 64-bit words of a token's ancestor mask
-    uint64_t off_prefix, off_ancestor, off_part_ml, off_part_o, bytes;
+    uint64_t off_prefix, off_flags, off_ancestor, off_part_ml, off_part_o, bytes;
 };
 int make_tree_plan(const pplb200_attn_params& p, int sm_count, TreePlan* plan);
 int launch_tree_attn(const pplb200_attn_params& p, const CacheGeom& geom, const TreePlan& plan, const void* query,

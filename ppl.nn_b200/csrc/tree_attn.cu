@@ -14,8 +14,8 @@
 //     per range), which tree_merge_kernel joins.
 //   * tree_plan_kernel turns the device-side lengths into the prefix sum of blocks, and the parents into one bit mask
 //     of ancestors per token.  Only blocks that reach behind the history look at the masks, 64 bits a row and block.
-//   * Roles of a CTA: 4 MT softmax warps, one thread per query row; four converter warps, which turn the raw codes and
-//     scales of a block into the swizzled fp16 K and V tiles; MT warps that issue the MMAs of a 128-row tile each; one
+//   * Roles of a CTA: 4 MT softmax warps, one thread per query row; four warps each that turn the raw codes and scales
+//     of a block into the swizzled fp16 K and V tiles; MT warps that issue the MMAs of a 128-row tile each; one
 //     warp that fetches the raw blocks by TMA into a ring of two, K and V apart.  S = Q K^T goes to a 64-column TMEM
 //     buffer, P returns to TMEM as the A operand of O += P V (two buffers), as in the prefill kernel.
 //   * MT = 1: two CTAs per SM.  MT = 2, for more than 128 rows per kv head: one CTA per SM, whose two tiles share the
@@ -44,9 +44,16 @@ constexpr float kRescaleSlack = 8.0f;
 template <int DH, int MT>
 struct TTraits {
     static constexpr int kBlockM = kTileM * MT;
-    static constexpr int kThreads = 32 * (4 * MT + 4 + MT + 1);
+    static constexpr int kThreads = 32 * (4 * MT + 8 + 4);  // whole warpgroups: registers are dealt to those
+    // registers of a softmax, converter and other thread; the launch gives all the same, 65 536 / kThreads / kCtasPerSm
+    // rounded down to the allocation's granularity (64 and 96)
+    // registers of a softmax, converter and other thread; the launch gives all the same, 65 536 / kThreads / kCtasPerSm
+    // rounded down to the allocation's granularity
+    static constexpr int kSoftmaxRegs = MT == 1 ? 96 : 128, kConvRegs = MT == 1 ? 56 : 72, kOtherRegs = MT == 1 ? 48 : 72;
+    static constexpr int kLaunchRegs = MT == 1 ? 64 : 96;
+    static_assert(4 * MT * kSoftmaxRegs + 8 * kConvRegs + 4 * kOtherRegs <= (4 * MT + 12) * kLaunchRegs, "register split");
     static constexpr int kCtasPerSm = MT == 1 ? 2 : 1;
-    static constexpr int kConvWarp = 4 * MT, kMmaWarp = kConvWarp + 4, kLoadWarp = kMmaWarp + MT;
+    static constexpr int kConvWarp = 4 * MT, kMmaWarp = kConvWarp + 8, kLoadWarp = kMmaWarp + MT;
     static constexpr int kColBlocks = DH / 64;
     static constexpr int kQBlockBytes = kTileM * 128;
     static constexpr int kKVBlockBytes = kBlockN * 128;
@@ -56,10 +63,11 @@ struct TTraits {
     static constexpr int kRawBytes = kCodeBytes + kBlockN * (DH / 8) * 2;  // codes and scales of K or V of a block
     // The same for every head size, so that never more CTAs share an SM than its TMEM holds; MT = 2 asks for more
     // than half of the SM's.
-    static constexpr int kSmemBytes = MT * 32768 + 2 * (kBlockN * 256) + 2 * kRawStages * (kBlockN * 160) + 512;
-    static constexpr uint32_t kPCols = kBlockN / 2;
-    static constexpr uint32_t kColS = 0, kColP = kBlockN, kColO = kColP + 2 * kPCols;
-    static constexpr uint32_t kTileCols = 256;  // TMEM columns of a tile: S 64 | P 2 x 32 | O 128
+    static constexpr int kJoinBytes = 2 * kTileM * 8 * 4;  // per tile: joining the replicas of few rows
+    static constexpr int kSmemBytes = MT * 32768 + 2 * (kBlockN * 256) + 2 * kRawStages * (kBlockN * 160) + MT * kJoinBytes + 512;
+    // TMEM columns of a tile: S0 64 | S1 64 | O 128; P of a block takes the first half of its S
+    static constexpr uint32_t kColO = 2 * kBlockN;
+    static constexpr uint32_t kTileCols = 256;
 };
 
 struct TreeHeader {
@@ -80,6 +88,7 @@ struct TreeArgs {
     __half* out;
     TreeHeader* hdr;
     int64_t* prefix;     // [batch + 1] blocks before each sequence
+    uint32_t* flags;     // [batch] what the planning of each sequence has to report
     uint64_t* ancestor;  // [total_tokens][words]
     float* part_o;       // [slots][128][Dh]
     float2* part_ml;     // [slots][128]
@@ -132,9 +141,12 @@ __global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(const TreeArgs 
     __shared__ int64_t carry;
     __shared__ int32_t up[kTreeMaxTokens];
     const int tid = threadIdx.x;
+    grid_launch_dependents();
+    grid_dependency_wait();  // the workspace may still be read by the previous call's kernels
     if (blockIdx.x == 0) {
         if (tid == 0) {
             carry = 0;
+            a.hdr->status = 0;
         }
         __syncthreads();
         for (int32_t base = 0; base < a.batch; base += kPlanThreads) {
@@ -166,21 +178,21 @@ __global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(const TreeArgs 
     }
     const int32_t b = blockIdx.x - 1;
     const Seq s = seq_of(a, b);
-    if (tid == 0) {
-        const int64_t n = a.seqstarts[b + 1] - s.tok0;
-        if (n != s.n || a.start_pos[b] != s.start || s.start + n > a.max_kvlen) {
-            atomicOr(&a.hdr->status, kDevLengthClamped);
-        }
-    }
+    const int64_t n = a.seqstarts[b + 1] - s.tok0;
+    bool bad = false;
     for (int32_t i = tid; i < s.n; i += kPlanThreads) {
         int64_t p = a.parents != nullptr ? a.parents[s.tok0 + i] : i - 1;
         if (p < -1 || p >= i) {
-            atomicOr(&a.hdr->status, kDevParentInvalid);
+            bad = true;
             p = -1;
         }
         up[i] = static_cast<int32_t>(p);
     }
-    __syncthreads();
+    bad = __syncthreads_or(bad);
+    if (tid == 0) {
+        const bool cut = n != s.n || a.start_pos[b] != s.start || s.start + n > a.max_kvlen;
+        a.flags[b] = (cut ? kDevLengthClamped : 0u) | (bad ? kDevParentInvalid : 0u);
+    }
     for (int32_t i = tid; i < s.n; i += kPlanThreads) {
         uint64_t* row = a.ancestor + (s.tok0 + i) * a.words;
         int32_t at = i;  // ancestors have strictly smaller indices: the words fill from the highest down
@@ -227,8 +239,10 @@ struct Barriers {
     uint64_t q_full, q_empty;
     uint64_t raw_full[2][kRawStages], raw_empty[2][kRawStages];  // [K | V]
     uint64_t k_full, k_empty, v_full, v_empty;
-    uint64_t o_free[MT], s_full[MT], s_free[MT];
-    uint64_t p_full[MT][2], pv_done[MT][2];
+    uint64_t o_free[MT];
+    // One per S buffer: who waits for block x knows that block x - 2 is done, and block x + 2 needs what it holds, so the
+    // parity of the phase is never mistaken.
+    uint64_t s_full[MT][2], p_full[MT][2], pv_done[MT][2];
     uint32_t tmem_slot;
     int abort_word;
 };
@@ -253,12 +267,15 @@ __device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
     return v;
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
     uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
 
@@ -316,6 +333,85 @@ __device__ __forceinline__ void load_rows(const TreeArgs& a, void* dst, const CU
     tma_load_5d(dst, map, bar, 0, c[0], c[1], c[2], c[3]);
 }
 
+// Few rows leave most of a tile's 128 lanes empty, and a softmax takes a warp the same time for one row as for 32.  Up to
+// 32 rows (64) are therefore put into the tile 4 (2) times, and each replica takes the softmax of a quarter (half) of
+// a block's positions; the weights of the other positions are zeros in its rows of P.  The replicas are joined like
+// the parts of a segment when the segment's part ends.
+__device__ __forceinline__ int replicas(int32_t rows) {
+    return rows <= 32 ? 4 : (rows <= 64 ? 2 : 1);
+}
+
+// Maximum of N raw scores, of which bit e of `seen` says whether score e counts
+template <int N>
+__device__ __forceinline__ float max_of(float (&v)[N], bool masked, uint32_t seen) {
+    if (masked) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            v[e] = (seen >> e) & 1u ? v[e] : -INFINITY;
+        }
+    }
+    float a = fmax3(v[0], v[1], v[2]), b = fmax3(v[3], v[4], v[5]);
+#pragma unroll
+    for (int e = 6; e + 3 < N; e += 4) {
+        a = fmax3(a, v[e], v[e + 1]);
+        b = fmax3(b, v[e + 2], v[e + 3]);
+    }
+    return fmax3(a, b, fmaxf(v[N - 2], v[N - 1]));
+}
+
+// N scores -> N / 2 columns of packed fp16 weights exp2(s * scale - m).  The row sum adds the rounded values that P V
+// uses, in four chains (one chain of N dependent additions would be as long as the exponentials).
+template <int N>
+__device__ __forceinline__ float weights_of(const float (&v)[N], float sc, float m, uint32_t (&pk)[N / 2]) {
+    float l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) {
+        const float2 x = __ffma2_rn(make_float2(v[2 * e], v[2 * e + 1]), make_float2(sc, sc), make_float2(-m, -m));
+        pk[e] = h2_as_u32(__floats2half2_rn(ex2_approx(x.x), ex2_approx(x.y)));
+        add_half2_to_float(l[e & 3], pk[e]);
+    }
+    return (l[0] + l[1]) + (l[2] + l[3]);
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void load_scores(uint32_t taddr, float (&v)[32]) {
+    uint32_t u[32];
+    tmem_ld32(taddr, u);
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+        v[e] = __uint_as_float(u[e]);
+    }
+}
+__device__ __forceinline__ void load_scores(uint32_t taddr, float (&v)[16]) {
+    tmem_ld16(taddr, v);
+    tmem_wait_ld();
+}
+
+// Barrier of the four softmax warps of tile t (it counts warps: the lanes have to come together)
+__device__ __forceinline__ void tile_barrier(int t) {
+    __syncwarp();
+    asm volatile("bar.sync %0, 128;" ::"r"(t + 1) : "memory");
+}
+
+// The warpgroup's registers per thread from here on
+template <int N, bool UP>
+__device__ __forceinline__ void set_registers() {
+    if constexpr (UP) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+    }
+}
+
 template <int DH, int MT>
 __global__ void __launch_bounds__(TTraits<DH, MT>::kThreads, TTraits<DH, MT>::kCtasPerSm)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_constant__ CUtensorMap tm_scale, const TreeArgs a) {
@@ -325,16 +421,26 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
     uint8_t* sK = sQ + MT * T::kQBytes;
     uint8_t* sV = sK + T::kKVBytes;
     uint8_t* sRaw = sV + T::kKVBytes;  // [stage][K | V]
-    Barriers<MT>& bars = *reinterpret_cast<Barriers<MT>*>(sRaw + 2 * kRawStages * T::kRawBytes);
+    float* sJoin = reinterpret_cast<float*>(sRaw + 2 * kRawStages * T::kRawBytes);  // [tile][2][128][8]
+    Barriers<MT>& bars = *reinterpret_cast<Barriers<MT>*>(reinterpret_cast<uint8_t*>(sJoin) + MT * T::kJoinBytes);
     volatile int* abort_flag = &bars.abort_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t* status = &a.hdr->status;
 
+    grid_launch_dependents();
+    grid_dependency_wait();
     if ((smem_u32(smem) & 1023u) != 0u) {  // no static shared memory: the window starts on a 1 KB boundary
         if (threadIdx.x == 0) {
             atomicOr(status, kDevMmaTimeout);
         }
         return;
+    }
+    if (blockIdx.x == 0) {  // the status word has been cleared: now it can take what the planning found
+        for (int32_t b = threadIdx.x; b < a.batch; b += T::kThreads) {
+            if (a.flags[b] != 0u) {
+                atomicOr(status, a.flags[b]);
+            }
+        }
     }
     const int lane_class = blockIdx.x % a.lanes;
     const int64_t begin = blockIdx.x / a.lanes * a.hdr->range;
@@ -359,11 +465,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
         mbar_init(&bars.v_empty, MT);
         for (int t = 0; t < MT; ++t) {
             mbar_init(&bars.o_free[t], 128);
-            mbar_init(&bars.s_full[t], 1);
-            mbar_init(&bars.s_free[t], 128);
             for (int i = 0; i < 2; ++i) {
-                mbar_init(&bars.p_full[t][i], 128);
                 mbar_init(&bars.pv_done[t][i], 1);
+                mbar_init(&bars.s_full[t][i], 1);
+                mbar_init(&bars.p_full[t][i], 128);
             }
         }
         mbar_fence_init();
@@ -379,6 +484,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
     tc_fence_after();
     const uint32_t tmem_base = bars.tmem_slot;
 
+    if (warp >= T::kMmaWarp) {
+        set_registers<T::kOtherRegs, false>();
+    } else if (warp >= T::kConvWarp) {
+        set_registers<T::kConvRegs, false>();
+    } else {
+        set_registers<T::kSoftmaxRegs, true>();
+    }
     if (warp == T::kLoadWarp) {
         // =========================== TMA producer ===========================
         bool ok = true;
@@ -436,7 +548,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                 }
             }
         }
-    } else if (warp >= T::kMmaWarp) {
+    } else if (warp >= T::kMmaWarp && warp < T::kMmaWarp + MT) {
         // =========================== MMA issuer of one 128-row tile ===========================
         constexpr uint32_t idesc_qk = instr_desc_f16(kBlockN, false);
         constexpr uint32_t idesc_pv = instr_desc_f16(DH, true);
@@ -446,10 +558,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
         const uint32_t k_lo = desc_lo(smem_u32(sK), 16);
         const uint32_t v_lo = desc_lo(smem_u32(sV), T::kKVBlockBytes);
         const uint32_t tm = tmem_base + t * T::kTileCols;
-        const uint32_t d_s = tm + T::kColS, d_o = tm + T::kColO, a_p = tm + T::kColP;
+        const uint32_t d_o = tm + T::kColO;
         bool ok = true;
-        int pieces = 0, blocks_done = 0;    // of the CTA
-        int mine = 0, kc = 0, vc = 0;       // pieces, Q K^T and P V of this tile
+        int pieces = 0, blocks_done = 0;  // of the CTA
+        int mine = 0, kc = 0, vc = 0;     // pieces, Q K^T and P V of this tile
         for (int64_t u = begin; ok && u < end; ++pieces) {
             Piece p;
             piece_at(a, u, end, lane_class, lane, p);
@@ -474,15 +586,18 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                 }
                 continue;
             }
+            // Q K^T runs a block ahead of P V.  The scores of block j take the buffer of block j - 2, whose P has to
+            // have been read: MMAs with different accumulators need not run in the order of their issue.
             for (int32_t j = 0; ok && j <= blocks; ++j) {
                 if (j < blocks) {
                     ok = wait_or_abort(&bars.k_full, (blocks_done + j) & 1, abort_flag, status, kDevMmaTimeout) &&
-                         (kc == 0 || wait_or_abort(&bars.s_free[t], (kc - 1) & 1, abort_flag, status, kDevMmaTimeout));
+                         (vc == 0 || wait_or_abort(&bars.pv_done[t][(vc - 1) & 1], ((vc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout));
                     if (!ok) {
                         break;
                     }
                     tc_fence_after();
                     if (elect_one()) {
+                        const uint32_t d_s = tm + (kc & 1) * kBlockN;
 #pragma unroll
                         for (int cb = 0; cb < T::kColBlocks; ++cb) {
 #pragma unroll
@@ -492,7 +607,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                                            (cb | k) ? 1u : 0u);
                             }
                         }
-                        tc_commit(&bars.s_full[t]);
+                        tc_commit(&bars.s_full[t][kc & 1]);
                         tc_commit(&bars.k_empty);
                         if (j == blocks - 1) {
                             tc_commit(&bars.q_empty);
@@ -512,7 +627,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                     }
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t pa = a_p + (vc & 1) * T::kPCols;
+                        const uint32_t pa = tm + (vc & 1) * kBlockN;
 #pragma unroll
                         for (int ks = 0; ks < kBlockN / 16; ++ks) {
                             tc_mma_f16_ts(d_o, pa + 8 * ks, desc_join(v_lo + ks * (2048 >> 4), hi_sw128), idesc_pv,
@@ -528,212 +643,226 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
             blocks_done += blocks;
             ++mine;
         }
-    } else if (warp >= T::kConvWarp) {
+    } else if (warp >= T::kConvWarp && warp < T::kMmaWarp) {
         // =========================== converters ===========================
+        // The first four warps convert K (and bring Q), the others V.  K of block j + 1 is thus never behind V of block
+        // j, which has to wait for P V (j - 1), i.e. for a softmax.
         const int ct = threadIdx.x - 32 * T::kConvWarp;
+        const int kv = ct >= 128 ? 1 : 0;
         constexpr int kPieces = Raw<DH>::kPieces;
         const int piece = lane % kPieces;
-        const int row = (warp - T::kConvWarp) * 16 + lane / kPieces;  // first of the thread's rows of a block
-        const uint32_t k_tile = smem_u32(sK), v_tile = smem_u32(sV), raw0 = smem_u32(sRaw), q_tile = smem_u32(sQ);
+        const int row = ((warp - T::kConvWarp) & 3) * 16 + lane / kPieces;  // first of the thread's rows of a block
+        const uint32_t tile = smem_u32(kv ? sV : sK), raw0 = smem_u32(sRaw) + kv * T::kRawBytes, q_tile = smem_u32(sQ);
+        uint64_t* full = kv ? &bars.v_full : &bars.k_full;
+        uint64_t* empty = kv ? &bars.v_empty : &bars.k_empty;
         bool ok = true;
         int pieces = 0, n = 0;  // pieces and blocks so far
-        // K (0) or V (1) of the CTA's block number `blk_no`, of which `rows` rows exist
-        auto convert = [&](int kv, int blk_no, int32_t rows) -> bool {
-            const int s = blk_no % kRawStages;
-            if (!wait_or_abort(&bars.raw_full[kv][s], (blk_no / kRawStages) & 1, abort_flag, status, kDevTmaTimeout)) {
-                return false;
-            }
-            Raw<DH> raw;
-            raw.load(raw0 + (2 * s + kv) * T::kRawBytes, row, piece, rows);
-            mbar_arrive(&bars.raw_empty[kv][s]);
-            if (blk_no > 0 && !wait_or_abort(kv ? &bars.v_empty : &bars.k_empty, (blk_no - 1) & 1, abort_flag, status,
-                                             kDevMmaTimeout)) {
-                return false;
-            }
-            raw.store(kv ? v_tile : k_tile, row, piece);
-            fence_proxy_async_smem();
-            mbar_arrive(kv ? &bars.v_full : &bars.k_full);
-            return true;
-        };
         for (int64_t u = begin; ok && u < end; ++pieces) {
             Piece p;
             piece_at(a, u, end, lane_class, lane, p);
             u += p.blk1 - p.blk0;
-            // Q: row r of the tile is query row row0 + r = token x head of the group
-            if (pieces > 0) {
-                ok = wait_or_abort(&bars.q_empty, (pieces - 1) & 1, abort_flag, status, kDevMmaTimeout);
+            if (kv == 0) {
+                // Q: row r of the tile is query row row0 + r = token x head of the group
+                if (pieces > 0) {
+                    ok = wait_or_abort(&bars.q_empty, (pieces - 1) & 1, abort_flag, status, kDevMmaTimeout);
+                    if (!ok) {
+                        break;
+                    }
+                }
+                constexpr int kQPieces = DH / 8;  // 16-byte pieces of a query row
+                const int copies0 = replicas(p.rows_valid), copies1 = replicas(p.rows_valid - kTileM);  // of either tile
+                for (int i = ct; i < p.rows_valid * kQPieces; i += 128) {
+                    const int r = i / kQPieces, c = i - r * kQPieces;
+                    const int32_t qrow = p.row0 + r;
+                    const int32_t tok = qrow / a.group;
+                    const uint4 v = *reinterpret_cast<const uint4*>(
+                        a.q + ((p.seq.tok0 + tok) * a.num_heads + p.kvh * a.group + (qrow - tok * a.group)) * DH + c * 8);
+                    const uint32_t at = q_tile + (r / kTileM) * T::kQBytes + (c >> 3) * T::kQBlockBytes + (r % kTileM) * 128 +
+                                        (((c & 7) ^ (r & 7)) << 4);
+                    const int copies = r < kTileM ? copies0 : copies1;
+                    for (int f = 0; f < copies; ++f) {
+                        sts128(at + f * (kTileM / copies) * 128, v);
+                    }
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&bars.q_full);
+            }
+            for (int32_t blk = p.blk0; blk < p.blk1; ++blk, ++n) {
+                const int s = n % kRawStages;
+                ok = wait_or_abort(&bars.raw_full[kv][s], (n / kRawStages) & 1, abort_flag, status, kDevTmaTimeout);
                 if (!ok) {
                     break;
                 }
-            }
-            constexpr int kQPieces = DH / 8;  // 16-byte pieces of a query row
-            for (int i = ct; i < p.rows_valid * kQPieces; i += 128) {
-                const int r = i / kQPieces, c = i - r * kQPieces;
-                const int32_t qrow = p.row0 + r;
-                const int32_t tok = qrow / a.group;
-                const uint4 v = *reinterpret_cast<const uint4*>(
-                    a.q + ((p.seq.tok0 + tok) * a.num_heads + p.kvh * a.group + (qrow - tok * a.group)) * DH + c * 8);
-                sts128(q_tile + (r / kTileM) * T::kQBytes + (c >> 3) * T::kQBlockBytes + (r % kTileM) * 128 +
-                           (((c & 7) ^ (r & 7)) << 4), v);
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(&bars.q_full);
-            // K runs one block ahead of V: V(j) has to wait for P V(j - 1), i.e. for a softmax, and the scores of block
-            // j + 1 should not wait with it
-            ok = convert(0, n, p.seq.len - p.blk0 * kBlockN);
-            for (int32_t blk = p.blk0; ok && blk < p.blk1; ++blk, ++n) {
-                if (blk + 1 < p.blk1) {
-                    ok = convert(0, n + 1, p.seq.len - (blk + 1) * kBlockN);
+                Raw<DH> raw;
+                raw.load(raw0 + 2 * s * T::kRawBytes, row, piece, p.seq.len - blk * kBlockN);
+                // The loads have to be over before the slot is handed back.  The arrival alone does not see to that: the
+                // scales were found loaded behind it, next to their use, when the next copy had overwritten them.
+                __threadfence_block();
+                mbar_arrive(&bars.raw_empty[kv][s]);
+                ok = n == 0 || wait_or_abort(empty, (n - 1) & 1, abort_flag, status, kDevMmaTimeout);
+                if (!ok) {
+                    break;
                 }
-                ok = ok && convert(1, n, p.seq.len - blk * kBlockN);
+                raw.store(tile, row, piece);
+                fence_proxy_async_smem();
+                mbar_arrive(full);
             }
         }
-    } else {
+    } else if (warp < T::kConvWarp) {
         // =========================== softmax / epilogue ===========================
         const int t = warp >> 2, quarter = warp & 3;
-        const int r = quarter * 32 + lane;  // row of the tile = TMEM lane
-        const uint32_t t_lane = (static_cast<uint32_t>(quarter * 32) << 16) + t * T::kTileCols;
-        const uint32_t t_s = tmem_base + t_lane + T::kColS;
-        const uint32_t t_o = tmem_base + t_lane + T::kColO;
-        const uint32_t t_p = tmem_base + t_lane + T::kColP;
+        const int lane_row = quarter * 32 + lane;  // row of the tile = TMEM lane
+        const uint32_t t_tile = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + t * T::kTileCols;
+        const uint32_t t_o = t_tile + T::kColO;
         const float sc = a.scale_log2;
+        float* join = sJoin + t * (T::kJoinBytes / 4);
         bool ok = true;
         int pc = 0;
         for (int64_t u = begin; ok && u < end;) {
             Piece p;
             piece_at(a, u, end, lane_class, lane, p);
             u += p.blk1 - p.blk0;
-            const int32_t rows_valid = p.rows_valid - t * kTileM;  // of this tile
-            if (rows_valid <= 0) {
+            int32_t rows = p.rows_valid - t * kTileM;  // of this tile
+            if (rows <= 0) {
                 continue;
             }
-            if (quarter * 32 >= rows_valid) {
-                // the rows of this warp are behind the last one: its lanes only keep the barriers going
+            rows = rows < kTileM ? rows : kTileM;
+            const int copies = replicas(rows), spread = kTileM / copies;
+            const int copy = lane_row / spread, r = lane_row - copy * spread;  // row r of the tile, its copy
+            if (quarter * 32 - copy * spread >= rows) {
+                // no row of this warp exists: its lanes only keep the barriers going
                 for (int32_t blk = p.blk0; ok && blk < p.blk1; ++blk, ++pc) {
-                    ok = wait_or_abort_parked(&bars.s_full[t], pc & 1, abort_flag, status, kDevMmaTimeout);
+                    ok = wait_or_abort_parked(&bars.s_full[t][pc & 1], (pc >> 1) & 1, abort_flag, status, kDevMmaTimeout);
                     if (ok) {
-                        mbar_arrive(&bars.s_free[t]);
                         mbar_arrive(&bars.p_full[t][pc & 1]);
                     }
                 }
-                ok = ok && wait_or_abort_parked(&bars.pv_done[t][(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status,
-                                                kDevMmaTimeout);
-                if (ok) {
-                    mbar_arrive(&bars.o_free[t]);
+                ok = ok && wait_or_abort_parked(&bars.pv_done[t][(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
+                if (!ok) {
+                    break;
                 }
-                continue;
             }
-            const bool live = r < rows_valid;
+            const bool live = r < rows;
             const int32_t row = p.row0 + t * kTileM + r;
             const int32_t tok = live ? row / a.group : 0;
             const uint64_t* anc = a.ancestor + (p.seq.tok0 + tok) * a.words;
             float m_ref = kNegBig, l_sum = 0.0f;
-            for (int32_t blk = p.blk0; ok && blk < p.blk1; ++blk, ++pc) {
-                if (pc >= 2) {
-                    ok = wait_or_abort(&bars.pv_done[t][pc & 1], ((pc - 2) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
-                    if (!ok) {
-                        break;
-                    }
+            // `grown`: a maximum above the reference by more than 2^8; O is rescaled in TMEM, eight columns at a time
+            auto raise = [&](float top, bool rescale) -> bool {
+                const bool grow = top > m_ref + kRescaleSlack;
+                if (!__any_sync(0xffffffffu, grow)) {
+                    return true;
                 }
-                ok = wait_or_abort(&bars.s_full[t], pc & 1, abort_flag, status, kDevMmaTimeout);
+                const float m_new = grow ? top : m_ref;
+                const float f = ex2_approx(m_ref - m_new);
+                m_ref = m_new;
+                l_sum *= f;
+                if (rescale) {
+                    if (!wait_or_abort(&bars.pv_done[t][(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout)) {
+                        return false;
+                    }
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < DH / 8; ++c) {
+                        uint32_t v[8];
+                        tmem_ld8(t_o + c * 8, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                        }
+                        tmem_st8(t_o + c * 8, v);
+                    }
+                    tmem_wait_st();
+                }
+                return true;
+            };
+            for (int32_t blk = quarter * 32 - copy * spread < rows ? p.blk0 : p.blk1; ok && blk < p.blk1; ++blk, ++pc) {
+                ok = wait_or_abort(&bars.s_full[t][pc & 1], (pc >> 1) & 1, abort_flag, status, kDevMmaTimeout);
                 if (!ok) {
                     break;
                 }
                 tc_fence_after();
-                float sv[kBlockN];
-                {
-                    uint32_t v[kBlockN / 32][32];
-#pragma unroll
-                    for (int c = 0; c < kBlockN / 32; ++c) {
-                        tmem_ld32(t_s + 32 * c, v[c]);
-                    }
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int c = 0; c < kBlockN / 32; ++c) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            sv[32 * c + e] = __uint_as_float(v[c][e]);
-                        }
-                    }
-                }
-                tc_fence_before();
-                mbar_arrive(&bars.s_free[t]);
+                const uint32_t t_s = t_tile + (pc & 1) * kBlockN;
+                // 64 positions of this row: bit e = position blk * 64 + e is visible
                 const int32_t a0 = blk * kBlockN - p.seq.start;  // index of the block's first position among the drafts
-                if (a0 + kBlockN > 0) {
-                    // 64 positions of this row: bit e = position blk * 64 + e is visible
-                    uint64_t seen = ~0ull;
-                    if (live) {
-                        if (a0 <= 0) {
-                            seen = (a0 == 0 ? 0ull : ~0ull >> (64 + a0)) | (anc[0] << -a0);
-                        } else {
-                            const int32_t w = a0 >> 6, sh = a0 & 63;
-                            seen = w < a.words ? anc[w] >> sh : 0ull;
-                            if (sh > 0 && w + 1 < a.words) {
-                                seen |= anc[w + 1] << (64 - sh);
-                            }
-                        }
-                        const int32_t room = p.seq.len - blk * kBlockN;  // positions that exist
-                        if (room < kBlockN) {
-                            seen &= ~0ull >> (64 - room);
+                const bool masked = a0 + kBlockN > 0;
+                uint64_t seen = ~0ull;
+                if (masked && live) {
+                    if (a0 <= 0) {
+                        seen = (a0 == 0 ? 0ull : ~0ull >> (64 + a0)) | (anc[0] << -a0);
+                    } else {
+                        const int32_t w = a0 >> 6, sh = a0 & 63;
+                        seen = w < a.words ? anc[w] >> sh : 0ull;
+                        if (sh > 0 && w + 1 < a.words) {
+                            seen |= anc[w + 1] << (64 - sh);
                         }
                     }
-                    const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
-#pragma unroll
-                    for (int e = 0; e < kBlockN; ++e) {
-                        sv[e] = ((e < 32 ? lo : hi) >> (e & 31)) & 1u ? sv[e] : -INFINITY;
+                    const int32_t room = p.seq.len - blk * kBlockN;  // positions that exist
+                    if (room < kBlockN) {
+                        seen &= ~0ull >> (64 - room);
                     }
                 }
-                float mx0 = fmax3(sv[0], sv[1], sv[2]), mx1 = fmax3(sv[3], sv[4], sv[5]);
-#pragma unroll
-                for (int e = 6; e + 3 < kBlockN; e += 4) {
-                    mx0 = fmax3(mx0, sv[e], sv[e + 1]);
-                    mx1 = fmax3(mx1, sv[e + 2], sv[e + 3]);
-                }
-                float mx = fmax3(mx0, mx1, fmaxf(sv[kBlockN - 2], sv[kBlockN - 1]));
-                mx *= sc;
-                const bool grow = mx > m_ref + kRescaleSlack;
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float m_new = grow ? mx : m_ref;
-                    const float f = ex2_approx(m_ref - m_new);
-                    m_ref = m_new;
-                    l_sum *= f;
-                    if (blk > p.blk0) {
-                        ok = wait_or_abort(&bars.pv_done[t][(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
-                        if (!ok) {
-                            break;
-                        }
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int c = 0; c < DH / 8; ++c) {  // eight columns at a time: the scores stay in registers
-                            uint32_t v[8];
-                            tmem_ld8(t_o + c * 8, v);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                            }
-                            tmem_st8(t_o + c * 8, v);
-                        }
-                        tmem_wait_st();
+                const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
+                const bool rescale = blk > p.blk0;
+                if (copies == 1) {
+                    // all 64 positions, in two halves; the second is read twice, which keeps it out of the registers
+                    // while the first is worked on.  P of the first half overwrites scores that are done with.
+                    float v[32];
+                    load_scores(t_s + 32, v);
+                    float top = max_of(v, masked, hi);
+                    load_scores(t_s, v);
+                    top = fmaxf(top, max_of(v, masked, lo)) * sc;
+                    ok = raise(top, rescale);
+                    if (!ok) {
+                        break;
                     }
-                }
-                // P = exp2(s * scale - m_ref) as packed fp16; the row sum adds the rounded values that P V uses, in
-                // four chains (one chain of 64 dependent additions would be as long as the exponentials)
-                const uint32_t t_pb = t_p + (pc & 1) * T::kPCols;
-                float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int q = 0; q < kBlockN / 32; ++q) {
                     uint32_t pk[16];
+                    l_sum += weights_of(v, sc, m_ref, pk);
+                    tmem_st16(t_s, pk);
+                    load_scores(t_s + 32, v);
+                    if (masked) {
+                        max_of(v, true, hi);
+                    }
+                    l_sum += weights_of(v, sc, m_ref, pk);
+                    tmem_st16(t_s + 16, pk);
+                } else if (copies == 2) {
+                    float v[32];
+                    load_scores(t_s + copy * 32, v);
+                    ok = raise(max_of(v, masked, copy == 0 ? lo : hi) * sc, rescale);
+                    if (!ok) {
+                        break;
+                    }
+                    uint32_t pk[16];
+                    l_sum += weights_of(v, sc, m_ref, pk);
+                    tmem_st16(t_s + copy * 16, pk);
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float2 x = __ffma2_rn(make_float2(sv[32 * q + 2 * e], sv[32 * q + 2 * e + 1]),
-                                                    make_float2(sc, sc), make_float2(-m_ref, -m_ref));
-                        pk[e] = h2_as_u32(__floats2half2_rn(ex2_approx(x.x), ex2_approx(x.y)));
-                        add_half2_to_float(l4[e & 3], pk[e]);
+                        pk[e] = 0u;
                     }
-                    tmem_st16(t_pb + 16 * q, pk);
+                    tmem_st16(t_s + (copy ^ 1) * 16, pk);
+                } else {
+                    float v[16];
+                    load_scores(t_s + copy * 16, v);
+                    ok = raise(max_of(v, masked, (copy & 2 ? hi : lo) >> ((copy & 1) * 16)) * sc, rescale);
+                    if (!ok) {
+                        break;
+                    }
+                    uint32_t pk[8], zero[8];
+                    l_sum += weights_of(v, sc, m_ref, pk);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        zero[e] = 0u;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (c == copy) {
+                            tmem_st8(t_s + c * 8, pk);
+                        } else {
+                            tmem_st8(t_s + c * 8, zero);
+                        }
+                    }
                 }
-                l_sum += (l4[0] + l4[1]) + (l4[2] + l4[3]);
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(&bars.p_full[t][pc & 1]);
@@ -742,19 +871,27 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
             if (ok) {
                 ok = wait_or_abort(&bars.pv_done[t][(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
             }
-            if (ok) {
-                tc_fence_after();
-                const bool whole = p.blk0 == 0 && p.blk1 == p.seq.blocks;
+            if (!ok) {
+                break;
+            }
+            tc_fence_after();
+            const bool whole = p.blk0 == 0 && p.blk1 == p.seq.blocks;
+            const int64_t slot0 = (2 * static_cast<int64_t>(blockIdx.x) + (p.blk0 == 0 ? 1 : 0)) * T::kBlockM + t * kTileM;
+            auto out_row = [&](int32_t of) -> __half* {  // output row of row `of` of the tile
+                const int32_t x = p.row0 + t * kTileM + of, i = x / a.group;
+                return a.out + ((p.seq.tok0 + i) * a.num_heads + p.kvh * a.group + (x - i * a.group)) * DH;
+            };
+            if (copies == 1) {
                 const float inv = l_sum > 0.0f ? 1.0f / l_sum : 0.0f;
-                __half* dst = a.out + ((p.seq.tok0 + tok) * a.num_heads + p.kvh * a.group + (row - tok * a.group)) * DH;
-                const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (p.blk0 == 0 ? 1 : 0)) * T::kBlockM + t * kTileM + r;
-                float* part = a.part_o + slot * DH;
+                __half* dst = out_row(live ? r : 0);
+                float* part = a.part_o + (slot0 + r) * DH;
                 if (!whole && live) {
-                    a.part_ml[slot] = make_float2(m_ref, l_sum);
+                    a.part_ml[slot0 + r] = make_float2(m_ref, l_sum);
                 }
 #pragma unroll
                 for (int c = 0; c < DH / 32; ++c) {
                     uint32_t v[32];
+                    __syncwarp();
                     tmem_ld32(t_o + c * 32, v);
                     tmem_wait_ld();
                     if (c == DH / 32 - 1) {
@@ -784,6 +921,63 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                         }
                     }
                 }
+            } else {
+                // join the copies: their maxima and sums first, then eight channels at a time through shared memory
+                join[2 * lane_row] = m_ref;
+                join[2 * lane_row + 1] = l_sum;
+                tile_barrier(t);
+                float top = kNegBig, sum = 0.0f;
+                for (int f = 0; f < copies; ++f) {
+                    top = fmaxf(top, join[2 * (f * spread + r)]);
+                }
+                for (int f = 0; f < copies; ++f) {
+                    sum += join[2 * (f * spread + r) + 1] * ex2_approx(join[2 * (f * spread + r)] - top);
+                }
+                const float factor = ex2_approx(m_ref - top) * (whole ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f);
+                if (!whole && live && copy == 0) {
+                    a.part_ml[slot0 + r] = make_float2(top, sum);
+                }
+                tile_barrier(t);
+                // thread -> (row, channels): 128 threads share spread rows x 8 channels
+                const int per = 8 / copies;                            // channels of a thread
+                const int out_r = (lane_row * per) >> 3, out_c = (lane_row * per) & 7;
+                __half* dst = out_r < rows ? out_row(out_r) : nullptr;
+                float* part = a.part_o + (slot0 + out_r) * DH;
+#pragma unroll 1
+                for (int c = 0; c < DH / 8; ++c) {
+                    uint32_t v[8];
+                    __syncwarp();
+                    tmem_ld8(t_o + c * 8, v);
+                    tmem_wait_ld();
+                    if (c == DH / 8 - 1) {
+                        tc_fence_before();
+                        mbar_arrive(&bars.o_free[t]);
+                    }
+                    float* buf = join + (c & 1) * (kTileM * 8);
+                    float4* mine = reinterpret_cast<float4*>(buf + lane_row * 8);
+                    mine[0] = make_float4(__uint_as_float(v[0]) * factor, __uint_as_float(v[1]) * factor,
+                                          __uint_as_float(v[2]) * factor, __uint_as_float(v[3]) * factor);
+                    mine[1] = make_float4(__uint_as_float(v[4]) * factor, __uint_as_float(v[5]) * factor,
+                                          __uint_as_float(v[6]) * factor, __uint_as_float(v[7]) * factor);
+                    tile_barrier(t);  // two buffers: the next round's writes cannot meet this round's reads
+                    if (out_r < rows) {
+#pragma unroll 2
+                        for (int e = 0; e < per; e += 2) {
+                            float2 x = make_float2(0.0f, 0.0f);
+                            for (int f = 0; f < copies; ++f) {
+                                const float2 y = *reinterpret_cast<const float2*>(buf + (f * spread + out_r) * 8 + out_c + e);
+                                x.x += y.x;
+                                x.y += y.y;
+                            }
+                            if (whole) {
+                                *reinterpret_cast<__half2*>(dst + c * 8 + out_c + e) = __floats2half2_rn(x.x, x.y);
+                            } else {
+                                *reinterpret_cast<float2*>(part + c * 8 + out_c + e) = x;
+                            }
+                        }
+                    }
+                }
+                tile_barrier(t);
             }
         }
     }
@@ -798,61 +992,63 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
 
 // ---- joining the parts of a segment that several ranges hold -----------------------------------------
 
-// One warp per (query token, head).
+// A CTA per range and 32 query rows: the segment that begins in the range and goes on behind it, if there is one.  A
+// warp per row.
+constexpr int kMergeThreads = 512;
+constexpr int kMergeRows = 32;
+
 template <int DH>
-__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a) {
+__global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArgs a) {
     constexpr int kPer = DH / 32;  // channels of a lane
     const int lane = threadIdx.x & 31;
-    const int64_t id = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
-    const int64_t tok = id / a.num_heads;
-    if (tok >= a.total_tokens) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int64_t range = a.hdr->range, first = blockIdx.x / a.lanes, lane_class = blockIdx.x % a.lanes;
+    const int64_t last_unit = (first + 1) * range - 1;
+    if (last_unit + 1 >= a.hdr->total) {
         return;
     }
-    const int32_t head = static_cast<int32_t>(id - tok * a.num_heads);
-    const int32_t b = warp_find_segment(a.seqstarts, a.batch, tok, lane);
-    const Seq s = seq_of(a, b);
-    const int64_t i = tok - s.tok0;
-    if (i < 0 || i >= s.n) {
-        return;
+    Piece p;  // of the range's last block: its segment
+    piece_at(a, last_unit, last_unit + 1, static_cast<int>(lane_class), lane, p);
+    const int64_t u0 = last_unit - p.blk0, u1 = u0 + p.seq.blocks;  // units of the segment
+    if (u0 < first * range || u1 <= last_unit + 1) {
+        return;  // it began before the range, or ends with it
     }
-    const int32_t kvh = head / a.group;
-    const int32_t row = static_cast<int32_t>(i) * a.group + (head - kvh * a.group);
-    const int32_t rt = row / a.tile_rows, r = row - rt * a.tile_rows;
-    const int32_t vc = kvh / a.lanes, lane_class = kvh - vc * a.lanes;
-    const int64_t u0 = a.prefix[b] + (static_cast<int64_t>(vc) * s.row_tiles + rt) * s.blocks;
-    const int64_t range = a.hdr->range;
-    const int64_t first = u0 / range, last = (u0 + s.blocks - 1) / range;
-    if (first == last) {
-        return;  // one range held all of it and wrote the output
-    }
-    auto slot_of = [&](int64_t w) -> int64_t {
-        return (2 * (w * a.lanes + lane_class) + (u0 >= w * range ? 1 : 0)) * a.tile_rows + r;
-    };
-    float m = kNegBig;
-    for (int64_t w = first; w <= last; ++w) {
-        m = fmaxf(m, a.part_ml[slot_of(w)].x);
-    }
-    float l = 0.0f, o[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        o[e] = 0.0f;
-    }
-    for (int64_t w = first; w <= last; ++w) {
-        const int64_t slot = slot_of(w);
-        const float2 ml = a.part_ml[slot];
-        const float f = ex2_approx(ml.x - m);
-        const float* part = a.part_o + slot * DH + lane * kPer;
-        l += ml.y * f;
+    const int64_t last = (u1 - 1) / range;
+    const int32_t r0 = blockIdx.y * kMergeRows, r1 = r0 + kMergeRows < p.rows_valid ? r0 + kMergeRows : p.rows_valid;
+    for (int32_t r = r0 + (threadIdx.x >> 5); r < r1; r += kMergeThreads / 32) {
+        // the segment's first part is the second of its range's two, the others are first ones
+        auto slot_of = [&](int64_t w) -> int64_t {
+            return (2 * (w * a.lanes + lane_class) + (w == first ? 1 : 0)) * a.tile_rows + r;
+        };
+        float m = kNegBig;
+        for (int64_t w = first; w <= last; ++w) {
+            m = fmaxf(m, a.part_ml[slot_of(w)].x);
+        }
+        float l = 0.0f, o[kPer];
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
-            o[e] += part[e] * f;
+            o[e] = 0.0f;
         }
-    }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    __half2* dst = reinterpret_cast<__half2*>(a.out + (tok * a.num_heads + head) * DH + lane * kPer);
+        for (int64_t w = first; w <= last; ++w) {
+            const int64_t slot = slot_of(w);
+            const float2 ml = a.part_ml[slot];
+            const float f = ex2_approx(ml.x - m);
+            const float* part = a.part_o + slot * DH + lane * kPer;
+            l += ml.y * f;
 #pragma unroll
-    for (int e = 0; e < kPer; e += 2) {
-        dst[e / 2] = __floats2half2_rn(o[e] * inv, o[e + 1] * inv);
+            for (int e = 0; e < kPer; ++e) {
+                o[e] += part[e] * f;
+            }
+        }
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const int32_t row = p.row0 + r, tok = row / a.group;
+        __half2* dst = reinterpret_cast<__half2*>(
+            a.out + ((p.seq.tok0 + tok) * a.num_heads + p.kvh * a.group + (row - tok * a.group)) * DH + lane * kPer);
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2) {
+            dst[e / 2] = __floats2half2_rn(o[e] * inv, o[e + 1] * inv);
+        }
     }
 }
 
@@ -889,18 +1085,19 @@ int launch_dh(const pplb200_attn_params& p, TreeArgs a, cudaStream_t stream) {
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    tree_plan_kernel<<<static_cast<unsigned>(a.batch + 1), kPlanThreads, 0, stream>>>(a);
+    // each kernel starts while the one before it drains, and waits for it before it touches anything
+    launch_dependent(tree_plan_kernel, dim3(static_cast<unsigned>(a.batch + 1)), dim3(kPlanThreads), 0, stream, a);
     rc = check_launch("tree_plan_kernel");
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    kernel<<<static_cast<unsigned>(a.ranges * a.lanes), T::kThreads, T::kSmemBytes, stream>>>(tm_code, tm_scale, a);
+    launch_dependent(kernel, dim3(static_cast<unsigned>(a.ranges * a.lanes)), dim3(T::kThreads), T::kSmemBytes, stream, tm_code,
+                     tm_scale, a);
     rc = check_launch("tree_attn_kernel");
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    const int64_t warps = a.total_tokens * a.num_heads;
-    tree_merge_kernel<DH><<<static_cast<unsigned>((warps * 32 + 255) / 256), 256, 0, stream>>>(a);
+    launch_dependent(tree_merge_kernel<DH>, dim3(static_cast<unsigned>(a.ranges * a.lanes), T::kBlockM / kMergeRows), dim3(kMergeThreads), 0, stream, a);
     return check_launch("tree_merge_kernel");
 }
 
@@ -923,7 +1120,8 @@ int make_tree_plan(const pplb200_attn_params& p, int sm_count, TreePlan* plan) {
     plan->words = (p.max_seqlen + 63) / 64;
     const uint64_t slot_rows = static_cast<uint64_t>(plan->ranges) * plan->lanes * 2 * tile_rows;
     plan->off_prefix = 256;
-    plan->off_ancestor = plan->off_prefix + align256(static_cast<uint64_t>(p.batch + 1) * 8);
+    plan->off_flags = plan->off_prefix + align256(static_cast<uint64_t>(p.batch + 1) * 8);
+    plan->off_ancestor = plan->off_flags + align256(static_cast<uint64_t>(p.batch) * 4);
     plan->off_part_ml = plan->off_ancestor + align256(static_cast<uint64_t>(p.total_tokens) * plan->words * 8);
     plan->off_part_o = plan->off_part_ml + slot_rows * 8;
     plan->bytes = plan->off_part_o + slot_rows * p.head_dim * 4;
@@ -949,6 +1147,7 @@ int launch_tree_attn(const pplb200_attn_params& p, const CacheGeom& geom, const 
     a.out = static_cast<__half*>(attn_output);
     a.hdr = reinterpret_cast<TreeHeader*>(ws);
     a.prefix = reinterpret_cast<int64_t*>(ws + plan.off_prefix);
+    a.flags = reinterpret_cast<uint32_t*>(ws + plan.off_flags);
     a.ancestor = reinterpret_cast<uint64_t*>(ws + plan.off_ancestor);
     a.part_ml = reinterpret_cast<float2*>(ws + plan.off_part_ml);
     a.part_o = reinterpret_cast<float*>(ws + plan.off_part_o);

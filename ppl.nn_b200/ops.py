@@ -385,102 +385,95 @@ class RotaryPositionEmbedding(_Base):
         return rotated_query, rotated_key
 
 
-def _require_index(device, **tensors):
-    """CUDA tensors of one device, int64, as the kernels read them."""
-    _require_cuda(**tensors)
+def _require(device: int, dtype: torch.dtype, **tensors) -> None:
+    """Contiguous CUDA tensors of one device (by index) and type."""
     for name, t in tensors.items():
-        if t.dtype != torch.int64:
-            raise OpError("RC_INVALID_VALUE", f"{name} must be int64")
-    _require_device(device, **tensors)
-
-
-def _require_device(device, **tensors):
-    for name, t in tensors.items():
-        if t.device != device:
-            raise OpError("RC_INVALID_VALUE", f"{name} is on {t.device}, not on {device}")
-
-
-def _require_cache(cache, scale, layout):
-    """Checks an INT8 cache and its scales against one another; returns (layers, kv heads, head_dim)."""
-    _require_cuda(cache=cache)
-    if scale is None or scale.numel() == 0:
-        raise OpError("RC_UNSUPPORTED", "currently only support qunatized cache but scale not found")
-    _require_cuda(scale=scale)
-    if cache.dtype != torch.int8 or scale.dtype != torch.float16:
-        raise OpError("RC_UNSUPPORTED", "the cache must be int8 with fp16 scales")
-    if layout not in (0, 3):
-        raise OpError("RC_UNSUPPORTED", "currently only support cache_layout == 0 or cache_layout == 3")
-    _require_device(cache.device, scale=scale)
-    if cache.dim() != 5 or cache.shape[:4] != scale.shape[:4] or cache.shape[4] != 8 * scale.shape[4]:
-        raise OpError("RC_INVALID_VALUE", "cache and scale do not belong together")
-    layers, heads = (cache.shape[1], cache.shape[3]) if layout == 0 else (cache.shape[0], cache.shape[2])
-    return layers, heads, cache.shape[4]
-
-
-def _require_weight(weight, num_layer):
-    _require_cuda(weight=weight)
-    if weight.dtype != torch.float32:
-        raise OpError("RC_UNSUPPORTED", "weight must be fp32")
-    if weight.dim() != 3 or weight.shape[0] != num_layer:
-        raise OpError("RC_INVALID_VALUE", "weight must be [num_layer, num_kv_heads, max_tokens]")
+        if t is None or not (t.is_cuda and t.is_contiguous()):
+            _require_cuda(**{name: t})
+        if t.get_device() != device:
+            raise OpError("RC_INVALID_VALUE", f"{name} is on {t.device}, not on cuda:{device}")
+        if t.dtype != dtype:
+            raise OpError("RC_INVALID_VALUE" if dtype == torch.int64 else "RC_UNSUPPORTED", f"{name} must be {dtype}")
 
 
 class _CacheOp(_Base):
-    """What the operators around the cache share: parameters from the cache's geometry, and a workspace whose first
-    word is the device status word.  The workspace is allocated per call, so that calls of one object on two streams,
-    or in two captured graphs, never share one; the last call's is kept for device_status()."""
+    """What the operators around the cache share: checks, parameters from the cache's geometry, and a workspace whose
+    first word is the device status word.  The workspace is allocated per call, so that calls of one object on two
+    streams, or in two captured graphs, never share one; the last call's is kept for device_status()."""
 
     def __init__(self, param):
         super().__init__()
         self.param = param
         self._workspace: torch.Tensor | None = None
 
-    def _params(self, *, num_heads, num_kv_heads, head_dim, batch, max_kvlen, max_tokens, cachestarts, max_seqlen=0,
+    def _check_cache(self, cache, scale):
+        """(device, kv heads, head_dim, rows) of an INT8 cache with num_layer layers and its scales."""
+        a = self.param
+        if scale is None or scale.numel() == 0:
+            raise OpError("RC_UNSUPPORTED", "currently only support qunatized cache but scale not found")
+        _require_cuda(cache=cache)
+        device = cache.get_device()
+        _require(device, torch.int8, cache=cache)
+        _require(device, torch.float16, scale=scale)
+        shape = cache.shape
+        if len(shape) != 5 or scale.shape != shape[:4] + (shape[4] // 8,):
+            raise OpError("RC_INVALID_VALUE", "cache and scale do not belong together")
+        if a.cache_layout == 0:
+            rows, layers, _, heads, dim = shape
+        elif a.cache_layout == 3:
+            layers, _, heads, rows, dim = shape
+        else:
+            raise OpError("RC_UNSUPPORTED", "currently only support cache_layout == 0 or cache_layout == 3")
+        if layers != a.num_layer:
+            raise OpError("RC_INVALID_VALUE", "cache does not have num_layer layers")
+        return device, heads, dim, rows
+
+    def _check_weight(self, device, weight, heads, rows) -> None:
+        _require(device, torch.float32, weight=weight)
+        if weight.shape != (self.param.num_layer, heads, rows):
+            raise OpError("RC_INVALID_VALUE", "weight must be [num_layer, num_kv_heads, max_tokens]")
+
+    def _params(self, num_heads, num_kv_heads, head_dim, batch, max_kvlen, max_tokens, cachestarts, max_seqlen=0,
                 total_tokens=0, is_causal=True) -> capi.AttnParams:
         a = self.param
-        if a.cache_mode == 1 and cachestarts.dim() != 2:
-            raise OpError("RC_INVALID_VALUE", "cachestarts must be a 2d tensor in cache_mode 1")
+        stride_b = 0
+        if a.cache_mode == 1:
+            if cachestarts.dim() != 2:
+                raise OpError("RC_INVALID_VALUE", "cachestarts must be a 2d tensor in cache_mode 1")
+            stride_b = cachestarts.shape[1]
         if cachestarts.shape[0] != batch or (a.cache_mode == 0 and cachestarts.dim() != 1):
             raise OpError("RC_INVALID_VALUE", "cachestarts must have an entry (cache_mode 1: a row) per sequence")
-        p = capi.AttnParams()
-        p.num_heads, p.num_kv_heads, p.head_dim = num_heads, num_kv_heads, head_dim
-        p.is_causal = int(is_causal)
-        p.num_layer, p.layer_idx = a.num_layer, a.layer_idx
-        p.quant_bit, p.quant_group = a.quant_bit, a.quant_group
-        p.cache_mode, p.cache_layout, p.page_size = a.cache_mode, a.cache_layout, a.page_size
-        p.batch, p.total_tokens, p.max_tokens = batch, total_tokens, max_tokens
-        p.max_seqlen, p.max_kvlen = int(max_seqlen), int(max_kvlen)
-        p.cachestart_stride_b = cachestarts.shape[1] if a.cache_mode == 1 else 0
+        p = capi.AttnParams(num_heads, num_kv_heads, head_dim, int(is_causal), a.num_layer, a.layer_idx, a.quant_bit,
+                            a.quant_group, a.cache_mode, a.cache_layout, a.page_size, 0, 0, 0, batch, 0,
+                            int(max_seqlen), int(max_kvlen), total_tokens, max_tokens, 0, 0, 0, 0, stride_b)
         self._raise("pplb200_fill_cache_strides", self.lib.fill_cache_strides(p))
         return p
 
     def _query_params(self, query, seqstarts, cachestarts, start_pos, max_seqlen, max_kvlen, cache, scale):
         """Checks and parameters of the operators whose query tokens attend to the cache."""
         a = self.param
-        layers, kv_heads, dim = _require_cache(cache, scale, a.cache_layout)
-        _require_cuda(query=query)
-        _require_device(cache.device, query=query)
-        _require_index(cache.device, seqstarts=seqstarts, cachestarts=cachestarts, start_pos=start_pos)
+        device, heads, dim, rows = self._check_cache(cache, scale)
+        _require(device, torch.float16, query=query)
+        _require(device, torch.int64, seqstarts=seqstarts, cachestarts=cachestarts, start_pos=start_pos)
         if a.is_alibi:
             raise OpError("RC_UNSUPPORTED", "currently only support is_alibi == false")
-        if query.dtype != torch.float16:
-            raise OpError("RC_UNSUPPORTED", "currently only support fp16")
-        if query.shape[1:] != (a.num_heads, a.head_dim) or (layers, kv_heads, dim) != (a.num_layer, a.num_kv_heads,
-                                                                                      a.head_dim):
+        if query.shape[1:] != (a.num_heads, a.head_dim) or heads != a.num_kv_heads or dim != a.head_dim:
             raise OpError("RC_INVALID_VALUE", "query or cache does not have the shape of the attributes")
-        if seqstarts.shape[0] != start_pos.shape[0] + 1:
+        batch = start_pos.shape[0]
+        if seqstarts.shape[0] != batch + 1:
             raise OpError("RC_INVALID_VALUE", "seqstarts must have one entry more than start_pos")
-        return self._params(num_heads=a.num_heads, num_kv_heads=kv_heads, head_dim=dim, batch=start_pos.shape[0],
-                            max_kvlen=max_kvlen, max_tokens=_max_tokens(cache, a.cache_layout), cachestarts=cachestarts,
-                            max_seqlen=max_seqlen, total_tokens=query.shape[0], is_causal=a.is_causal)
+        return device, self._params(a.num_heads, heads, dim, batch, max_kvlen, rows, cachestarts, max_seqlen,
+                                    query.shape[0], a.is_causal)
 
-    def _call(self, name, size_fn, fn, p, device, *args) -> None:
+    def _call(self, name, size_fn, fn, p, device: int, *args) -> None:
         """Runs fn(p, *args, workspace, bytes, stream) on the tensors' device and its current stream."""
+        if device != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                return self._call(name, size_fn, fn, p, device, *args)
         rc, nbytes = size_fn(p)
-        self._raise(name, rc)
-        with torch.cuda.device(device):
-            self._workspace = ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-            rc = fn(p, *args, _ptr(ws), nbytes, _stream())
+        if rc == capi.SUCCESS:
+            self._workspace = ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+            rc = fn(p, *args, ws.data_ptr(), nbytes, _stream())
         self._raise(name, rc)
 
     def device_status(self) -> int:
@@ -503,21 +496,20 @@ class TreeAttention(_CacheOp):
 
     def forward(self, query, parents, seqstarts, cachestarts, start_pos, max_seqlen: int, max_kvlen: int, cache, scale,
                 attn_output: torch.Tensor | None = None) -> torch.Tensor:
-        a = self.param
-        p = self._query_params(query, seqstarts, cachestarts, start_pos, max_seqlen, max_kvlen, cache, scale)
+        device, p = self._query_params(query, seqstarts, cachestarts, start_pos, max_seqlen, max_kvlen, cache, scale)
         if parents is not None:
-            _require_index(cache.device, parents=parents)
+            _require(device, torch.int64, parents=parents)
             if parents.shape != query.shape[:1]:
                 raise OpError("RC_INVALID_VALUE", "parents must have an entry per query token")
         if attn_output is None:
             attn_output = torch.empty_like(query)
-        _require_cuda(attn_output=attn_output)
-        _require_device(cache.device, attn_output=attn_output)
-        if attn_output.shape != query.shape or attn_output.dtype != query.dtype:
-            raise OpError("RC_INVALID_VALUE", "attn_output must be like query")
-        self._call("pplb200_tree_attn_forward", self.lib.tree_attn_workspace_size, self.lib.tree_attn_forward, p,
-                   cache.device, _ptr(query), _ptr(parents), _ptr(seqstarts), _ptr(cachestarts), _ptr(start_pos),
-                   _ptr(cache), _ptr(scale), _ptr(attn_output))
+        else:
+            _require(device, torch.float16, attn_output=attn_output)
+            if attn_output.shape != query.shape:
+                raise OpError("RC_INVALID_VALUE", "attn_output must be like query")
+        self._call("pplb200_tree_attn_forward", self.lib.tree_attn_workspace_size, self.lib.tree_attn_forward, p, device,
+                   _ptr(query), _ptr(parents), _ptr(seqstarts), _ptr(cachestarts), _ptr(start_pos), _ptr(cache),
+                   _ptr(scale), _ptr(attn_output))
         return attn_output
 
 
@@ -531,14 +523,11 @@ class AttentionWeight(_CacheOp):
 
     def forward(self, query, seqstarts, cachestarts, start_pos, max_seqlen: int, max_kvlen: int, cache, scale,
                 weight) -> torch.Tensor:
-        p = self._query_params(query, seqstarts, cachestarts, start_pos, max_seqlen, max_kvlen, cache, scale)
-        _require_weight(weight, self.param.num_layer)
-        _require_device(cache.device, weight=weight)
-        if weight.shape[1:] != (p.num_kv_heads, p.max_tokens):
-            raise OpError("RC_INVALID_VALUE", "weight does not have the shape of the cache")
-        self._call("pplb200_attn_weight_accumulate", self.lib.attn_weight_workspace_size,
-                   self.lib.attn_weight_accumulate, p, cache.device, _ptr(query), _ptr(seqstarts), _ptr(cachestarts),
-                   _ptr(start_pos), _ptr(cache), _ptr(scale), _ptr(weight))
+        device, p = self._query_params(query, seqstarts, cachestarts, start_pos, max_seqlen, max_kvlen, cache, scale)
+        self._check_weight(device, weight, p.num_kv_heads, p.max_tokens)
+        self._call("pplb200_attn_weight_accumulate", self.lib.attn_weight_workspace_size, self.lib.attn_weight_accumulate,
+                   p, device, _ptr(query), _ptr(seqstarts), _ptr(cachestarts), _ptr(start_pos), _ptr(cache), _ptr(scale),
+                   _ptr(weight))
         return weight
 
 
@@ -560,22 +549,25 @@ class KeyValueCacheEvict(_CacheOp):
     def forward(self, weight, cachestarts, kvlens, budgets, max_kvlen: int, max_budget: int,
                 kept: torch.Tensor | None = None) -> torch.Tensor:
         a = self.param
-        _require_weight(weight, a.num_layer)
-        _require_index(weight.device, cachestarts=cachestarts, kvlens=kvlens, budgets=budgets)
-        batch, heads = kvlens.shape[0], weight.shape[1]
+        _require_cuda(weight=weight)
+        if weight.dim() != 3:
+            raise OpError("RC_INVALID_VALUE", "weight must be [num_layer, num_kv_heads, max_tokens]")
+        device, heads, rows = weight.get_device(), weight.shape[1], weight.shape[2]
+        self._check_weight(device, weight, heads, rows)
+        _require(device, torch.int64, cachestarts=cachestarts, kvlens=kvlens, budgets=budgets)
+        batch, max_budget = kvlens.shape[0], int(max_budget)
         if budgets.shape != kvlens.shape or max_budget < 0:
             raise OpError("RC_INVALID_VALUE", "budgets must have an entry per sequence and max_budget not be negative")
         if kept is None:
-            kept = torch.empty((batch, heads, int(max_budget)), dtype=torch.int64, device=weight.device)
-        _require_index(weight.device, kept=kept)
-        if kept.shape != (batch, heads, int(max_budget)):
-            raise OpError("RC_INVALID_VALUE", "kept must be [batch, num_kv_heads, max_budget]")
+            kept = torch.empty((batch, heads, max_budget), dtype=torch.int64, device=weight.device)
+        else:
+            _require(device, torch.int64, kept=kept)
+            if kept.shape != (batch, heads, max_budget):
+                raise OpError("RC_INVALID_VALUE", "kept must be [batch, num_kv_heads, max_budget]")
         # the choice does not depend on the head size; any supported one describes the rows
-        p = self._params(num_heads=heads, num_kv_heads=heads, head_dim=128, batch=batch, max_kvlen=max_kvlen,
-                         max_tokens=weight.shape[2], cachestarts=cachestarts)
-        self._call("pplb200_kv_evict_select", self.lib.kv_evict_workspace_size, self.lib.kv_evict_select, p,
-                   weight.device, _ptr(weight), _ptr(cachestarts), _ptr(kvlens), _ptr(budgets), a.sink, a.recent,
-                   max_budget, _ptr(kept))
+        p = self._params(heads, heads, 128, batch, max_kvlen, rows, cachestarts)
+        self._call("pplb200_kv_evict_select", self.lib.kv_evict_workspace_size, self.lib.kv_evict_select, p, device,
+                   _ptr(weight), _ptr(cachestarts), _ptr(kvlens), _ptr(budgets), a.sink, a.recent, max_budget, _ptr(kept))
         return kept
 
 
@@ -590,23 +582,15 @@ class KeyValueCacheCompact(_CacheOp):
 
     def forward(self, kept, cachestarts, base, kvlens, max_kvlen: int, cache, scale, weight=None,
                 num_layers: int = 1) -> None:
-        a = self.param
-        layers, heads, dim = _require_cache(cache, scale, a.cache_layout)
-        _require_index(cache.device, kept=kept, cachestarts=cachestarts, base=base, kvlens=kvlens)
-        max_tokens = _max_tokens(cache, a.cache_layout)
-        if layers != a.num_layer:
-            raise OpError("RC_INVALID_VALUE", "cache does not have num_layer layers")
+        device, heads, dim, rows = self._check_cache(cache, scale)
+        _require(device, torch.int64, kept=kept, cachestarts=cachestarts, base=base, kvlens=kvlens)
         batch = kvlens.shape[0]
         if kept.dim() != 3 or kept.shape[0] != batch or kept.shape[1] not in (1, heads) or base.shape != kvlens.shape:
             raise OpError("RC_INVALID_VALUE", "kept must be [batch, num_kv_heads or 1, K], base and kvlens [batch]")
         if weight is not None:
-            _require_weight(weight, a.num_layer)
-            _require_device(cache.device, weight=weight)
-            if weight.shape[1:] != (heads, max_tokens):
-                raise OpError("RC_INVALID_VALUE", "weight does not have the shape of the cache")
-        p = self._params(num_heads=heads, num_kv_heads=heads, head_dim=dim, batch=batch, max_kvlen=max_kvlen,
-                         max_tokens=max_tokens, cachestarts=cachestarts)
-        size = lambda q: self.lib.kv_compact_workspace_size(q, kept.shape[1], kept.shape[2], num_layers)  # noqa: E731
-        self._call("pplb200_kv_compact", size, self.lib.kv_compact, p, cache.device,
-                   _ptr(kept), kept.shape[1], kept.shape[2], _ptr(base), _ptr(kvlens), _ptr(cachestarts), num_layers,
-                   _ptr(cache), _ptr(scale), _ptr(weight))
+            self._check_weight(device, weight, heads, rows)
+        p = self._params(heads, heads, dim, batch, max_kvlen, rows, cachestarts)
+        _, kept_heads, most = kept.shape
+        self._call("pplb200_kv_compact", lambda q: self.lib.kv_compact_workspace_size(q, kept_heads, most, num_layers),
+                   self.lib.kv_compact, p, device, _ptr(kept), kept_heads, most, _ptr(base), _ptr(kvlens),
+                   _ptr(cachestarts), num_layers, _ptr(cache), _ptr(scale), _ptr(weight))
