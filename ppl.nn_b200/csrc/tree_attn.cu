@@ -14,8 +14,8 @@
 //     per range), which tree_merge_kernel joins.
 //   * tree_plan_kernel turns the device-side lengths into the prefix sum of blocks, and the parents into one bit mask
 //     of ancestors per token.  Only blocks that reach behind the history look at the masks, 64 bits a row and block.
-//   * Roles of a CTA: 4 MT softmax warps, one thread per query row; four warps each that turn the raw codes and scales
-//     of a block into the swizzled fp16 K and V tiles; MT warps that issue the MMAs of a 128-row tile each; one
+//   * Roles of a CTA: 4 MT softmax warps, one thread per query row; warps that turn the raw codes and scales of a block
+//     into the swizzled fp16 tiles, some for K and some for V; MT warps that issue the MMAs of a 128-row tile each; one
 //     warp that fetches the raw blocks by TMA into a ring of two, K and V apart.  S = Q K^T goes to a 64-column TMEM
 //     buffer, P returns to TMEM as the A operand of O += P V (two buffers), as in the prefill kernel.
 //   * MT = 1: two CTAs per SM.  MT = 2, for more than 128 rows per kv head: one CTA per SM, whose two tiles share the
@@ -44,16 +44,11 @@ constexpr float kRescaleSlack = 8.0f;
 template <int DH, int MT>
 struct TTraits {
     static constexpr int kBlockM = kTileM * MT;
-    static constexpr int kThreads = 32 * (4 * MT + 8 + 4);  // whole warpgroups: registers are dealt to those
-    // registers of a softmax, converter and other thread; the launch gives all the same, 65 536 / kThreads / kCtasPerSm
-    // rounded down to the allocation's granularity (64 and 96)
-    // registers of a softmax, converter and other thread; the launch gives all the same, 65 536 / kThreads / kCtasPerSm
-    // rounded down to the allocation's granularity
-    static constexpr int kSoftmaxRegs = MT == 1 ? 96 : 128, kConvRegs = MT == 1 ? 56 : 72, kOtherRegs = MT == 1 ? 48 : 72;
-    static constexpr int kLaunchRegs = MT == 1 ? 64 : 96;
-    static_assert(4 * MT * kSoftmaxRegs + 8 * kConvRegs + 4 * kOtherRegs <= (4 * MT + 12) * kLaunchRegs, "register split");
+    static constexpr int kConvWarps = MT == 1 ? 2 : 4;  // for K, and as many for V
+    static constexpr int kConvThreads = 32 * kConvWarps;
+    static constexpr int kThreads = 32 * (4 * MT + 2 * kConvWarps + MT + 1);
     static constexpr int kCtasPerSm = MT == 1 ? 2 : 1;
-    static constexpr int kConvWarp = 4 * MT, kMmaWarp = kConvWarp + 8, kLoadWarp = kMmaWarp + MT;
+    static constexpr int kConvWarp = 4 * MT, kMmaWarp = kConvWarp + 2 * kConvWarps, kLoadWarp = kMmaWarp + MT;
     static constexpr int kColBlocks = DH / 64;
     static constexpr int kQBlockBytes = kTileM * 128;
     static constexpr int kKVBlockBytes = kBlockN * 128;
@@ -280,11 +275,12 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
 }
 
 // One thread's share of a raw K or V block: 16-byte piece `piece` of the rows row, row + kRowsPerStep, ..
-template <int DH>
+template <int DH, int WARPS>
 struct Raw {
     static constexpr int kPieces = DH / 16;            // 16-byte pieces of a row
     static constexpr int kRowsPerStep = 32 / kPieces;  // rows of a warp at once
-    static constexpr int kRows = 16 / kRowsPerStep;    // steps over the warp's 16 rows
+    static constexpr int kWarpRows = kBlockN / WARPS;
+    static constexpr int kRows = kWarpRows / kRowsPerStep;
     uint4 code[kRows];
     uint32_t sc[kRows];
 
@@ -402,16 +398,6 @@ __device__ __forceinline__ void tile_barrier(int t) {
     asm volatile("bar.sync %0, 128;" ::"r"(t + 1) : "memory");
 }
 
-// The warpgroup's registers per thread from here on
-template <int N, bool UP>
-__device__ __forceinline__ void set_registers() {
-    if constexpr (UP) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-    }
-}
-
 template <int DH, int MT>
 __global__ void __launch_bounds__(TTraits<DH, MT>::kThreads, TTraits<DH, MT>::kCtasPerSm)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_constant__ CUtensorMap tm_scale, const TreeArgs a) {
@@ -451,16 +437,16 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
     }
     if (threadIdx.x == 0) {
         bars.abort_word = 0;
-        mbar_init(&bars.q_full, 128);
+        mbar_init(&bars.q_full, T::kConvThreads);
         mbar_init(&bars.q_empty, MT);
         for (int s = 0; s < kRawStages; ++s) {
             for (int kv = 0; kv < 2; ++kv) {
                 mbar_init(&bars.raw_full[kv][s], 1);
-                mbar_init(&bars.raw_empty[kv][s], 128);
+                mbar_init(&bars.raw_empty[kv][s], T::kConvThreads);
             }
         }
-        mbar_init(&bars.k_full, 128);
-        mbar_init(&bars.v_full, 128);
+        mbar_init(&bars.k_full, T::kConvThreads);
+        mbar_init(&bars.v_full, T::kConvThreads);
         mbar_init(&bars.k_empty, MT);
         mbar_init(&bars.v_empty, MT);
         for (int t = 0; t < MT; ++t) {
@@ -484,13 +470,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
     tc_fence_after();
     const uint32_t tmem_base = bars.tmem_slot;
 
-    if (warp >= T::kMmaWarp) {
-        set_registers<T::kOtherRegs, false>();
-    } else if (warp >= T::kConvWarp) {
-        set_registers<T::kConvRegs, false>();
-    } else {
-        set_registers<T::kSoftmaxRegs, true>();
-    }
     if (warp == T::kLoadWarp) {
         // =========================== TMA producer ===========================
         bool ok = true;
@@ -645,13 +624,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
         }
     } else if (warp >= T::kConvWarp && warp < T::kMmaWarp) {
         // =========================== converters ===========================
-        // The first four warps convert K (and bring Q), the others V.  K of block j + 1 is thus never behind V of block
+        // The first half of the warps converts K (and brings Q), the other V.  K of block j + 1 is thus never behind V of block
         // j, which has to wait for P V (j - 1), i.e. for a softmax.
         const int ct = threadIdx.x - 32 * T::kConvWarp;
-        const int kv = ct >= 128 ? 1 : 0;
-        constexpr int kPieces = Raw<DH>::kPieces;
+        const int kv = ct >= T::kConvThreads ? 1 : 0;
+        constexpr int kPieces = Raw<DH, T::kConvWarps>::kPieces;
         const int piece = lane % kPieces;
-        const int row = ((warp - T::kConvWarp) & 3) * 16 + lane / kPieces;  // first of the thread's rows of a block
+        const int row = (warp - T::kConvWarp) % T::kConvWarps * Raw<DH, T::kConvWarps>::kWarpRows + lane / kPieces;  // first of the thread's rows of a block
         const uint32_t tile = smem_u32(kv ? sV : sK), raw0 = smem_u32(sRaw) + kv * T::kRawBytes, q_tile = smem_u32(sQ);
         uint64_t* full = kv ? &bars.v_full : &bars.k_full;
         uint64_t* empty = kv ? &bars.v_empty : &bars.k_empty;
@@ -671,7 +650,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                 }
                 constexpr int kQPieces = DH / 8;  // 16-byte pieces of a query row
                 const int copies0 = replicas(p.rows_valid), copies1 = replicas(p.rows_valid - kTileM);  // of either tile
-                for (int i = ct; i < p.rows_valid * kQPieces; i += 128) {
+                for (int i = ct; i < p.rows_valid * kQPieces; i += T::kConvThreads) {
                     const int r = i / kQPieces, c = i - r * kQPieces;
                     const int32_t qrow = p.row0 + r;
                     const int32_t tok = qrow / a.group;
@@ -693,7 +672,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                 if (!ok) {
                     break;
                 }
-                Raw<DH> raw;
+                Raw<DH, T::kConvWarps> raw;
                 raw.load(raw0 + 2 * s * T::kRawBytes, row, piece, p.seq.len - blk * kBlockN);
                 // The loads have to be over before the slot is handed back.  The arrival alone does not see to that: the
                 // scales were found loaded behind it, next to their use, when the next copy had overwritten them.
