@@ -14,8 +14,8 @@
 //     per range), which tree_merge_kernel joins.
 //   * tree_plan_kernel turns the device-side lengths into the prefix sum of blocks, and the parents into one bit mask
 //     of ancestors per token.  Only blocks that reach behind the history look at the masks, 64 bits a row and block.
-//   * Roles of a CTA: 4 MT softmax warps, one thread per query row; warps that turn the raw codes and scales of a block
-//     into the swizzled fp16 tiles, some for K and some for V; MT warps that issue the MMAs of a 128-row tile each; one
+//   * Roles of a CTA: 4 MT softmax warps, one thread per query row; four converter warps, which turn the raw codes and
+//     scales of a block into the swizzled fp16 K and V tiles; MT warps that issue the MMAs of a 128-row tile each; one
 //     warp that fetches the raw blocks by TMA into a ring of two, K and V apart.  S = Q K^T goes to a 64-column TMEM
 //     buffer, P returns to TMEM as the A operand of O += P V (two buffers), as in the prefill kernel.
 //   * MT = 1: two CTAs per SM.  MT = 2, for more than 128 rows per kv head: one CTA per SM, whose two tiles share the
@@ -44,11 +44,9 @@ constexpr float kRescaleSlack = 8.0f;
 template <int DH, int MT>
 struct TTraits {
     static constexpr int kBlockM = kTileM * MT;
-    static constexpr int kConvWarps = MT == 1 ? 2 : 4;  // for K, and as many for V
-    static constexpr int kConvThreads = 32 * kConvWarps;
-    static constexpr int kThreads = 32 * (4 * MT + 2 * kConvWarps + MT + 1);
+    static constexpr int kThreads = 32 * (4 * MT + 4 + MT + 1);
     static constexpr int kCtasPerSm = MT == 1 ? 2 : 1;
-    static constexpr int kConvWarp = 4 * MT, kMmaWarp = kConvWarp + 2 * kConvWarps, kLoadWarp = kMmaWarp + MT;
+    static constexpr int kConvWarp = 4 * MT, kMmaWarp = kConvWarp + 4, kLoadWarp = kMmaWarp + MT;
     static constexpr int kColBlocks = DH / 64;
     static constexpr int kQBlockBytes = kTileM * 128;
     static constexpr int kKVBlockBytes = kBlockN * 128;
@@ -58,11 +56,10 @@ struct TTraits {
     static constexpr int kRawBytes = kCodeBytes + kBlockN * (DH / 8) * 2;  // codes and scales of K or V of a block
     // The same for every head size, so that never more CTAs share an SM than its TMEM holds; MT = 2 asks for more
     // than half of the SM's.
-    static constexpr int kJoinBytes = 2 * kTileM * 8 * 4;  // per tile: joining the replicas of few rows
-    static constexpr int kSmemBytes = MT * 32768 + 2 * (kBlockN * 256) + 2 * kRawStages * (kBlockN * 160) + MT * kJoinBytes + 512;
-    // TMEM columns of a tile: S0 64 | S1 64 | O 128; P of a block takes the first half of its S
-    static constexpr uint32_t kColO = 2 * kBlockN;
-    static constexpr uint32_t kTileCols = 256;
+    static constexpr int kSmemBytes = MT * 32768 + 2 * (kBlockN * 256) + 2 * kRawStages * (kBlockN * 160) + 512;
+    static constexpr uint32_t kPCols = kBlockN / 2;
+    static constexpr uint32_t kColS = 0, kColP = kBlockN, kColO = kColP + 2 * kPCols;
+    static constexpr uint32_t kTileCols = 256;  // TMEM columns of a tile: S 64 | P 2 x 32 | O 128
 };
 
 struct TreeHeader {
@@ -234,10 +231,8 @@ struct Barriers {
     uint64_t q_full, q_empty;
     uint64_t raw_full[2][kRawStages], raw_empty[2][kRawStages];  // [K | V]
     uint64_t k_full, k_empty, v_full, v_empty;
-    uint64_t o_free[MT];
-    // One per S buffer: who waits for block x knows that block x - 2 is done, and block x + 2 needs what it holds, so the
-    // parity of the phase is never mistaken.
-    uint64_t s_full[MT][2], p_full[MT][2], pv_done[MT][2];
+    uint64_t o_free[MT], s_full[MT], s_free[MT];
+    uint64_t p_full[MT][2], pv_done[MT][2];
     uint32_t tmem_slot;
     int abort_word;
 };
@@ -275,12 +270,11 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
 }
 
 // One thread's share of a raw K or V block: 16-byte piece `piece` of the rows row, row + kRowsPerStep, ..
-template <int DH, int WARPS>
+template <int DH>
 struct Raw {
     static constexpr int kPieces = DH / 16;            // 16-byte pieces of a row
     static constexpr int kRowsPerStep = 32 / kPieces;  // rows of a warp at once
-    static constexpr int kWarpRows = kBlockN / WARPS;
-    static constexpr int kRows = kWarpRows / kRowsPerStep;
+    static constexpr int kRows = 16 / kRowsPerStep;    // steps over the warp's 16 rows
     uint4 code[kRows];
     uint32_t sc[kRows];
 
@@ -329,75 +323,6 @@ __device__ __forceinline__ void load_rows(const TreeArgs& a, void* dst, const CU
     tma_load_5d(dst, map, bar, 0, c[0], c[1], c[2], c[3]);
 }
 
-// Few rows leave most of a tile's 128 lanes empty, and a softmax takes a warp the same time for one row as for 32.  Up to
-// 32 rows (64) are therefore put into the tile 4 (2) times, and each replica takes the softmax of a quarter (half) of
-// a block's positions; the weights of the other positions are zeros in its rows of P.  The replicas are joined like
-// the parts of a segment when the segment's part ends.
-__device__ __forceinline__ int replicas(int32_t rows) {
-    return rows <= 32 ? 4 : (rows <= 64 ? 2 : 1);
-}
-
-// Maximum of N raw scores, of which bit e of `seen` says whether score e counts
-template <int N>
-__device__ __forceinline__ float max_of(float (&v)[N], bool masked, uint32_t seen) {
-    if (masked) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            v[e] = (seen >> e) & 1u ? v[e] : -INFINITY;
-        }
-    }
-    float a = fmax3(v[0], v[1], v[2]), b = fmax3(v[3], v[4], v[5]);
-#pragma unroll
-    for (int e = 6; e + 3 < N; e += 4) {
-        a = fmax3(a, v[e], v[e + 1]);
-        b = fmax3(b, v[e + 2], v[e + 3]);
-    }
-    return fmax3(a, b, fmaxf(v[N - 2], v[N - 1]));
-}
-
-// N scores -> N / 2 columns of packed fp16 weights exp2(s * scale - m).  The row sum adds the rounded values that P V
-// uses, in four chains (one chain of N dependent additions would be as long as the exponentials).
-template <int N>
-__device__ __forceinline__ float weights_of(const float (&v)[N], float sc, float m, uint32_t (&pk)[N / 2]) {
-    float l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int e = 0; e < N / 2; ++e) {
-        const float2 x = __ffma2_rn(make_float2(v[2 * e], v[2 * e + 1]), make_float2(sc, sc), make_float2(-m, -m));
-        pk[e] = h2_as_u32(__floats2half2_rn(ex2_approx(x.x), ex2_approx(x.y)));
-        add_half2_to_float(l[e & 3], pk[e]);
-    }
-    return (l[0] + l[1]) + (l[2] + l[3]);
-}
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void load_scores(uint32_t taddr, float (&v)[32]) {
-    uint32_t u[32];
-    tmem_ld32(taddr, u);
-    tmem_wait_ld();
-#pragma unroll
-    for (int e = 0; e < 32; ++e) {
-        v[e] = __uint_as_float(u[e]);
-    }
-}
-__device__ __forceinline__ void load_scores(uint32_t taddr, float (&v)[16]) {
-    tmem_ld16(taddr, v);
-    tmem_wait_ld();
-}
-
-// Barrier of the four softmax warps of tile t (it counts warps: the lanes have to come together)
-__device__ __forceinline__ void tile_barrier(int t) {
-    __syncwarp();
-    asm volatile("bar.sync %0, 128;" ::"r"(t + 1) : "memory");
-}
-
 template <int DH, int MT>
 __global__ void __launch_bounds__(TTraits<DH, MT>::kThreads, TTraits<DH, MT>::kCtasPerSm)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_constant__ CUtensorMap tm_scale, const TreeArgs a) {
@@ -407,8 +332,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
     uint8_t* sK = sQ + MT * T::kQBytes;
     uint8_t* sV = sK + T::kKVBytes;
     uint8_t* sRaw = sV + T::kKVBytes;  // [stage][K | V]
-    float* sJoin = reinterpret_cast<float*>(sRaw + 2 * kRawStages * T::kRawBytes);  // [tile][2][128][8]
-    Barriers<MT>& bars = *reinterpret_cast<Barriers<MT>*>(reinterpret_cast<uint8_t*>(sJoin) + MT * T::kJoinBytes);
+    Barriers<MT>& bars = *reinterpret_cast<Barriers<MT>*>(sRaw + 2 * kRawStages * T::kRawBytes);
     volatile int* abort_flag = &bars.abort_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t* status = &a.hdr->status;
@@ -437,24 +361,25 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
     }
     if (threadIdx.x == 0) {
         bars.abort_word = 0;
-        mbar_init(&bars.q_full, T::kConvThreads);
+        mbar_init(&bars.q_full, 128);
         mbar_init(&bars.q_empty, MT);
         for (int s = 0; s < kRawStages; ++s) {
             for (int kv = 0; kv < 2; ++kv) {
                 mbar_init(&bars.raw_full[kv][s], 1);
-                mbar_init(&bars.raw_empty[kv][s], T::kConvThreads);
+                mbar_init(&bars.raw_empty[kv][s], 128);
             }
         }
-        mbar_init(&bars.k_full, T::kConvThreads);
-        mbar_init(&bars.v_full, T::kConvThreads);
+        mbar_init(&bars.k_full, 128);
+        mbar_init(&bars.v_full, 128);
         mbar_init(&bars.k_empty, MT);
         mbar_init(&bars.v_empty, MT);
         for (int t = 0; t < MT; ++t) {
             mbar_init(&bars.o_free[t], 128);
+            mbar_init(&bars.s_full[t], 1);
+            mbar_init(&bars.s_free[t], 128);
             for (int i = 0; i < 2; ++i) {
-                mbar_init(&bars.pv_done[t][i], 1);
-                mbar_init(&bars.s_full[t][i], 1);
                 mbar_init(&bars.p_full[t][i], 128);
+                mbar_init(&bars.pv_done[t][i], 1);
             }
         }
         mbar_fence_init();
@@ -527,7 +452,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                 }
             }
         }
-    } else if (warp >= T::kMmaWarp && warp < T::kMmaWarp + MT) {
+    } else if (warp >= T::kMmaWarp) {
         // =========================== MMA issuer of one 128-row tile ===========================
         constexpr uint32_t idesc_qk = instr_desc_f16(kBlockN, false);
         constexpr uint32_t idesc_pv = instr_desc_f16(DH, true);
@@ -537,10 +462,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
         const uint32_t k_lo = desc_lo(smem_u32(sK), 16);
         const uint32_t v_lo = desc_lo(smem_u32(sV), T::kKVBlockBytes);
         const uint32_t tm = tmem_base + t * T::kTileCols;
-        const uint32_t d_o = tm + T::kColO;
+        const uint32_t d_s = tm + T::kColS, d_o = tm + T::kColO, a_p = tm + T::kColP;
         bool ok = true;
-        int pieces = 0, blocks_done = 0;  // of the CTA
-        int mine = 0, kc = 0, vc = 0;     // pieces, Q K^T and P V of this tile
+        int pieces = 0, blocks_done = 0;    // of the CTA
+        int mine = 0, kc = 0, vc = 0;       // pieces, Q K^T and P V of this tile
         for (int64_t u = begin; ok && u < end; ++pieces) {
             Piece p;
             piece_at(a, u, end, lane_class, lane, p);
@@ -565,18 +490,15 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                 }
                 continue;
             }
-            // Q K^T runs a block ahead of P V.  The scores of block j take the buffer of block j - 2, whose P has to
-            // have been read: MMAs with different accumulators need not run in the order of their issue.
             for (int32_t j = 0; ok && j <= blocks; ++j) {
                 if (j < blocks) {
                     ok = wait_or_abort(&bars.k_full, (blocks_done + j) & 1, abort_flag, status, kDevMmaTimeout) &&
-                         (vc == 0 || wait_or_abort(&bars.pv_done[t][(vc - 1) & 1], ((vc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout));
+                         (kc == 0 || wait_or_abort(&bars.s_free[t], (kc - 1) & 1, abort_flag, status, kDevMmaTimeout));
                     if (!ok) {
                         break;
                     }
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t d_s = tm + (kc & 1) * kBlockN;
 #pragma unroll
                         for (int cb = 0; cb < T::kColBlocks; ++cb) {
 #pragma unroll
@@ -586,7 +508,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                                            (cb | k) ? 1u : 0u);
                             }
                         }
-                        tc_commit(&bars.s_full[t][kc & 1]);
+                        tc_commit(&bars.s_full[t]);
                         tc_commit(&bars.k_empty);
                         if (j == blocks - 1) {
                             tc_commit(&bars.q_empty);
@@ -606,7 +528,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                     }
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t pa = tm + (vc & 1) * kBlockN;
+                        const uint32_t pa = a_p + (vc & 1) * T::kPCols;
 #pragma unroll
                         for (int ks = 0; ks < kBlockN / 16; ++ks) {
                             tc_mma_f16_ts(d_o, pa + 8 * ks, desc_join(v_lo + ks * (2048 >> 4), hi_sw128), idesc_pv,
@@ -622,226 +544,215 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
             blocks_done += blocks;
             ++mine;
         }
-    } else if (warp >= T::kConvWarp && warp < T::kMmaWarp) {
+    } else if (warp >= T::kConvWarp) {
         // =========================== converters ===========================
-        // The first half of the warps converts K (and brings Q), the other V.  K of block j + 1 is thus never behind V of block
-        // j, which has to wait for P V (j - 1), i.e. for a softmax.
         const int ct = threadIdx.x - 32 * T::kConvWarp;
-        const int kv = ct >= T::kConvThreads ? 1 : 0;
-        constexpr int kPieces = Raw<DH, T::kConvWarps>::kPieces;
+        constexpr int kPieces = Raw<DH>::kPieces;
         const int piece = lane % kPieces;
-        const int row = (warp - T::kConvWarp) % T::kConvWarps * Raw<DH, T::kConvWarps>::kWarpRows + lane / kPieces;  // first of the thread's rows of a block
-        const uint32_t tile = smem_u32(kv ? sV : sK), raw0 = smem_u32(sRaw) + kv * T::kRawBytes, q_tile = smem_u32(sQ);
-        uint64_t* full = kv ? &bars.v_full : &bars.k_full;
-        uint64_t* empty = kv ? &bars.v_empty : &bars.k_empty;
+        const int row = (warp - T::kConvWarp) * 16 + lane / kPieces;  // first of the thread's rows of a block
+        const uint32_t k_tile = smem_u32(sK), v_tile = smem_u32(sV), raw0 = smem_u32(sRaw), q_tile = smem_u32(sQ);
         bool ok = true;
         int pieces = 0, n = 0;  // pieces and blocks so far
+        // K (0) or V (1) of the CTA's block number `blk_no`, of which `rows` rows exist
+        auto convert = [&](int kv, int blk_no, int32_t rows) -> bool {
+            const int s = blk_no % kRawStages;
+            if (!wait_or_abort(&bars.raw_full[kv][s], (blk_no / kRawStages) & 1, abort_flag, status, kDevTmaTimeout)) {
+                return false;
+            }
+            Raw<DH> raw;
+            raw.load(raw0 + (2 * s + kv) * T::kRawBytes, row, piece, rows);
+            // The loads have to be over before the slot is handed back.  The arrival alone does not see to that: the
+            // scales were found loaded behind it, next to their use, when the next copy had overwritten them.
+            __threadfence_block();
+            mbar_arrive(&bars.raw_empty[kv][s]);
+            if (blk_no > 0 && !wait_or_abort(kv ? &bars.v_empty : &bars.k_empty, (blk_no - 1) & 1, abort_flag, status,
+                                             kDevMmaTimeout)) {
+                return false;
+            }
+            raw.store(kv ? v_tile : k_tile, row, piece);
+            fence_proxy_async_smem();
+            mbar_arrive(kv ? &bars.v_full : &bars.k_full);
+            return true;
+        };
         for (int64_t u = begin; ok && u < end; ++pieces) {
             Piece p;
             piece_at(a, u, end, lane_class, lane, p);
             u += p.blk1 - p.blk0;
-            if (kv == 0) {
-                // Q: row r of the tile is query row row0 + r = token x head of the group
-                if (pieces > 0) {
-                    ok = wait_or_abort(&bars.q_empty, (pieces - 1) & 1, abort_flag, status, kDevMmaTimeout);
-                    if (!ok) {
-                        break;
-                    }
+            // Q: row r of the tile is query row row0 + r = token x head of the group
+            if (pieces > 0) {
+                ok = wait_or_abort(&bars.q_empty, (pieces - 1) & 1, abort_flag, status, kDevMmaTimeout);
+                if (!ok) {
+                    break;
                 }
-                constexpr int kQPieces = DH / 8;  // 16-byte pieces of a query row
-                const int copies0 = replicas(p.rows_valid), copies1 = replicas(p.rows_valid - kTileM);  // of either tile
-                for (int i = ct; i < p.rows_valid * kQPieces; i += T::kConvThreads) {
-                    const int r = i / kQPieces, c = i - r * kQPieces;
-                    const int32_t qrow = p.row0 + r;
-                    const int32_t tok = qrow / a.group;
-                    const uint4 v = *reinterpret_cast<const uint4*>(
-                        a.q + ((p.seq.tok0 + tok) * a.num_heads + p.kvh * a.group + (qrow - tok * a.group)) * DH + c * 8);
-                    const uint32_t at = q_tile + (r / kTileM) * T::kQBytes + (c >> 3) * T::kQBlockBytes + (r % kTileM) * 128 +
-                                        (((c & 7) ^ (r & 7)) << 4);
-                    const int copies = r < kTileM ? copies0 : copies1;
-                    for (int f = 0; f < copies; ++f) {
-                        sts128(at + f * (kTileM / copies) * 128, v);
-                    }
-                }
-                fence_proxy_async_smem();
-                mbar_arrive(&bars.q_full);
             }
-            for (int32_t blk = p.blk0; blk < p.blk1; ++blk, ++n) {
-                const int s = n % kRawStages;
-                ok = wait_or_abort(&bars.raw_full[kv][s], (n / kRawStages) & 1, abort_flag, status, kDevTmaTimeout);
-                if (!ok) {
-                    break;
+            constexpr int kQPieces = DH / 8;  // 16-byte pieces of a query row
+            for (int i = ct; i < p.rows_valid * kQPieces; i += 128) {
+                const int r = i / kQPieces, c = i - r * kQPieces;
+                const int32_t qrow = p.row0 + r;
+                const int32_t tok = qrow / a.group;
+                const uint4 v = *reinterpret_cast<const uint4*>(
+                    a.q + ((p.seq.tok0 + tok) * a.num_heads + p.kvh * a.group + (qrow - tok * a.group)) * DH + c * 8);
+                sts128(q_tile + (r / kTileM) * T::kQBytes + (c >> 3) * T::kQBlockBytes + (r % kTileM) * 128 +
+                           (((c & 7) ^ (r & 7)) << 4), v);
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&bars.q_full);
+            // K runs one block ahead of V: V(j) has to wait for P V(j - 1), i.e. for a softmax, and the scores of block
+            // j + 1 should not wait with it
+            ok = convert(0, n, p.seq.len - p.blk0 * kBlockN);
+            for (int32_t blk = p.blk0; ok && blk < p.blk1; ++blk, ++n) {
+                if (blk + 1 < p.blk1) {
+                    ok = convert(0, n + 1, p.seq.len - (blk + 1) * kBlockN);
                 }
-                Raw<DH, T::kConvWarps> raw;
-                raw.load(raw0 + 2 * s * T::kRawBytes, row, piece, p.seq.len - blk * kBlockN);
-                // The loads have to be over before the slot is handed back.  The arrival alone does not see to that: the
-                // scales were found loaded behind it, next to their use, when the next copy had overwritten them.
-                __threadfence_block();
-                mbar_arrive(&bars.raw_empty[kv][s]);
-                ok = n == 0 || wait_or_abort(empty, (n - 1) & 1, abort_flag, status, kDevMmaTimeout);
-                if (!ok) {
-                    break;
-                }
-                raw.store(tile, row, piece);
-                fence_proxy_async_smem();
-                mbar_arrive(full);
+                ok = ok && convert(1, n, p.seq.len - blk * kBlockN);
             }
         }
-    } else if (warp < T::kConvWarp) {
+    } else {
         // =========================== softmax / epilogue ===========================
         const int t = warp >> 2, quarter = warp & 3;
-        const int lane_row = quarter * 32 + lane;  // row of the tile = TMEM lane
-        const uint32_t t_tile = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + t * T::kTileCols;
-        const uint32_t t_o = t_tile + T::kColO;
+        const int r = quarter * 32 + lane;  // row of the tile = TMEM lane
+        const uint32_t t_lane = (static_cast<uint32_t>(quarter * 32) << 16) + t * T::kTileCols;
+        const uint32_t t_s = tmem_base + t_lane + T::kColS;
+        const uint32_t t_o = tmem_base + t_lane + T::kColO;
+        const uint32_t t_p = tmem_base + t_lane + T::kColP;
         const float sc = a.scale_log2;
-        float* join = sJoin + t * (T::kJoinBytes / 4);
         bool ok = true;
         int pc = 0;
         for (int64_t u = begin; ok && u < end;) {
             Piece p;
             piece_at(a, u, end, lane_class, lane, p);
             u += p.blk1 - p.blk0;
-            int32_t rows = p.rows_valid - t * kTileM;  // of this tile
-            if (rows <= 0) {
+            const int32_t rows_valid = p.rows_valid - t * kTileM;  // of this tile
+            if (rows_valid <= 0) {
                 continue;
             }
-            rows = rows < kTileM ? rows : kTileM;
-            const int copies = replicas(rows), spread = kTileM / copies;
-            const int copy = lane_row / spread, r = lane_row - copy * spread;  // row r of the tile, its copy
-            if (quarter * 32 - copy * spread >= rows) {
-                // no row of this warp exists: its lanes only keep the barriers going
+            if (quarter * 32 >= rows_valid) {
+                // the rows of this warp are behind the last one: its lanes only keep the barriers going
                 for (int32_t blk = p.blk0; ok && blk < p.blk1; ++blk, ++pc) {
-                    ok = wait_or_abort_parked(&bars.s_full[t][pc & 1], (pc >> 1) & 1, abort_flag, status, kDevMmaTimeout);
+                    ok = wait_or_abort_parked(&bars.s_full[t], pc & 1, abort_flag, status, kDevMmaTimeout);
                     if (ok) {
+                        mbar_arrive(&bars.s_free[t]);
                         mbar_arrive(&bars.p_full[t][pc & 1]);
                     }
                 }
-                ok = ok && wait_or_abort_parked(&bars.pv_done[t][(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
-                if (!ok) {
-                    break;
+                ok = ok && wait_or_abort_parked(&bars.pv_done[t][(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status,
+                                                kDevMmaTimeout);
+                if (ok) {
+                    mbar_arrive(&bars.o_free[t]);
                 }
+                continue;
             }
-            const bool live = r < rows;
+            const bool live = r < rows_valid;
             const int32_t row = p.row0 + t * kTileM + r;
             const int32_t tok = live ? row / a.group : 0;
             const uint64_t* anc = a.ancestor + (p.seq.tok0 + tok) * a.words;
             float m_ref = kNegBig, l_sum = 0.0f;
-            // `grown`: a maximum above the reference by more than 2^8; O is rescaled in TMEM, eight columns at a time
-            auto raise = [&](float top, bool rescale) -> bool {
-                const bool grow = top > m_ref + kRescaleSlack;
-                if (!__any_sync(0xffffffffu, grow)) {
-                    return true;
-                }
-                const float m_new = grow ? top : m_ref;
-                const float f = ex2_approx(m_ref - m_new);
-                m_ref = m_new;
-                l_sum *= f;
-                if (rescale) {
-                    if (!wait_or_abort(&bars.pv_done[t][(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout)) {
-                        return false;
+            for (int32_t blk = p.blk0; ok && blk < p.blk1; ++blk, ++pc) {
+                if (pc >= 2) {
+                    ok = wait_or_abort(&bars.pv_done[t][pc & 1], ((pc - 2) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
+                    if (!ok) {
+                        break;
                     }
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < DH / 8; ++c) {
-                        uint32_t v[8];
-                        tmem_ld8(t_o + c * 8, v);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                        }
-                        tmem_st8(t_o + c * 8, v);
-                    }
-                    tmem_wait_st();
                 }
-                return true;
-            };
-            for (int32_t blk = quarter * 32 - copy * spread < rows ? p.blk0 : p.blk1; ok && blk < p.blk1; ++blk, ++pc) {
-                ok = wait_or_abort(&bars.s_full[t][pc & 1], (pc >> 1) & 1, abort_flag, status, kDevMmaTimeout);
+                ok = wait_or_abort(&bars.s_full[t], pc & 1, abort_flag, status, kDevMmaTimeout);
                 if (!ok) {
                     break;
                 }
                 tc_fence_after();
-                const uint32_t t_s = t_tile + (pc & 1) * kBlockN;
-                // 64 positions of this row: bit e = position blk * 64 + e is visible
-                const int32_t a0 = blk * kBlockN - p.seq.start;  // index of the block's first position among the drafts
-                const bool masked = a0 + kBlockN > 0;
-                uint64_t seen = ~0ull;
-                if (masked && live) {
-                    if (a0 <= 0) {
-                        seen = (a0 == 0 ? 0ull : ~0ull >> (64 + a0)) | (anc[0] << -a0);
-                    } else {
-                        const int32_t w = a0 >> 6, sh = a0 & 63;
-                        seen = w < a.words ? anc[w] >> sh : 0ull;
-                        if (sh > 0 && w + 1 < a.words) {
-                            seen |= anc[w + 1] << (64 - sh);
+                float sv[kBlockN];
+                {
+                    uint32_t v[kBlockN / 32][32];
+#pragma unroll
+                    for (int c = 0; c < kBlockN / 32; ++c) {
+                        tmem_ld32(t_s + 32 * c, v[c]);
+                    }
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < kBlockN / 32; ++c) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            sv[32 * c + e] = __uint_as_float(v[c][e]);
                         }
                     }
-                    const int32_t room = p.seq.len - blk * kBlockN;  // positions that exist
-                    if (room < kBlockN) {
-                        seen &= ~0ull >> (64 - room);
+                }
+                tc_fence_before();
+                mbar_arrive(&bars.s_free[t]);
+                const int32_t a0 = blk * kBlockN - p.seq.start;  // index of the block's first position among the drafts
+                if (a0 + kBlockN > 0) {
+                    // 64 positions of this row: bit e = position blk * 64 + e is visible
+                    uint64_t seen = ~0ull;
+                    if (live) {
+                        if (a0 <= 0) {
+                            seen = (a0 == 0 ? 0ull : ~0ull >> (64 + a0)) | (anc[0] << -a0);
+                        } else {
+                            const int32_t w = a0 >> 6, sh = a0 & 63;
+                            seen = w < a.words ? anc[w] >> sh : 0ull;
+                            if (sh > 0 && w + 1 < a.words) {
+                                seen |= anc[w + 1] << (64 - sh);
+                            }
+                        }
+                        const int32_t room = p.seq.len - blk * kBlockN;  // positions that exist
+                        if (room < kBlockN) {
+                            seen &= ~0ull >> (64 - room);
+                        }
+                    }
+                    const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
+#pragma unroll
+                    for (int e = 0; e < kBlockN; ++e) {
+                        sv[e] = ((e < 32 ? lo : hi) >> (e & 31)) & 1u ? sv[e] : -INFINITY;
                     }
                 }
-                const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
-                const bool rescale = blk > p.blk0;
-                if (copies == 1) {
-                    // all 64 positions, in two halves; the second is read twice, which keeps it out of the registers
-                    // while the first is worked on.  P of the first half overwrites scores that are done with.
-                    float v[32];
-                    load_scores(t_s + 32, v);
-                    float top = max_of(v, masked, hi);
-                    load_scores(t_s, v);
-                    top = fmaxf(top, max_of(v, masked, lo)) * sc;
-                    ok = raise(top, rescale);
-                    if (!ok) {
-                        break;
+                float mx0 = fmax3(sv[0], sv[1], sv[2]), mx1 = fmax3(sv[3], sv[4], sv[5]);
+#pragma unroll
+                for (int e = 6; e + 3 < kBlockN; e += 4) {
+                    mx0 = fmax3(mx0, sv[e], sv[e + 1]);
+                    mx1 = fmax3(mx1, sv[e + 2], sv[e + 3]);
+                }
+                float mx = fmax3(mx0, mx1, fmaxf(sv[kBlockN - 2], sv[kBlockN - 1]));
+                mx *= sc;
+                const bool grow = mx > m_ref + kRescaleSlack;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float m_new = grow ? mx : m_ref;
+                    const float f = ex2_approx(m_ref - m_new);
+                    m_ref = m_new;
+                    l_sum *= f;
+                    if (blk > p.blk0) {
+                        ok = wait_or_abort(&bars.pv_done[t][(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
+                        if (!ok) {
+                            break;
+                        }
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < DH / 8; ++c) {  // eight columns at a time: the scores stay in registers
+                            uint32_t v[8];
+                            tmem_ld8(t_o + c * 8, v);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                            }
+                            tmem_st8(t_o + c * 8, v);
+                        }
+                        tmem_wait_st();
                     }
+                }
+                // P = exp2(s * scale - m_ref) as packed fp16; the row sum adds the rounded values that P V uses, in
+                // four chains (one chain of 64 dependent additions would be as long as the exponentials)
+                const uint32_t t_pb = t_p + (pc & 1) * T::kPCols;
+                float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int q = 0; q < kBlockN / 32; ++q) {
                     uint32_t pk[16];
-                    l_sum += weights_of(v, sc, m_ref, pk);
-                    tmem_st16(t_s, pk);
-                    load_scores(t_s + 32, v);
-                    if (masked) {
-                        max_of(v, true, hi);
-                    }
-                    l_sum += weights_of(v, sc, m_ref, pk);
-                    tmem_st16(t_s + 16, pk);
-                } else if (copies == 2) {
-                    float v[32];
-                    load_scores(t_s + copy * 32, v);
-                    ok = raise(max_of(v, masked, copy == 0 ? lo : hi) * sc, rescale);
-                    if (!ok) {
-                        break;
-                    }
-                    uint32_t pk[16];
-                    l_sum += weights_of(v, sc, m_ref, pk);
-                    tmem_st16(t_s + copy * 16, pk);
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        pk[e] = 0u;
+                        const float2 x = __ffma2_rn(make_float2(sv[32 * q + 2 * e], sv[32 * q + 2 * e + 1]),
+                                                    make_float2(sc, sc), make_float2(-m_ref, -m_ref));
+                        pk[e] = h2_as_u32(__floats2half2_rn(ex2_approx(x.x), ex2_approx(x.y)));
+                        add_half2_to_float(l4[e & 3], pk[e]);
                     }
-                    tmem_st16(t_s + (copy ^ 1) * 16, pk);
-                } else {
-                    float v[16];
-                    load_scores(t_s + copy * 16, v);
-                    ok = raise(max_of(v, masked, (copy & 2 ? hi : lo) >> ((copy & 1) * 16)) * sc, rescale);
-                    if (!ok) {
-                        break;
-                    }
-                    uint32_t pk[8], zero[8];
-                    l_sum += weights_of(v, sc, m_ref, pk);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        zero[e] = 0u;
-                    }
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        if (c == copy) {
-                            tmem_st8(t_s + c * 8, pk);
-                        } else {
-                            tmem_st8(t_s + c * 8, zero);
-                        }
-                    }
+                    tmem_st16(t_pb + 16 * q, pk);
                 }
+                l_sum += (l4[0] + l4[1]) + (l4[2] + l4[3]);
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(&bars.p_full[t][pc & 1]);
@@ -850,27 +761,19 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
             if (ok) {
                 ok = wait_or_abort(&bars.pv_done[t][(pc - 1) & 1], ((pc - 1) >> 1) & 1, abort_flag, status, kDevMmaTimeout);
             }
-            if (!ok) {
-                break;
-            }
-            tc_fence_after();
-            const bool whole = p.blk0 == 0 && p.blk1 == p.seq.blocks;
-            const int64_t slot0 = (2 * static_cast<int64_t>(blockIdx.x) + (p.blk0 == 0 ? 1 : 0)) * T::kBlockM + t * kTileM;
-            auto out_row = [&](int32_t of) -> __half* {  // output row of row `of` of the tile
-                const int32_t x = p.row0 + t * kTileM + of, i = x / a.group;
-                return a.out + ((p.seq.tok0 + i) * a.num_heads + p.kvh * a.group + (x - i * a.group)) * DH;
-            };
-            if (copies == 1) {
+            if (ok) {
+                tc_fence_after();
+                const bool whole = p.blk0 == 0 && p.blk1 == p.seq.blocks;
                 const float inv = l_sum > 0.0f ? 1.0f / l_sum : 0.0f;
-                __half* dst = out_row(live ? r : 0);
-                float* part = a.part_o + (slot0 + r) * DH;
+                __half* dst = a.out + ((p.seq.tok0 + tok) * a.num_heads + p.kvh * a.group + (row - tok * a.group)) * DH;
+                const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (p.blk0 == 0 ? 1 : 0)) * T::kBlockM + t * kTileM + r;
+                float* part = a.part_o + slot * DH;
                 if (!whole && live) {
-                    a.part_ml[slot0 + r] = make_float2(m_ref, l_sum);
+                    a.part_ml[slot] = make_float2(m_ref, l_sum);
                 }
 #pragma unroll
                 for (int c = 0; c < DH / 32; ++c) {
                     uint32_t v[32];
-                    __syncwarp();
                     tmem_ld32(t_o + c * 32, v);
                     tmem_wait_ld();
                     if (c == DH / 32 - 1) {
@@ -900,63 +803,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                         }
                     }
                 }
-            } else {
-                // join the copies: their maxima and sums first, then eight channels at a time through shared memory
-                join[2 * lane_row] = m_ref;
-                join[2 * lane_row + 1] = l_sum;
-                tile_barrier(t);
-                float top = kNegBig, sum = 0.0f;
-                for (int f = 0; f < copies; ++f) {
-                    top = fmaxf(top, join[2 * (f * spread + r)]);
-                }
-                for (int f = 0; f < copies; ++f) {
-                    sum += join[2 * (f * spread + r) + 1] * ex2_approx(join[2 * (f * spread + r)] - top);
-                }
-                const float factor = ex2_approx(m_ref - top) * (whole ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f);
-                if (!whole && live && copy == 0) {
-                    a.part_ml[slot0 + r] = make_float2(top, sum);
-                }
-                tile_barrier(t);
-                // thread -> (row, channels): 128 threads share spread rows x 8 channels
-                const int per = 8 / copies;                            // channels of a thread
-                const int out_r = (lane_row * per) >> 3, out_c = (lane_row * per) & 7;
-                __half* dst = out_r < rows ? out_row(out_r) : nullptr;
-                float* part = a.part_o + (slot0 + out_r) * DH;
-#pragma unroll 1
-                for (int c = 0; c < DH / 8; ++c) {
-                    uint32_t v[8];
-                    __syncwarp();
-                    tmem_ld8(t_o + c * 8, v);
-                    tmem_wait_ld();
-                    if (c == DH / 8 - 1) {
-                        tc_fence_before();
-                        mbar_arrive(&bars.o_free[t]);
-                    }
-                    float* buf = join + (c & 1) * (kTileM * 8);
-                    float4* mine = reinterpret_cast<float4*>(buf + lane_row * 8);
-                    mine[0] = make_float4(__uint_as_float(v[0]) * factor, __uint_as_float(v[1]) * factor,
-                                          __uint_as_float(v[2]) * factor, __uint_as_float(v[3]) * factor);
-                    mine[1] = make_float4(__uint_as_float(v[4]) * factor, __uint_as_float(v[5]) * factor,
-                                          __uint_as_float(v[6]) * factor, __uint_as_float(v[7]) * factor);
-                    tile_barrier(t);  // two buffers: the next round's writes cannot meet this round's reads
-                    if (out_r < rows) {
-#pragma unroll 2
-                        for (int e = 0; e < per; e += 2) {
-                            float2 x = make_float2(0.0f, 0.0f);
-                            for (int f = 0; f < copies; ++f) {
-                                const float2 y = *reinterpret_cast<const float2*>(buf + (f * spread + out_r) * 8 + out_c + e);
-                                x.x += y.x;
-                                x.y += y.y;
-                            }
-                            if (whole) {
-                                *reinterpret_cast<__half2*>(dst + c * 8 + out_c + e) = __floats2half2_rn(x.x, x.y);
-                            } else {
-                                *reinterpret_cast<float2*>(part + c * 8 + out_c + e) = x;
-                            }
-                        }
-                    }
-                }
-                tile_barrier(t);
             }
         }
     }
