@@ -25,6 +25,7 @@
 #include <cub/block/block_scan.cuh>
 
 #include "common.cuh"
+#include "kv_tiles.cuh"
 #include "launch.h"
 #include "ragged.cuh"
 #include "tcgen05.cuh"
@@ -35,7 +36,7 @@ namespace pplb200 {
 namespace {
 
 constexpr int kTileM = 128;  // rows of an MMA
-constexpr int kBlockN = 64;
+constexpr int kBlockN = kTileRows;  // positions of a block
 constexpr int kRawStages = 2;
 constexpr int kMinRange = 4;  // blocks: no range is cut finer
 constexpr float kNegBig = -1.0e30f;
@@ -238,91 +239,6 @@ struct Barriers {
 };
 static_assert(sizeof(Barriers<2>) <= 512, "barrier block");
 
-// 16 codes -> 16 halves of value, scaled by two groups' scales (s = scale of channels 0..7 | 8..15 << 16)
-__device__ __forceinline__ void dequant16(const uint4& c, uint32_t s, uint4& lo, uint4& hi) {
-    const __half2 s0 = u32_as_h2(prmt(s, 0u, 0x1010u)), s1 = u32_as_h2(prmt(s, 0u, 0x3232u));
-    const uint32_t x0 = c.x ^ 0x80808080u, x1 = c.y ^ 0x80808080u, x2 = c.z ^ 0x80808080u, x3 = c.w ^ 0x80808080u;
-    lo.x = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5140u>(x0), s0));
-    lo.y = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5342u>(x0), s0));
-    lo.z = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5140u>(x1), s0));
-    lo.w = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5342u>(x1), s0));
-    hi.x = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5140u>(x2), s1));
-    hi.y = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5342u>(x2), s1));
-    hi.z = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5140u>(x3), s1));
-    hi.w = h2_as_u32(__hmul2(biased_bytes_to_half2<0x5342u>(x3), s1));
-}
-
-__device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
-    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "r"(addr)
-                 : "memory");
-    return v;
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-}
-
-// One thread's share of a raw K or V block: 16-byte piece `piece` of the rows row, row + kRowsPerStep, ..
-template <int DH>
-struct Raw {
-    static constexpr int kPieces = DH / 16;            // 16-byte pieces of a row
-    static constexpr int kRowsPerStep = 32 / kPieces;  // rows of a warp at once
-    static constexpr int kRows = 16 / kRowsPerStep;    // steps over the warp's 16 rows
-    uint4 code[kRows];
-    uint32_t sc[kRows];
-
-    __device__ __forceinline__ void load(uint32_t raw, int32_t row, int32_t piece, int32_t rows) {
-#pragma unroll
-        for (int k = 0; k < kRows; ++k) {
-            const int32_t r = row + k * kRowsPerStep;
-            const int32_t chunk = DH == 128 ? piece ^ (r & 7) : piece;  // as the 128-byte swizzle of the copy left it
-            code[k] = lds128(raw + r * DH + chunk * 16);
-            sc[k] = lds32(raw + kBlockN * DH + r * (DH / 4) + piece * 4);
-            if (r >= rows) {  // rows behind the sequence's end may hold anything
-                code[k] = make_uint4(0u, 0u, 0u, 0u);
-                sc[k] = 0u;
-            }
-        }
-    }
-
-    // -> the swizzled fp16 tile at `tile`: [64 rows][64 halves] blocks, 16-byte chunk c of row r at chunk c ^ (r & 7)
-    __device__ __forceinline__ void store(uint32_t tile, int32_t row, int32_t piece) const {
-        const int32_t cb = piece >> 2, c = (piece & 3) * 2;
-#pragma unroll
-        for (int k = 0; k < kRows; ++k) {
-            const int32_t r = row + k * kRowsPerStep;
-            const uint32_t at = tile + cb * (kBlockN * 128) + r * 128;
-            uint4 lo, hi;
-            dequant16(code[k], sc[k], lo, hi);
-            const uint32_t c0 = at + ((c ^ (r & 7)) << 4), c1 = at + (((c + 1) ^ (r & 7)) << 4);
-            // the two column blocks start with different chunks: eight lanes then fill all banks once
-            const bool odd = cb != 0;
-            sts128(odd ? c1 : c0, odd ? hi : lo);
-            sts128(odd ? c0 : c1, odd ? lo : hi);
-        }
-    }
-};
-
-// `rows` rows of one head, K (0) or V (1), from cache row `row` on
-__device__ __forceinline__ void load_rows(const TreeArgs& a, void* dst, const CUtensorMap* map, uint64_t* bar, int row,
-                                          int head, int kv) {
-    int c[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int pos = i + 1;
-        c[i] = a.order.pos_row == pos ? row
-                                      : (a.order.pos_head == pos ? head : (a.order.pos_kv == pos ? kv : static_cast<int>(a.geom.layer_idx)));
-    }
-    tma_load_5d(dst, map, bar, 0, c[0], c[1], c[2], c[3]);
-}
-
 template <int DH, int MT>
 __global__ void __launch_bounds__(TTraits<DH, MT>::kThreads, TTraits<DH, MT>::kCtasPerSm)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_constant__ CUtensorMap tm_scale, const TreeArgs a) {
@@ -435,8 +351,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                     }
                     __syncwarp();
                     if (lane < boxes) {
-                        load_rows(a, dst + lane * a.box_rows * DH, &tm_code, bar, row, p.kvh, kv);
-                        load_rows(a, dst + T::kCodeBytes + lane * a.box_rows * (DH / 4), &tm_scale, bar, row, p.kvh, kv);
+                        load_rows(dst + lane * a.box_rows * DH, &tm_code, bar, a.order, row, p.kvh, kv, a.geom.layer_idx);
+                        load_rows(dst + T::kCodeBytes + lane * a.box_rows * (DH / 4), &tm_scale, bar, a.order, row, p.kvh, kv, a.geom.layer_idx);
                     }
                     __syncwarp();
                 }
@@ -561,10 +477,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
             }
             Raw<DH> raw;
             raw.load(raw0 + (2 * s + kv) * T::kRawBytes, row, piece, rows);
-            // The loads have to be over before the slot is handed back.  The arrival alone does not see to that: the
-            // scales were found loaded behind it, next to their use, when the next copy had overwritten them.
-            __threadfence_block();
-            mbar_arrive(&bars.raw_empty[kv][s]);
+            hand_back(&bars.raw_empty[kv][s]);
             if (blk_no > 0 && !wait_or_abort(kv ? &bars.v_empty : &bars.k_empty, (blk_no - 1) & 1, abort_flag, status,
                                              kDevMmaTimeout)) {
                 return false;
