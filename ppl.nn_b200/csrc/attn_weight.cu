@@ -1,22 +1,20 @@
 // Accumulated attention weight: w[row(j)] += sum over the query heads of a kv group and over the query tokens of
 // softmax_j(q . k_j / sqrt(Dh)), for every cached position j of every sequence.  Only K is read.
 //
-// The normaliser of a row needs all its scores before any weight is known.  attn_weight_stats_kernel leaves, per query
-// row and chunk of positions, the maximum and the sum of exponentials, and attn_weight_merge_kernel joins the chunks.
-// With up to 8 query rows per kv head (decode steps) the scores themselves go to the workspace as well (4 bytes a row
-// against the 160 of a K row at Dh 128), and attn_weight_spread_kernel joins the chunks and reads the scores; with more
-// rows attn_weight_apply_kernel forms them again and adds each position's normalised weights up.
+// The normaliser of a row needs all its scores before any weight is known.  This file has the form for up to 8 query
+// rows (token x head of the group) per kv head, i.e. for decode steps; attn_window.cu the one for more.
+// attn_weight_stats_kernel leaves, per query row and chunk of positions, the maximum and the sum of exponentials, and
+// writes the raw scores to the workspace (4 bytes a row against the 160 of a K row at Dh 128), so that K is read once;
+// attn_weight_spread_kernel joins the chunks and turns the scores into weights.
 //
-// Both score kernels: a CTA takes a chunk of the positions of one (sequence, kv head), a warp 16 positions at a
-// time.  Positions are the M dimension of mma.m16n8k16, the query rows (token x head of the group) come in octets as
-// its N dimension.  A thread needs the channels 2t, 2t+1, 2t+8, 2t+9 of each block of 16 for rows g and g+8 of the
-// A operand; as the order of the channels does not matter as long as Q has the same, thread t takes 16 consecutive
-// code bytes per 64 channels straight from global memory.
+// The score kernel: a CTA takes a chunk of the positions of one (sequence, kv head), a warp 16 positions at a time.
+// Positions are the M dimension of mma.m16n8k16, the query rows its N dimension.  A thread needs the channels 2t, 2t+1,
+// 2t+8, 2t+9 of each block of 16 for rows g and g+8 of the A operand; as the order of the channels does not matter as
+// long as Q has the same, thread t takes 16 consecutive code bytes per 64 channels.
 //
 // The weights are fp32 and proportional to exp(score), so a key rounded to fp16 would cost 1e-4 of their value;
-// k = code * scale is therefore split into fp16(k) and the exact remainder, and both enter the accumulator.
-#include "common.cuh"
-#include "launch.h"
+// k = code * scale is therefore split into fp16(k) and the exact remainder, which have accumulators of their own.
+#include "attn_weight.cuh"
 
 namespace pplb200 {
 
@@ -24,32 +22,10 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kChunk = 512;     // positions of a CTA where the scores are formed twice
+constexpr int kChunk = 512;     // positions of a CTA, at least
 constexpr int kSpread = 2048;   // positions of a CTA of attn_weight_spread_kernel
-constexpr int kRowBlock = 32;   // query rows whose fragments are held in registers at a time
-constexpr int kScoreRows = 8;   // up to so many query rows per kv head the scores are kept
 constexpr int kStages = 3;      // tiles of a warp's ring
-constexpr float kNegBig = -1.0e30f;
-
-struct WeightArgs {
-    const __half* q;
-    const int64_t* seqstarts;
-    const int64_t* cachestarts;
-    const int64_t* start_pos;
-    const int8_t* cache;
-    const __half* scale;
-    float* weight;   // [L, Hkv, MaxT]
-    float2* part;    // [chunks][T][Hq]: maximum (exp2 domain) and sum
-    float2* norm;    // [T][Hq]: maximum and reciprocal sum
-    float* score;    // [batch][Hkv][max_kvlen][kScoreRows or fewer]: raw scores, -inf where hidden, or null
-    int32_t score_rows;
-    uint32_t* status;
-    CacheGeom geom;
-    int64_t max_seqlen, max_kvlen, max_tokens, total_tokens;
-    int32_t num_heads, num_kv_heads, group, causal, chunks;
-    int32_t chunk;   // positions of a chunk
-    float scale_log2;
-};
+constexpr float kNegBig = kWeightNegBig;
 
 // D = A B, without an accumulator to start from
 __device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -70,37 +46,6 @@ __device__ __forceinline__ void split_key_word(uint32_t w, __half2 s2, uint32_t&
     k1 = h2_as_u32(p1);
     e0 = h2_as_u32(__hfma2(c0, s2, __hneg2(p0)));
     e1 = h2_as_u32(__hfma2(c1, s2, __hneg2(p1)));
-}
-
-// What a CTA works on
-struct Span {
-    int64_t tok0;   // first query row of the sequence
-    int64_t start;  // positions before its first query token
-    int32_t rows;   // query rows: tokens * group
-    int32_t len;    // positions
-};
-
-__device__ __forceinline__ Span span_of(const WeightArgs& a, int64_t b) {
-    Span s;
-    s.tok0 = a.seqstarts[b];
-    int64_t n = a.seqstarts[b + 1] - s.tok0;
-    if (s.tok0 < 0 || s.tok0 + n > a.total_tokens) {
-        n = 0;
-    }
-    bool cut = n > a.max_seqlen;
-    n = cut ? a.max_seqlen : (n < 0 ? 0 : n);
-    s.start = a.start_pos[b];
-    int64_t len = s.start < 0 ? 0 : s.start + n;
-    if (len > a.max_kvlen) {
-        len = a.max_kvlen;
-        cut = true;
-    }
-    if (cut && threadIdx.x == 0) {
-        atomicOr(a.status, kDevLengthClamped);
-    }
-    s.rows = static_cast<int32_t>(n) * a.group;
-    s.len = n > 0 ? static_cast<int32_t>(len) : 0;
-    return s;
 }
 
 // A warp's ring of tiles in shared memory: 16 K rows of one (sequence, kv head), codes and scales, copied
@@ -181,9 +126,9 @@ struct Ring {
     }
 };
 
-// Scores (unscaled) of 16 positions against NOCT octets of query rows whose fragments are in qf.
-// acc[o][0..1]: position g, rows 2t and 2t+1 of octet o; acc[o][2..3]: position g + 8.
-template <int DH, int NOCT>
+// Scores (unscaled) of 16 positions against the query rows whose fragments are in qf.
+// acc[0..1]: position g, rows 2t and 2t+1; acc[2..3]: position g + 8.
+template <int DH>
 struct Tile {
     static constexpr int kWords = DH / 16;
     uint4 code[2][DH / 64];
@@ -216,11 +161,10 @@ struct Tile {
         }
     }
 
-    // The keys and their remainders have accumulators of their own, and with one octet there are two of each: shorter
-    // chains of dependent instructions, and of roundings.
-    __device__ __forceinline__ void scores(const uint2 (&qf)[NOCT][kWords], float (&acc)[NOCT][4]) const {
-        constexpr int kChains = NOCT == 1 ? 2 : 1;
-        float key[kChains][NOCT][4], rest[kChains][NOCT][4];
+    // The keys and their remainders have two accumulators each: short chains of dependent instructions, and of
+    // roundings.
+    __device__ __forceinline__ void scores(const uint2 (&qf)[kWords], float (&acc)[4]) const {
+        float key[2][4], rest[2][4];
 #pragma unroll
         for (int w = 0; w < kWords; ++w) {
             uint32_t k[2][2], e[2][2];
@@ -231,112 +175,28 @@ struct Tile {
                 const uint32_t s = prmt(sc[r][w / 4], 0u, (w & 2) ? 0x3232u : 0x1010u);
                 split_key_word(word, u32_as_h2(s), k[r][0], k[r][1], e[r][0], e[r][1]);
             }
-#pragma unroll
-            for (int o = 0; o < NOCT; ++o) {
-                if (w < kChains) {
-                    mma_first(key[w % kChains][o], k[0][0], k[1][0], k[0][1], k[1][1], qf[o][w].x, qf[o][w].y);
-                } else {
-                    mma_m16n8k16_f16f32(key[w % kChains][o], k[0][0], k[1][0], k[0][1], k[1][1], qf[o][w].x, qf[o][w].y);
-                }
-            }
-#pragma unroll
-            for (int o = 0; o < NOCT; ++o) {
-                if (w < kChains) {
-                    mma_first(rest[w % kChains][o], e[0][0], e[1][0], e[0][1], e[1][1], qf[o][w].x, qf[o][w].y);
-                } else {
-                    mma_m16n8k16_f16f32(rest[w % kChains][o], e[0][0], e[1][0], e[0][1], e[1][1], qf[o][w].x, qf[o][w].y);
-                }
+            if (w < 2) {
+                mma_first(key[w & 1], k[0][0], k[1][0], k[0][1], k[1][1], qf[w].x, qf[w].y);
+                mma_first(rest[w & 1], e[0][0], e[1][0], e[0][1], e[1][1], qf[w].x, qf[w].y);
+            } else {
+                mma_m16n8k16_f16f32(key[w & 1], k[0][0], k[1][0], k[0][1], k[1][1], qf[w].x, qf[w].y);
+                mma_m16n8k16_f16f32(rest[w & 1], e[0][0], e[1][0], e[0][1], e[1][1], qf[w].x, qf[w].y);
             }
         }
 #pragma unroll
-        for (int o = 0; o < NOCT; ++o) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                acc[o][e] = key[0][o][e] + rest[0][o][e];
-                if constexpr (kChains == 2) {
-                    acc[o][e] = (key[0][o][e] + key[1][o][e]) + (rest[0][o][e] + rest[1][o][e]);
-                }
-            }
+        for (int e = 0; e < 4; ++e) {
+            acc[e] = (key[0][e] + key[1][e]) + (rest[0][e] + rest[1][e]);
         }
     }
 };
 
-// Query fragments of the rows [row0, row0 + 8 NOCT): rows behind the last read as zeros
-template <int DH, int NOCT>
-__device__ __forceinline__ void load_queries(const WeightArgs& a, const Span& s, int head, int32_t row0, int lane,
-                                             uint2 (&qf)[NOCT][DH / 16]) {
-    const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-    for (int o = 0; o < NOCT; ++o) {
-        const int32_t r = row0 + o * 8 + g;
-        const int32_t i = r / a.group;
-        const __half* src = a.q + ((s.tok0 + i) * a.num_heads + head * a.group + (r - i * a.group)) * DH;
-#pragma unroll
-        for (int w = 0; w < DH / 16; ++w) {
-            qf[o][w] = make_uint2(0u, 0u);
-            if (r < s.rows) {
-                qf[o][w] = *reinterpret_cast<const uint2*>(src + (w / 4) * 64 + t * 16 + (w & 3) * 4);
-            }
-        }
-    }
-}
-
-// -inf in the places of `acc` that a query row may not see
-template <int NOCT>
-__device__ __forceinline__ void hide(const WeightArgs& a, const Span& s, int32_t row0, int32_t tile0, int lane,
-                                     float (&acc)[NOCT][4]) {
-    const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-    for (int o = 0; o < NOCT; ++o) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int32_t r = row0 + o * 8 + 2 * t + c;
-            const int64_t last = a.causal ? s.start + r / a.group : s.len - 1;
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const int32_t j = tile0 + g + 8 * p;
-                if (j > last || j >= s.len) {
-                    acc[o][2 * p + c] = -INFINITY;
-                }
-            }
-        }
-    }
-}
-
-// work(tile, position) for this warp's tiles of [tile0, end)
-template <int DH, int NOCT, typename Work>
-__device__ __forceinline__ void for_tiles(const WeightArgs& a, const Ring<DH>& ring, int64_t b, int32_t tile0, int32_t end,
-                                          int32_t len, int lane, Work work) {
-    constexpr int kStep = kWarps * 16;
-    __syncwarp();  // the ring may still be read for the rows before
-#pragma unroll
-    for (int k = 0; k < kStages - 1; ++k) {
-        ring.issue(a, b, tile0 + k * kStep, end, len, k, lane);
-    }
-    const uint32_t code_addr = ring.base + Tile<DH, NOCT>::code_offset(lane);
-    const uint32_t scale_addr = ring.base + Tile<DH, NOCT>::scale_offset(lane);
-    int stage = 0, ahead = kStages - 1;
-    for (; tile0 < end; tile0 += kStep) {
-        ring.issue(a, b, tile0 + (kStages - 1) * kStep, end, len, ahead, lane);
-        cp_async_wait<kStages - 1>();
-        __syncwarp();
-        Tile<DH, NOCT> tile;
-        tile.read(code_addr + stage * Ring<DH>::kTileBytes, scale_addr + stage * Ring<DH>::kTileBytes);
-        __syncwarp();  // everyone has read: the next round may overwrite the stage
-        work(tile, tile0);
-        ahead = stage;
-        stage = stage + 1 == kStages ? 0 : stage + 1;
-    }
-    cp_async_wait<0>();
-}
-
-template <int DH, int NOCT>
-__global__ void __launch_bounds__(kThreads, NOCT == 1 ? 6 : 3) attn_weight_stats_kernel(const WeightArgs a) {
+template <int DH>
+__global__ void __launch_bounds__(kThreads, 6) attn_weight_stats_kernel(const WeightArgs a) {
     grid_launch_dependents();
     grid_dependency_wait();
-    __shared__ float2 red[kWarps][NOCT * 8];
+    __shared__ float2 red[kWarps][kScoreRows];
     __shared__ __align__(128) uint8_t smem[kWarps * Ring<DH>::kWarpBytes];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int64_t b = blockIdx.z;
     const int head = blockIdx.x, chunk = blockIdx.y;  // neighbouring CTAs read neighbouring heads of the same rows
     const Span s = span_of(a, b);
@@ -346,219 +206,105 @@ __global__ void __launch_bounds__(kThreads, NOCT == 1 ? 6 : 3) attn_weight_stats
     }
     const int32_t end = first + a.chunk < s.len ? first + a.chunk : s.len;
     const Ring<DH> ring(a, s, b, head, warp, lane, smem);
-    float* score = a.score + (b * a.num_kv_heads + head) * a.max_kvlen * a.score_rows;  // NOCT == 1
-    for (int32_t row0 = 0; row0 < s.rows; row0 += NOCT * 8) {
-        uint2 qf[NOCT][DH / 16];
-        load_queries<DH, NOCT>(a, s, head, row0, lane, qf);
-        float m[NOCT][2], l[NOCT][2];
+    float* score = a.score + (b * a.num_kv_heads + head) * a.max_kvlen * a.score_rows;
+    // query fragments: row g (zeros behind the last)
+    uint2 qf[DH / 16];
+    {
+        const int32_t i = g / a.group;
+        const __half* src = a.q + ((s.tok0 + i) * a.num_heads + head * a.group + (g - i * a.group)) * DH;
 #pragma unroll
-        for (int o = 0; o < NOCT; ++o) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                m[o][c] = kNegBig;
-                l[o][c] = 0.0f;
+        for (int w = 0; w < DH / 16; ++w) {
+            qf[w] = make_uint2(0u, 0u);
+            if (g < s.rows) {
+                qf[w] = *reinterpret_cast<const uint2*>(src + (w / 4) * 64 + t * 16 + (w & 3) * 4);
             }
         }
-        auto work = [&](const Tile<DH, NOCT>& tile, int32_t tile0) {
-            float acc[NOCT][4];
-            tile.scores(qf, acc);
-            if (tile0 + 15 > s.start || tile0 + 15 >= s.len) {
-                hide<NOCT>(a, s, row0, tile0, lane, acc);
-            }
-            if constexpr (NOCT == 1) {
-                const int g = lane >> 2, t = lane & 3;
-                if (2 * t < s.rows) {
-                    float* dst = score + (tile0 + g) * a.score_rows + 2 * t;
+    }
+    // the last position that rows 2t and 2t + 1 see
+    int64_t last[2];
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        if (tile0 + g + 8 * p < s.len) {
-                            dst[p * 8 * a.score_rows] = acc[0][2 * p];
-                            if (2 * t + 1 < s.rows) {
-                                dst[p * 8 * a.score_rows + 1] = acc[0][2 * p + 1];
-                            }
-                        }
-                    }
-                }
-            }
+    for (int c = 0; c < 2; ++c) {
+        last[c] = a.causal ? s.start + (2 * t + c) / a.group : s.len - 1;
+        last[c] = last[c] < s.len - 1 ? last[c] : s.len - 1;
+    }
+    float m[2] = {kNegBig, kNegBig}, l[2] = {0.0f, 0.0f};
+    constexpr int kStep = kWarps * 16;
+    int32_t tile0 = first + warp * 16;
 #pragma unroll
-            for (int o = 0; o < NOCT; ++o) {
+    for (int k = 0; k < kStages - 1; ++k) {
+        ring.issue(a, b, tile0 + k * kStep, end, s.len, k, lane);
+    }
+    const uint32_t code_addr = ring.base + Tile<DH>::code_offset(lane);
+    const uint32_t scale_addr = ring.base + Tile<DH>::scale_offset(lane);
+    int stage = 0, ahead = kStages - 1;
+    for (; tile0 < end; tile0 += kStep) {
+        ring.issue(a, b, tile0 + (kStages - 1) * kStep, end, s.len, ahead, lane);
+        cp_async_wait<kStages - 1>();
+        __syncwarp();
+        Tile<DH> tile;
+        tile.read(code_addr + stage * Ring<DH>::kTileBytes, scale_addr + stage * Ring<DH>::kTileBytes);
+        __syncwarp();  // everyone has read: the next round may overwrite the stage
+        ahead = stage;
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        float acc[4];
+        tile.scores(qf, acc);
+        if (tile0 + 15 > s.start || tile0 + 15 >= s.len) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const float x = acc[o][c] * a.scale_log2, y = acc[o][2 + c] * a.scale_log2;
-                    const float top = fmaxf(m[o][c], fmaxf(x, y));
-                    l[o][c] = l[o][c] * ex2_approx(m[o][c] - top) + ex2_approx(x - top) + ex2_approx(y - top);
-                    m[o][c] = top;
-                }
-            }
-        };
-        for_tiles<DH, NOCT>(a, ring, b, first + warp * 16, end, s.len, lane, work);
-        // over the eight positions a column's values are spread over, then over the warps
-#pragma unroll
-        for (int o = 0; o < NOCT; ++o) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) {
-                    const float om = __shfl_xor_sync(0xffffffffu, m[o][c], x);
-                    const float ol = __shfl_xor_sync(0xffffffffu, l[o][c], x);
-                    const float top = fmaxf(m[o][c], om);
-                    l[o][c] = l[o][c] * ex2_approx(m[o][c] - top) + ol * ex2_approx(om - top);
-                    m[o][c] = top;
-                }
-                if (lane < 4) {
-                    red[warp][o * 8 + 2 * lane + c] = make_float2(m[o][c], l[o][c]);
+            for (int e = 0; e < 4; ++e) {
+                if (tile0 + g + 8 * (e >> 1) > last[e & 1]) {
+                    acc[e] = -INFINITY;
                 }
             }
         }
-        __syncthreads();
-        const int32_t r = row0 + threadIdx.x;
-        if (threadIdx.x < NOCT * 8 && r < s.rows) {
-            float2 v = red[0][threadIdx.x];
-#pragma unroll
-            for (int k = 1; k < kWarps; ++k) {
-                const float2 u = red[k][threadIdx.x];
-                const float top = fmaxf(v.x, u.x);
-                v.y = v.y * ex2_approx(v.x - top) + u.y * ex2_approx(u.x - top);
-                v.x = top;
-            }
-            const int32_t i = r / a.group;
-            const int64_t at = (s.tok0 + i) * a.num_heads + head * a.group + (r - i * a.group);
-            a.part[chunk * a.total_tokens * a.num_heads + at] = v;
-        }
-        __syncthreads();
-    }
-}
-
-// Maximum and reciprocal sum of row `at` over its chunks; all lanes of a warp call it.
-__device__ __forceinline__ float2 join_chunks(const WeightArgs& a, int64_t at, int32_t chunks, int lane) {
-    float m = kNegBig, l = 0.0f;
-    for (int32_t c = lane; c < chunks; c += 32) {
-        const float2 v = a.part[c * a.total_tokens * a.num_heads + at];
-        const float top = fmaxf(m, v.x);
-        l = l * ex2_approx(m - top) + v.y * ex2_approx(v.x - top);
-        m = top;
-    }
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, x), ol = __shfl_xor_sync(0xffffffffu, l, x);
-        const float top = fmaxf(m, om);
-        l = l * ex2_approx(m - top) + ol * ex2_approx(om - top);
-        m = top;
-    }
-    return make_float2(m, l > 0.0f ? 1.0f / l : 0.0f);
-}
-
-// One warp per (query token, head): joins the chunks of its sequence.
-__global__ void __launch_bounds__(256) attn_weight_merge_kernel(const WeightArgs a, int32_t batch) {
-    grid_launch_dependents();
-    grid_dependency_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t id = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
-    const int64_t tok = id / a.num_heads;
-    if (tok >= a.total_tokens) {
-        return;
-    }
-    int32_t lo = 0, hi = batch;  // sequence of the token
-    while (hi - lo > 1) {
-        const int32_t mid = (lo + hi) >> 1;
-        if (a.seqstarts[mid] <= tok) {
-            lo = mid;
-        } else {
-            hi = mid;
-        }
-    }
-    const int64_t i = tok - a.seqstarts[lo], start = a.start_pos[lo];
-    int64_t n = a.seqstarts[lo + 1] - a.seqstarts[lo];
-    n = n > a.max_seqlen ? a.max_seqlen : n;
-    int64_t len = start < 0 ? 0 : start + n;
-    len = len > a.max_kvlen ? a.max_kvlen : len;
-    if (i < 0 || i >= n) {
-        return;
-    }
-    const float2 v = join_chunks(a, id, static_cast<int32_t>((len + a.chunk - 1) / a.chunk), lane);
-    if (lane == 0) {
-        a.norm[id] = v;
-    }
-}
-
-template <int DH, int NOCT>
-__global__ void __launch_bounds__(kThreads, 3) attn_weight_apply_kernel(const WeightArgs a) {
-    grid_launch_dependents();
-    grid_dependency_wait();
-    __shared__ float sum[kChunk];
-    __shared__ __align__(128) uint8_t smem[kWarps * Ring<DH>::kWarpBytes];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int64_t b = blockIdx.z;
-    const int head = blockIdx.x, chunk = blockIdx.y;  // neighbouring CTAs read neighbouring heads of the same rows
-    const Span s = span_of(a, b);
-    const int32_t first = chunk * kChunk;
-    if (first >= s.len) {
-        return;
-    }
-    const int32_t end = first + kChunk < s.len ? first + kChunk : s.len;
-    const Ring<DH> ring(a, s, b, head, warp, lane, smem);
-    float* w = a.weight + (a.geom.layer_idx * a.num_kv_heads + head) * a.max_tokens;
-    for (int32_t row0 = 0; row0 < s.rows; row0 += NOCT * 8) {
-        uint2 qf[NOCT][DH / 16];
-        load_queries<DH, NOCT>(a, s, head, row0, lane, qf);
-        float neg_m[NOCT][2], inv[NOCT][2];
-#pragma unroll
-        for (int o = 0; o < NOCT; ++o) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int32_t r = row0 + o * 8 + 2 * t + c;
-                neg_m[o][c] = -INFINITY;  // rows behind the last: no weight
-                inv[o][c] = 0.0f;
-                if (r < s.rows) {
-                    const int32_t i = r / a.group;
-                    const float2 v = a.norm[(s.tok0 + i) * a.num_heads + head * a.group + (r - i * a.group)];
-                    neg_m[o][c] = -v.x;
-                    inv[o][c] = v.y;
-                }
-            }
-        }
-        const bool last_rows = row0 + NOCT * 8 >= s.rows;
-        auto work = [&](const Tile<DH, NOCT>& tile, int32_t tile0) {
-            float acc[NOCT][4];
-            tile.scores(qf, acc);
-            if (tile0 + 15 > s.start || tile0 + 15 >= s.len) {
-                hide<NOCT>(a, s, row0, tile0, lane, acc);
-            }
-            float part[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (int o = 0; o < NOCT; ++o) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        part[p] = fmaf(ex2_approx(fmaf(acc[o][2 * p + c], a.scale_log2, neg_m[o][c])), inv[o][c], part[p]);
-                    }
-                }
-            }
+        if (2 * t < s.rows) {
+            float* dst = score + static_cast<int64_t>(tile0 + g) * a.score_rows + 2 * t;
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-                part[p] += __shfl_xor_sync(0xffffffffu, part[p], 1);
-                part[p] += __shfl_xor_sync(0xffffffffu, part[p], 2);
-            }
-            // lane t = 0 of a quad owns position g, t = 1 position g + 8: one addition per position and call
-            if (t < 2) {
-                const int i = g + 8 * t;
-                float x = t == 0 ? part[0] : part[1];
-                float* acc_row = &sum[tile0 - first + i];
-                if (row0 > 0) {
-                    x += *acc_row;
-                }
-                if (!last_rows) {
-                    *acc_row = x;
-                } else if (tile0 + i < s.len) {
-                    const int64_t row = ring.row_of(a, b, tile0);
-                    if (row >= 0 && cache_row_ok(row + i, a.max_tokens)) {
-                        atomicAdd(w + row + i, x);
+                if (tile0 + g + 8 * p < s.len) {
+                    dst[p * 8 * a.score_rows] = acc[2 * p];
+                    if (2 * t + 1 < s.rows) {
+                        dst[p * 8 * a.score_rows + 1] = acc[2 * p + 1];
                     }
                 }
             }
-        };
-        for_tiles<DH, NOCT>(a, ring, b, first + warp * 16, end, s.len, lane, work);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const float x = acc[c] * a.scale_log2, y = acc[2 + c] * a.scale_log2;
+            const float top = fmaxf(m[c], fmaxf(x, y));
+            l[c] = l[c] * ex2_approx(m[c] - top) + ex2_approx(x - top) + ex2_approx(y - top);
+            m[c] = top;
+        }
+    }
+    cp_async_wait<0>();
+    // over the eight positions a column's values are spread over, then over the warps
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+            const float om = __shfl_xor_sync(0xffffffffu, m[c], x);
+            const float ol = __shfl_xor_sync(0xffffffffu, l[c], x);
+            const float top = fmaxf(m[c], om);
+            l[c] = l[c] * ex2_approx(m[c] - top) + ol * ex2_approx(om - top);
+            m[c] = top;
+        }
+        if (lane < 4) {
+            red[warp][2 * lane + c] = make_float2(m[c], l[c]);
+        }
+    }
+    __syncthreads();
+    if (static_cast<int32_t>(threadIdx.x) < s.rows) {
+        float2 v = red[0][threadIdx.x];
+#pragma unroll
+        for (int k = 1; k < kWarps; ++k) {
+            const float2 u = red[k][threadIdx.x];
+            const float top = fmaxf(v.x, u.x);
+            v.y = v.y * ex2_approx(v.x - top) + u.y * ex2_approx(u.x - top);
+            v.x = top;
+        }
+        const int32_t i = threadIdx.x / a.group;
+        const int64_t at = (s.tok0 + i) * a.num_heads + head * a.group + (threadIdx.x - i * a.group);
+        a.part[chunk * a.total_tokens * a.num_heads + at] = v;
     }
 }
 
@@ -624,30 +370,14 @@ template <int DH>
 int launch_dh(const pplb200_attn_params& p, const WeightArgs& a, cudaStream_t stream) {
     const dim3 grid(static_cast<unsigned>(p.num_kv_heads), static_cast<unsigned>(a.chunks), static_cast<unsigned>(p.batch));
     // each kernel starts while the one before it drains, and waits for it before it reads anything
-    if (p.max_seqlen * a.group <= kScoreRows) {
-        launch_dependent(attn_weight_stats_kernel<DH, 1>, grid, dim3(kThreads), 0, stream, a);
-        const int rc = check_launch("attn_weight_stats_kernel");
-        if (rc != PPLB200_SUCCESS) {
-            return rc;
-        }
-        const dim3 spread(grid.x, static_cast<unsigned>((p.max_kvlen + kSpread - 1) / kSpread), grid.z);
-        launch_dependent(attn_weight_spread_kernel, spread, dim3(256), 0, stream, a);
-        return check_launch("attn_weight_spread_kernel");
-    }
-    launch_dependent(attn_weight_stats_kernel<DH, kRowBlock / 8>, grid, dim3(kThreads), 0, stream, a);
-    int rc = check_launch("attn_weight_stats_kernel");
+    launch_dependent(attn_weight_stats_kernel<DH>, grid, dim3(kThreads), 0, stream, a);
+    const int rc = check_launch("attn_weight_stats_kernel");
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    const int64_t warps = p.total_tokens * p.num_heads;
-    launch_dependent(attn_weight_merge_kernel, dim3(static_cast<unsigned>((warps * 32 + 255) / 256)), dim3(256), 0, stream, a,
-                     static_cast<int32_t>(p.batch));
-    rc = check_launch("attn_weight_merge_kernel");
-    if (rc != PPLB200_SUCCESS) {
-        return rc;
-    }
-    launch_dependent(attn_weight_apply_kernel<DH, kRowBlock / 8>, grid, dim3(kThreads), 0, stream, a);
-    return check_launch("attn_weight_apply_kernel");
+    const dim3 spread(grid.x, static_cast<unsigned>((p.max_kvlen + kSpread - 1) / kSpread), grid.z);
+    launch_dependent(attn_weight_spread_kernel, spread, dim3(256), 0, stream, a);
+    return check_launch("attn_weight_spread_kernel");
 }
 
 }  // namespace
@@ -656,7 +386,7 @@ int make_weight_plan(const pplb200_attn_params& p, WeightPlan* plan) {
     // With kept scores a CTA's start (lengths, rows and queries, each waiting for the one before) is worth longer chunks
     // as long as there are some 8 CTAs for each place on the chip.
     const bool kept = p.max_seqlen > 0 && p.max_seqlen * (p.num_heads / p.num_kv_heads) <= kScoreRows;
-    plan->chunk = kChunk;
+    plan->chunk = kept ? kChunk : kWindowChunk;
     while (kept && plan->chunk < 8 * kChunk &&
            p.batch * p.num_kv_heads * ((p.max_kvlen + 2 * plan->chunk - 1) / (2 * plan->chunk)) >= 148 * 4 * 8) {
         plan->chunk *= 2;
@@ -704,6 +434,9 @@ int launch_attn_weight(const pplb200_attn_params& p, const CacheGeom& geom, cons
     a.chunks = static_cast<int32_t>(plan.chunks);
     a.chunk = plan.chunk;
     a.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(p.head_dim));
+    if (p.max_seqlen * a.group > kScoreRows) {
+        return launch_weight_window(p, a, stream);
+    }
     return p.head_dim == 128 ? launch_dh<128>(p, a, stream) : launch_dh<64>(p, a, stream);
 }
 
