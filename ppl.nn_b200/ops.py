@@ -436,13 +436,9 @@ class _CacheOp(_Base):
     def _params(self, num_heads, num_kv_heads, head_dim, batch, max_kvlen, max_tokens, cachestarts, max_seqlen=0,
                 total_tokens=0, is_causal=True) -> capi.AttnParams:
         a = self.param
-        stride_b = 0
-        if a.cache_mode == 1:
-            if cachestarts.dim() != 2:
-                raise OpError("RC_INVALID_VALUE", "cachestarts must be a 2d tensor in cache_mode 1")
-            stride_b = cachestarts.shape[1]
-        if cachestarts.shape[0] != batch or (a.cache_mode == 0 and cachestarts.dim() != 1):
+        if cachestarts.dim() != 1 + (a.cache_mode == 1) or cachestarts.shape[0] != batch:
             raise OpError("RC_INVALID_VALUE", "cachestarts must have an entry (cache_mode 1: a row) per sequence")
+        stride_b = cachestarts.shape[1] if a.cache_mode == 1 else 0
         p = capi.AttnParams(num_heads, num_kv_heads, head_dim, int(is_causal), a.num_layer, a.layer_idx, a.quant_bit,
                             a.quant_group, a.cache_mode, a.cache_layout, a.page_size, 0, 0, 0, batch, 0,
                             int(max_seqlen), int(max_kvlen), total_tokens, max_tokens, 0, 0, 0, 0, stride_b)
@@ -459,21 +455,22 @@ class _CacheOp(_Base):
             raise OpError("RC_UNSUPPORTED", "currently only support is_alibi == false")
         if query.shape[1:] != (a.num_heads, a.head_dim) or heads != a.num_kv_heads or dim != a.head_dim:
             raise OpError("RC_INVALID_VALUE", "query or cache does not have the shape of the attributes")
-        batch = start_pos.shape[0]
-        if seqstarts.shape[0] != batch + 1:
+        batch = start_pos.numel()
+        if start_pos.dim() != 1 or seqstarts.shape != (batch + 1,):
             raise OpError("RC_INVALID_VALUE", "seqstarts must have one entry more than start_pos")
         return device, self._params(a.num_heads, heads, dim, batch, max_kvlen, rows, cachestarts, max_seqlen,
                                     query.shape[0], a.is_causal)
 
     def _call(self, name, size_fn, fn, p, device: int, *args) -> None:
         """Runs fn(p, *args, workspace, bytes, stream) on the tensors' device and its current stream."""
-        if device != torch.cuda.current_device():
+        if device != torch._C._cuda_getDevice():
             with torch.cuda.device(device):
                 return self._call(name, size_fn, fn, p, device, *args)
         rc, nbytes = size_fn(p)
         if rc == capi.SUCCESS:
             self._workspace = ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
-            rc = fn(p, *args, ws.data_ptr(), nbytes, _stream())
+            # the current stream's handle; a Stream object around it costs 5 us, a fifth of a small call
+            rc = fn(p, *args, ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(device))
         self._raise(name, rc)
 
     def device_status(self) -> int:
@@ -555,8 +552,8 @@ class KeyValueCacheEvict(_CacheOp):
         device, heads, rows = weight.get_device(), weight.shape[1], weight.shape[2]
         self._check_weight(device, weight, heads, rows)
         _require(device, torch.int64, cachestarts=cachestarts, kvlens=kvlens, budgets=budgets)
-        batch, max_budget = kvlens.shape[0], int(max_budget)
-        if budgets.shape != kvlens.shape or max_budget < 0:
+        batch, max_budget = kvlens.numel(), int(max_budget)
+        if kvlens.dim() != 1 or budgets.shape != kvlens.shape or max_budget < 0:
             raise OpError("RC_INVALID_VALUE", "budgets must have an entry per sequence and max_budget not be negative")
         if kept is None:
             kept = torch.empty((batch, heads, max_budget), dtype=torch.int64, device=weight.device)
@@ -584,8 +581,8 @@ class KeyValueCacheCompact(_CacheOp):
                 num_layers: int = 1) -> None:
         device, heads, dim, rows = self._check_cache(cache, scale)
         _require(device, torch.int64, kept=kept, cachestarts=cachestarts, base=base, kvlens=kvlens)
-        batch = kvlens.shape[0]
-        if kept.dim() != 3 or kept.shape[0] != batch or kept.shape[1] not in (1, heads) or base.shape != kvlens.shape:
+        batch = kvlens.numel()
+        if kvlens.dim() != 1 or kept.dim() != 3 or kept.shape[0] != batch or kept.shape[1] not in (1, heads) or base.shape != kvlens.shape:
             raise OpError("RC_INVALID_VALUE", "kept must be [batch, num_kv_heads or 1, K], base and kvlens [batch]")
         if weight is not None:
             self._check_weight(device, weight, heads, rows)
