@@ -8,12 +8,15 @@
 // attn_weight_spread_kernel joins the chunks and turns the scores into weights.
 //
 // The score kernel: a CTA takes a chunk of the positions of one (sequence, kv head), a warp 16 positions at a time.
-// Positions are the M dimension of mma.m16n8k16, the query rows its N dimension.  A thread needs the channels 2t, 2t+1,
-// 2t+8, 2t+9 of each block of 16 for rows g and g+8 of the A operand; as the order of the channels does not matter as
-// long as Q has the same, thread t takes 16 consecutive code bytes per 64 channels.
+// Positions are the M dimension of mma.m16n8k16.  A thread needs the channels 2t, 2t+1, 2t+8, 2t+9 of each block of 16 for
+// rows g and g+8 of the A operand; as the order of the channels does not matter as long as Q has the same, thread t takes
+// 16 consecutive code bytes per 64 channels.
 //
-// The weights are fp32 and proportional to exp(score), so a key rounded to fp16 would cost 1e-4 of their value;
-// k = code * scale is therefore split into fp16(k) and the exact remainder, which have accumulators of their own.
+// The weights are fp32 and proportional to exp(score), so a key rounded to fp16 would cost 1e-4 of their value.  With up
+// to 4 query rows the codes themselves (exact in fp16) are the A operand and the columns of B are (scale group, query
+// row) pairs, each zero outside its group: the accumulators hold a row's products of one group, which are scaled in
+// fp32.  With more rows there are too few columns for that, and k = code * scale is split into fp16(k) and the exact
+// remainder, which have accumulators of their own.
 #include "attn_weight.cuh"
 
 namespace pplb200 {
@@ -126,13 +129,33 @@ struct Ring {
     }
 };
 
+// Where the score of a thread belongs: RB is the number of query rows that the columns of B have room for.
+// RB 8: positions g and g + 8, rows 2t and 2t + 1.  Below, the four threads of a g share the positions out.
+template <int RB>
+struct Place {
+    static constexpr int kPos = RB == 8 ? 2 : 1;      // positions of a thread, 8 apart
+    static constexpr int kCols = RB >= 4 ? 2 : 1;     // rows of a thread
+    static __device__ __forceinline__ int position(int lane) {
+        return (lane >> 2) + (RB == 8 ? 0 : 8 * (RB == 4 ? (lane >> 1) & 1 : lane & 1));
+    }
+    static __device__ __forceinline__ int row(int lane) {
+        return RB == 8 ? 2 * (lane & 3) : (RB == 4 ? 2 * (lane & 1) : (RB == 2 ? (lane >> 1) & 1 : 0));
+    }
+    // lanes (by their differences) that hold other positions of the same rows; RB 1 has each score twice
+    static constexpr uint32_t kPeers = RB == 8 ? 4 + 8 + 16 : (RB == 4 ? 2 + 4 + 8 + 16 : 1 + 4 + 8 + 16);
+    static __device__ __forceinline__ bool first(int lane) { return (lane & kPeers) == 0 && (RB > 1 || lane == 0); }
+    static __device__ __forceinline__ bool stores(int lane) { return RB > 1 || (lane & 2) == 0; }
+};
+
 // Scores (unscaled) of 16 positions against the query rows whose fragments are in qf.
-// acc[0..1]: position g, rows 2t and 2t+1; acc[2..3]: position g + 8.
-template <int DH>
+template <int DH, int RB>
 struct Tile {
     static constexpr int kWords = DH / 16;
+    static constexpr int kHalves = RB == 4 ? 2 : 1;  // RB 4: two of the four groups of a k-step at a time
+    static constexpr int kPos = Place<RB>::kPos, kCols = Place<RB>::kCols;
+    using Query = uint2[kHalves][kWords];
     uint4 code[2][DH / 64];
-    uint32_t sc[2][DH / 64];
+    uint32_t sc[kHalves][2][DH / 64];
 
     // Where in a tile a lane reads its 16 code bytes of row g (Dh 128: of the first 64 channels; the others are 64
     // bytes up or down, as the copy left them) and its scales
@@ -141,7 +164,7 @@ struct Tile {
         return g * DH + (DH == 128 ? t ^ ((g & 1) << 2) : t) * 16;
     }
     static __device__ __forceinline__ uint32_t scale_offset(int lane) {
-        return Ring<DH>::kCodeBytes + (lane >> 2) * (DH / 4) + (lane & 3) * 4;
+        return Ring<DH>::kCodeBytes + (lane >> 2) * (DH / 4) + (RB == 4 ? (lane & 3) >> 1 : lane & 3) * 4;
     }
 
     __device__ __forceinline__ void read(uint32_t code_addr, uint32_t scale_addr) {
@@ -153,50 +176,133 @@ struct Tile {
                              : "=r"(code[r][h].x), "=r"(code[r][h].y), "=r"(code[r][h].z), "=r"(code[r][h].w)
                              : "r"((h == 0 ? code_addr : code_addr ^ 64u) + r * 8 * DH)
                              : "memory");
-                asm volatile("ld.shared.u32 %0, [%1];"
-                             : "=r"(sc[r][h])
-                             : "r"(scale_addr + r * 8 * (DH / 4) + h * 16)
-                             : "memory");
+#pragma unroll
+                for (int x = 0; x < kHalves; ++x) {
+                    asm volatile("ld.shared.u32 %0, [%1];"
+                                 : "=r"(sc[x][r][h])
+                                 : "r"(scale_addr + r * 8 * (DH / 4) + h * 16 + x * 8)
+                                 : "memory");
+                }
             }
         }
     }
 
-    // The keys and their remainders have two accumulators each: short chains of dependent instructions, and of
-    // roundings.
-    __device__ __forceinline__ void scores(const uint2 (&qf)[kWords], float (&acc)[4]) const {
-        float key[2][4], rest[2][4];
+    __device__ __forceinline__ uint32_t word(int r, int w) const {
+        const uint4 c = code[r][w / 4];
+        return (w & 3) == 0 ? c.x : ((w & 3) == 1 ? c.y : ((w & 3) == 2 ? c.z : c.w));
+    }
+
+    // Query fragments: row g of this CTA's rows, or of column g's (group, row) pair; zeros elsewhere.  Thread t holds the
+    // channels of the groups 2t (words 0 and 1 of a block of 64) and 2t + 1.
+    static __device__ __forceinline__ void load_queries(const WeightArgs& a, const Span& s, int head, int lane, Query& qf) {
+        const int g = lane >> 2, t = lane & 3, row = RB == 8 ? g : (RB == 1 ? 0 : g % RB);
+        const int32_t i = row / a.group;
+        const __half* src = a.q + ((s.tok0 + i) * a.num_heads + head * a.group + (row - i * a.group)) * DH;
 #pragma unroll
         for (int w = 0; w < kWords; ++w) {
-            uint32_t k[2][2], e[2][2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const uint4 c = code[r][w / 4];
-                const uint32_t word = (w & 3) == 0 ? c.x : ((w & 3) == 1 ? c.y : ((w & 3) == 2 ? c.z : c.w));
-                const uint32_t s = prmt(sc[r][w / 4], 0u, (w & 2) ? 0x3232u : 0x1010u);
-                split_key_word(word, u32_as_h2(s), k[r][0], k[r][1], e[r][0], e[r][1]);
+            uint2 q = make_uint2(0u, 0u);
+            if (row < s.rows) {
+                q = *reinterpret_cast<const uint2*>(src + (w / 4) * 64 + t * 16 + (w & 3) * 4);
             }
-            if (w < 2) {
-                mma_first(key[w & 1], k[0][0], k[1][0], k[0][1], k[1][1], qf[w].x, qf[w].y);
-                mma_first(rest[w & 1], e[0][0], e[1][0], e[0][1], e[1][1], qf[w].x, qf[w].y);
-            } else {
-                mma_m16n8k16_f16f32(key[w & 1], k[0][0], k[1][0], k[0][1], k[1][1], qf[w].x, qf[w].y);
-                mma_m16n8k16_f16f32(rest[w & 1], e[0][0], e[1][0], e[0][1], e[1][1], qf[w].x, qf[w].y);
+#pragma unroll
+            for (int x = 0; x < kHalves; ++x) {
+                const bool mine = RB == 8 || (RB == 4 ? t == 2 * x + (g >> 2) : (RB == 2 ? t == g >> 1 : g == 2 * t + ((w & 3) >> 1)));
+                qf[x][w] = mine ? q : make_uint2(0u, 0u);
             }
         }
+    }
+
+    __device__ __forceinline__ void scores(const Query& qf, int lane, float (&out)[kPos][kCols]) const {
+        if constexpr (RB == 8) {
+            // two accumulators each for the keys and their remainders: short chains of dependent instructions, and of
+            // roundings
+            float key[2][4], rest[2][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            acc[e] = (key[0][e] + key[1][e]) + (rest[0][e] + rest[1][e]);
+            for (int w = 0; w < kWords; ++w) {
+                uint32_t k[2][2], e[2][2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const uint32_t s = prmt(sc[0][r][w / 4], 0u, (w & 2) ? 0x3232u : 0x1010u);
+                    split_key_word(word(r, w), u32_as_h2(s), k[r][0], k[r][1], e[r][0], e[r][1]);
+                }
+                const uint2 q = qf[0][w];
+                if (w < 2) {
+                    mma_first(key[w & 1], k[0][0], k[1][0], k[0][1], k[1][1], q.x, q.y);
+                    mma_first(rest[w & 1], e[0][0], e[1][0], e[0][1], e[1][1], q.x, q.y);
+                } else {
+                    mma_m16n8k16_f16f32(key[w & 1], k[0][0], k[1][0], k[0][1], k[1][1], q.x, q.y);
+                    mma_m16n8k16_f16f32(rest[w & 1], e[0][0], e[1][0], e[0][1], e[1][1], q.x, q.y);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                out[e >> 1][e & 1] = (key[0][e] + key[1][e]) + (rest[0][e] + rest[1][e]);
+            }
+        } else {
+            constexpr int kSteps = RB == 1 ? 4 : 2;  // k-steps of the same groups
+            float sum[2][2] = {};                    // positions g and g + 8; RB 1: [.][0] alone
+#pragma unroll
+            for (int w0 = 0; w0 < kWords; w0 += kSteps) {
+                uint32_t k[kSteps][2][2];
+#pragma unroll
+                for (int w = 0; w < kSteps; ++w) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const uint32_t x = word(r, w0 + w) ^ 0x80808080u;
+                        k[w][r][0] = h2_as_u32(biased_bytes_to_half2<0x5140u>(x));
+                        k[w][r][1] = h2_as_u32(biased_bytes_to_half2<0x5342u>(x));
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < kHalves; ++x) {
+                    float acc[4];
+                    mma_first(acc, k[0][0][0], k[0][1][0], k[0][0][1], k[0][1][1], qf[x][w0].x, qf[x][w0].y);
+#pragma unroll
+                    for (int w = 1; w < kSteps; ++w) {
+                        mma_m16n8k16_f16f32(acc, k[w][0][0], k[w][1][0], k[w][0][1], k[w][1][1], qf[x][w0 + w].x,
+                                            qf[x][w0 + w].y);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float2 g2 = __half22float2(u32_as_h2(sc[x][r][w0 / 4]));
+                        if constexpr (RB == 1) {  // columns 2t, 2t + 1: this thread's own two groups
+                            sum[r][0] = fmaf(acc[2 * r], g2.x, fmaf(acc[2 * r + 1], g2.y, sum[r][0]));
+                        } else {  // two rows of one group
+                            const float f = (w0 & 2) ? g2.y : g2.x;
+                            sum[r][0] = fmaf(acc[2 * r], f, sum[r][0]);
+                            sum[r][1] = fmaf(acc[2 * r + 1], f, sum[r][1]);
+                        }
+                    }
+                }
+            }
+            // over the threads of a g: each keeps one of the two positions, RB 2 one of the two rows as well
+            constexpr int kFirst = RB == 4 ? 2 : 1;
+            const bool upper = (lane & kFirst) != 0;
+            float x[2];
+#pragma unroll
+            for (int c = 0; c < (RB == 1 ? 1 : 2); ++c) {
+                x[c] = (upper ? sum[1][c] : sum[0][c]) + __shfl_xor_sync(0xffffffffu, upper ? sum[0][c] : sum[1][c], kFirst);
+            }
+            if constexpr (RB == 1) {
+                out[0][0] = x[0] + __shfl_xor_sync(0xffffffffu, x[0], 2);
+            } else if constexpr (RB == 2) {
+                const bool second = (lane & 2) != 0;
+                out[0][0] = (second ? x[1] : x[0]) + __shfl_xor_sync(0xffffffffu, second ? x[0] : x[1], 2);
+            } else {
+                out[0][0] = x[0];
+                out[0][1] = x[1];
+            }
         }
     }
 };
 
-template <int DH>
-__global__ void __launch_bounds__(kThreads, 6) attn_weight_stats_kernel(const WeightArgs a) {
+template <int DH, int RB>
+__global__ void __launch_bounds__(kThreads, RB >= 4 ? 5 : 6) attn_weight_stats_kernel(const WeightArgs a) {
     grid_launch_dependents();
     grid_dependency_wait();
     __shared__ float2 red[kWarps][kScoreRows];
     __shared__ __align__(128) uint8_t smem[kWarps * Ring<DH>::kWarpBytes];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t b = blockIdx.z;
     const int head = blockIdx.x, chunk = blockIdx.y;  // neighbouring CTAs read neighbouring heads of the same rows
     const Span s = span_of(a, b);
@@ -207,89 +313,97 @@ __global__ void __launch_bounds__(kThreads, 6) attn_weight_stats_kernel(const We
     const int32_t end = first + a.chunk < s.len ? first + a.chunk : s.len;
     const Ring<DH> ring(a, s, b, head, warp, lane, smem);
     float* score = a.score + (b * a.num_kv_heads + head) * a.max_kvlen * a.score_rows;
-    // query fragments: row g (zeros behind the last)
-    uint2 qf[DH / 16];
-    {
-        const int32_t i = g / a.group;
-        const __half* src = a.q + ((s.tok0 + i) * a.num_heads + head * a.group + (g - i * a.group)) * DH;
+    using T = Tile<DH, RB>;
+    using At = Place<RB>;
+    typename T::Query qf;
+    T::load_queries(a, s, head, lane, qf);
+    const int my_pos = At::position(lane), my_row = At::row(lane);
+    // the last position that this thread's rows see
+    int64_t last[At::kCols];
+    float m[At::kCols], l[At::kCols];
 #pragma unroll
-        for (int w = 0; w < DH / 16; ++w) {
-            qf[w] = make_uint2(0u, 0u);
-            if (g < s.rows) {
-                qf[w] = *reinterpret_cast<const uint2*>(src + (w / 4) * 64 + t * 16 + (w & 3) * 4);
-            }
-        }
-    }
-    // the last position that rows 2t and 2t + 1 see
-    int64_t last[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        last[c] = a.causal ? s.start + (2 * t + c) / a.group : s.len - 1;
+    for (int c = 0; c < At::kCols; ++c) {
+        last[c] = a.causal ? s.start + (my_row + c) / a.group : s.len - 1;
         last[c] = last[c] < s.len - 1 ? last[c] : s.len - 1;
+        m[c] = kNegBig;
+        l[c] = 0.0f;
     }
-    float m[2] = {kNegBig, kNegBig}, l[2] = {0.0f, 0.0f};
     constexpr int kStep = kWarps * 16;
     int32_t tile0 = first + warp * 16;
 #pragma unroll
     for (int k = 0; k < kStages - 1; ++k) {
         ring.issue(a, b, tile0 + k * kStep, end, s.len, k, lane);
     }
-    const uint32_t code_addr = ring.base + Tile<DH>::code_offset(lane);
-    const uint32_t scale_addr = ring.base + Tile<DH>::scale_offset(lane);
+    const uint32_t code_addr = ring.base + T::code_offset(lane);
+    const uint32_t scale_addr = ring.base + T::scale_offset(lane);
     int stage = 0, ahead = kStages - 1;
     for (; tile0 < end; tile0 += kStep) {
         ring.issue(a, b, tile0 + (kStages - 1) * kStep, end, s.len, ahead, lane);
         cp_async_wait<kStages - 1>();
         __syncwarp();
-        Tile<DH> tile;
+        T tile;
         tile.read(code_addr + stage * Ring<DH>::kTileBytes, scale_addr + stage * Ring<DH>::kTileBytes);
         __syncwarp();  // everyone has read: the next round may overwrite the stage
         ahead = stage;
         stage = stage + 1 == kStages ? 0 : stage + 1;
-        float acc[4];
-        tile.scores(qf, acc);
+        float x[At::kPos][At::kCols];
+        tile.scores(qf, lane, x);
+        const int32_t pos = tile0 + my_pos;
         if (tile0 + 15 > s.start || tile0 + 15 >= s.len) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (tile0 + g + 8 * (e >> 1) > last[e & 1]) {
-                    acc[e] = -INFINITY;
+            for (int p = 0; p < At::kPos; ++p) {
+#pragma unroll
+                for (int c = 0; c < At::kCols; ++c) {
+                    if (pos + 8 * p > last[c]) {
+                        x[p][c] = -INFINITY;
+                    }
                 }
             }
         }
-        if (2 * t < s.rows) {
-            float* dst = score + static_cast<int64_t>(tile0 + g) * a.score_rows + 2 * t;
+        if (my_row < s.rows && At::stores(lane)) {
+            float* dst = score + static_cast<int64_t>(pos) * a.score_rows + my_row;
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                if (tile0 + g + 8 * p < s.len) {
-                    dst[p * 8 * a.score_rows] = acc[2 * p];
-                    if (2 * t + 1 < s.rows) {
-                        dst[p * 8 * a.score_rows + 1] = acc[2 * p + 1];
+            for (int p = 0; p < At::kPos; ++p) {
+                if (pos + 8 * p < s.len) {
+                    dst[p * 8 * a.score_rows] = x[p][0];
+                    if (At::kCols > 1 && my_row + 1 < s.rows) {
+                        dst[p * 8 * a.score_rows + 1] = x[p][At::kCols - 1];
                     }
                 }
             }
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const float x = acc[c] * a.scale_log2, y = acc[2 + c] * a.scale_log2;
-            const float top = fmaxf(m[c], fmaxf(x, y));
-            l[c] = l[c] * ex2_approx(m[c] - top) + ex2_approx(x - top) + ex2_approx(y - top);
+        for (int c = 0; c < At::kCols; ++c) {
+            float top = m[c], sum = 0.0f;
+#pragma unroll
+            for (int p = 0; p < At::kPos; ++p) {
+                x[p][c] *= a.scale_log2;
+                top = fmaxf(top, x[p][c]);
+            }
+#pragma unroll
+            for (int p = 0; p < At::kPos; ++p) {
+                sum += ex2_approx(x[p][c] - top);
+            }
+            l[c] = fmaf(l[c], ex2_approx(m[c] - top), sum);
             m[c] = top;
         }
     }
     cp_async_wait<0>();
-    // over the eight positions a column's values are spread over, then over the warps
+    // over the positions a row's values are spread over, then over the warps
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < At::kCols; ++c) {
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) {
-            const float om = __shfl_xor_sync(0xffffffffu, m[c], x);
-            const float ol = __shfl_xor_sync(0xffffffffu, l[c], x);
-            const float top = fmaxf(m[c], om);
-            l[c] = l[c] * ex2_approx(m[c] - top) + ol * ex2_approx(om - top);
-            m[c] = top;
+        for (int x = 1; x < 32; x <<= 1) {
+            if (At::kPeers & x) {
+                const float om = __shfl_xor_sync(0xffffffffu, m[c], x);
+                const float ol = __shfl_xor_sync(0xffffffffu, l[c], x);
+                const float top = fmaxf(m[c], om);
+                l[c] = l[c] * ex2_approx(m[c] - top) + ol * ex2_approx(om - top);
+                m[c] = top;
+            }
         }
-        if (lane < 4) {
-            red[warp][2 * lane + c] = make_float2(m[c], l[c]);
+        if (At::first(lane)) {
+            red[warp][my_row + c] = make_float2(m[c], l[c]);
         }
     }
     __syncthreads();
@@ -341,12 +455,36 @@ __global__ void __launch_bounds__(256) attn_weight_spread_kernel(const WeightArg
     for (int k = 0; k < kPer; ++k) {
         sum[k] = 0.0f;
     }
-    for (int32_t r = 0; r < s.rows; ++r) {
-        const float2 v = norm[r];
+    int32_t r0 = 0;
+    if ((a.score_rows & 3) == 0) {  // four rows of a position at once
+        for (; r0 < s.rows; r0 += 4) {
+            float4 x[kPer];
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                x[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if (pos0 + k * 256 < s.len) {
+                    x[k] = *reinterpret_cast<const float4*>(score + static_cast<int64_t>(pos0 + k * 256) * a.score_rows + r0);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (r0 + c < s.rows) {  // rows behind the last were not written
+                    const float2 v = norm[r0 + c];
+#pragma unroll
+                    for (int k = 0; k < kPer; ++k) {
+                        const float y = c == 0 ? x[k].x : (c == 1 ? x[k].y : (c == 2 ? x[k].z : x[k].w));
+                        sum[k] = fmaf(ex2_approx(fmaf(y, a.scale_log2, -v.x)), v.y, sum[k]);
+                    }
+                }
+            }
+        }
+    }
+    for (; r0 < s.rows; ++r0) {
+        const float2 v = norm[r0];
         float x[kPer];
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
-            x[k] = pos0 + k * 256 < s.len ? score[static_cast<int64_t>(pos0 + k * 256) * a.score_rows + r] : -INFINITY;
+            x[k] = pos0 + k * 256 < s.len ? score[static_cast<int64_t>(pos0 + k * 256) * a.score_rows + r0] : -INFINITY;
         }
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
@@ -370,7 +508,12 @@ template <int DH>
 int launch_dh(const pplb200_attn_params& p, const WeightArgs& a, cudaStream_t stream) {
     const dim3 grid(static_cast<unsigned>(p.num_kv_heads), static_cast<unsigned>(a.chunks), static_cast<unsigned>(p.batch));
     // each kernel starts while the one before it drains, and waits for it before it reads anything
-    launch_dependent(attn_weight_stats_kernel<DH>, grid, dim3(kThreads), 0, stream, a);
+    const int32_t rows = a.score_rows;
+    launch_dependent(rows <= 1   ? attn_weight_stats_kernel<DH, 1>
+                     : rows <= 2 ? attn_weight_stats_kernel<DH, 2>
+                     : rows <= 4 ? attn_weight_stats_kernel<DH, 4>
+                                 : attn_weight_stats_kernel<DH, 8>,
+                     grid, dim3(kThreads), 0, stream, a);
     const int rc = check_launch("attn_weight_stats_kernel");
     if (rc != PPLB200_SUCCESS) {
         return rc;
