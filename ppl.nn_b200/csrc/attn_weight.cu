@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(256) attn_weight_spread_kernel(const WeightArg
             const int64_t row = a.geom.cache_mode == 0 ? (start_row < 0 ? -1 : start_row + pos)
                                                        : cache_row(a.geom, a.cachestarts, b, pos);
             if (cache_row_ok(row, a.max_tokens)) {
-                atomicAdd(w + row, sum[k]);  // one addition per position and call
+                add_weight(w + row, sum[k]);  // one addition per position and call
             }
         }
     }

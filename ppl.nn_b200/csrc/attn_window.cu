@@ -10,8 +10,9 @@
 // Roles of a CTA (two per SM): four softmax warps, one thread per query row; they also bring Q, which is the A operand
 // in TMEM (64 columns), so that the MMAs read only K from shared memory.  Four converter warps turn raw codes and scales
 // into the two swizzled tiles (two stages); one warp issues the MMAs, one fetches raw blocks by TMA.  TMEM: Q 64 | S 2 x
-// 64 columns.  The column sums of the weights: each thread has 64 positions of its row; 31 exchanges within the warp
-// leave every lane with the sums of two positions over the warp's 32 rows, shared memory adds the four warps up.
+// 64 columns.  The column sums of the weights: scores are read in the fragment layout, four rows and sixteen positions a
+// thread; 14 exchanges within the warp leave every lane with the sums of two positions over the warp's 32 rows, shared
+// memory adds the four warps up.
 // The order of every sum is fixed.
 #include "attn_weight.cuh"
 #include "kv_tiles.cuh"
@@ -61,16 +62,17 @@ struct WindowMaps {
     CacheMapOrder order;
 };
 
-// v[e] = this lane's value for position e.  Afterwards v[0] and v[1] are the sums over the warp's lanes for the positions
-// 2 * lane and 2 * lane + 1: halves of the positions are exchanged with the lane 16, 8, 4, 2, 1 away.
-__device__ __forceinline__ void sum_positions(float (&v)[64], int lane) {
+// v[2j + c] = this lane's value for position 8j + 2t + c (t = lane % 4).  Afterwards v[0] and v[1] are the sums over the
+// lanes of the same t for j = lane / 4, i.e. for the positions 2 * lane and 2 * lane + 1: halves of the positions are
+// exchanged with the lane 16, 8 and 4 away.
+__device__ __forceinline__ void sum_positions(float (&v)[16], int lane) {
 #pragma unroll
-    for (int half = 32; half >= 2; half >>= 1) {
-        const bool upper = (lane & (half >> 1)) != 0;
+    for (int half = 8; half >= 2; half >>= 1) {
+        const bool upper = (lane & (2 * half)) != 0;
 #pragma unroll
         for (int e = 0; e < half; ++e) {
             const float give = upper ? v[e] : v[e + half], keep = upper ? v[e + half] : v[e];
-            v[e] = keep + __shfl_xor_sync(0xffffffffu, give, half >> 1);
+            v[e] = keep + __shfl_xor_sync(0xffffffffu, give, 2 * half);
         }
     }
 }
@@ -281,16 +283,23 @@ attn_window_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_con
             tc_fence_before();
             mbar_arrive(&bars.q_full);
 
-            // the last position this row sees
-            int64_t last = a.causal ? s.start + i : s.len - 1;
-            last = last < s.len - 1 ? last : s.len - 1;
-            float m = kWeightNegBig, l = 0.0f, inv = 0.0f;
-            if constexpr (APPLY) {
-                m = INFINITY;  // rows behind the last: no weight
-                if (live) {
-                    const float2 v = a.norm[at];
-                    m = v.x;
-                    inv = v.y;
+            // Statistics: one thread per row.  Weights: a thread has the rows g + 8k (k = 0..3) of its warp's 32, two of
+            // eight positions each, so that most of the sum over the rows stays within it.
+            constexpr int kMine = APPLY ? 4 : 1;
+            int64_t last[kMine];  // the last position a row sees
+            float m[kMine], l[kMine];
+#pragma unroll
+            for (int k = 0; k < kMine; ++k) {
+                const int32_t x = APPLY ? rt * kRows + warp * 32 + (lane >> 2) + 8 * k : row;
+                const int32_t tok = x < s.rows ? x / a.group : 0;
+                last[k] = a.causal ? s.start + tok : s.len - 1;
+                last[k] = last[k] < s.len - 1 ? last[k] : s.len - 1;
+                m[k] = APPLY ? INFINITY : kWeightNegBig;  // INFINITY: rows behind the last have no weight
+                l[k] = 0.0f;
+                if (APPLY && x < s.rows) {
+                    const float2 v = a.norm[(s.tok0 + tok) * a.num_heads + head * a.group + (x - tok * a.group)];
+                    m[k] = v.x;
+                    l[k] = v.y;  // the reciprocal sum
                 }
             }
             for (int32_t blk = 0; blk < blocks; ++blk) {
@@ -301,36 +310,40 @@ attn_window_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_con
                     break;
                 }
                 tc_fence_after();
-                float v[kBlockN];
-                {
-                    uint32_t u[2][32];
-                    __syncwarp();
+                uint32_t u[2][32];
+                __syncwarp();
+                if constexpr (APPLY) {
+                    tmem_ld_16x64(t_lane + T::kColS + sb * kBlockN, u[0]);
+                    tmem_ld_16x64(t_lane + (16u << 16) + T::kColS + sb * kBlockN, u[1]);
+                } else {
                     tmem_ld32(t_lane + T::kColS + sb * kBlockN, u[0]);
                     tmem_ld32(t_lane + T::kColS + sb * kBlockN + 32, u[1]);
-                    tmem_wait_ld();
+                }
+                tmem_wait_ld();
+                tc_fence_before();
+                mbar_arrive(&bars.s_free[sb]);
+                const int32_t pos0 = first + blk * kBlockN;
+                const bool edge = pos0 + kBlockN - 1 > s.start || pos0 + kBlockN > s.len;  // the first row sees up to s.start
+                if constexpr (!APPLY) {
+                    float v[kBlockN];
 #pragma unroll
                     for (int e = 0; e < kBlockN; ++e) {
                         v[e] = __uint_as_float(u[e >> 5][e & 31]);
                     }
-                }
-                tc_fence_before();
-                mbar_arrive(&bars.s_free[sb]);
-                const int32_t pos0 = first + blk * kBlockN;
-                if (pos0 + kBlockN - 1 > s.start || pos0 + kBlockN > s.len) {  // the first row's last position is s.start
-                    const int32_t limit = last - pos0 > kBlockN ? kBlockN : static_cast<int32_t>(last - pos0);
+                    if (edge) {
+                        const int32_t limit = last[0] - pos0 > kBlockN ? kBlockN : static_cast<int32_t>(last[0] - pos0);
 #pragma unroll
-                    for (int e = 0; e < kBlockN; ++e) {
-                        v[e] = e <= limit ? v[e] : -INFINITY;
+                        for (int e = 0; e < kBlockN; ++e) {
+                            v[e] = e <= limit ? v[e] : -INFINITY;
+                        }
                     }
-                }
-                if constexpr (!APPLY) {
                     float x = fmax3(v[0], v[1], v[2]), y = fmax3(v[3], v[4], v[5]);
 #pragma unroll
                     for (int e = 6; e + 3 < kBlockN; e += 4) {
                         x = fmax3(x, v[e], v[e + 1]);
                         y = fmax3(y, v[e + 2], v[e + 3]);
                     }
-                    const float top = fmaxf(m, fmax3(x, y, fmaxf(v[kBlockN - 2], v[kBlockN - 1])) * sc);
+                    const float top = fmaxf(m[0], fmax3(x, y, fmaxf(v[kBlockN - 2], v[kBlockN - 1])) * sc);
                     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int e = 0; e < kBlockN; e += 2) {
@@ -338,14 +351,34 @@ attn_window_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_con
                         sum[e & 2] += ex2_approx(z.x);
                         sum[(e & 2) + 1] += ex2_approx(z.y);
                     }
-                    l = l * ex2_approx(m - top) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-                    m = top;
+                    l[0] = l[0] * ex2_approx(m[0] - top) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                    m[0] = top;
                 } else {
+                    if (edge) {
 #pragma unroll
-                    for (int e = 0; e < kBlockN; e += 2) {
-                        const float2 z = __ffma2_rn(make_float2(v[e], v[e + 1]), make_float2(sc, sc), make_float2(-m, -m));
-                        v[e] = ex2_approx(z.x) * inv;
-                        v[e + 1] = ex2_approx(z.y) * inv;
+                        for (int k = 0; k < 4; ++k) {
+                            const int64_t rest = last[k] - pos0 - 2 * (lane & 3);
+                            const int32_t limit = rest > kBlockN ? kBlockN : static_cast<int32_t>(rest);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                uint32_t& x = u[k >> 1][4 * (e >> 1) + 2 * (k & 1) + (e & 1)];
+                                x = 8 * (e >> 1) + (e & 1) <= limit ? x : 0xff800000u;  // -inf
+                            }
+                        }
+                    }
+                    float v[16];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {  // row g + 8k
+                            const float2 x = make_float2(__uint_as_float(u[k >> 1][4 * j + 2 * (k & 1)]),
+                                                         __uint_as_float(u[k >> 1][4 * j + 2 * (k & 1) + 1]));
+                            const float2 y = __ffma2_rn(x, make_float2(sc, sc), make_float2(-m[k], -m[k]));
+                            sum = __ffma2_rn(make_float2(ex2_approx(y.x), ex2_approx(y.y)), make_float2(l[k], l[k]), sum);
+                        }
+                        v[2 * j] = sum.x;
+                        v[2 * j + 1] = sum.y;
                     }
                     sum_positions(v, lane);
                     float* buf = sSum + (n % kSumStages) * (4 * kBlockN);
@@ -358,29 +391,26 @@ attn_window_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_con
                     if (!ok) {
                         break;
                     }
-                    const int32_t e = threadIdx.x, pos = pos0 + e;
-                    if (pos < s.len) {
-                        float x = (buf[e] + buf[kBlockN + e]) + (buf[2 * kBlockN + e] + buf[3 * kBlockN + e]);
-                        float* sum = &sChunk[pos - first];
-                        if (rt > 0) {
-                            x += *sum;
-                        }
-                        if (rt + 1 < row_tiles) {
-                            *sum = x;
-                        } else {
-                            const int64_t at_row = a.geom.cache_mode == 0 ? (first_row < 0 ? -1 : first_row + pos)
-                                                                          : cache_row(a.geom, a.cachestarts, b, pos);
-                            if (cache_row_ok(at_row, a.max_tokens)) {
-                                atomicAdd(w + at_row, x);  // one addition per position and call
-                            }
-                        }
-                    }
+                    const int32_t e = threadIdx.x;
+                    float* sum = &sChunk[blk * kBlockN + e];
+                    const float x = (buf[e] + buf[kBlockN + e]) + (buf[2 * kBlockN + e] + buf[3 * kBlockN + e]);
+                    *sum = rt > 0 ? *sum + x : x;
                     __syncwarp();
                 }
             }
             if constexpr (!APPLY) {
                 if (ok && live) {
-                    a.part[chunk * a.total_tokens * a.num_heads + at] = make_float2(m, l);
+                    a.part[chunk * a.total_tokens * a.num_heads + at] = make_float2(m[0], l[0]);
+                }
+            }
+        }
+        if constexpr (APPLY) {
+            // behind the last row tile, not block by block: a row of the cache gets one addition per call
+            for (int32_t pos = first + static_cast<int32_t>(threadIdx.x); ok && warp < 2 && pos < end; pos += kBlockN) {
+                const int64_t at_row = a.geom.cache_mode == 0 ? (first_row < 0 ? -1 : first_row + pos)
+                                                              : cache_row(a.geom, a.cachestarts, b, pos);
+                if (cache_row_ok(at_row, a.max_tokens)) {
+                    add_weight(w + at_row, sChunk[pos - first]);
                 }
             }
         }
