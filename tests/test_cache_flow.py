@@ -1,0 +1,474 @@
+"""The operators around the INT8 cache as they are used together -- drafting, eviction, captured steps, several streams,
+long caches -- and the forms of each that its own tests leave out."""
+import numpy as np
+import pytest
+
+from test_cache_ops import HostCache, dev, gpu, starts_of, weight_reference  # noqa: F401  (gpu is a fixture)
+from test_tree_attention import draw_parents, run_tree, tree_reference
+
+I64 = np.int64
+
+
+def attention_param(hc, heads, layer=0, **kw):
+    from ppl_nn_b200 import ops
+    return ops.MultiHeadCacheAttentionParam(num_heads=heads, num_kv_heads=hc.heads, head_dim=hc.dim, **hc.param(layer), **kw)
+
+
+def i64(x):
+    return dev(np.array(x, dtype=I64))
+
+
+# ---- refusals by the Python layer -----------------------------------------------------------------
+
+def test_host_tensors_are_refused(pkg, built_lib):
+    import torch
+    from ppl_nn_b200 import ops
+    hc = HostCache(np.random.default_rng(0), [5, 9], 2, 64)
+    t = torch.from_numpy
+    cache, scale, weight = t(hc.cache), t(hc.scale), t(hc.weight)
+    q, one = torch.zeros(2, 4, 64, dtype=torch.float16), torch.zeros(2, dtype=torch.int64)
+    seq = torch.tensor([0, 1, 2])
+    p = attention_param(hc, 4)
+    for call in (lambda: ops.TreeAttention(p).forward(q, None, seq, one, one, 1, 9, cache, scale),
+                 lambda: ops.AttentionWeight(p).forward(q, seq, one, one, 1, 9, cache, scale, weight),
+                 lambda: ops.KeyValueCacheEvict(ops.KeyValueCacheEvictParam(**hc.param())).forward(weight, one, one, one, 9, 4),
+                 lambda: ops.KeyValueCacheCompact(ops.KeyValueCacheParam(**hc.param())).forward(
+                     torch.zeros(2, 2, 4, dtype=torch.int64), one, one, one, 9, cache, scale)):
+        with pytest.raises(ops.OpError):
+            call()
+
+
+@pytest.mark.gpu
+def test_wrong_types_and_shapes_are_refused(gpu, pkg):  # noqa: F811
+    import torch
+    from ppl_nn_b200 import ops
+    hc = HostCache(np.random.default_rng(0), [5, 9], 2, 64)
+    good = dict(q=torch.zeros(2, 4, 64, dtype=torch.float16, device=gpu), parents=i64([-1, -1]), seq=i64([0, 1, 2]),
+                cs=dev(hc.starts), start=i64([4, 8]), cache=dev(hc.cache), scale=dev(hc.scale), weight=dev(hc.weight),
+                kept=i64(np.zeros((2, 2, 3))), base=i64([0, 0]), lens=i64([5, 9]), budgets=i64([3, 3]))
+    p = attention_param(hc, 4)
+    tree, weigh = ops.TreeAttention(p), ops.AttentionWeight(p)
+    evict = ops.KeyValueCacheEvict(ops.KeyValueCacheEvictParam(**hc.param()))
+    compact = ops.KeyValueCacheCompact(ops.KeyValueCacheParam(**hc.param()))
+
+    def calls(d):
+        return dict(
+            tree=lambda: tree.forward(d["q"], d["parents"], d["seq"], d["cs"], d["start"], 1, 9, d["cache"], d["scale"]),
+            weight=lambda: weigh.forward(d["q"], d["seq"], d["cs"], d["start"], 1, 9, d["cache"], d["scale"], d["weight"]),
+            evict=lambda: evict.forward(d["weight"], d["cs"], d["lens"], d["budgets"], 9, 3),
+            compact=lambda: compact.forward(d["kept"], d["cs"], d["base"], d["lens"], 9, d["cache"], d["scale"], d["weight"]))
+
+    for f in calls(good).values():  # the calls themselves are right (kept: position 0 alone, then not ascending)
+        f()
+    torch.cuda.synchronize()
+    for name, bad, which in (
+            ("q", good["q"].float(), "tree weight"), ("q", good["q"][:, :3], "tree weight"),
+            ("q", good["q"].transpose(0, 1).contiguous().transpose(0, 1), "tree weight"),
+            ("parents", good["parents"].int(), "tree"), ("parents", i64([-1]), "tree"),
+            ("seq", i64([0, 1]), "tree weight"), ("seq", good["seq"].int(), "tree weight"),
+            ("seq", i64([[0], [1], [2]]), "tree weight"), ("start", i64([[4], [8]]), "tree weight"),
+            ("cs", good["cs"][:1], "tree weight evict compact"), ("cs", good["cs"].cpu(), "tree weight evict compact"),
+            ("cs", good["cs"][:, None].contiguous(), "tree weight evict compact"),
+            ("cache", good["cache"].half(), "tree weight compact"), ("cache", good["cache"][..., :32].contiguous(), "tree weight compact"),
+            ("scale", good["scale"].float(), "tree weight compact"), ("scale", None, "tree weight compact"),
+            ("scale", good["scale"][:3], "tree weight compact"),
+            ("weight", good["weight"].double(), "weight evict compact"), ("weight", good["weight"][0], "weight evict compact"),
+            ("weight", good["weight"][..., 1:].contiguous(), "weight compact"),
+            ("lens", i64([[5], [9]]), "evict compact"), ("budgets", i64([3]), "evict"),
+            ("base", i64([0]), "compact"), ("kept", i64(np.zeros((2, 3, 3))), "compact"), ("kept", i64(np.zeros((2, 3))), "compact"),
+            ("kept", good["kept"].int(), "compact")):
+        for op in which.split():
+            with pytest.raises(ops.OpError):
+                calls(dict(good, **{name: bad}))[op]()
+    if torch.cuda.device_count() > 1:
+        with pytest.raises(ops.OpError):
+            calls(dict(good, cs=good["cs"].to("cuda:1")))["tree"]()
+
+
+# ---- a run of them, as they are used -----------------------------------------------------------------
+
+def decode_output(hc, cache, scale, starts, heads, start, q, k, v):
+    """One decode step of the framework's attention: appends k and v at `start`, attends over start + 1 positions."""
+    from ppl_nn_b200 import ops
+    batch = len(start)
+    op = ops.MultiHeadCacheAttention(attention_param(hc, heads))
+    kvlens = [s + 1 for s in start]
+    out = op.forward(q, k, v, i64(range(batch + 1)), dev(starts_of(kvlens)), starts, i64(start), batch, 1, max(kvlens),
+                     cache, scale)
+    assert op.device_status() == 0
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout,page", [(0, 0), (3, 0), (0, 16), (3, 128)])
+def test_a_drafted_step_is_a_run_of_decode_steps(gpu, pkg, layout, page):  # noqa: F811
+    """History and drafted tokens are appended by the cache operator, the tree is attended to, an accepted path is moved
+    to the front; the next decode step then gives, bit by bit, what it gives on a cache that never held the rest."""
+    import torch
+    from ppl_nn_b200 import ops
+    rng = np.random.default_rng(layout + page)
+    heads, kv_heads, dim = 8, 2, 128
+    start, n = [37, 0, 200], [9, 4, 16]
+    hc = HostCache(rng, [s + m + 1 for s, m in zip(start, n)], kv_heads, dim, layout, page)
+    cache, scale, starts = dev(hc.cache), dev(hc.scale), dev(hc.starts)
+    append = ops.KeyValueCache(ops.KeyValueCacheParam(**hc.param()))
+
+    def put(to_cache, to_scale, counts, first, k, v):
+        ends = [f + c for f, c in zip(first, counts)]
+        append.forward(dev(k), dev(v), dev(starts_of(counts)), dev(starts_of(ends)), starts, i64(first), max(counts), max(ends),
+                       to_cache, to_scale)
+
+    def draw(total):
+        return [rng.standard_normal((total, kv_heads, dim)).astype(np.float16) for _ in range(2)]
+
+    hist_k, hist_v = draw(sum(start))
+    tok_k, tok_v = draw(sum(n))
+    put(cache, scale, start, [0] * 3, hist_k, hist_v)
+    put(cache, scale, n, start, tok_k, tok_v)
+    parents = sum([draw_parents(rng, m, "tree") for m in n], [])
+    q = rng.standard_normal((sum(n), heads, dim)).astype(np.float16)
+    tree = ops.TreeAttention(attention_param(hc, heads))
+    got = tree.forward(dev(q), i64(parents), dev(starts_of(n)), starts, i64(start), max(n), max(s + m for s, m in zip(start, n)),
+                       cache, scale)
+    assert tree.device_status() == 0
+    hc.cache, hc.scale = cache.cpu().numpy(), scale.cpu().numpy()
+    hc.lens = [s + m for s, m in zip(start, n)]
+    want, tol = tree_reference(hc, q, parents, start, n, heads, 0)
+    assert np.all(np.abs(got.cpu().numpy() - want) <= tol)
+
+    paths = []  # from a drafted token up to the root
+    for b, first in enumerate(starts_of(n)[:-1]):
+        at, path = n[b] - 1 - b, []
+        while at >= 0:
+            path.append(at)
+            at = parents[first + at]
+        paths.append(path[::-1])
+    most = max(len(p) for p in paths) + 1
+    kept = np.full((3, 1, most), -1, dtype=I64)
+    for b, path in enumerate(paths):
+        kept[b, 0, :len(path)] = path
+    compact = ops.KeyValueCacheCompact(ops.KeyValueCacheParam(**hc.param()))
+    compact.forward(dev(kept), starts, i64(start), i64(hc.lens), max(hc.lens), cache, scale)
+    assert compact.device_status() == 0
+
+    plain, plain_scale = torch.zeros_like(cache), torch.zeros_like(scale)
+    put(plain, plain_scale, start, [0] * 3, hist_k, hist_v)
+    rows = np.concatenate([[first + i for i in path] for first, path in zip(starts_of(n)[:-1], paths)]).astype(I64)
+    put(plain, plain_scale, [len(p) for p in paths], start, tok_k[rows], tok_v[rows])
+    now = [s + len(p) for s, p in zip(start, paths)]
+    q1 = dev(rng.standard_normal((3, heads, dim)).astype(np.float16))
+    k1, v1 = (dev(x) for x in draw(3))
+    one = decode_output(hc, cache, scale, starts, heads, now, q1, k1, v1)
+    two = decode_output(hc, plain, plain_scale, starts, heads, now, q1, k1, v1)
+    assert torch.equal(one, two)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout,page", [(0, 0), (3, 48)])
+def test_an_evicted_cache_decodes_like_one_of_the_kept_rows(gpu, pkg, layout, page):  # noqa: F811
+    """Prompt window and decode steps add up weights, the highest stay, their rows move to the front with their weights;
+    a decode step then gives what it gives on a cache into which the host gathered the same rows."""
+    import torch
+    from ppl_nn_b200 import ops
+    rng = np.random.default_rng(layout)
+    heads, kv_heads, dim = 8, 2, 64
+    lens = [300, 90, 31]
+    hc = HostCache(rng, [m + 1 for m in lens], kv_heads, dim, layout, page)
+    hc.weight[:] = 0
+    cache, scale, starts, weight = dev(hc.cache), dev(hc.scale), dev(hc.starts), dev(hc.weight)
+    weigh = ops.AttentionWeight(attention_param(hc, heads))
+    want, tol = np.zeros_like(hc.weight, dtype=np.float64), 0.0
+    for n in ([16, 16, 16], [1, 1, 1]):  # the window at the end of the prompt, then a step
+        q = rng.standard_normal((sum(n), heads, dim)).astype(np.float16)
+        first = [m - x for m, x in zip(lens, n)]
+        part, off = weight_reference(hc, q, first, n, heads, 0, True)
+        want, tol = want + part, tol + off
+        weigh.forward(dev(q), dev(starts_of(n)), starts, i64(first), max(n), max(lens), cache, scale, weight)
+        assert weigh.device_status() == 0
+    w = weight.cpu().numpy()
+    # the second sum's rounding counts the first's weights as well
+    assert np.all(np.abs(w - want) <= tol + 2.0 ** -23 * np.abs(want))
+    budgets = [64, 90, 20]
+    evict = ops.KeyValueCacheEvict(ops.KeyValueCacheEvictParam(**hc.param(), sink=2, recent=8))
+    kept = evict.forward(weight, starts, i64(lens), i64(budgets), max(lens), max(budgets))
+    compact = ops.KeyValueCacheCompact(ops.KeyValueCacheParam(**hc.param()))
+    compact.forward(kept, starts, i64([0, 0, 0]), i64(lens), max(lens), cache, scale, weight)
+    assert evict.device_status() == 0 and compact.device_status() == 0
+    kept = kept.cpu().numpy()
+    gathered, gathered_scale, gathered_w = hc.cache.copy(), hc.scale.copy(), w.copy()
+    for b, m in enumerate(budgets):
+        dst = hc.rows(b, np.arange(m))
+        for h in range(kv_heads):
+            assert (kept[b, h, :m] >= 0).all() and (kept[b, h, m:] == -1).all()
+            src = hc.rows(b, kept[b, h, :m])
+            if layout == 0:
+                gathered[dst, :, :, h], gathered_scale[dst, :, :, h] = hc.cache[src, :, :, h], hc.scale[src, :, :, h]
+            else:
+                gathered[:, :, h, dst], gathered_scale[:, :, h, dst] = hc.cache[:, :, h, src], hc.scale[:, :, h, src]
+            gathered_w[:, h, dst] = w[:, h, src]
+            gathered_w[:, h, hc.rows(b, np.arange(m, lens[b]))] = 0
+    assert np.array_equal(weight.cpu().numpy(), gathered_w)
+    q1 = dev(rng.standard_normal((3, heads, dim)).astype(np.float16))
+    k1, v1 = (dev(rng.standard_normal((3, kv_heads, dim)).astype(np.float16)) for _ in range(2))
+    one = decode_output(hc, cache, scale, starts, heads, budgets, q1, k1, v1)
+    two = decode_output(hc, dev(gathered), dev(gathered_scale), starts, heads, budgets, q1, k1, v1)
+    assert torch.equal(one, two)
+
+
+# ---- streams and captured calls ------------------------------------------------------------------------
+
+class Step:
+    """All four operators once, on inputs that stay where they are."""
+
+    def __init__(self, seed, heads=8, kv_heads=2, dim=128):
+        from ppl_nn_b200 import ops
+        self.rng = np.random.default_rng(seed)
+        self.heads, self.n = heads, [5, 1, 12]
+        self.hc = hc = HostCache(self.rng, [700, 90, 330], kv_heads, dim, 3, 48)
+        p = attention_param(hc, heads)
+        self.tree, self.weigh = ops.TreeAttention(p), ops.AttentionWeight(p)
+        self.evict = ops.KeyValueCacheEvict(ops.KeyValueCacheEvictParam(**hc.param(), sink=1, recent=9))
+        self.compact = ops.KeyValueCacheCompact(ops.KeyValueCacheParam(**hc.param()))
+        self.seq, self.starts, self.budgets = dev(starts_of(self.n)), dev(hc.starts), i64([100, 90, 40])
+        self.base = i64([0, 0, 0])
+        self.cache, self.scale, self.weight = dev(hc.cache), dev(hc.scale), dev(hc.weight)
+        self.q = dev(self.rng.standard_normal((sum(self.n), heads, dim)).astype(np.float16))
+        self.parents = i64(sum([draw_parents(self.rng, m, "tree") for m in self.n], []))
+        self.lens = i64(hc.lens)
+        self.start = self.lens - i64(self.n)
+
+    def refill(self, seed):
+        """New contents in the same places: other codes, queries, parents and lengths."""
+        rng = np.random.default_rng(seed)
+        lens = [int(rng.integers(m // 2, m + 1)) for m in self.hc.lens]
+        for t, a in ((self.cache, rng.integers(-127, 128, size=self.hc.cache.shape, dtype=np.int8)),
+                     (self.weight, rng.exponential(0.01, size=self.hc.weight.shape).astype(np.float32)),
+                     (self.scale, self.hc.scale), (self.q, rng.standard_normal(tuple(self.q.shape)).astype(np.float16)),
+                     (self.parents, np.array(sum([draw_parents(rng, m, "tree") for m in self.n], []))),
+                     (self.lens, np.array(lens)), (self.start, np.array(lens) - np.array(self.n))):
+            t.copy_(dev(a))
+
+    def run(self):
+        most = max(self.hc.lens)
+        out = self.tree.forward(self.q, self.parents, self.seq, self.starts, self.start, 12, most, self.cache, self.scale)
+        self.weigh.forward(self.q, self.seq, self.starts, self.start, 12, most, self.cache, self.scale, self.weight)
+        kept = self.evict.forward(self.weight, self.starts, self.lens, self.budgets, most, 100)
+        self.compact.forward(kept, self.starts, self.base, self.lens, most, self.cache, self.scale, self.weight)
+        return [out, kept, self.cache, self.scale, self.weight]
+
+
+@pytest.mark.gpu
+def test_captured_steps_are_replayed_on_new_contents(gpu, pkg):  # noqa: F811
+    import torch
+    steps = [Step(1), Step(1)]
+    # what the steps give in turn, eagerly
+    want = []
+    for seed in (11, 12, 13):
+        steps[0].refill(seed)
+        want.append([t.clone() for t in steps[0].run()])
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in steps:  # two graphs; the second's operators are the first's, too
+        s.tree, s.weigh, s.evict, s.compact = steps[0].tree, steps[0].weigh, steps[0].evict, steps[0].compact
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(s.run())
+        graphs.append(g)
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for seeds in ((11, 12), (13, 11), (12, 13)):
+        for s, seed in zip(steps, seeds):
+            s.refill(seed)
+        torch.cuda.synchronize()
+        for g, stream in zip(graphs, side):  # at the same time
+            with torch.cuda.stream(stream):
+                g.replay()
+        torch.cuda.synchronize()
+        for out, seed in zip(outs, seeds):
+            for x, y in zip(out, want[seed - 11]):
+                assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_steps_on_two_streams_share_the_operators(gpu, pkg):  # noqa: F811
+    import torch
+    alone = []
+    for seed in (21, 22):
+        s = Step(1)
+        s.refill(seed)
+        alone.append([t.clone() for t in s.run()])
+    pair = [Step(1), Step(1)]
+    pair[1].tree, pair[1].weigh, pair[1].evict, pair[1].compact = pair[0].tree, pair[0].weigh, pair[0].evict, pair[0].compact
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for s, seed in zip(pair, (21, 22)):
+            s.refill(seed)
+        torch.cuda.synchronize()
+        outs = []
+        for s, stream in zip(pair, streams):
+            with torch.cuda.stream(stream):
+                outs.append(s.run())
+        torch.cuda.synchronize()
+        for out, want in zip(outs, alone):
+            for x, y in zip(out, want):
+                assert torch.equal(x, y)
+
+
+# ---- long caches -------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout,page", [(0, 0), (3, 0), (0, 128)])
+def test_rows_beyond_two_to_the_31(gpu, pkg, layout, page):  # noqa: F811
+    """Sequences at the end of a cache of 2.3 GB give what the same rows give in a small one, bit by bit."""
+    import torch
+    from ppl_nn_b200 import ops
+    torch.manual_seed(layout + page)
+    heads, kv_heads, dim, layers, tokens = 8, 4, 128, 4, 1 << 19
+    lead = (tokens + 65536, layers, 2, kv_heads) if layout == 0 else (layers, 2, kv_heads, tokens + 65536)
+    shift = 65536 + tokens - 4096  # the small cache's row 0
+    big = torch.zeros(lead + (dim,), dtype=torch.int8, device=gpu)
+    big_scale = torch.zeros(lead + (dim // 8,), dtype=torch.float16, device=gpu)
+    assert big.numel() > 1 << 31
+    rows = slice(shift, shift + 4096)
+    cut = (rows,) if layout == 0 else (slice(None), slice(None), slice(None), rows)
+    small = torch.randint(-127, 128, tuple(big[cut].shape), dtype=torch.int8, device=gpu)
+    small_scale = torch.rand(tuple(big_scale[cut].shape), device=gpu).mul_(0.02).add_(0.005).half()
+    big[cut], big_scale[cut] = small, small_scale
+    n, start = [20, 3], [1500, 2000]
+    starts = torch.tensor([100, 2000] if not page else [[i * 128 for i in order] for order in (range(0, 16), range(31, 15, -1))],
+                          device=gpu, dtype=torch.int64)
+    q = torch.randn(sum(n), heads, dim, device=gpu).half()
+    parents = i64(sum([draw_parents(np.random.default_rng(3), m, "tree") for m in n], []))
+    seq, first, lens = dev(starts_of(n)), i64(start), i64([s + m for s, m in zip(start, n)])
+    geometry = dict(num_layer=layers, layer_idx=layers - 1, quant_bit=8, cache_mode=1 if page else 0, cache_layout=layout,
+                    page_size=page or 128)
+    p = ops.MultiHeadCacheAttentionParam(num_heads=heads, num_kv_heads=kv_heads, head_dim=dim, **geometry)
+    res = []
+    for cache, scale, at in ((small, small_scale, starts), (big, big_scale, starts + shift)):
+        weight = torch.zeros(layers, kv_heads, cache.shape[0 if layout == 0 else 3], device=gpu)
+        tree, weigh = ops.TreeAttention(p), ops.AttentionWeight(p)
+        out = tree.forward(q, parents, seq, at, first, 20, 2003, cache, scale)
+        weigh.forward(q, seq, at, first, 20, 2003, cache, scale, weight)
+        last = torch.stack([q[19], q[22]])
+        weigh.forward(last, i64([0, 1, 2]), at, lens - 1, 1, 2003, cache, scale, weight)
+        evict = ops.KeyValueCacheEvict(ops.KeyValueCacheEvictParam(**geometry, sink=1, recent=4))
+        kept = evict.forward(weight, at, lens, i64([700, 333]), 2003, 700)
+        compact = ops.KeyValueCacheCompact(ops.KeyValueCacheParam(**geometry))
+        compact.forward(kept, at, i64([0, 0]), lens, 2003, cache, scale, weight)
+        assert [o.device_status() for o in (tree, weigh, evict, compact)] == [0] * 4
+        part = cut if cache is big else (slice(None),)
+        res.append([out, kept, cache[part].clone(), scale[part].clone(), weight[..., -4096:].clone()])
+        if cache is big:  # nothing in front of the rows was touched
+            rest = (slice(0, shift),) if layout == 0 else (slice(None), slice(None), slice(None), slice(0, shift))
+            assert not cache[rest].any() and not weight[..., :-4096].any()
+    for x, y in zip(*res):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["spread", "equal", "two values", "sampled high", "sorted"])
+@pytest.mark.parametrize("n", [40000, 262144, 300001])
+def test_select_of_long_lists(gpu, pkg, kind, n):  # noqa: F811
+    """Lists beyond the shared memory, samples that mislead, and more equal weights than a list holds."""
+    import torch
+    from ppl_nn_b200 import ops
+    rng = np.random.default_rng(n)
+    budget, sink, recent = n // 3, 4, 100
+    w = rng.exponential(1.0, size=n).astype(np.float32)
+    if kind == "equal":
+        w[:] = 0.25
+    elif kind == "two values":
+        w[:] = rng.integers(0, 2, size=n)
+    elif kind == "sampled high":  # the sample's positions hold the highest weights
+        have = n - recent - sink
+        w[sink + (np.arange(4096) * (have / 4096)).astype(I64)] += 100
+    elif kind == "sorted":
+        w.sort()
+    full = np.zeros((1, 1, n + 7), dtype=np.float32)
+    full[0, 0, 3:3 + n] = w
+    op = ops.KeyValueCacheEvict(ops.KeyValueCacheEvictParam(num_layer=1, layer_idx=0, quant_bit=8, cache_mode=0, cache_layout=0,
+                                                            sink=sink, recent=recent))
+    got = op.forward(dev(full), i64([3]), i64([n]), i64([budget]), n, budget)
+    assert op.device_status() == 0
+    cand = np.arange(sink, n - recent)
+    order = cand[np.argsort(-w[cand], kind="stable")][:budget - sink - recent]
+    want = np.sort(np.concatenate([np.arange(sink), order, np.arange(n - recent, n)]))
+    assert torch.equal(got[0, 0].cpu(), torch.from_numpy(want))
+
+
+# ---- forms of the weights and of the tree --------------------------------------------------------------
+
+MORE_WEIGHT_CASES = [
+    # heads, kv heads, dim, start, n, layout, page, layers, layer, causal: 1, 2, 3..4, 5..8 and many rows, both head sizes
+    (4, 4, 128, [0, 31, 600], [1, 1, 1], 0, 0, 1, 0, True),
+    (3, 3, 64, [5, 1023], [1, 1], 3, 48, 1, 0, True),
+    (4, 2, 128, [0, 16, 1500], [1, 1, 1], 3, 0, 1, 0, True),
+    (4, 2, 64, [47, 200], [1, 1], 0, 16, 1, 0, True),
+    (2, 2, 64, [0, 100, 33], [2, 1, 0], 0, 0, 2, 1, True),
+    (2, 2, 128, [64, 9], [2, 2], 0, 0, 1, 0, False),
+    (8, 2, 64, [15, 700], [1, 1], 0, 0, 1, 0, True),
+    (6, 2, 64, [300, 2], [1, 1], 3, 128, 1, 0, True),
+    (2, 1, 128, [0, 515], [2, 2], 0, 16, 1, 0, True),
+    (16, 2, 128, [0, 900], [1, 1], 0, 0, 1, 0, True),
+    (5, 1, 128, [63], [1], 3, 0, 1, 0, True),
+    (9, 1, 64, [64, 0], [1, 1], 0, 0, 1, 0, True),
+    (32, 4, 64, [0, 1100], [40, 17], 0, 0, 1, 0, True),
+    (32, 4, 128, [980, 3], [33, 2], 3, 64, 2, 0, False),
+    (4, 1, 128, [2040], [300], 0, 128, 1, 0, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", MORE_WEIGHT_CASES, ids=str)
+def test_attention_weight_forms(gpu, pkg, case):  # noqa: F811
+    from ppl_nn_b200 import ops
+    heads, kv_heads, dim, start, n, layout, page, layers, layer, causal = case
+    rng = np.random.default_rng(sum(start) + dim)
+    hc = HostCache(rng, [s + m for s, m in zip(start, n)], kv_heads, dim, layout, page, layers)
+    q = rng.standard_normal((sum(n), heads, dim)).astype(np.float16)
+    want, tol = weight_reference(hc, q, start, n, heads, layer, causal)
+    op = ops.AttentionWeight(attention_param(hc, heads, layer, is_causal=causal))
+    for max_n, max_len in ((max(n), hc.max_len), (max(n), hc.max_len + (0 if page else 1000))):
+        weight, cache, scale = dev(hc.weight), dev(hc.cache), dev(hc.scale)
+        op.forward(dev(q), dev(starts_of(n)), dev(hc.starts), i64(start), max_n, max_len, cache, scale, weight)
+        assert op.device_status() == 0
+        got = weight.cpu().numpy()
+        assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+        assert np.array_equal(cache.cpu().numpy(), hc.cache) and np.array_equal(scale.cpu().numpy(), hc.scale)
+    # a larger bound on the query tokens picks another form, not another result
+    weight = dev(hc.weight)
+    op.forward(dev(q), dev(starts_of(n)), dev(hc.starts), i64(start), max(n) + 9, hc.max_len, dev(hc.cache), dev(hc.scale), weight)
+    assert op.device_status() == 0
+    assert np.all(np.abs(weight.cpu().numpy() - want) <= tol)
+
+
+@pytest.mark.gpu
+def test_weights_of_sequences_that_share_rows_add_up(gpu, pkg):  # noqa: F811
+    """Two sequences over the same cache rows: both add to them (a shared prefix)."""
+    from ppl_nn_b200 import ops
+    rng = np.random.default_rng(8)
+    hc = HostCache(rng, [200, 200], 2, 64)
+    hc.starts[1] = hc.starts[0]
+    for n in ([1, 1], [9, 9]):
+        start = [200 - m for m in n]
+        q = rng.standard_normal((sum(n), 4, 64)).astype(np.float16)
+        want, tol = weight_reference(hc, q, start, n, 4, 0, True)
+        weight = dev(hc.weight)
+        ops.AttentionWeight(attention_param(hc, 4)).forward(dev(q), dev(starts_of(n)), dev(hc.starts), i64(start), max(n), 200,
+                                                             dev(hc.cache), dev(hc.scale), weight)
+        # one more rounding than the reference counts: two additions to a row
+        assert np.all(np.abs(weight.cpu().numpy() - want) <= tol + 2.0 ** -23 * np.abs(want))
+
+
+@pytest.mark.gpu
+def test_the_largest_tree(gpu, pkg):  # noqa: F811
+    rng = np.random.default_rng(5)
+    start, n = [70, 3], [1024, 129]
+    hc = HostCache(rng, [s + m for s, m in zip(start, n)], 1, 64)
+    q = rng.standard_normal((sum(n), 2, 64)).astype(np.float16)
+    parents = draw_parents(rng, 1024, "tree") + draw_parents(rng, 129, "star")
+    want, tol = tree_reference(hc, q, parents, start, n, 2, 0)
+    got, status = run_tree(hc, q, parents, start, n, 2, 0)
+    assert status == 0
+    assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+    again, _ = run_tree(hc, q, parents, start, n, 2, 0)
+    assert np.array_equal(again, got)
