@@ -21,6 +21,8 @@
 // where many positions were dropped.  Persistent CTAs draw their segments from a counter in an order in which a list's
 // earlier segments come first.  Nobody waits before it has raised the flags of the segments it has begun, so the lowest
 // flag not yet up always belongs to a CTA that can go on.
+#include <type_traits>
+
 #include "common.cuh"
 #include "launch.h"
 
@@ -287,46 +289,47 @@ __global__ void __launch_bounds__(NT) kv_evict_select_kernel(const SelectArgs a)
             }
             cp_async_commit();
         };
-        fetch(0, first);
-        int stage = 0;
-        for (int32_t pos0 = first; pos0 - lane < hi; pos0 += step, stage ^= 1) {
-            fetch(stage ^ 1, pos0 + step);
-            cp_async_wait<1>();
-            uint32_t mid[kAhead], count = 0, in_list = 0, my_up = 0;
-            float x[kAhead];
-            const bool inner = pos0 - lane >= lo && pos0 - lane + (kAhead - 1) * NT + 32 <= hi;  // all of the stage
+        // The list's order does not matter: a lane with keys for it takes their places by itself.  ALL: every position
+        // of the stage is a candidate.
+        auto scan = [&](auto all, int stage, int32_t pos0) {
+            constexpr bool ALL = decltype(all)::value;
+            const float* mine_now = ring + stage * kAhead * NT + tid;
+            uint32_t in_list = 0, my_up = 0;
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
                 const int32_t pos = pos0 + i * NT;
-                const bool in = inner || (pos >= lo && pos < hi);
-                x[i] = in ? ring[(stage * kAhead + i) * NT + tid] : 0.0f;
-                const bool up_here = in && x[i] > high_w;
-                const bool listed = in && !up_here && (list_all || x[i] >= low_w);
+                const bool in = ALL || (pos >= lo && pos < hi);
+                const float x = in ? mine_now[i * NT] : 0.0f;
+                const bool up_here = in && x > high_w;
                 const uint32_t up = __ballot_sync(0xffffffffu, up_here);
-                mid[i] = __ballot_sync(0xffffffffu, listed);
                 my_up = lane == i ? up : my_up;
-                count += __popc(mid[i]);
-                in_list |= (listed ? 1u : 0u) << i;
+                if (in && !up_here && (list_all || x >= low_w)) {
+                    in_list |= 1u << i;
+                }
             }
             if (my_up != 0u) {  // lanes 0 .. kAhead - 1 hold a word each; this warp alone owns them
                 mask[(pos0 >> 5) + lane * (NT / 32)] |= my_up;
                 above += __popc(my_up);
             }
-            if (count != 0u) {
-                uint32_t at = 0;
-                if (lane == 0) {
-                    at = atomicAdd(&sh.listed, count);
+            if (in_list != 0u) {
+                uint32_t slot = atomicAdd(&sh.listed, __popc(in_list));
+                for (; in_list != 0u && slot < static_cast<uint32_t>(a.list_cap); in_list &= in_list - 1u, ++slot) {
+                    const int i = __ffs(in_list) - 1;
+                    list_key[slot] = order_key(mine_now[i * NT]);
+                    list_pos[slot] = pos0 + i * NT;
                 }
-                at = __shfl_sync(0xffffffffu, at, 0);
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    const uint32_t slot = at + __popc(mid[i] & ((1u << lane) - 1u));
-                    if (((in_list >> i) & 1u) != 0u && slot < static_cast<uint32_t>(a.list_cap)) {
-                        list_key[slot] = order_key(x[i]);
-                        list_pos[slot] = pos0 + i * NT;
-                    }
-                    at += __popc(mid[i]);
-                }
+            }
+            __syncwarp();
+        };
+        fetch(0, first);
+        int stage = 0;
+        for (int32_t pos0 = first; pos0 - lane < hi; pos0 += step, stage ^= 1) {
+            fetch(stage ^ 1, pos0 + step);
+            cp_async_wait<1>();
+            if (pos0 - lane >= lo && pos0 - lane + (kAhead - 1) * NT + 32 <= hi) {
+                scan(std::true_type{}, stage, pos0);
+            } else {
+                scan(std::false_type{}, stage, pos0);
             }
         }
         cp_async_wait<0>();
