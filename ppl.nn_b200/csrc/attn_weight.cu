@@ -1,8 +1,8 @@
 // Accumulated attention weight: w[row(j)] += sum over the query heads of a kv group and over the query tokens of
 // softmax_j(q . k_j / sqrt(Dh)), for every cached position j of every sequence.  Only K is read.
 //
-// The normaliser of a row needs all its scores before any weight is known.  This file has the form for up to 8 query
-// rows (token x head of the group) per kv head, i.e. for decode steps; attn_window.cu the one for more.
+// The normaliser of a row needs all its scores before any weight is known.  This file has the form for up to 32 query
+// rows (token x head of the group) per kv head, i.e. for decode steps and short windows; attn_window.cu the one for more.
 // attn_weight_stats_kernel leaves, per query row and chunk of positions, the maximum and the sum of exponentials, and
 // writes the raw scores to the workspace (4 bytes a row against the 160 of a K row at Dh 128), so that K is read once;
 // attn_weight_spread_kernel joins the chunks and turns the scores into weights.
@@ -17,6 +17,13 @@
 // row) pairs, each zero outside its group: the accumulators hold a row's products of one group, which are scaled in
 // fp32.  With more rows there are too few columns for that, and k = code * scale is split into fp16(k) and the exact
 // remainder, which have accumulators of their own.
+//
+// Measured: 64 sequences of 128 to 4096 positions, 32 kv heads of 128 (771 MB of keys), one row: scores 127 us (6.1 TB/s,
+// 92 % of a copy's rate), 155 us with the spread kernel, whose traffic is 4 + 4 + 8 bytes a position against 160.  With
+// split keys, bound by their instructions, it was 190.  64 sequences of up to 16384 positions, 8 kv heads (739 MB): 4 rows
+// 160, 8 rows 185, 16 rows 255, 32 rows 480 us; attn_window.cu takes 785 us for up to 32 rows and 839 for 128, the kept
+// scores of more than 32 rows would be twice the bytes of K and more.  Chunks of 512 positions waste a CTA's start, so
+// they grow to 4096 while the chip stays full.
 #include "attn_weight.cuh"
 
 namespace pplb200 {
@@ -129,20 +136,23 @@ struct Ring {
     }
 };
 
-// Where the score of a thread belongs: RB is the number of query rows that the columns of B have room for.
-// RB 8: positions g and g + 8, rows 2t and 2t + 1.  Below, the four threads of a g share the positions out.
+// Where the scores of a thread belong: RB is the number of query rows that the columns of B have room for.
+// RB 8, 16, 32: positions g and g + 8, rows 2t and 2t + 1 of each octet.  Below, the four threads of a g share the
+// positions out.
 template <int RB>
 struct Place {
-    static constexpr int kPos = RB == 8 ? 2 : 1;      // positions of a thread, 8 apart
-    static constexpr int kCols = RB >= 4 ? 2 : 1;     // rows of a thread
+    static constexpr int kOctets = RB < 8 ? 1 : RB / 8;
+    static constexpr int kPos = RB >= 8 ? 2 : 1;                         // positions of a thread, 8 apart
+    static constexpr int kCols = (RB >= 4 ? 2 : 1) * kOctets;            // rows of a thread
     static __device__ __forceinline__ int position(int lane) {
-        return (lane >> 2) + (RB == 8 ? 0 : 8 * (RB == 4 ? (lane >> 1) & 1 : lane & 1));
+        return (lane >> 2) + (RB >= 8 ? 0 : 8 * (RB == 4 ? (lane >> 1) & 1 : lane & 1));
     }
-    static __device__ __forceinline__ int row(int lane) {
-        return RB == 8 ? 2 * (lane & 3) : (RB == 4 ? 2 * (lane & 1) : (RB == 2 ? (lane >> 1) & 1 : 0));
+    static __device__ __forceinline__ int row(int lane, int c) {
+        return RB >= 8 ? 8 * (c >> 1) + 2 * (lane & 3) + (c & 1)
+                       : (RB == 4 ? 2 * (lane & 1) + c : (RB == 2 ? (lane >> 1) & 1 : 0));
     }
     // lanes (by their differences) that hold other positions of the same rows; RB 1 has each score twice
-    static constexpr uint32_t kPeers = RB == 8 ? 4 + 8 + 16 : (RB == 4 ? 2 + 4 + 8 + 16 : 1 + 4 + 8 + 16);
+    static constexpr uint32_t kPeers = RB >= 8 ? 4 + 8 + 16 : (RB == 4 ? 2 + 4 + 8 + 16 : 1 + 4 + 8 + 16);
     static __device__ __forceinline__ bool first(int lane) { return (lane & kPeers) == 0 && (RB > 1 || lane == 0); }
     static __device__ __forceinline__ bool stores(int lane) { return RB > 1 || (lane & 2) == 0; }
 };
@@ -152,8 +162,9 @@ template <int DH, int RB>
 struct Tile {
     static constexpr int kWords = DH / 16;
     static constexpr int kHalves = RB == 4 ? 2 : 1;  // RB 4: two of the four groups of a k-step at a time
+    static constexpr int kFrags = kHalves * Place<RB>::kOctets;
     static constexpr int kPos = Place<RB>::kPos, kCols = Place<RB>::kCols;
-    using Query = uint2[kHalves][kWords];
+    using Query = uint2[kFrags][kWords];
     uint4 code[2][DH / 64];
     uint32_t sc[kHalves][2][DH / 64];
 
@@ -192,31 +203,32 @@ struct Tile {
         return (w & 3) == 0 ? c.x : ((w & 3) == 1 ? c.y : ((w & 3) == 2 ? c.z : c.w));
     }
 
-    // Query fragments: row g of this CTA's rows, or of column g's (group, row) pair; zeros elsewhere.  Thread t holds the
+    // Query fragments: row g of an octet, or of column g's (group, row) pair; zeros elsewhere.  Thread t holds the
     // channels of the groups 2t (words 0 and 1 of a block of 64) and 2t + 1.
     static __device__ __forceinline__ void load_queries(const WeightArgs& a, const Span& s, int head, int lane, Query& qf) {
-        const int g = lane >> 2, t = lane & 3, row = RB == 8 ? g : (RB == 1 ? 0 : g % RB);
-        const int32_t i = row / a.group;
-        const __half* src = a.q + ((s.tok0 + i) * a.num_heads + head * a.group + (row - i * a.group)) * DH;
+        const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-        for (int w = 0; w < kWords; ++w) {
-            uint2 q = make_uint2(0u, 0u);
-            if (row < s.rows) {
-                q = *reinterpret_cast<const uint2*>(src + (w / 4) * 64 + t * 16 + (w & 3) * 4);
-            }
+        for (int x = 0; x < kFrags; ++x) {
+            const int row = RB >= 8 ? 8 * x + g : (RB == 1 ? 0 : g % RB);
+            const int32_t i = row / a.group;
+            const __half* src = a.q + ((s.tok0 + i) * a.num_heads + head * a.group + (row - i * a.group)) * DH;
 #pragma unroll
-            for (int x = 0; x < kHalves; ++x) {
-                const bool mine = RB == 8 || (RB == 4 ? t == 2 * x + (g >> 2) : (RB == 2 ? t == g >> 1 : g == 2 * t + ((w & 3) >> 1)));
-                qf[x][w] = mine ? q : make_uint2(0u, 0u);
+            for (int w = 0; w < kWords; ++w) {
+                const bool mine = RB >= 8 || (RB == 4 ? t == 2 * x + (g >> 2) : (RB == 2 ? t == g >> 1 : g == 2 * t + ((w & 3) >> 1)));
+                qf[x][w] = make_uint2(0u, 0u);
+                if (row < s.rows && mine) {
+                    qf[x][w] = *reinterpret_cast<const uint2*>(src + (w / 4) * 64 + t * 16 + (w & 3) * 4);
+                }
             }
         }
     }
 
     __device__ __forceinline__ void scores(const Query& qf, int lane, float (&out)[kPos][kCols]) const {
-        if constexpr (RB == 8) {
-            // two accumulators each for the keys and their remainders: short chains of dependent instructions, and of
-            // roundings
-            float key[2][4], rest[2][4];
+        if constexpr (RB >= 8) {
+            // with one octet two accumulators each for the keys and their remainders: short chains of dependent
+            // instructions, and of roundings
+            constexpr int kOctets = RB / 8, kChains = RB == 8 ? 2 : 1;
+            float key[kChains * kOctets][4], rest[kChains * kOctets][4];
 #pragma unroll
             for (int w = 0; w < kWords; ++w) {
                 uint32_t k[2][2], e[2][2];
@@ -225,18 +237,27 @@ struct Tile {
                     const uint32_t s = prmt(sc[0][r][w / 4], 0u, (w & 2) ? 0x3232u : 0x1010u);
                     split_key_word(word(r, w), u32_as_h2(s), k[r][0], k[r][1], e[r][0], e[r][1]);
                 }
-                const uint2 q = qf[0][w];
-                if (w < 2) {
-                    mma_first(key[w & 1], k[0][0], k[1][0], k[0][1], k[1][1], q.x, q.y);
-                    mma_first(rest[w & 1], e[0][0], e[1][0], e[0][1], e[1][1], q.x, q.y);
-                } else {
-                    mma_m16n8k16_f16f32(key[w & 1], k[0][0], k[1][0], k[0][1], k[1][1], q.x, q.y);
-                    mma_m16n8k16_f16f32(rest[w & 1], e[0][0], e[1][0], e[0][1], e[1][1], q.x, q.y);
+#pragma unroll
+                for (int o = 0; o < kOctets; ++o) {
+                    const uint2 q = qf[o][w];
+                    const int x = o * kChains + w % kChains;
+                    if (w < kChains) {
+                        mma_first(key[x], k[0][0], k[1][0], k[0][1], k[1][1], q.x, q.y);
+                        mma_first(rest[x], e[0][0], e[1][0], e[0][1], e[1][1], q.x, q.y);
+                    } else {
+                        mma_m16n8k16_f16f32(key[x], k[0][0], k[1][0], k[0][1], k[1][1], q.x, q.y);
+                        mma_m16n8k16_f16f32(rest[x], e[0][0], e[1][0], e[0][1], e[1][1], q.x, q.y);
+                    }
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                out[e >> 1][e & 1] = (key[0][e] + key[1][e]) + (rest[0][e] + rest[1][e]);
+            for (int o = 0; o < kOctets; ++o) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int x = o * kChains, y = x + kChains - 1;
+                    out[e >> 1][2 * o + (e & 1)] =
+                        kChains == 2 ? (key[x][e] + key[y][e]) + (rest[x][e] + rest[y][e]) : key[x][e] + rest[x][e];
+                }
             }
         } else {
             constexpr int kSteps = RB == 1 ? 4 : 2;  // k-steps of the same groups
@@ -297,10 +318,10 @@ struct Tile {
 };
 
 template <int DH, int RB>
-__global__ void __launch_bounds__(kThreads, RB >= 4 ? 5 : 6) attn_weight_stats_kernel(const WeightArgs a) {
+__global__ void __launch_bounds__(kThreads, RB == 32 ? 3 : RB == 16 ? 4 : RB >= 4 ? 5 : 6) attn_weight_stats_kernel(const WeightArgs a) {
     grid_launch_dependents();
     grid_dependency_wait();
-    __shared__ float2 red[kWarps][kScoreRows];
+    __shared__ float2 red[kWarps][RB];
     __shared__ __align__(128) uint8_t smem[kWarps * Ring<DH>::kWarpBytes];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t b = blockIdx.z;
@@ -317,13 +338,13 @@ __global__ void __launch_bounds__(kThreads, RB >= 4 ? 5 : 6) attn_weight_stats_k
     using At = Place<RB>;
     typename T::Query qf;
     T::load_queries(a, s, head, lane, qf);
-    const int my_pos = At::position(lane), my_row = At::row(lane);
+    const int my_pos = At::position(lane);
     // the last position that this thread's rows see
     int64_t last[At::kCols];
     float m[At::kCols], l[At::kCols];
 #pragma unroll
     for (int c = 0; c < At::kCols; ++c) {
-        last[c] = a.causal ? s.start + (my_row + c) / a.group : s.len - 1;
+        last[c] = a.causal ? s.start + At::row(lane, c) / a.group : s.len - 1;
         last[c] = last[c] < s.len - 1 ? last[c] : s.len - 1;
         m[c] = kNegBig;
         l[c] = 0.0f;
@@ -360,14 +381,19 @@ __global__ void __launch_bounds__(kThreads, RB >= 4 ? 5 : 6) attn_weight_stats_k
                 }
             }
         }
-        if (my_row < s.rows && At::stores(lane)) {
-            float* dst = score + static_cast<int64_t>(pos) * a.score_rows + my_row;
+        if (At::stores(lane)) {
+            float* dst = score + static_cast<int64_t>(pos) * a.score_rows;
 #pragma unroll
             for (int p = 0; p < At::kPos; ++p) {
                 if (pos + 8 * p < s.len) {
-                    dst[p * 8 * a.score_rows] = x[p][0];
-                    if (At::kCols > 1 && my_row + 1 < s.rows) {
-                        dst[p * 8 * a.score_rows + 1] = x[p][At::kCols - 1];
+#pragma unroll
+                    for (int c = 0; c < At::kCols; c += 2) {
+                        const int row = At::row(lane, c);
+                        if (At::kCols > 1 && row + 1 < a.score_rows) {  // score_rows is even here
+                            *reinterpret_cast<float2*>(dst + p * 8 * a.score_rows + row) = make_float2(x[p][c], x[p][(c + 1) % At::kCols]);
+                        } else if (row < a.score_rows) {
+                            dst[p * 8 * a.score_rows + row] = x[p][c];
+                        }
                     }
                 }
             }
@@ -403,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, RB >= 4 ? 5 : 6) attn_weight_stats_k
             }
         }
         if (At::first(lane)) {
-            red[warp][my_row + c] = make_float2(m[c], l[c]);
+            red[warp][At::row(lane, c)] = make_float2(m[c], l[c]);
         }
     }
     __syncthreads();
@@ -422,7 +448,9 @@ __global__ void __launch_bounds__(kThreads, RB >= 4 ? 5 : 6) attn_weight_stats_k
     }
 }
 
-// One thread per position: the weights of the kept scores.
+// A thread per position at a time: the weights of the kept scores.  V: how many float4 the rows of a position take; 0: one
+// or two rows.
+template <int V>
 __global__ void __launch_bounds__(256) attn_weight_spread_kernel(const WeightArgs a) {
     grid_launch_dependents();
     grid_dependency_wait();
@@ -435,70 +463,74 @@ __global__ void __launch_bounds__(256) attn_weight_spread_kernel(const WeightArg
         return;
     }
     // a warp per query row joins its chunks
-    const int32_t my_row = threadIdx.x >> 5;
-    if (my_row < s.rows) {
-        const int32_t i = my_row / a.group;
-        const int64_t at = (s.tok0 + i) * a.num_heads + head * a.group + (my_row - i * a.group);
+    for (int32_t row = threadIdx.x >> 5; row < s.rows; row += 8) {
+        const int32_t i = row / a.group;
+        const int64_t at = (s.tok0 + i) * a.num_heads + head * a.group + (row - i * a.group);
         const float2 v = join_chunks(a, at, (s.len + a.chunk - 1) / a.chunk, threadIdx.x & 31);
         if ((threadIdx.x & 31) == 0) {
-            norm[my_row] = v;
+            norm[row] = v;
         }
     }
     __syncthreads();
     float* w = a.weight + (a.geom.layer_idx * a.num_kv_heads + head) * a.max_tokens;
     const float* score = a.score + (b * a.num_kv_heads + head) * a.max_kvlen * a.score_rows;
     const int64_t start_row = a.geom.cache_mode == 0 ? a.cachestarts[b] : 0;
-    constexpr int kPer = kSpread / 256;  // positions of a thread: their loads go out together
-    const int32_t pos0 = first + threadIdx.x;
-    float sum[kPer];
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        sum[k] = 0.0f;
-    }
-    int32_t r0 = 0;
-    if ((a.score_rows & 3) == 0) {  // four rows of a position at once
-        for (; r0 < s.rows; r0 += 4) {
-            float4 x[kPer];
+    auto add = [&](int32_t pos, float x) {
+        const int64_t row = a.geom.cache_mode == 0 ? (start_row < 0 ? -1 : start_row + pos)
+                                                   : cache_row(a.geom, a.cachestarts, b, pos);
+        if (cache_row_ok(row, a.max_tokens)) {
+            add_weight(w + row, x);  // one addition per position and call
+        }
+    };
+    auto weight_of = [&](float x, int32_t r) -> float {
+        const float2 v = norm[r];
+        return ex2_approx(fmaf(x, a.scale_log2, -v.x)) * v.y;
+    };
+    constexpr int kPer = V == 0 ? 8 : (V >= 8 ? 1 : 8 / V);  // positions of a thread whose loads go out together
+    for (int32_t pos0 = first + threadIdx.x; pos0 < first + kSpread && pos0 < s.len; pos0 += kPer * 256) {
+        float sum[kPer];
+        if constexpr (V == 0) {
+            float x[kPer][2];
 #pragma unroll
             for (int k = 0; k < kPer; ++k) {
-                x[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                if (pos0 + k * 256 < s.len) {
-                    x[k] = *reinterpret_cast<const float4*>(score + static_cast<int64_t>(pos0 + k * 256) * a.score_rows + r0);
-                }
+                const float* src = score + static_cast<int64_t>(pos0 + k * 256) * a.score_rows;
+                const bool there = pos0 + k * 256 < s.len;
+                x[k][0] = there ? src[0] : -INFINITY;
+                x[k][1] = there && s.rows > 1 ? src[1] : -INFINITY;
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                if (r0 + c < s.rows) {  // rows behind the last were not written
-                    const float2 v = norm[r0 + c];
+            for (int k = 0; k < kPer; ++k) {
+                sum[k] = weight_of(x[k][0], 0) + (s.rows > 1 ? weight_of(x[k][1], 1) : 0.0f);
+            }
+        } else {
+            float4 x[kPer][V];
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                const float* src = score + static_cast<int64_t>(pos0 + k * 256) * a.score_rows;
+#pragma unroll
+                for (int c = 0; c < V; ++c) {
+                    x[k][c] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    if (pos0 + k * 256 < s.len && 4 * c < s.rows) {
+                        x[k][c] = *reinterpret_cast<const float4*>(src + 4 * c);
+                    }
+                }
+                sum[k] = 0.0f;
+            }
+#pragma unroll
+            for (int c = 0; c < 4 * V; ++c) {
+                if (c < s.rows) {  // rows behind the last were not written, or are another call's
 #pragma unroll
                     for (int k = 0; k < kPer; ++k) {
-                        const float y = c == 0 ? x[k].x : (c == 1 ? x[k].y : (c == 2 ? x[k].z : x[k].w));
-                        sum[k] = fmaf(ex2_approx(fmaf(y, a.scale_log2, -v.x)), v.y, sum[k]);
+                        const float4 y = x[k][c / 4];
+                        sum[k] += weight_of(c % 4 == 0 ? y.x : (c % 4 == 1 ? y.y : (c % 4 == 2 ? y.z : y.w)), c);
                     }
                 }
             }
         }
-    }
-    for (; r0 < s.rows; ++r0) {
-        const float2 v = norm[r0];
-        float x[kPer];
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
-            x[k] = pos0 + k * 256 < s.len ? score[static_cast<int64_t>(pos0 + k * 256) * a.score_rows + r0] : -INFINITY;
-        }
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            sum[k] = fmaf(ex2_approx(fmaf(x[k], a.scale_log2, -v.x)), v.y, sum[k]);
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        const int32_t pos = pos0 + k * 256;
-        if (pos < s.len) {
-            const int64_t row = a.geom.cache_mode == 0 ? (start_row < 0 ? -1 : start_row + pos)
-                                                       : cache_row(a.geom, a.cachestarts, b, pos);
-            if (cache_row_ok(row, a.max_tokens)) {
-                add_weight(w + row, sum[k]);  // one addition per position and call
+            if (pos0 + k * 256 < s.len) {
+                add(pos0 + k * 256, sum[k]);
             }
         }
     }
@@ -508,18 +540,25 @@ template <int DH>
 int launch_dh(const pplb200_attn_params& p, const WeightArgs& a, cudaStream_t stream) {
     const dim3 grid(static_cast<unsigned>(p.num_kv_heads), static_cast<unsigned>(a.chunks), static_cast<unsigned>(p.batch));
     // each kernel starts while the one before it drains, and waits for it before it reads anything
-    const int32_t rows = a.score_rows;
-    launch_dependent(rows <= 1   ? attn_weight_stats_kernel<DH, 1>
-                     : rows <= 2 ? attn_weight_stats_kernel<DH, 2>
-                     : rows <= 4 ? attn_weight_stats_kernel<DH, 4>
-                                 : attn_weight_stats_kernel<DH, 8>,
+    const int64_t rows = p.max_seqlen * a.group;
+    launch_dependent(rows <= 1    ? attn_weight_stats_kernel<DH, 1>
+                     : rows <= 2  ? attn_weight_stats_kernel<DH, 2>
+                     : rows <= 4  ? attn_weight_stats_kernel<DH, 4>
+                     : rows <= 8  ? attn_weight_stats_kernel<DH, 8>
+                     : rows <= 16 ? attn_weight_stats_kernel<DH, 16>
+                                  : attn_weight_stats_kernel<DH, 32>,
                      grid, dim3(kThreads), 0, stream, a);
     const int rc = check_launch("attn_weight_stats_kernel");
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
     const dim3 spread(grid.x, static_cast<unsigned>((p.max_kvlen + kSpread - 1) / kSpread), grid.z);
-    launch_dependent(attn_weight_spread_kernel, spread, dim3(256), 0, stream, a);
+    launch_dependent(rows <= 2    ? attn_weight_spread_kernel<0>
+                     : rows <= 4  ? attn_weight_spread_kernel<1>
+                     : rows <= 8  ? attn_weight_spread_kernel<2>
+                     : rows <= 16 ? attn_weight_spread_kernel<4>
+                                  : attn_weight_spread_kernel<8>,
+                     spread, dim3(256), 0, stream, a);
     return check_launch("attn_weight_spread_kernel");
 }
 
@@ -528,18 +567,19 @@ int launch_dh(const pplb200_attn_params& p, const WeightArgs& a, cudaStream_t st
 int make_weight_plan(const pplb200_attn_params& p, WeightPlan* plan) {
     // With kept scores a CTA's start (lengths, rows and queries, each waiting for the one before) is worth longer chunks
     // as long as there are some 8 CTAs for each place on the chip.
-    const bool kept = p.max_seqlen > 0 && p.max_seqlen * (p.num_heads / p.num_kv_heads) <= kScoreRows;
+    const int64_t rows = p.max_seqlen * (p.num_heads / p.num_kv_heads);
+    const bool kept = rows > 0 && rows <= kScoreRows;
     plan->chunk = kept ? kChunk : kWindowChunk;
     while (kept && plan->chunk < 8 * kChunk &&
            p.batch * p.num_kv_heads * ((p.max_kvlen + 2 * plan->chunk - 1) / (2 * plan->chunk)) >= 148 * 4 * 8) {
         plan->chunk *= 2;
     }
     plan->chunks = (p.max_kvlen + plan->chunk - 1) / plan->chunk;
-    const uint64_t rows = static_cast<uint64_t>(p.total_tokens) * p.num_heads;
+    plan->score_rows = static_cast<int32_t>(rows <= 2 ? rows : (rows + 3) / 4 * 4);
+    const uint64_t all_rows = static_cast<uint64_t>(p.total_tokens) * p.num_heads;
     plan->off_norm = 256;  // behind the status word
-    plan->off_part = plan->off_norm + (rows * 8 + 255) / 256 * 256;
-    plan->off_score = plan->off_part + (rows * plan->chunks * 8 + 255) / 256 * 256;
-    plan->score_rows = static_cast<int32_t>(p.max_seqlen * (p.num_heads / p.num_kv_heads));
+    plan->off_part = plan->off_norm + (all_rows * 8 + 255) / 256 * 256;
+    plan->off_score = plan->off_part + (all_rows * plan->chunks * 8 + 255) / 256 * 256;
     const uint64_t positions = static_cast<uint64_t>(p.batch) * p.num_kv_heads * p.max_kvlen;
     plan->bytes = plan->off_score + (kept ? (positions * plan->score_rows * 4 + 255) / 256 * 256 : 0);
     return plan->chunks > 65535 ? PPLB200_UNSUPPORTED : PPLB200_SUCCESS;  // a grid dimension

@@ -7,7 +7,7 @@
 
 namespace pplb200 {
 
-constexpr int kScoreRows = 8;       // up to so many query rows per kv head the scores are kept
+constexpr int kScoreRows = 32;      // up to so many query rows per kv head the scores are kept
 constexpr int kWindowChunk = 1024;  // positions of a CTA where they are formed twice
 constexpr float kWeightNegBig = -1.0e30f;
 
@@ -86,7 +86,7 @@ __device__ __forceinline__ void add_weight(float* w, float x) {
     asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(w), "f"(x) : "memory");
 }
 
-// More than 8 query rows per kv head: statistics, join and weights (attn_window.cu).
+// More than kScoreRows query rows per kv head: statistics, join and weights (attn_window.cu).
 int launch_weight_window(const pplb200_attn_params& p, WeightArgs a, cudaStream_t stream);
 
 }  // namespace pplb200

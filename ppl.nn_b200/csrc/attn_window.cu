@@ -14,6 +14,12 @@
 // thread; 14 exchanges within the warp leave every lane with the sums of two positions over the warp's 32 rows, shared
 // memory adds the four warps up.
 // The order of every sum is fixed.
+//
+// Measured: 4 sequences of 8192 to 32768 positions, 8 kv heads of 128, 116 to 128 rows: statistics 68 us, weights 80 us,
+// 163 us in all; with warp-level products (mma.sync, 32 rows at a time) 408 us.  For up to 32 rows attn_weight.cu is the
+// faster one (figures there).  Bound by neither pipe: a block takes a CTA 2150 cycles for the statistics and 2600 for the
+// weights, the converters work 1500 of them, the tensor pipe is busy 40 % and 25 %; 760 CTAs on 296 places leave the third
+// wave partly empty, but with chunks of 512 or 2048 positions the two passes take longer (196 and 208 us against 180).
 #include "attn_weight.cuh"
 #include "kv_tiles.cuh"
 #include "ragged.cuh"

@@ -13,6 +13,10 @@
 //   4. The masks are walked in order of position: bits of the first mask, and the first so many of the second.
 // Should the bracket miss (too many keys above, or too few down to its end) or the list overflow (many equal weights),
 // the radix descent runs over the weights themselves, and so it does for lists too long for the masks.
+// Measured: 128 lists of 32768 to 131072 positions, 4096 kept: 40 us (49 us a call), of which the longest list takes 7 us
+// for the sample, 21 for the scan, 5 for the descent and 3 for the output.  A read of the weights alone would take 7 us:
+// a list is one CTA's, because its mask and list fill an SM's shared memory, and 128 CTAs of unequal length fill the chip
+// 60 %.
 //
 // Compact.  Row base + kept[i] moves to row base + i.  kept is strictly ascending, so kept[i] >= i.  A list is cut into
 // segments; a segment reads all its sources before it writes.  Its destinations may still be the sources of EARLIER
@@ -21,6 +25,9 @@
 // where many positions were dropped.  Persistent CTAs draw their segments from a counter in an order in which a list's
 // earlier segments come first.  Nobody waits before it has raised the flags of the segments it has begun, so the lowest
 // flag not yet up always belongs to a CTA that can go on.
+// Measured: 16 sequences of up to 16384 positions, 2048 kept per kv head, weights too (176 MB): 47 us (3.7 TB/s); 4 of up
+// to 131072, paged, 16001 kept (347 MB): 100 us (3.4 TB/s); the accepted paths of 32 sequences in 32 layers (26 MB): 7 us
+// of a 20 us call.  Scattered rows of 128 + 32 bytes are read in whole sectors but not in whole DRAM bursts.
 #include <type_traits>
 
 #include "common.cuh"

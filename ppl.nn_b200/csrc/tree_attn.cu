@@ -21,6 +21,20 @@
 //   * MT = 1: two CTAs per SM.  MT = 2, for more than 128 rows per kv head: one CTA per SM, whose two tiles share the
 //     fetched and converted K and V.
 //
+// Roundings: keys, weights and values enter the tensor cores as fp16 (code * scale rounded once, as in the prefill
+// kernel); scores, maxima, sums and outputs are held in fp32.  The keys' rounding dominates: 7e-4 to 1.2e-3 of the
+// output's magnitude against 2e-4 for exact keys and the same fp16 output.  Exact keys (a second tile of remainders, as
+// attn_window.cu has it) would need 16 KB more of shared memory than two CTAs per SM leave, and half as much again of
+// the converters' work, which is what the kernel waits for.
+//
+// Measured (8 kv heads of 128): 32 sequences of 256 to 8192 positions, 4 to 64 rows per kv head, 392 MB of cache: 145 us,
+// 163 us with plan and merge (2.4 TB/s); 64 such sequences, 200 to 264 rows: 445 us, 514 us in all (530 TFLOP/s); 4 of up
+// to 131072, paged, 228 to 256 rows: 470 us, 549 us in all (710 TFLOP/s).  What bounds it: a block takes a CTA 3300 cycles
+// at MT = 1, of which the converters work 2600 and wait 700; the MMA warp waits 1050 of them for converted tiles, the
+// tensor pipe is busy 31 % and DRAM 36 %.  More converter warps do not pay at 96 registers a thread (spills), with
+// converters apart for K and V and double-buffered scores the three cases take 177, 565 and 574 us.  MT = 2 against
+// MT = 1 for 256 rows: K and V are fetched and converted once for both tiles.
+//
 // Waits on mbarriers are bounded and give up together (see tcgen05.cuh).
 #include <cub/block/block_scan.cuh>
 

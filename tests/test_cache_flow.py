@@ -398,7 +398,8 @@ def test_select_of_long_lists(gpu, pkg, kind, n):  # noqa: F811
 # ---- forms of the weights and of the tree --------------------------------------------------------------
 
 MORE_WEIGHT_CASES = [
-    # heads, kv heads, dim, start, n, layout, page, layers, layer, causal: 1, 2, 3..4, 5..8 and many rows, both head sizes
+    # heads, kv heads, dim, start, n, layout, page, layers, layer, causal: 1, 2, 3..4, 5..8, 9..16, 17..32 and many rows, both
+    # head sizes
     (4, 4, 128, [0, 31, 600], [1, 1, 1], 0, 0, 1, 0, True),
     (3, 3, 64, [5, 1023], [1, 1], 3, 48, 1, 0, True),
     (4, 2, 128, [0, 16, 1500], [1, 1, 1], 3, 0, 1, 0, True),
@@ -411,6 +412,11 @@ MORE_WEIGHT_CASES = [
     (16, 2, 128, [0, 900], [1, 1], 0, 0, 1, 0, True),
     (5, 1, 128, [63], [1], 3, 0, 1, 0, True),
     (9, 1, 64, [64, 0], [1, 1], 0, 0, 1, 0, True),
+    (8, 2, 128, [300, 0, 77], [3, 4, 1], 0, 0, 1, 0, True),
+    (4, 1, 64, [50, 600], [4, 3], 3, 48, 1, 0, False),
+    (8, 1, 128, [700, 3], [4, 3], 3, 0, 1, 0, True),
+    (8, 2, 64, [100, 1030], [5, 2], 0, 16, 1, 0, True),
+    (7, 1, 128, [0, 2000], [1, 3], 0, 0, 2, 0, False),
     (32, 4, 64, [0, 1100], [40, 17], 0, 0, 1, 0, True),
     (32, 4, 128, [980, 3], [33, 2], 3, 64, 2, 0, False),
     (4, 1, 128, [2040], [300], 0, 128, 1, 0, True),
