@@ -577,10 +577,13 @@ int make_weight_plan(const pplb200_attn_params& p, WeightPlan* plan) {
     plan->chunks = (p.max_kvlen + plan->chunk - 1) / plan->chunk;
     plan->score_rows = static_cast<int32_t>(rows <= 2 ? rows : (rows + 3) / 4 * 4);
     const uint64_t all_rows = static_cast<uint64_t>(p.total_tokens) * p.num_heads;
+    const uint64_t positions = static_cast<uint64_t>(p.batch) * p.num_kv_heads * p.max_kvlen;
+    if (positions > 1ull << 50 || all_rows > 1ull << 40) {  // keeps the sizes below from wrapping around
+        return PPLB200_UNSUPPORTED;
+    }
     plan->off_norm = 256;  // behind the status word
     plan->off_part = plan->off_norm + (all_rows * 8 + 255) / 256 * 256;
     plan->off_score = plan->off_part + (all_rows * plan->chunks * 8 + 255) / 256 * 256;
-    const uint64_t positions = static_cast<uint64_t>(p.batch) * p.num_kv_heads * p.max_kvlen;
     plan->bytes = plan->off_score + (kept ? (positions * plan->score_rows * 4 + 255) / 256 * 256 : 0);
     return plan->chunks > 65535 ? PPLB200_UNSUPPORTED : PPLB200_SUCCESS;  // a grid dimension
 }

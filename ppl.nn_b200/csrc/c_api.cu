@@ -693,6 +693,9 @@ static int validate_cache_op(const pplb200_attn_params* p) {
     if (p->max_kvlen > 0x7fff0000) {
         return fail(PPLB200_UNSUPPORTED, "max_kvlen above 2^31 - 2^16");
     }
+    if (p->max_seqlen > 0x7fffffff) {
+        return fail(PPLB200_UNSUPPORTED, "max_seqlen above 2^31 - 1");
+    }
     if (p->batch > 65535 || p->num_kv_heads > 65535) {
         return fail(PPLB200_UNSUPPORTED, "more than 65535 sequences or kv heads");
     }
@@ -754,6 +757,9 @@ int pplb200_tree_attn_forward(const pplb200_attn_params* p, const void* query, c
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
+    if (query == attn_output) {
+        return fail(PPLB200_INVALID_VALUE, "attn_output must not be query: other CTAs still read it");
+    }
     TreePlan plan;
     rc = make_tree_plan(*p, di.sm_count, &plan);
     if (rc != PPLB200_SUCCESS) {
@@ -779,7 +785,7 @@ int pplb200_attn_weight_workspace_size(const pplb200_attn_params* p, uint64_t* b
     if (!bytes) {
         return fail(PPLB200_NOT_FOUND, "bytes is null");
     }
-    WeightPlan plan;
+    WeightPlan plan = {};
     rc = make_weight_plan(*p, &plan);
     *bytes = plan.bytes;
     return rc;
@@ -811,7 +817,7 @@ int pplb200_attn_weight_accumulate(const pplb200_attn_params* p, const void* que
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    WeightPlan plan;
+    WeightPlan plan = {};
     rc = make_weight_plan(*p, &plan);
     if (rc != PPLB200_SUCCESS) {
         return rc;
@@ -902,7 +908,7 @@ static int validate_compact(const pplb200_attn_params* p, int64_t kept_heads, in
 
 int pplb200_kv_compact_workspace_size(const pplb200_attn_params* p, int64_t kept_heads, int64_t max_kept,
                                       int64_t layers, uint64_t* bytes) {
-    CompactPlan plan;
+    CompactPlan plan = {};
     const int rc = validate_compact(p, kept_heads, max_kept, layers, &plan);
     if (rc != PPLB200_SUCCESS) {
         return rc;
@@ -918,7 +924,7 @@ int pplb200_kv_compact(const pplb200_attn_params* p, const int64_t* kept, int64_
                        const int64_t* base, const int64_t* kvlens, const int64_t* cachestarts, int64_t layers,
                        void* cache, void* scale, float* weight, void* workspace, uint64_t workspace_bytes,
                        void* stream_v) {
-    CompactPlan plan;
+    CompactPlan plan = {};
     int rc = validate_compact(p, kept_heads, max_kept, layers, &plan);
     if (rc != PPLB200_SUCCESS) {
         return rc;

@@ -835,6 +835,10 @@ int make_compact_plan(const pplb200_attn_params& p, int64_t kept_heads, int64_t 
     plan->rows_per_seg = kSegmentRows / plan->heads_per_cta;
     plan->lists = p.batch * layers * (p.num_kv_heads / plan->heads_per_cta);
     plan->segments = (max_kept + plan->rows_per_seg - 1) / plan->rows_per_seg;
+    plan->bytes = 0;
+    if (plan->lists > 0x7fffffff) {
+        return PPLB200_UNSUPPORTED;
+    }
     plan->off_flags = 256;  // behind the status word and the ticket counter
     plan->bytes = plan->off_flags + (static_cast<uint64_t>(plan->segments) * plan->lists * 4 + 255) / 256 * 256;
     const int64_t clears = (p.max_kvlen + kClearRows - 1) / kClearRows;

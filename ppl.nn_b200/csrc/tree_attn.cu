@@ -867,8 +867,10 @@ int make_tree_plan(const pplb200_attn_params& p, int sm_count, TreePlan* plan) {
     // no more ranges than there can be work for
     const int64_t row_tiles = (p.max_seqlen * (p.num_heads / p.num_kv_heads) + tile_rows - 1) / tile_rows;
     const int64_t blocks = (p.max_kvlen + kBlockN - 1) / kBlockN;
-    const int64_t most = (p.batch * (p.num_kv_heads / plan->lanes) * row_tiles * blocks + kMinRange - 1) / kMinRange;
-    plan->ranges = most > resident / plan->lanes ? resident / plan->lanes : most;
+    // (in floating point: the product of the largest sizes does not fit 64 bits)
+    const double units = static_cast<double>(p.batch) * (p.num_kv_heads / plan->lanes) * row_tiles * blocks;
+    const int64_t places = resident / plan->lanes;
+    plan->ranges = units > static_cast<double>(places) * kMinRange ? places : (static_cast<int64_t>(units) + kMinRange - 1) / kMinRange;
     plan->words = (p.max_seqlen + 63) / 64;
     const uint64_t slot_rows = static_cast<uint64_t>(plan->ranges) * plan->lanes * 2 * tile_rows;
     plan->off_prefix = 256;

@@ -438,6 +438,8 @@ class _CacheOp(_Base):
         a = self.param
         if cachestarts.dim() != 1 + (a.cache_mode == 1) or cachestarts.shape[0] != batch:
             raise OpError("RC_INVALID_VALUE", "cachestarts must have an entry (cache_mode 1: a row) per sequence")
+        if getattr(a, "num_repeat", 1) != 1:
+            raise OpError("RC_UNSUPPORTED", "currently only support num_repeat == 1")
         stride_b = cachestarts.shape[1] if a.cache_mode == 1 else 0
         p = capi.AttnParams(num_heads, num_kv_heads, head_dim, int(is_causal), a.num_layer, a.layer_idx, a.quant_bit,
                             a.quant_group, a.cache_mode, a.cache_layout, a.page_size, 0, 0, 0, batch, 0,
@@ -461,13 +463,16 @@ class _CacheOp(_Base):
         return device, self._params(a.num_heads, heads, dim, batch, max_kvlen, rows, cachestarts, max_seqlen,
                                     query.shape[0], a.is_causal)
 
-    def _call(self, name, size_fn, fn, p, device: int, *args) -> None:
-        """Runs fn(p, *args, workspace, bytes, stream) on the tensors' device and its current stream."""
+    def _call(self, name, size_fn, fn, p, device: int, empty: bool, *args) -> None:
+        """Runs fn(p, *args, workspace, bytes, stream) on the tensors' device and its current stream.  A call without
+        anything to do launches nothing and leaves no status word."""
         if device != torch._C._cuda_getDevice():
             with torch.cuda.device(device):
-                return self._call(name, size_fn, fn, p, device, *args)
+                return self._call(name, size_fn, fn, p, device, empty, *args)
         rc, nbytes = size_fn(p)
-        if rc == capi.SUCCESS:
+        if empty and rc == capi.SUCCESS:
+            self._workspace = None
+        elif rc == capi.SUCCESS:
             self._workspace = ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
             # the current stream's handle; a Stream object around it costs 5 us, a fifth of a small call
             rc = fn(p, *args, ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(device))
@@ -505,7 +510,7 @@ class TreeAttention(_CacheOp):
             if attn_output.shape != query.shape:
                 raise OpError("RC_INVALID_VALUE", "attn_output must be like query")
         self._call("pplb200_tree_attn_forward", self.lib.tree_attn_workspace_size, self.lib.tree_attn_forward, p, device,
-                   _ptr(query), _ptr(parents), _ptr(seqstarts), _ptr(cachestarts), _ptr(start_pos), _ptr(cache),
+                   p.batch == 0 or p.total_tokens == 0, _ptr(query), _ptr(parents), _ptr(seqstarts), _ptr(cachestarts), _ptr(start_pos), _ptr(cache),
                    _ptr(scale), _ptr(attn_output))
         return attn_output
 
@@ -523,7 +528,7 @@ class AttentionWeight(_CacheOp):
         device, p = self._query_params(query, seqstarts, cachestarts, start_pos, max_seqlen, max_kvlen, cache, scale)
         self._check_weight(device, weight, p.num_kv_heads, p.max_tokens)
         self._call("pplb200_attn_weight_accumulate", self.lib.attn_weight_workspace_size, self.lib.attn_weight_accumulate,
-                   p, device, _ptr(query), _ptr(seqstarts), _ptr(cachestarts), _ptr(start_pos), _ptr(cache), _ptr(scale),
+                   p, device, p.batch == 0 or p.total_tokens == 0, _ptr(query), _ptr(seqstarts), _ptr(cachestarts), _ptr(start_pos), _ptr(cache), _ptr(scale),
                    _ptr(weight))
         return weight
 
@@ -564,7 +569,7 @@ class KeyValueCacheEvict(_CacheOp):
         # the choice does not depend on the head size; any supported one describes the rows
         p = self._params(heads, heads, 128, batch, max_kvlen, rows, cachestarts)
         self._call("pplb200_kv_evict_select", self.lib.kv_evict_workspace_size, self.lib.kv_evict_select, p, device,
-                   _ptr(weight), _ptr(cachestarts), _ptr(kvlens), _ptr(budgets), a.sink, a.recent, max_budget, _ptr(kept))
+                   batch == 0 or max_budget == 0, _ptr(weight), _ptr(cachestarts), _ptr(kvlens), _ptr(budgets), a.sink, a.recent, max_budget, _ptr(kept))
         return kept
 
 
@@ -589,5 +594,5 @@ class KeyValueCacheCompact(_CacheOp):
         p = self._params(heads, heads, dim, batch, max_kvlen, rows, cachestarts)
         _, kept_heads, most = kept.shape
         self._call("pplb200_kv_compact", lambda q: self.lib.kv_compact_workspace_size(q, kept_heads, most, num_layers),
-                   self.lib.kv_compact, p, device, _ptr(kept), kept_heads, most, _ptr(base), _ptr(kvlens),
+                   self.lib.kv_compact, p, device, batch == 0 or (most == 0 and weight is None), _ptr(kept), kept_heads, most, _ptr(base), _ptr(kvlens),
                    _ptr(cachestarts), num_layers, _ptr(cache), _ptr(scale), _ptr(weight))

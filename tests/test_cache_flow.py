@@ -3,7 +3,7 @@ long caches -- and the forms of each that its own tests leave out."""
 import numpy as np
 import pytest
 
-from test_cache_ops import HostCache, dev, gpu, starts_of, weight_reference  # noqa: F401  (gpu is a fixture)
+from test_cache_ops import HostCache, _params, _weight_call, dev, gpu, starts_of, weight_reference  # noqa: F401  (gpu is a fixture)
 from test_tree_attention import draw_parents, run_tree, tree_reference
 
 I64 = np.int64
@@ -36,6 +36,48 @@ def test_host_tensors_are_refused(pkg, built_lib):
                      torch.zeros(2, 2, 4, dtype=torch.int64), one, one, one, 9, cache, scale)):
         with pytest.raises(ops.OpError):
             call()
+
+
+def test_sizes_that_would_wrap_around_are_refused(pkg, built_lib):
+    from ppl_nn_b200 import capi
+    most = dict(num_heads=65535, num_kv_heads=65535, batch=65535, max_tokens=0x7fffffff, total_tokens=0x7fffffff)
+    p = _params(built_lib, capi, **most, max_kvlen=1 << 27, max_seqlen=1)
+    assert built_lib.status_str(built_lib.attn_weight_workspace_size(p)[0]) == "RC_UNSUPPORTED"
+    assert built_lib.status_str(built_lib.kv_compact_workspace_size(p, 65535, 1 << 30, 1)[0]) == "RC_UNSUPPORTED"
+    for longest in (1 << 31, 1 << 62):  # times the group of four: 2^64
+        p = _params(built_lib, capi, max_seqlen=longest)
+        assert built_lib.status_str(built_lib.attn_weight_workspace_size(p)[0]) == "RC_UNSUPPORTED"
+        assert built_lib.status_str(_weight_call(built_lib, p)) == "RC_UNSUPPORTED"
+    # the tree's work is cut into as many parts as there are places, however much it is
+    p = _params(built_lib, capi, **most, max_kvlen=0x7fff0000, max_seqlen=1024)
+    rc, n = built_lib.tree_attn_workspace_size(p)
+    assert rc == capi.SUCCESS and n > 0x7fffffff * 16 * 8
+
+
+@pytest.mark.gpu
+def test_calls_without_work_leave_no_status(gpu, pkg):  # noqa: F811
+    import torch
+    from ppl_nn_b200 import ops
+    hc = HostCache(np.random.default_rng(0), [5, 9], 2, 64)
+    cache, scale, weight, none = dev(hc.cache), dev(hc.scale), dev(hc.weight), i64([])
+    q = torch.zeros(0, 4, 64, dtype=torch.float16, device=gpu)
+    p = attention_param(hc, 4)
+    tree, weigh = ops.TreeAttention(p), ops.AttentionWeight(p)
+    evict = ops.KeyValueCacheEvict(ops.KeyValueCacheEvictParam(**hc.param()))
+    compact = ops.KeyValueCacheCompact(ops.KeyValueCacheParam(**hc.param()))
+    junk = torch.full((1 << 16,), 255, dtype=torch.uint8, device=gpu)  # what a new workspace would hold
+    del junk
+    tree.forward(q, None, i64([0]), none, none, 0, 0, cache, scale)
+    weigh.forward(q, i64([0]), none, none, 0, 0, cache, scale, weight)
+    tree.forward(q, None, i64([0, 0, 0]), dev(hc.starts), i64([5, 9]), 0, 9, cache, scale)
+    assert evict.forward(weight, none, none, none, 0, 4).shape == (0, 2, 4)
+    assert evict.forward(weight, dev(hc.starts), i64([5, 9]), i64([0, 0]), 9, 0).shape == (2, 2, 0)
+    compact.forward(i64(np.zeros((2, 1, 0))), dev(hc.starts), i64([0, 0]), i64([5, 9]), 9, cache, scale)
+    assert [o.device_status() for o in (tree, weigh, evict, compact)] == [0] * 4
+    assert np.array_equal(weight.cpu().numpy(), hc.weight) and np.array_equal(cache.cpu().numpy(), hc.cache)
+    with pytest.raises(ops.OpError):
+        ops.KeyValueCacheCompact(ops.KeyValueCacheParam(**hc.param(), num_repeat=2)).forward(
+            i64(np.zeros((2, 1, 1))), dev(hc.starts), i64([0, 0]), i64([5, 9]), 9, cache, scale)
 
 
 @pytest.mark.gpu
@@ -80,6 +122,9 @@ def test_wrong_types_and_shapes_are_refused(gpu, pkg):  # noqa: F811
         for op in which.split():
             with pytest.raises(ops.OpError):
                 calls(dict(good, **{name: bad}))[op]()
+    with pytest.raises(ops.OpError):  # other parts of the call still read the query
+        tree.forward(good["q"], None, good["seq"], good["cs"], good["start"], 1, 9, good["cache"], good["scale"],
+                     attn_output=good["q"])
     if torch.cuda.device_count() > 1:
         with pytest.raises(ops.OpError):
             calls(dict(good, cs=good["cs"].to("cuda:1")))["tree"]()
