@@ -21,7 +21,7 @@ struct WeightArgs {
     float* weight;   // [L, Hkv, MaxT]
     float2* part;    // [chunks][T][Hq]: maximum (exp2 domain) and sum
     float2* norm;    // [T][Hq]: maximum and reciprocal sum
-    float* score;    // [batch][Hkv][max_kvlen][kScoreRows or fewer]: raw scores, -inf where hidden, or null
+    float* score;    // [batch][Hkv][max_kvlen][score_rows]: raw scores, -inf where hidden; up to kScoreRows rows
     int32_t score_rows;
     uint32_t* status;
     CacheGeom geom;

@@ -138,7 +138,7 @@ int launch_tree_attn(const pplb200_attn_params& p, const CacheGeom& geom, const 
 struct WeightPlan {
     int32_t chunk;   // positions of a chunk
     int64_t chunks;  // chunks per sequence
-    int32_t score_rows;  // query rows per kv head
+    int32_t score_rows;  // kept scores of a position: the query rows per kv head, above 2 a multiple of 4
     uint64_t off_norm, off_part, off_score, bytes;
 };
 int make_weight_plan(const pplb200_attn_params& p, WeightPlan* plan);

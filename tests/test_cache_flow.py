@@ -511,6 +511,33 @@ def test_weights_of_sequences_that_share_rows_add_up(gpu, pkg):  # noqa: F811
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [[3, 1], [40, 9]])
+def test_tokens_behind_the_last_sequence_are_padding(gpu, pkg, n):  # noqa: F811
+    """A padded batch: queries behind seqstarts[-1] are not read, their outputs stay as they were."""
+    import torch
+    from ppl_nn_b200 import ops
+    rng = np.random.default_rng(n[0])
+    start = [130, 7]
+    hc = HostCache(rng, [s + m for s, m in zip(start, n)], 2, 64)
+    q = rng.standard_normal((sum(n) + 5, 8, 64)).astype(np.float16)
+    q[sum(n):] = np.nan
+    args = (dev(q), dev(starts_of(n)), dev(hc.starts), i64(start), max(n), hc.max_len, dev(hc.cache), dev(hc.scale))
+    parents = sum([draw_parents(rng, m, "tree") for m in n], [])
+    want, tol = tree_reference(hc, q[:sum(n)], parents, start, n, 8, 0)
+    out = torch.full(q.shape, 7.0, dtype=torch.float16, device=gpu)
+    tree = ops.TreeAttention(attention_param(hc, 8))
+    tree.forward(args[0], i64(parents + [99] * 5), *args[1:], attn_output=out)
+    assert tree.device_status() == 0
+    got = out.cpu().numpy()
+    assert np.all(np.abs(got[:sum(n)] - want) <= tol) and (got[sum(n):] == 7).all()
+    want, tol = weight_reference(hc, q[:sum(n)], start, n, 8, 0, True)
+    weight = dev(hc.weight)
+    weigh = ops.AttentionWeight(attention_param(hc, 8))
+    weigh.forward(*args, weight)
+    assert weigh.device_status() == 0 and np.all(np.abs(weight.cpu().numpy() - want) <= tol)
+
+
+@pytest.mark.gpu
 def test_the_largest_tree(gpu, pkg):  # noqa: F811
     rng = np.random.default_rng(5)
     start, n = [70, 3], [1024, 129]
