@@ -131,10 +131,11 @@ __device__ __forceinline__ void load_rows(void* dst, const CUtensorMap* map, uin
     tma_load_5d(dst, map, bar, 0, c[0], c[1], c[2], c[3]);
 }
 
-// A thread is done reading a raw slot.  The loads have to be over before the slot is handed back, and the arrival alone
-// does not see to that: scale loads were found behind it, next to their use, when the next copy had overwritten them.
+// A thread is done reading a raw slot, which the next tensor copy overwrites through the asynchronous proxy.  The loads
+// have to be over before: the arrival alone, and the arrival behind a fence of the CTA's ordinary accesses, let copies
+// overtake loads (seen as wrong scores in up to half of the runs of a busy kernel), the proxy fence does not.
 __device__ __forceinline__ void hand_back(uint64_t* bar) {
-    __threadfence_block();
+    fence_proxy_async_smem();
     mbar_arrive(bar);
 }
 
