@@ -241,14 +241,12 @@ attn_window_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_con
             }
             Raw<DH> raw;
             raw.load(raw0 + rs * T::kRawBytes, row, piece, s.len - (first + n % blocks * kBlockN));
-            hand_back(&bars.raw_empty[rs]);
             if (n >= kTileStages && !wait_or_abort(&bars.k_empty[st], ((n / kTileStages) - 1) & 1, abort_flag, a.status, kDevMmaTimeout)) {
                 break;
             }
             const uint32_t tile = tiles + st * 2 * T::kTileBytes;
             raw.store_split(tile, tile + T::kTileBytes, row, piece);
-            fence_proxy_async_smem();
-            mbar_arrive(&bars.k_full[st]);
+            hand_over(&bars.k_full[st], &bars.raw_empty[rs]);
         }
     } else {
         // =========================== softmax ===========================

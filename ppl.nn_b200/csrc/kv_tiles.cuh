@@ -131,12 +131,14 @@ __device__ __forceinline__ void load_rows(void* dst, const CUtensorMap* map, uin
     tma_load_5d(dst, map, bar, 0, c[0], c[1], c[2], c[3]);
 }
 
-// A thread is done reading a raw slot, which the next tensor copy overwrites through the asynchronous proxy.  The loads
-// have to be over before: the arrival alone, and the arrival behind a fence of the CTA's ordinary accesses, let copies
-// overtake loads (seen as wrong scores in up to half of the runs of a busy kernel), the proxy fence does not.
-__device__ __forceinline__ void hand_back(uint64_t* bar) {
+// A thread has stored its share of the operand tiles at `full` and is done with the raw slot of `empty`.  The proxy fence
+// orders both for what comes next: the stores ahead of the MMAs that read the tiles, and the loads from the slot ahead of
+// the tensor copy that overwrites it.  (An arrival behind a fence of ordinary accesses alone lets such a copy overtake the
+// loads: seen as wrong scores in up to half of the runs of a busy kernel.)
+__device__ __forceinline__ void hand_over(uint64_t* full, uint64_t* empty) {
     fence_proxy_async_smem();
-    mbar_arrive(bar);
+    mbar_arrive(empty);
+    mbar_arrive(full);
 }
 
 }  // namespace pplb200

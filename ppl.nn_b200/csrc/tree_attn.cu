@@ -15,25 +15,26 @@
 //   * tree_plan_kernel turns the device-side lengths into the prefix sum of blocks, and the parents into one bit mask
 //     of ancestors per token.  Only blocks that reach behind the history look at the masks, 64 bits a row and block.
 //   * Roles of a CTA: 4 MT softmax warps, one thread per query row; four converter warps, which turn the raw codes and
-//     scales of a block into the swizzled fp16 K and V tiles; MT warps that issue the MMAs of a 128-row tile each; one
-//     warp that fetches the raw blocks by TMA into a ring of two, K and V apart.  S = Q K^T goes to a 64-column TMEM
+//     scales of a block into the swizzled fp16 tiles of K, its remainders and V; MT warps that issue the MMAs of a 128-row
+//     tile each; one warp that fetches the raw blocks by TMA into a ring of three (MT = 1) or four, in the converters'
+//     order.  S = Q K^T goes to a 64-column TMEM
 //     buffer, P returns to TMEM as the A operand of O += P V (two buffers), as in the prefill kernel.
 //   * MT = 1: two CTAs per SM.  MT = 2, for more than 128 rows per kv head: one CTA per SM, whose two tiles share the
 //     fetched and converted K and V.
 //
-// Roundings: keys, weights and values enter the tensor cores as fp16 (code * scale rounded once, as in the prefill
-// kernel); scores, maxima, sums and outputs are held in fp32.  The keys' rounding dominates: 7e-4 to 1.2e-3 of the
-// output's magnitude against 2e-4 for exact keys and the same fp16 output.  Exact keys (a second tile of remainders, as
-// attn_window.cu has it) would need 16 KB more of shared memory than two CTAs per SM leave, and half as much again of
-// the converters' work, which is what the kernel waits for.
+// Roundings: a key rounded to fp16 costs 1e-3 of the output's magnitude where keys have outlying channels, and 3e-3 where
+// several positions compete for a row (against 2e-4 for the fp16 output itself), so K is split into fp16(k) and the exact
+// remainder, two tiles whose products with Q meet in one accumulator.  Weights and values are rounded to fp16, by 2^-12 of
+// each and independently, which averages out; scores, maxima, sums and outputs are held in fp32.
 //
-// Measured (8 kv heads of 128): 32 sequences of 256 to 8192 positions, 4 to 64 rows per kv head, 392 MB of cache: 145 us,
-// 163 us with plan and merge (2.4 TB/s); 64 such sequences, 200 to 264 rows: 445 us, 514 us in all (530 TFLOP/s); 4 of up
-// to 131072, paged, 228 to 256 rows: 470 us, 549 us in all (710 TFLOP/s).  What bounds it: a block takes a CTA 3300 cycles
-// at MT = 1, of which the converters work 2600 and wait 700; the MMA warp waits 1050 of them for converted tiles, the
-// tensor pipe is busy 31 % and DRAM 36 %.  More converter warps do not pay at 96 registers a thread (spills), with
-// converters apart for K and V and double-buffered scores the three cases take 177, 565 and 574 us.  MT = 2 against
-// MT = 1 for 256 rows: K and V are fetched and converted once for both tiles.
+// Measured (8 kv heads of 128): 32 sequences of 256 to 8192 positions, 4 to 64 rows per kv head, 392 MB of cache: 164 us,
+// with rounded keys 145; 64 such sequences, 200 to 264 rows: 537 us (445); 4 of up to 131072, paged, 228 to 256 rows: 620
+// us (470).  What bounds it: the converters, the MMAs' reads of shared memory and the softmax are about as long as one
+// another (at MT = 1 and with rounded keys a block took a CTA 3300 cycles, of which the converters worked 2600, the MMA
+// warp waited 1050 for tiles and the softmax 790 for scores; tensor pipe 31 %, DRAM 36 %).  More converter warps do not
+// pay at 96 registers a thread: with converters apart for K and V and double-buffered scores the three cases took 177, 565
+// and 574 us in all against 163, 515 and 549.  MT = 2 against MT = 1 for 256 rows: K and V are fetched and converted once
+// for both tiles.
 //
 // Waits on mbarriers are bounded and give up together (see tcgen05.cuh).
 #include <cub/block/block_scan.cuh>
@@ -51,7 +52,6 @@ namespace {
 
 constexpr int kTileM = 128;  // rows of an MMA
 constexpr int kBlockN = kTileRows;  // positions of a block
-constexpr int kRawStages = 2;
 constexpr int kMinRange = 4;  // blocks: no range is cut finer
 constexpr float kNegBig = -1.0e30f;
 constexpr float kRescaleSlack = 8.0f;
@@ -69,9 +69,10 @@ struct TTraits {
     static constexpr int kKVBytes = kColBlocks * kKVBlockBytes;
     static constexpr int kCodeBytes = kBlockN * DH;
     static constexpr int kRawBytes = kCodeBytes + kBlockN * (DH / 8) * 2;  // codes and scales of K or V of a block
+    static constexpr int kRawSlots = MT == 1 ? 3 : 4;  // what fits beside a second CTA, or more
     // The same for every head size, so that never more CTAs share an SM than its TMEM holds; MT = 2 asks for more
     // than half of the SM's.
-    static constexpr int kSmemBytes = MT * 32768 + 2 * (kBlockN * 256) + 2 * kRawStages * (kBlockN * 160) + 512;
+    static constexpr int kSmemBytes = MT * 32768 + 3 * (kBlockN * 256) + kRawSlots * (kBlockN * 160) + 512;
     static constexpr uint32_t kPCols = kBlockN / 2;
     static constexpr uint32_t kColS = 0, kColP = kBlockN, kColO = kColP + 2 * kPCols;
     static constexpr uint32_t kTileCols = 256;  // TMEM columns of a tile: S 64 | P 2 x 32 | O 128
@@ -244,7 +245,7 @@ __device__ __forceinline__ void piece_at(const TreeArgs& a, int64_t u, int64_t e
 template <int MT>
 struct Barriers {
     uint64_t q_full, q_empty;
-    uint64_t raw_full[2][kRawStages], raw_empty[2][kRawStages];  // [K | V]
+    uint64_t raw_full[4], raw_empty[4];
     uint64_t k_full, k_empty, v_full, v_empty;
     uint64_t o_free[MT], s_full[MT], s_free[MT];
     uint64_t p_full[MT][2], pv_done[MT][2];
@@ -260,9 +261,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sQ = smem;
     uint8_t* sK = sQ + MT * T::kQBytes;
-    uint8_t* sV = sK + T::kKVBytes;
-    uint8_t* sRaw = sV + T::kKVBytes;  // [stage][K | V]
-    Barriers<MT>& bars = *reinterpret_cast<Barriers<MT>*>(sRaw + 2 * kRawStages * T::kRawBytes);
+    uint8_t* sV = sK + 2 * T::kKVBytes;  // K: keys, then their remainders
+    uint8_t* sRaw = sV + T::kKVBytes;    // a ring of raw K and V blocks
+    Barriers<MT>& bars = *reinterpret_cast<Barriers<MT>*>(sRaw + T::kRawSlots * T::kRawBytes);
     volatile int* abort_flag = &bars.abort_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t* status = &a.hdr->status;
@@ -293,11 +294,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
         bars.abort_word = 0;
         mbar_init(&bars.q_full, 128);
         mbar_init(&bars.q_empty, MT);
-        for (int s = 0; s < kRawStages; ++s) {
-            for (int kv = 0; kv < 2; ++kv) {
-                mbar_init(&bars.raw_full[kv][s], 1);
-                mbar_init(&bars.raw_empty[kv][s], 128);
-            }
+        for (int s = 0; s < T::kRawSlots; ++s) {
+            mbar_init(&bars.raw_full[s], 1);
+            mbar_init(&bars.raw_empty[s], 128);
         }
         mbar_init(&bars.k_full, 128);
         mbar_init(&bars.v_full, 128);
@@ -328,13 +327,17 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
     if (warp == T::kLoadWarp) {
         // =========================== TMA producer ===========================
         bool ok = true;
-        int n = 0;  // blocks requested so far
+        int n = 0;  // raw blocks requested so far
         for (int64_t u = begin; ok && u < end;) {
             Piece p;
             piece_at(a, u, end, lane_class, lane, p);
-            const int boxes = kBlockN / a.box_rows;
-            for (int32_t blk = p.blk0; ok && blk < p.blk1; ++blk, ++n) {
-                const int s = n % kRawStages;
+            const int boxes = kBlockN / a.box_rows, blocks = p.blk1 - p.blk0;
+            u += blocks;
+            for (int i = 0; ok && i < 2 * blocks; ++i, ++n) {
+                // the converters' order: K(0) K(1) V(0) K(2) V(1) ..
+                const int kv = i == 2 * blocks - 1 || (i > 0 && (i & 1) == 0) ? 1 : 0;
+                const int32_t blk = p.blk0 + (kv == 0 ? (i + 1) / 2 : (i & 1) ? blocks - 1 : i / 2 - 1);
+                const int s = n % T::kRawSlots;
                 // lane i < boxes: cache row of the i-th copy; rows outside the cache are flagged and read as zeros
                 int row = static_cast<int>(a.max_tokens);
                 if (lane < boxes) {
@@ -350,36 +353,30 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                         }
                     }
                 }
-                for (int kv = 0; ok && kv < 2; ++kv) {
-                    if (n >= kRawStages) {
-                        ok = wait_or_abort_parked(&bars.raw_empty[kv][s], ((n / kRawStages) - 1) & 1, abort_flag, status,
-                                                  kDevMmaTimeout);
-                        if (!ok) {
-                            break;
-                        }
+                if (n >= T::kRawSlots) {
+                    ok = wait_or_abort_parked(&bars.raw_empty[s], ((n / T::kRawSlots) - 1) & 1, abort_flag, status, kDevMmaTimeout);
+                    if (!ok) {
+                        break;
                     }
-                    uint8_t* dst = sRaw + (2 * s + kv) * T::kRawBytes;
-                    uint64_t* bar = &bars.raw_full[kv][s];
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(bar, T::kRawBytes);
-                    }
-                    __syncwarp();
-                    if (lane < boxes) {
-                        load_rows(dst + lane * a.box_rows * DH, &tm_code, bar, a.order, row, p.kvh, kv, a.geom.layer_idx);
-                        load_rows(dst + T::kCodeBytes + lane * a.box_rows * (DH / 4), &tm_scale, bar, a.order, row, p.kvh, kv, a.geom.layer_idx);
-                    }
-                    __syncwarp();
                 }
+                uint8_t* dst = sRaw + s * T::kRawBytes;
+                uint64_t* bar = &bars.raw_full[s];
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(bar, T::kRawBytes);
+                }
+                __syncwarp();
+                if (lane < boxes) {
+                    load_rows(dst + lane * a.box_rows * DH, &tm_code, bar, a.order, row, p.kvh, kv, a.geom.layer_idx);
+                    load_rows(dst + T::kCodeBytes + lane * a.box_rows * (DH / 4), &tm_scale, bar, a.order, row, p.kvh, kv, a.geom.layer_idx);
+                }
+                __syncwarp();
             }
-            u += p.blk1 - p.blk0;
         }
         if (*abort_flag) {
-            // every copy this warp issued must have landed before the CTA may exit; a stage whose copies were issued
-            // is complete at the latest parity it was armed with (a stage that was never armed is left alone)
-            for (int j = n > kRawStages ? n - kRawStages : 0; j < n; ++j) {
-                for (int kv = 0; kv < 2; ++kv) {
-                    mbar_wait_bounded(&bars.raw_full[kv][j % kRawStages], (j / kRawStages) & 1);
-                }
+            // every copy this warp issued must have landed before the CTA may exit; a slot whose copies were issued
+            // is complete at the latest parity it was armed with (a slot that was never armed is left alone)
+            for (int j = n > T::kRawSlots ? n - T::kRawSlots : 0; j < n; ++j) {
+                mbar_wait_bounded(&bars.raw_full[j % T::kRawSlots], (j / T::kRawSlots) & 1);
             }
         }
     } else if (warp >= T::kMmaWarp) {
@@ -430,12 +427,15 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                     tc_fence_after();
                     if (elect_one()) {
 #pragma unroll
-                        for (int cb = 0; cb < T::kColBlocks; ++cb) {
+                        for (int part = 1; part >= 0; --part) {  // the remainders' products first, the large ones on top
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                tc_mma_f16(d_s, desc_join(q_lo + cb * (T::kQBlockBytes >> 4) + 2 * k, hi_sw128),
-                                           desc_join(k_lo + cb * (T::kKVBlockBytes >> 4) + 2 * k, hi_sw128), idesc_qk,
-                                           (cb | k) ? 1u : 0u);
+                            for (int cb = 0; cb < T::kColBlocks; ++cb) {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    tc_mma_f16(d_s, desc_join(q_lo + cb * (T::kQBlockBytes >> 4) + 2 * k, hi_sw128),
+                                               desc_join(k_lo + (part * T::kKVBytes + cb * T::kKVBlockBytes) / 16 + 2 * k, hi_sw128),
+                                               idesc_qk, (part == 0 || (cb | k)) ? 1u : 0u);
+                                }
                             }
                         }
                         tc_commit(&bars.s_full[t]);
@@ -482,23 +482,26 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
         const int row = (warp - T::kConvWarp) * 16 + lane / kPieces;  // first of the thread's rows of a block
         const uint32_t k_tile = smem_u32(sK), v_tile = smem_u32(sV), raw0 = smem_u32(sRaw), q_tile = smem_u32(sQ);
         bool ok = true;
-        int pieces = 0, n = 0;  // pieces and blocks so far
-        // K (0) or V (1) of the CTA's block number `blk_no`, of which `rows` rows exist
+        int pieces = 0, n = 0, taken = 0;  // pieces, blocks and raw blocks so far
+        // K (0) or V (1) of the CTA's block number `blk_no`, of which `rows` rows exist: the next one of the ring
         auto convert = [&](int kv, int blk_no, int32_t rows) -> bool {
-            const int s = blk_no % kRawStages;
-            if (!wait_or_abort(&bars.raw_full[kv][s], (blk_no / kRawStages) & 1, abort_flag, status, kDevTmaTimeout)) {
+            const int s = taken % T::kRawSlots;
+            if (!wait_or_abort(&bars.raw_full[s], (taken / T::kRawSlots) & 1, abort_flag, status, kDevTmaTimeout)) {
                 return false;
             }
+            ++taken;
             Raw<DH> raw;
-            raw.load(raw0 + (2 * s + kv) * T::kRawBytes, row, piece, rows);
-            hand_back(&bars.raw_empty[kv][s]);
+            raw.load(raw0 + s * T::kRawBytes, row, piece, rows);
             if (blk_no > 0 && !wait_or_abort(kv ? &bars.v_empty : &bars.k_empty, (blk_no - 1) & 1, abort_flag, status,
                                              kDevMmaTimeout)) {
                 return false;
             }
-            raw.store(kv ? v_tile : k_tile, row, piece);
-            fence_proxy_async_smem();
-            mbar_arrive(kv ? &bars.v_full : &bars.k_full);
+            if (kv) {
+                raw.store(v_tile, row, piece);
+            } else {
+                raw.store_split(k_tile, k_tile + T::kKVBytes, row, piece);
+            }
+            hand_over(kv ? &bars.v_full : &bars.k_full, &bars.raw_empty[s]);
             return true;
         };
         for (int64_t u = begin; ok && u < end; ++pieces) {

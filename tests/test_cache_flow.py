@@ -511,6 +511,40 @@ def test_weights_of_sequences_that_share_rows_add_up(gpu, pkg):  # noqa: F811
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,dim,n", [(8, 2, 128, [3, 12]), (8, 2, 64, [5, 1]), (8, 1, 128, [40, 9]), (16, 1, 64, [17, 30])])
+def test_keys_of_a_tree_are_not_rounded(gpu, pkg, heads, kv_heads, dim, n):  # noqa: F811
+    """One group of channels whose keys are 40 times the others', as after outlying activations: scores of tens, which a
+    rounding of the keys to fp16 would move by hundredths.
+
+    A score is a sum of 2 Dh exact products in fp32: Dh / 8 tensor-core instructions, each off by at most 2^-22 of the
+    products' magnitudes; that is an error of the exponent, of a weight and of the normaliser.  Weights, values and the
+    output are rounded to fp16 (2^-11), weights below its normal range by 2^-25 of the largest; 2^-16 covers the
+    exponentials and the sums."""
+    rng = np.random.default_rng(dim + n[0])
+    start, u = [700, 90], 2.0 ** -11
+    hc = HostCache(rng, [s + m for s, m in zip(start, n)], kv_heads, dim)
+    hc.scale[:, :, 0, :, 3] = (hc.scale[:, :, 0, :, 3].astype(np.float32) * 40).astype(np.float16)
+    q = rng.standard_normal((sum(n), heads, dim)).astype(np.float16)
+    parents = sum([draw_parents(rng, m, "tree") for m in n], [])
+    want, _ = tree_reference(hc, q, parents, start, n, heads, 0)
+    tol, first, group = np.zeros(q.shape), 0, heads // kv_heads
+    for b, m in enumerate(n):
+        rows = hc.rows(b, np.arange(start[b] + m))
+        for g in range(kv_heads):
+            k, v = hc.values(0, 0, g, rows), hc.values(1, 0, g, rows)
+            for i in range(first, first + m):
+                for h in range(g * group, (g + 1) * group):
+                    x = q[i, h].astype(np.float64)
+                    off = (dim / 8) * 2.0 ** -22 * (np.abs(k) @ np.abs(x)).max() / np.sqrt(dim)
+                    tol[i, h] = (np.abs(v).max(0) * (2 * off + 2 * u + 2.0 ** -16) + u * np.abs(want[i, h])
+                                 + 2 * len(k) * 2.0 ** -25 * np.abs(v).max())
+        first += m
+    got, status = run_tree(hc, q, parents, start, n, heads, 0)
+    assert status == 0
+    assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [[3, 1], [40, 9]])
 def test_tokens_behind_the_last_sequence_are_padding(gpu, pkg, n):  # noqa: F811
     """A padded batch: queries behind seqstarts[-1] are not read, their outputs stay as they were."""
