@@ -27,14 +27,14 @@
 // remainder, two tiles whose products with Q meet in one accumulator.  Weights and values are rounded to fp16, by 2^-12 of
 // each and independently, which averages out; scores, maxima, sums and outputs are held in fp32.
 //
-// Measured (8 kv heads of 128): 32 sequences of 256 to 8192 positions, 4 to 64 rows per kv head, 392 MB of cache: 164 us,
-// with rounded keys 145; 64 such sequences, 200 to 264 rows: 537 us (445); 4 of up to 131072, paged, 228 to 256 rows: 620
-// us (470).  What bounds it: the converters, the MMAs' reads of shared memory and the softmax are about as long as one
+// Measured (8 kv heads of 128), main kernel and whole call: 32 sequences of 256 to 8192 positions, 4 to 64 rows per kv
+// head, 392 MB of cache: 165 and 198 us (with rounded keys 145 and 163); 64 such sequences, 200 to 264 rows: 508 and 602
+// us (445 and 515), 537 and 637 with one stage of tiles; 4 of up to 131072, paged, 228 to 256 rows: 650 and 712 us (470
+// and 549).  What bounds it: the converters, the MMAs' reads of shared memory and the softmax are about as long as one
 // another (at MT = 1 and with rounded keys a block took a CTA 3300 cycles, of which the converters worked 2600, the MMA
 // warp waited 1050 for tiles and the softmax 790 for scores; tensor pipe 31 %, DRAM 36 %).  More converter warps do not
-// pay at 96 registers a thread: with converters apart for K and V and double-buffered scores the three cases took 177, 565
-// and 574 us in all against 163, 515 and 549.  MT = 2 against MT = 1 for 256 rows: K and V are fetched and converted once
-// for both tiles.
+// pay at 96 registers a thread: with rounded keys, converters apart for K and V and double-buffered scores the three calls
+// took 177, 565 and 574 us.  MT = 2 against MT = 1 for 256 rows: K and V are fetched and converted once for both tiles.
 //
 // Waits on mbarriers are bounded and give up together (see tcgen05.cuh).
 #include <cub/block/block_scan.cuh>
@@ -69,10 +69,11 @@ struct TTraits {
     static constexpr int kKVBytes = kColBlocks * kKVBlockBytes;
     static constexpr int kCodeBytes = kBlockN * DH;
     static constexpr int kRawBytes = kCodeBytes + kBlockN * (DH / 8) * 2;  // codes and scales of K or V of a block
-    static constexpr int kRawSlots = MT == 1 ? 3 : 4;  // what fits beside a second CTA, or more
+    static constexpr int kRawSlots = MT == 1 ? 3 : 4;    // what fits beside a second CTA, or more
+    static constexpr int kTileStages = MT == 1 ? 1 : 2;  // converted tiles of K (with remainders) and of V
     // The same for every head size, so that never more CTAs share an SM than its TMEM holds; MT = 2 asks for more
     // than half of the SM's.
-    static constexpr int kSmemBytes = MT * 32768 + 3 * (kBlockN * 256) + kRawSlots * (kBlockN * 160) + 512;
+    static constexpr int kSmemBytes = MT * 32768 + 3 * kTileStages * (kBlockN * 256) + kRawSlots * (kBlockN * 160) + 512;
     static constexpr uint32_t kPCols = kBlockN / 2;
     static constexpr uint32_t kColS = 0, kColP = kBlockN, kColO = kColP + 2 * kPCols;
     static constexpr uint32_t kTileCols = 256;  // TMEM columns of a tile: S 64 | P 2 x 32 | O 128
@@ -246,7 +247,7 @@ template <int MT>
 struct Barriers {
     uint64_t q_full, q_empty;
     uint64_t raw_full[4], raw_empty[4];
-    uint64_t k_full, k_empty, v_full, v_empty;
+    uint64_t k_full[MT], k_empty[MT], v_full[MT], v_empty[MT];  // MT stages
     uint64_t o_free[MT], s_full[MT], s_free[MT];
     uint64_t p_full[MT][2], pv_done[MT][2];
     uint32_t tmem_slot;
@@ -261,8 +262,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sQ = smem;
     uint8_t* sK = sQ + MT * T::kQBytes;
-    uint8_t* sV = sK + 2 * T::kKVBytes;  // K: keys, then their remainders
-    uint8_t* sRaw = sV + T::kKVBytes;    // a ring of raw K and V blocks
+    uint8_t* sV = sK + T::kTileStages * 2 * T::kKVBytes;  // K: keys, then their remainders
+    uint8_t* sRaw = sV + T::kTileStages * T::kKVBytes;    // a ring of raw K and V blocks
     Barriers<MT>& bars = *reinterpret_cast<Barriers<MT>*>(sRaw + T::kRawSlots * T::kRawBytes);
     volatile int* abort_flag = &bars.abort_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -298,10 +299,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
             mbar_init(&bars.raw_full[s], 1);
             mbar_init(&bars.raw_empty[s], 128);
         }
-        mbar_init(&bars.k_full, 128);
-        mbar_init(&bars.v_full, 128);
-        mbar_init(&bars.k_empty, MT);
-        mbar_init(&bars.v_empty, MT);
+        for (int s = 0; s < T::kTileStages; ++s) {
+            mbar_init(&bars.k_full[s], 128);
+            mbar_init(&bars.v_full[s], 128);
+            mbar_init(&bars.k_empty[s], MT);
+            mbar_init(&bars.v_empty[s], MT);
+        }
         for (int t = 0; t < MT; ++t) {
             mbar_init(&bars.o_free[t], 128);
             mbar_init(&bars.s_full[t], 1);
@@ -402,16 +405,17 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
             if (t * kTileM >= p.rows_valid) {
                 // no rows for this tile: only hand the operands back
                 for (int32_t j = 0; ok && j < blocks; ++j, ++blocks_done) {
-                    ok = wait_or_abort_parked(&bars.k_full, blocks_done & 1, abort_flag, status, kDevMmaTimeout);
+                    const int st = blocks_done % T::kTileStages, parity = (blocks_done / T::kTileStages) & 1;
+                    ok = wait_or_abort_parked(&bars.k_full[st], parity, abort_flag, status, kDevMmaTimeout);
                     if (ok && lane == 0) {
-                        mbar_arrive(&bars.k_empty);
+                        mbar_arrive(&bars.k_empty[st]);
                         if (j == blocks - 1) {
                             mbar_arrive(&bars.q_empty);
                         }
                     }
-                    ok = ok && wait_or_abort_parked(&bars.v_full, blocks_done & 1, abort_flag, status, kDevMmaTimeout);
+                    ok = ok && wait_or_abort_parked(&bars.v_full[st], parity, abort_flag, status, kDevMmaTimeout);
                     if (ok && lane == 0) {
-                        mbar_arrive(&bars.v_empty);
+                        mbar_arrive(&bars.v_empty[st]);
                     }
                     __syncwarp();
                 }
@@ -419,7 +423,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
             }
             for (int32_t j = 0; ok && j <= blocks; ++j) {
                 if (j < blocks) {
-                    ok = wait_or_abort(&bars.k_full, (blocks_done + j) & 1, abort_flag, status, kDevMmaTimeout) &&
+                    const int st = (blocks_done + j) % T::kTileStages;
+                    ok = wait_or_abort(&bars.k_full[st], ((blocks_done + j) / T::kTileStages) & 1, abort_flag, status, kDevMmaTimeout) &&
                          (kc == 0 || wait_or_abort(&bars.s_free[t], (kc - 1) & 1, abort_flag, status, kDevMmaTimeout));
                     if (!ok) {
                         break;
@@ -433,13 +438,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
 #pragma unroll
                                 for (int k = 0; k < 4; ++k) {
                                     tc_mma_f16(d_s, desc_join(q_lo + cb * (T::kQBlockBytes >> 4) + 2 * k, hi_sw128),
-                                               desc_join(k_lo + (part * T::kKVBytes + cb * T::kKVBlockBytes) / 16 + 2 * k, hi_sw128),
+                                               desc_join(k_lo + ((2 * st + part) * T::kKVBytes + cb * T::kKVBlockBytes) / 16 + 2 * k, hi_sw128),
                                                idesc_qk, (part == 0 || (cb | k)) ? 1u : 0u);
                                 }
                             }
                         }
                         tc_commit(&bars.s_full[t]);
-                        tc_commit(&bars.k_empty);
+                        tc_commit(&bars.k_empty[st]);
                         if (j == blocks - 1) {
                             tc_commit(&bars.q_empty);
                         }
@@ -448,7 +453,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                     ++kc;
                 }
                 if (j > 0) {
-                    ok = wait_or_abort(&bars.v_full, (blocks_done + j - 1) & 1, abort_flag, status, kDevMmaTimeout) &&
+                    const int st = (blocks_done + j - 1) % T::kTileStages;
+                    ok = wait_or_abort(&bars.v_full[st], ((blocks_done + j - 1) / T::kTileStages) & 1, abort_flag, status, kDevMmaTimeout) &&
                          wait_or_abort(&bars.p_full[t][vc & 1], (vc >> 1) & 1, abort_flag, status, kDevMmaTimeout);
                     if (ok && j == 1 && mine > 0) {
                         ok = wait_or_abort(&bars.o_free[t], (mine - 1) & 1, abort_flag, status, kDevMmaTimeout);
@@ -461,10 +467,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                         const uint32_t pa = a_p + (vc & 1) * T::kPCols;
 #pragma unroll
                         for (int ks = 0; ks < kBlockN / 16; ++ks) {
-                            tc_mma_f16_ts(d_o, pa + 8 * ks, desc_join(v_lo + ks * (2048 >> 4), hi_sw128), idesc_pv,
+                            tc_mma_f16_ts(d_o, pa + 8 * ks, desc_join(v_lo + st * (T::kKVBytes >> 4) + ks * (2048 >> 4), hi_sw128), idesc_pv,
                                           ((j - 1) | ks) ? 1u : 0u);
                         }
-                        tc_commit(&bars.v_empty);
+                        tc_commit(&bars.v_empty[st]);
                         tc_commit(&bars.pv_done[t][vc & 1]);
                     }
                     __syncwarp();
@@ -492,16 +498,17 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
             ++taken;
             Raw<DH> raw;
             raw.load(raw0 + s * T::kRawBytes, row, piece, rows);
-            if (blk_no > 0 && !wait_or_abort(kv ? &bars.v_empty : &bars.k_empty, (blk_no - 1) & 1, abort_flag, status,
-                                             kDevMmaTimeout)) {
+            const int st = blk_no % T::kTileStages;
+            if (blk_no >= T::kTileStages && !wait_or_abort(kv ? &bars.v_empty[st] : &bars.k_empty[st],
+                                                           ((blk_no / T::kTileStages) - 1) & 1, abort_flag, status, kDevMmaTimeout)) {
                 return false;
             }
             if (kv) {
-                raw.store(v_tile, row, piece);
+                raw.store(v_tile + st * T::kKVBytes, row, piece);
             } else {
-                raw.store_split(k_tile, k_tile + T::kKVBytes, row, piece);
+                raw.store_split(k_tile + 2 * st * T::kKVBytes, k_tile + (2 * st + 1) * T::kKVBytes, row, piece);
             }
-            hand_over(kv ? &bars.v_full : &bars.k_full, &bars.raw_empty[s]);
+            hand_over(kv ? &bars.v_full[st] : &bars.k_full[st], &bars.raw_empty[s]);
             return true;
         };
         for (int64_t u = begin; ok && u < end; ++pieces) {
