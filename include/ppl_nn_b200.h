@@ -362,7 +362,7 @@ int pplb200_kv_evict_select(const pplb200_attn_params* p, const float* weight, c
 /*
  * Compaction in place: for every sequence b, layer in [layer_idx, layer_idx + layers) and kv head, the row of
  * position base[b] + kept[i] moves to position base[b] + i, codes and scales of K and V, and the weight where `weight`
- * is given.  A kept list is strictly ascending and ends at its first negative entry.
+ * is given.  A kept list is strictly ascending and ends at its first negative entry; what follows that is not looked at.
  *   kept    [batch, kept_heads, max_kept] int64; kept_heads is num_kv_heads (a list per kv head: the survivors of
  *           an eviction, base 0) or 1 (one list for all: the accepted path of a tree of drafts, base = start_pos)
  *   kvlens  [batch]: the positions the sequence had; base[b] + kept[i] has to be below

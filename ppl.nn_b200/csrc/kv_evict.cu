@@ -22,7 +22,8 @@
 // segments; a segment reads all its sources before it writes.  Its destinations may still be the sources of EARLIER
 // segments (kept[i'] = i with i' < i), never of later ones, so a segment raises a flag once it has read, and before it
 // writes waits for the flags of those earlier segments whose sources lie among its destinations -- few, and long done
-// where many positions were dropped.  Persistent CTAs draw their segments from a counter in an order in which a list's
+// where many positions were dropped.  A list ends at its first negative entry, whatever follows; a kernel of its own finds
+// it (the lists are a twentieth of the bytes).  Persistent CTAs draw their segments from a counter in an order in which a list's
 // earlier segments come first.  Nobody waits before it has raised the flags of the segments it has begun, so the lowest
 // flag not yet up always belongs to a CTA that can go on.
 // Measured: 16 sequences of up to 16384 positions, 2048 kept per kv head, weights too (176 MB): 47 us (3.7 TB/s); 4 of up
@@ -488,9 +489,11 @@ struct CompactArgs {
     float* weight;  // [L, Hkv, MaxT] or null
     uint32_t* status;
     uint32_t* ticket;
+    int32_t* ends;    // [batch, kept_heads]: the entries of a kept list
     uint32_t* flags;  // [segments][lists]
     CacheGeom geom;
     int64_t max_kept, max_kvlen, max_tokens;
+    int64_t flag_words;
     uint32_t lists;       // batch * layers * head groups
     uint32_t move_tasks;  // segments * lists
     uint32_t tasks;       // and the clearing of weights
@@ -499,6 +502,7 @@ struct CompactArgs {
     int32_t heads_shift, rows_per_seg, segments;  // 1 << heads_shift heads per CTA
 };
 
+constexpr int kEndThreads = 1024;
 constexpr int kCompactThreads = 256;
 constexpr int kCompactCtas = 8;       // per SM: 160 KB on their way
 constexpr int kSegmentRows = 64;      // rows x heads of a segment
@@ -527,10 +531,51 @@ __device__ __forceinline__ bool wait_flag(const uint32_t* flag) {
     }
 }
 
+// A CTA per kept list: where it ends.  What follows its first negative entry may be anything, so the entries are looked at
+// one and all: a bisection would have to trust them.  Clears the status word, the ticket and the flags on the way, so that
+// the call needs no other launch before the moving one.
+__global__ void __launch_bounds__(kEndThreads) kv_compact_end_kernel(const CompactArgs a) {
+    __shared__ int32_t end;
+    grid_launch_dependents();
+    if (threadIdx.x == 0) {
+        end = static_cast<int32_t>(a.max_kept);
+    }
+    __syncthreads();
+    grid_dependency_wait();  // the workspace may still be in use, and the list still be written
+    const int64_t id = blockIdx.x * static_cast<int64_t>(kEndThreads) + threadIdx.x;
+    if (id < 2) {
+        a.status[id] = 0;  // and the ticket behind it
+    }
+    for (int64_t i = id; i < a.flag_words; i += gridDim.x * static_cast<int64_t>(kEndThreads)) {
+        a.flags[i] = 0;
+    }
+    const int64_t* kept = a.kept + blockIdx.x * a.max_kept;
+    constexpr int kUnroll = 8;  // entries of a thread whose loads go out together
+    for (int64_t i0 = threadIdx.x; i0 < a.max_kept; i0 += kUnroll * kEndThreads) {
+        int64_t p[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int64_t i = i0 + u * kEndThreads;
+            p[u] = i < a.max_kept ? kept[i] : 0;
+        }
+#pragma unroll
+        for (int u = kUnroll - 1; u >= 0; --u) {
+            if (p[u] < 0) {
+                atomicMin(&end, static_cast<int32_t>(i0 + u * kEndThreads));
+            }
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        a.ends[blockIdx.x] = end;
+    }
+}
+
 // What a task works on
 struct Task {
     int64_t b, base, n;   // sequence, its base, the positions it had
     const int64_t* kept;
+    int64_t end;          // entries of the kept list: up to its first negative one
     int32_t seg, head0;
     int64_t layer_idx;
     uint32_t list;
@@ -554,7 +599,9 @@ __device__ __forceinline__ Task task_of(const CompactArgs& a, uint32_t ticket) {
     t.head0 = static_cast<int>(t.list % a.head_groups) << a.heads_shift;
     t.layer_idx = a.geom.layer_idx + t.list / a.head_groups % a.layers;
     t.b = t.list / a.head_groups / a.layers;
-    t.kept = a.kept + (t.b * a.kept_heads + (a.kept_heads > 1 ? t.head0 : 0)) * a.max_kept;
+    const int64_t kept_list = t.b * a.kept_heads + (a.kept_heads > 1 ? t.head0 : 0);
+    t.kept = a.kept + kept_list * a.max_kept;
+    t.end = a.ends[kept_list];
     t.base = a.base[t.b];
     t.n = a.kvlens[t.b];
     if (t.n > a.max_kvlen) {
@@ -565,15 +612,13 @@ __device__ __forceinline__ Task task_of(const CompactArgs& a, uint32_t ticket) {
 }
 
 // The last segment in [0, seg] whose first entry is at most `pos` (0 if none is); all lanes of a warp call it.
-__device__ __forceinline__ int32_t segment_of(const CompactArgs& a, const int64_t* kept, int32_t seg, int64_t pos,
-                                              int lane) {
-    int32_t lo = 0, hi = seg + 1;  // answer in [lo, hi)
+__device__ __forceinline__ int32_t segment_of(const CompactArgs& a, const Task& t, int64_t pos, int lane) {
+    int32_t lo = 0, hi = t.seg + 1;  // answer in [lo, hi)
     while (hi - lo > 1) {
         const int32_t step = (hi - lo + 31) >> 5;
         const int32_t pivot = lo + (lane + 1) * step;
-        // entries behind the end of the list are negative: above every position when read as unsigned
-        const bool le = pivot < hi && static_cast<uint64_t>(kept[static_cast<int64_t>(pivot) * a.rows_per_seg]) <=
-                                          static_cast<uint64_t>(pos);
+        const int64_t i = static_cast<int64_t>(pivot) * a.rows_per_seg;
+        const bool le = pivot < hi && i < t.end && t.kept[i] <= pos;
         const int32_t next = lo + __popc(__ballot_sync(0xffffffffu, le)) * step;
         hi = next + step < hi ? next + step : hi;
         lo = next;
@@ -590,7 +635,7 @@ __device__ __forceinline__ void prepare_segment(const CompactArgs& a, uint32_t t
     const Task t = task_of(a, ticket);
     const int64_t first = static_cast<int64_t>(t.seg) * a.rows_per_seg;
     if (tid >= kSegmentRows) {
-        const int32_t e = segment_of(a, t.kept, t.seg, tid < 96 ? first : first + a.rows_per_seg - 1, lane);
+        const int32_t e = segment_of(a, t, tid < 96 ? first : first + a.rows_per_seg - 1, lane);
         if (lane == 0) {
             *(tid < 96 ? &rows.wait_from : &rows.wait_to) = e;
         }
@@ -600,12 +645,12 @@ __device__ __forceinline__ void prepare_segment(const CompactArgs& a, uint32_t t
         return;
     }
     const int64_t i = first + tid;
-    const int64_t p = i < a.max_kept ? t.kept[i] : -1;
-    const int64_t before = i > 0 && i < a.max_kept ? t.kept[i - 1] : -1;
+    const int64_t p = i < t.end ? t.kept[i] : -1;
+    const int64_t before = i > 0 && i < t.end ? t.kept[i - 1] : -1;
     CacheGeom geom = a.geom;
     int64_t src = -1, dst = 0;
     if (p >= 0) {
-        if (t.base < 0 || p < i || (i > 0 && (before < 0 || p <= before)) || t.base + p >= t.n) {
+        if (t.base < 0 || p < i || (i > 0 && p <= before) || t.base + p >= t.n) {
             atomicOr(a.status, kDevKeptInvalid);
         } else if (p != i) {
             src = cache_row(geom, a.cachestarts, t.b, t.base + p);
@@ -628,16 +673,7 @@ __device__ __forceinline__ bool clear_weights(const CompactArgs& a, uint32_t tic
     if (t.base < 0) {
         return true;
     }
-    int64_t count = 0, top = a.max_kept;  // first negative entry
-    while (count < top) {
-        const int64_t mid = (count + top) >> 1;
-        if (t.kept[mid] >= 0) {
-            count = mid + 1;
-        } else {
-            top = mid;
-        }
-    }
-    const int64_t from = t.base + count + static_cast<int64_t>(t.seg) * kClearRows;
+    const int64_t from = t.base + t.end + static_cast<int64_t>(t.seg) * kClearRows;
     const int64_t end = from + kClearRows < t.n ? from + kClearRows : t.n;
     if (from >= end) {
         return true;
@@ -673,6 +709,8 @@ __global__ void __launch_bounds__(kCompactThreads, kCompactCtas) kv_compact_kern
     __shared__ uint4 stage[(kCodeSteps + 1) * kCompactThreads];
     __shared__ float stage_w[kSegmentRows];
     const int tid = threadIdx.x;
+    grid_launch_dependents();
+    grid_dependency_wait();
     if (tid == 0) {
         s_rows[0].ticket = atomicAdd(a.ticket, 1u);
     }
@@ -839,7 +877,8 @@ int make_compact_plan(const pplb200_attn_params& p, int64_t kept_heads, int64_t 
     if (plan->lists > 0x7fffffff) {
         return PPLB200_UNSUPPORTED;
     }
-    plan->off_flags = 256;  // behind the status word and the ticket counter
+    plan->off_ends = 256;  // behind the status word and the ticket counter
+    plan->off_flags = plan->off_ends + (static_cast<uint64_t>(p.batch) * kept_heads * 4 + 255) / 256 * 256;
     plan->bytes = plan->off_flags + (static_cast<uint64_t>(plan->segments) * plan->lists * 4 + 255) / 256 * 256;
     const int64_t clears = (p.max_kvlen + kClearRows - 1) / kClearRows;
     return (plan->segments + clears) * plan->lists > 0x7fffffff ? PPLB200_UNSUPPORTED : PPLB200_SUCCESS;
@@ -859,7 +898,9 @@ int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const
     a.weight = weight;
     a.status = static_cast<uint32_t*>(workspace);
     a.ticket = a.status + 1;
+    a.ends = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + plan.off_ends);
     a.flags = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + plan.off_flags);
+    a.flag_words = plan.segments * plan.lists;
     a.geom = geom;
     a.max_kept = max_kept;
     a.max_kvlen = p.max_kvlen;
@@ -875,9 +916,11 @@ int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const
     a.head_groups = p.num_kv_heads / plan.heads_per_cta;
     a.rows_per_seg = plan.rows_per_seg;
     a.segments = static_cast<int32_t>(plan.segments);
-    if (cudaMemsetAsync(workspace, 0, plan.bytes, stream) != cudaSuccess) {
-        (void)cudaGetLastError();
-        return PPLB200_DEVICE_RUNTIME_ERROR;
+    // each kernel starts while the one before it drains, and waits for it before it reads or writes anything
+    launch_dependent(kv_compact_end_kernel, dim3(static_cast<unsigned>(p.batch * kept_heads)), dim3(kEndThreads), 0, stream, a);
+    const int rc = check_launch("kv_compact_end_kernel");
+    if (rc != PPLB200_SUCCESS) {
+        return rc;
     }
     const int64_t clears = weight == nullptr ? 0 : (p.max_kvlen + kClearRows - 1) / kClearRows;
     const int64_t tasks = (plan.segments + clears) * plan.lists;
@@ -888,7 +931,7 @@ int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const
     const int64_t resident = static_cast<int64_t>(sm_count) * kCompactCtas;
     const int64_t ctas = tasks < resident ? tasks : resident;
     auto kernel = p.head_dim == 128 ? kv_compact_kernel<128> : kv_compact_kernel<64>;
-    kernel<<<static_cast<unsigned>(ctas), kCompactThreads, 0, stream>>>(a);
+    launch_dependent(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kCompactThreads), 0, stream, a);
     return check_launch("kv_compact_kernel");
 }
 

@@ -576,7 +576,7 @@ class KeyValueCacheEvict(_CacheOp):
 class KeyValueCacheCompact(_CacheOp):
     """Moves the cache rows of the kept positions to the front, in place: position base + kept[i] to base + i, of
     ``num_layers`` layers from layer_idx on.  ``kept`` [batch, num_kv_heads or 1, K] is strictly ascending and ends at
-    its first negative entry; ``kvlens`` are the positions the sequences had.  ``weight`` (as of AttentionWeight)
+    its first negative entry, whatever follows it; ``kvlens`` are the positions the sequences had.  ``weight`` (as of AttentionWeight)
     moves along and is zeroed behind the kept positions."""
 
     def __init__(self, param: KeyValueCacheParam):

@@ -427,3 +427,33 @@ def test_compact_shifts_by_a_few_rows(gpu, pkg, drop, per_head):
         assert op.device_status() == 0
         for g, x in zip(got, want):
             assert np.array_equal(g.cpu().numpy(), x)
+
+
+# ---- lists that end before their row does --------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout,page", [(0, 0), (3, 48)])
+@pytest.mark.parametrize("per_head,with_weight", [(True, True), (False, True), (False, False)])
+def test_compact_ends_a_list_at_its_first_negative_entry(gpu, pkg, layout, page, per_head, with_weight):
+    """What stands behind the terminator -- the list of an earlier step, anything -- is not looked at: neither moved, nor
+    reported, nor taken for a part of the list where weights are cleared."""
+    from ppl_nn_b200 import ops
+    rng = np.random.default_rng(layout + per_head)
+    lens = [9, 700, 2000, 300, 64]
+    hc = HostCache(rng, lens, 8, 64, layout, page, 2)
+    kept = np.sort(rng.integers(0, 2000, size=(len(lens), 8 if per_head else 1, 700)), axis=-1)  # stale: plausible rows
+    kept[1] = rng.integers(-3, 1 << 40, size=kept.shape[1:])  # stale: anything, other negative entries too
+    for g in range(kept.shape[1]):
+        for b, count in enumerate([2, 130 + g, 65, 0, 64]):
+            kept[b, g, :count] = np.sort(rng.permutation(lens[b])[:count])
+            kept[b, g, count] = -1 - g
+    kept[0, 0, :5] = [0, 2, -1, 5, 6]
+    want = compact_reference(hc, kept, np.zeros(len(lens), dtype=np.int64), 0, 2, with_weight)
+    op = ops.KeyValueCacheCompact(ops.KeyValueCacheParam(**hc.param()))
+    for _ in range(3):
+        got = [dev(hc.cache), dev(hc.scale), dev(hc.weight)]
+        op.forward(dev(kept), dev(hc.starts), dev(np.zeros(len(lens), dtype=np.int64)), dev(np.array(lens)), hc.max_len,
+                   got[0], got[1], weight=got[2] if with_weight else None, num_layers=2)
+        assert op.device_status() == 0
+        for g, x in zip(got, want):
+            assert np.array_equal(g.cpu().numpy(), x)
