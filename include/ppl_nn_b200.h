@@ -369,8 +369,9 @@ int pplb200_kv_evict_select(const pplb200_attn_params* p, const float* weight, c
  *   weight  nullable; [num_layer, num_kv_heads, max_tokens] fp32.  The weights of the positions from
  *           base[b] + (entries of the list) up to kvlens[b] are set to zero
  * Positions behind the kept ones keep their codes and scales; the caller's lengths become base[b] + entries.  Two
- * sequences of a call must not share rows that either of them moves.  An entry that breaks these rules is skipped
- * and reported (PPLB200_DEV_KEPT_INVALID).  `workspace`: pplb200_kv_compact_workspace_size() bytes, 256-byte aligned
+ * sequences of a call must not share rows that either of them moves.  An entry that is below its own index, outside
+ * its sequence, or not above every entry before it that is neither, is skipped and reported
+ * (PPLB200_DEV_KEPT_INVALID); the others move as they would without it.  `workspace`: pplb200_kv_compact_workspace_size() bytes, 256-byte aligned
  * (its first word is the status word).  No counterpart in the reference.
  */
 int pplb200_kv_compact_workspace_size(const pplb200_attn_params* p, int64_t kept_heads, int64_t max_kept,

@@ -18,17 +18,22 @@
 // a list is one CTA's, because its mask and list fill an SM's shared memory, and 128 CTAs of unequal length fill the chip
 // 60 %.
 //
-// Compact.  Row base + kept[i] moves to row base + i.  kept is strictly ascending, so kept[i] >= i.  A list is cut into
+// Compact.  Row base + kept[i] moves to row base + i.  kept is strictly ascending, so kept[i] >= i; an entry below its
+// index, outside its sequence or not above every such entry before it is skipped, so that the rows that do move are
+// strictly ascending in any list.  A list is cut into
 // segments; a segment reads all its sources before it writes.  Its destinations may still be the sources of EARLIER
 // segments (kept[i'] = i with i' < i), never of later ones, so a segment raises a flag once it has read, and before it
 // writes waits for the flags of those earlier segments whose sources lie among its destinations -- few, and long done
-// where many positions were dropped.  A list ends at its first negative entry, whatever follows; a kernel of its own finds
-// it (the lists are a twentieth of the bytes).  Persistent CTAs draw their segments from a counter in an order in which a list's
+// where many positions were dropped.  A list ends at its first negative entry, whatever follows.  A kernel of its own looks
+// at all the entries (a twentieth of the bytes) and leaves that end, and for each segment the entries that move and the
+// earlier segments to wait for.  The highest positions that move before each segment do not fall, whatever the list holds,
+// so those are found by bisection.  Persistent CTAs draw their segments from a counter in an order in which a list's
 // earlier segments come first.  Nobody waits before it has raised the flags of the segments it has begun, so the lowest
 // flag not yet up always belongs to a CTA that can go on.
-// Measured: 16 sequences of up to 16384 positions, 2048 kept per kv head, weights too (176 MB): 47 us (3.7 TB/s); 4 of up
-// to 131072, paged, 16001 kept (347 MB): 100 us (3.4 TB/s); the accepted paths of 32 sequences in 32 layers (26 MB): 7 us
-// of a 20 us call.  Scattered rows of 128 + 32 bytes are read in whole sectors but not in whole DRAM bursts.
+// Measured: 16 sequences of up to 16384 positions, 2048 kept per kv head, weights too (176 MB): 49 us behind 6 for the
+// lists, 58 a call (3.0 TB/s); 4 of up to 131072, paged, 16001 kept (347 MB): 103 behind 9, 115 a call (3.0 TB/s); the
+// accepted paths of 32 sequences in 32 layers (26 MB): 7 us behind 4, 19 a call.  Scattered rows of 128 + 32 bytes are read
+// in whole sectors but not in whole DRAM bursts.
 #include <type_traits>
 
 #include "common.cuh"
@@ -479,6 +484,12 @@ __global__ void __launch_bounds__(NT) kv_evict_select_kernel(const SelectArgs a)
 
 // ---- compaction ----------------------------------------------------------------------------------
 
+// What the entries of a segment amount to
+struct __align__(16) SegmentPlan {
+    int32_t wait_from, wait_to;  // earlier segments whose sources may be among the destinations
+    uint32_t moves[2];           // bit i: entry i counts
+};
+
 struct CompactArgs {
     const int64_t* kept;  // [batch, kept_heads, max_kept]
     const int64_t* base;
@@ -489,7 +500,9 @@ struct CompactArgs {
     float* weight;  // [L, Hkv, MaxT] or null
     uint32_t* status;
     uint32_t* ticket;
-    int32_t* ends;    // [batch, kept_heads]: the entries of a kept list
+    int2* ends;       // [batch, kept_heads]: the entries of a kept list, and whether all of them move (or stay)
+    SegmentPlan* plans;  // [batch, kept_heads][segments]
+    int32_t* tops;    // [batch, kept_heads][segments]: the highest of the positions that move before a segment, or -1
     uint32_t* flags;  // [segments][lists]
     CacheGeom geom;
     int64_t max_kept, max_kvlen, max_tokens;
@@ -497,12 +510,12 @@ struct CompactArgs {
     uint32_t lists;       // batch * layers * head groups
     uint32_t move_tasks;  // segments * lists
     uint32_t tasks;       // and the clearing of weights
-    int32_t kept_heads, num_kv_heads;
+    int32_t kept_lists, kept_heads, num_kv_heads;
     uint32_t layers, head_groups;
     int32_t heads_shift, rows_per_seg, segments;  // 1 << heads_shift heads per CTA
 };
 
-constexpr int kEndThreads = 1024;
+constexpr int kScanThreads = 1024;
 constexpr int kCompactThreads = 256;
 constexpr int kCompactCtas = 8;       // per SM: 160 KB on their way
 constexpr int kSegmentRows = 64;      // rows x heads of a segment
@@ -531,51 +544,179 @@ __device__ __forceinline__ bool wait_flag(const uint32_t* flag) {
     }
 }
 
-// A CTA per kept list: where it ends.  What follows its first negative entry may be anything, so the entries are looked at
-// one and all: a bisection would have to trust them.  Clears the status word, the ticket and the flags on the way, so that
-// the call needs no other launch before the moving one.
-__global__ void __launch_bounds__(kEndThreads) kv_compact_end_kernel(const CompactArgs a) {
-    __shared__ int32_t end;
+// Entry i of a list; -1 where it leaves the sequence or would move up.  Of the entries in range those above all before them
+// count, so the highest that counts before i is the highest in range before i.
+__device__ __forceinline__ int32_t in_range(int64_t p, int64_t i, int64_t base, int64_t n) {
+    return base >= 0 && p >= i && p < n - base ? static_cast<int32_t>(p) : -1;
+}
+
+__device__ __forceinline__ int32_t warp_max_scan(int32_t x, int lane) {  // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int32_t other = __shfl_up_sync(0xffffffffu, x, o);
+        x = lane >= o && other > x ? other : x;
+    }
+    return x;
+}
+
+// How many of tops[0 .. count) are below `pos`; tops do not fall.
+__device__ __forceinline__ int32_t count_below(const int32_t* tops, int32_t count, int64_t pos) {
+    int32_t lo = 0, hi = count;
+    while (lo < hi) {
+        const int32_t mid = (lo + hi) >> 1;
+        if (tops[mid] < pos) {
+            lo = mid + 1;
+        } else {
+            hi = mid;
+        }
+    }
+    return lo;
+}
+
+// A CTA per kept list: where it ends, and the plans of its segments.  Behind the first negative entry there may be
+// anything, and a list may be out of order, so the entries are looked at one and all: a bisection would have to trust
+// them.  (What stands behind the end enters the maxima of segments that have nothing to move.)  Clears the status word,
+// the ticket and the flags on the way, so that the call needs no other launch before the moving one.
+__global__ void __launch_bounds__(kScanThreads) kv_compact_scan_kernel(const CompactArgs a) {
+    __shared__ int32_t s_end, s_bad, warp_top[kScanThreads / 32], seg_top[kScanThreads];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     grid_launch_dependents();
-    if (threadIdx.x == 0) {
-        end = static_cast<int32_t>(a.max_kept);
+    if (tid == 0) {
+        s_end = static_cast<int32_t>(a.max_kept);
+        s_bad = s_end;  // the first entry that does not count
     }
     __syncthreads();
     grid_dependency_wait();  // the workspace may still be in use, and the list still be written
-    const int64_t id = blockIdx.x * static_cast<int64_t>(kEndThreads) + threadIdx.x;
+    const int64_t id = blockIdx.x * static_cast<int64_t>(kScanThreads) + tid;
     if (id < 2) {
         a.status[id] = 0;  // and the ticket behind it
     }
-    for (int64_t i = id; i < a.flag_words; i += gridDim.x * static_cast<int64_t>(kEndThreads)) {
+    for (int64_t i = id; i < a.flag_words; i += gridDim.x * static_cast<int64_t>(kScanThreads)) {
         a.flags[i] = 0;
     }
     const int64_t* kept = a.kept + blockIdx.x * a.max_kept;
-    constexpr int kUnroll = 8;  // entries of a thread whose loads go out together
-    for (int64_t i0 = threadIdx.x; i0 < a.max_kept; i0 += kUnroll * kEndThreads) {
+    int32_t* tops = a.segments <= kScanThreads ? seg_top : a.tops + blockIdx.x * static_cast<int64_t>(a.segments);
+    const int64_t b = blockIdx.x / a.kept_heads, base = a.base[b];
+    const int rows = a.rows_per_seg, shift = 31 - __clz(rows);  // 8, 16, 32 or 64
+    int64_t n = a.kvlens[b];
+    n = n > a.max_kvlen ? a.max_kvlen : n;
+    constexpr int kUnroll = 8;  // entries of a thread whose loads go out together; a warp's 256 are neighbours
+    for (int64_t i0 = warp * (32 * kUnroll) + lane; i0 - lane < a.max_kept; i0 += kUnroll * kScanThreads) {
         int64_t p[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            const int64_t i = i0 + u * kEndThreads;
-            p[u] = i < a.max_kept ? kept[i] : 0;
+            p[u] = i0 + u * 32 < a.max_kept ? kept[i0 + u * 32] : 0;
         }
+        int32_t top[kUnroll];
+        int32_t last = i0 > lane && lane == 0 ? in_range(kept[i0 - 1], i0 - 1, base, n) : -1;
 #pragma unroll
-        for (int u = kUnroll - 1; u >= 0; --u) {
-            if (p[u] < 0) {
-                atomicMin(&end, static_cast<int32_t>(i0 + u * kEndThreads));
+        for (int u = 0; u < kUnroll; ++u) {
+            const int64_t i = i0 + u * 32;
+            top[u] = i < a.max_kept ? in_range(p[u], i, base, n) : -1;
+            const int32_t left = __shfl_up_sync(0xffffffffu, top[u], 1);
+            if (i < a.max_kept) {
+                if (p[u] < 0) {
+                    atomicMin(&s_end, static_cast<int32_t>(i));
+                } else if (top[u] <= (lane > 0 ? left : last)) {  // as long as all count, the one before is the highest
+                    atomicMin(&s_bad, static_cast<int32_t>(i));
+                }
+            }
+            last = __shfl_sync(0xffffffffu, top[u], 31);
+        }
+        if (rows >= 32) {  // one step of the warp, or two
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                top[u] = __reduce_max_sync(0xffffffffu, top[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                const int64_t i = i0 + u * 32;
+                if (lane == 0 && i < a.max_kept && (rows == 32 || (u & 1) == 0)) {
+                    tops[i >> shift] = rows == 32 || top[u] > top[u | 1] ? top[u] : top[u | 1];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+#pragma unroll
+                for (int o = 1; o < 16; o <<= 1) {
+                    const int32_t other = __shfl_xor_sync(0xffffffffu, top[u], o);
+                    top[u] = o < rows && other > top[u] ? other : top[u];
+                }
+                if ((lane & (rows - 1)) == 0 && i0 + u * 32 < a.max_kept) {
+                    tops[(i0 + u * 32) >> shift] = top[u];
+                }
             }
         }
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        a.ends[blockIdx.x] = end;
+    const int32_t end = s_end;
+    const bool orderly = s_bad >= end;
+    if (tid == 0) {
+        a.ends[blockIdx.x] = make_int2(end, orderly);
+    }
+    // each segment's own maximum -> the maximum of those before it
+    int32_t carry = -1;
+    for (int32_t e0 = 0; e0 < a.segments; e0 += kScanThreads) {
+        const int32_t e = e0 + tid;
+        const int32_t top = warp_max_scan(e < a.segments ? tops[e] : -1, lane);
+        __syncthreads();
+        if (lane == 31) {
+            warp_top[warp] = top;
+        }
+        __syncthreads();
+        const int32_t all = warp_max_scan(warp_top[lane], lane);
+        int32_t before = __shfl_sync(0xffffffffu, all, warp > 0 ? warp - 1 : 0);  // of the warps before
+        before = warp > 0 && before > carry ? before : carry;
+        const int32_t mine = __shfl_up_sync(0xffffffffu, top, 1);
+        if (e < a.segments) {
+            tops[e] = lane > 0 && mine > before ? mine : before;
+        }
+        const int32_t most = __shfl_sync(0xffffffffu, all, 31);
+        carry = most > carry ? most : carry;
+    }
+    __syncthreads();
+    // What counts in segment e lies above tops[e], up to tops[e + 1].  So of the segments before e it has to wait for those
+    // from the first whose highest reaches its destinations to the last that begins below their end.
+    SegmentPlan* plans = a.plans + blockIdx.x * static_cast<int64_t>(a.segments);
+    for (int32_t e = tid; e < a.segments; e += kScanThreads) {
+        const int64_t first = static_cast<int64_t>(e) * rows;
+        SegmentPlan plan = {0, -1, {0u, 0u}};  // behind the end: nothing to move, nothing to wait for
+        if (first < end) {
+            plan.wait_from = count_below(tops + 1, e, first);
+            plan.wait_to = count_below(tops, e, first + rows - 1) - 1;
+            const int32_t count = end - first < rows ? static_cast<int32_t>(end - first) : rows;
+            plan.moves[0] = count >= 32 ? ~0u : (1u << count) - 1u;
+            plan.moves[1] = count <= 32 ? 0u : (count == 64 ? ~0u : (1u << (count - 32)) - 1u);
+        }
+        plans[e] = plan;
+    }
+    if (orderly) {
+        return;
+    }
+    __syncthreads();
+    for (int32_t e = warp; e < a.segments; e += kScanThreads / 32) {  // a warp per segment
+        const int64_t first = static_cast<int64_t>(e) * rows;
+        int32_t before = tops[e];
+        for (int32_t j = lane; j - lane < rows; j += 32) {
+            const int64_t i = first + j;
+            const int32_t p = j < rows && i < end ? in_range(kept[i], i, base, n) : -1;
+            const int32_t incl = warp_max_scan(p, lane);
+            const int32_t left = __shfl_up_sync(0xffffffffu, incl, 1);
+            const uint32_t moves = __ballot_sync(0xffffffffu, p > (lane > 0 && left > before ? left : before));
+            const int32_t most = __shfl_sync(0xffffffffu, incl, 31);
+            before = most > before ? most : before;
+            if (lane == 0) {
+                plans[e].moves[j >> 5] = moves;
+            }
+        }
     }
 }
 
 // What a task works on
 struct Task {
     int64_t b, base, n;   // sequence, its base, the positions it had
-    const int64_t* kept;
-    int64_t end;          // entries of the kept list: up to its first negative one
+    int64_t kept_list;
     int32_t seg, head0;
     int64_t layer_idx;
     uint32_t list;
@@ -599,9 +740,7 @@ __device__ __forceinline__ Task task_of(const CompactArgs& a, uint32_t ticket) {
     t.head0 = static_cast<int>(t.list % a.head_groups) << a.heads_shift;
     t.layer_idx = a.geom.layer_idx + t.list / a.head_groups % a.layers;
     t.b = t.list / a.head_groups / a.layers;
-    const int64_t kept_list = t.b * a.kept_heads + (a.kept_heads > 1 ? t.head0 : 0);
-    t.kept = a.kept + kept_list * a.max_kept;
-    t.end = a.ends[kept_list];
+    t.kept_list = t.b * a.kept_heads + (a.kept_heads > 1 ? t.head0 : 0);
     t.base = a.base[t.b];
     t.n = a.kvlens[t.b];
     if (t.n > a.max_kvlen) {
@@ -611,54 +750,29 @@ __device__ __forceinline__ Task task_of(const CompactArgs& a, uint32_t ticket) {
     return t;
 }
 
-// The last segment in [0, seg] whose first entry is at most `pos` (0 if none is); all lanes of a warp call it.
-__device__ __forceinline__ int32_t segment_of(const CompactArgs& a, const Task& t, int64_t pos, int lane) {
-    int32_t lo = 0, hi = t.seg + 1;  // answer in [lo, hi)
-    while (hi - lo > 1) {
-        const int32_t step = (hi - lo + 31) >> 5;
-        const int32_t pivot = lo + (lane + 1) * step;
-        const int64_t i = static_cast<int64_t>(pivot) * a.rows_per_seg;
-        const bool le = pivot < hi && i < t.end && t.kept[i] <= pos;
-        const int32_t next = lo + __popc(__ballot_sync(0xffffffffu, le)) * step;
-        hi = next + step < hi ? next + step : hi;
-        lo = next;
-    }
-    return lo;
-}
-
-// Warps 0 and 1 look up the rows of the segment that `ticket` names, warps 2 and 3 the segments it has to wait for.
+// Looks up the rows of the segment that `ticket` names, and its plan.
 __device__ __forceinline__ void prepare_segment(const CompactArgs& a, uint32_t ticket, SegmentRows& rows) {
-    const int tid = threadIdx.x, lane = tid & 31;
-    if (tid >= 128 || ticket >= a.move_tasks) {
+    const int tid = threadIdx.x;
+    if (tid >= a.rows_per_seg || ticket >= a.move_tasks) {
         return;
     }
     const Task t = task_of(a, ticket);
-    const int64_t first = static_cast<int64_t>(t.seg) * a.rows_per_seg;
-    if (tid >= kSegmentRows) {
-        const int32_t e = segment_of(a, t, tid < 96 ? first : first + a.rows_per_seg - 1, lane);
-        if (lane == 0) {
-            *(tid < 96 ? &rows.wait_from : &rows.wait_to) = e;
-        }
-        return;
+    const int64_t i = static_cast<int64_t>(t.seg) * a.rows_per_seg + tid;
+    const int4 plan = *reinterpret_cast<const int4*>(a.plans + t.kept_list * a.segments + t.seg);  // a SegmentPlan
+    if (tid == 0) {
+        rows.wait_from = plan.x;
+        rows.wait_to = plan.y;
     }
-    if (tid >= a.rows_per_seg) {
-        return;
-    }
-    const int64_t i = first + tid;
-    const int64_t p = i < t.end ? t.kept[i] : -1;
-    const int64_t before = i > 0 && i < t.end ? t.kept[i - 1] : -1;
+    const bool counts = ((tid < 32 ? plan.z : plan.w) >> (tid & 31) & 1) != 0;
+    const int64_t p = i < a.max_kept ? a.kept[t.kept_list * a.max_kept + i] : 0;  // loaded without waiting for the plan
     CacheGeom geom = a.geom;
     int64_t src = -1, dst = 0;
-    if (p >= 0) {
-        if (t.base < 0 || p < i || (i > 0 && p <= before) || t.base + p >= t.n) {
-            atomicOr(a.status, kDevKeptInvalid);
-        } else if (p != i) {
-            src = cache_row(geom, a.cachestarts, t.b, t.base + p);
-            dst = cache_row(geom, a.cachestarts, t.b, t.base + i);
-            if (!cache_row_ok(src, a.max_tokens) || !cache_row_ok(dst, a.max_tokens)) {
-                atomicOr(a.status, kDevRowOutOfRange);
-                src = -1;
-            }
+    if (counts && p != i) {
+        src = cache_row(geom, a.cachestarts, t.b, t.base + p);
+        dst = cache_row(geom, a.cachestarts, t.b, t.base + i);
+        if (!cache_row_ok(src, a.max_tokens) || !cache_row_ok(dst, a.max_tokens)) {
+            atomicOr(a.status, kDevRowOutOfRange);
+            src = -1;
         }
     }
     const int64_t fixed = t.layer_idx * geom.stride_l + t.head0 * geom.stride_h;
@@ -673,7 +787,7 @@ __device__ __forceinline__ bool clear_weights(const CompactArgs& a, uint32_t tic
     if (t.base < 0) {
         return true;
     }
-    const int64_t from = t.base + t.end + static_cast<int64_t>(t.seg) * kClearRows;
+    const int64_t from = t.base + a.ends[t.kept_list].x + static_cast<int64_t>(t.seg) * kClearRows;
     const int64_t end = from + kClearRows < t.n ? from + kClearRows : t.n;
     if (from >= end) {
         return true;
@@ -711,6 +825,13 @@ __global__ void __launch_bounds__(kCompactThreads, kCompactCtas) kv_compact_kern
     const int tid = threadIdx.x;
     grid_launch_dependents();
     grid_dependency_wait();
+    if (blockIdx.x == 0) {  // the status word has been cleared: now it can take what the scan found
+        for (int32_t l = tid; l < a.kept_lists; l += kCompactThreads) {
+            if (a.ends[l].y == 0) {
+                atomicOr(a.status, kDevKeptInvalid);
+            }
+        }
+    }
     if (tid == 0) {
         s_rows[0].ticket = atomicAdd(a.ticket, 1u);
     }
@@ -781,8 +902,7 @@ __global__ void __launch_bounds__(kCompactThreads, kCompactCtas) kv_compact_kern
             raise_flag(a.flags + static_cast<int64_t>(seg) * a.lists + list);
         }
         bool ok = true;
-        const int32_t wait_to = rows.wait_to < seg ? rows.wait_to : seg - 1;
-        for (int32_t e = rows.wait_from + tid; e <= wait_to; e += kCompactThreads) {
+        for (int32_t e = rows.wait_from + tid; e <= rows.wait_to; e += kCompactThreads) {
             ok = wait_flag(a.flags + static_cast<int64_t>(e) * a.lists + list) && ok;
         }
         if (!__syncthreads_and(ok)) {
@@ -878,7 +998,11 @@ int make_compact_plan(const pplb200_attn_params& p, int64_t kept_heads, int64_t 
         return PPLB200_UNSUPPORTED;
     }
     plan->off_ends = 256;  // behind the status word and the ticket counter
-    plan->off_flags = plan->off_ends + (static_cast<uint64_t>(p.batch) * kept_heads * 4 + 255) / 256 * 256;
+    const uint64_t kept_lists = static_cast<uint64_t>(p.batch) * kept_heads;
+    plan->off_tops = plan->off_ends + (kept_lists * 8 + 255) / 256 * 256;
+    const bool spills = plan->segments > kScanThreads;  // else the scan has them in shared memory
+    plan->off_plans = plan->off_tops + (spills ? (kept_lists * plan->segments * 4 + 255) / 256 * 256 : 0);
+    plan->off_flags = plan->off_plans + (kept_lists * plan->segments * sizeof(SegmentPlan) + 255) / 256 * 256;
     plan->bytes = plan->off_flags + (static_cast<uint64_t>(plan->segments) * plan->lists * 4 + 255) / 256 * 256;
     const int64_t clears = (p.max_kvlen + kClearRows - 1) / kClearRows;
     return (plan->segments + clears) * plan->lists > 0x7fffffff ? PPLB200_UNSUPPORTED : PPLB200_SUCCESS;
@@ -898,7 +1022,9 @@ int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const
     a.weight = weight;
     a.status = static_cast<uint32_t*>(workspace);
     a.ticket = a.status + 1;
-    a.ends = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + plan.off_ends);
+    a.ends = reinterpret_cast<int2*>(static_cast<uint8_t*>(workspace) + plan.off_ends);
+    a.tops = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + plan.off_tops);
+    a.plans = reinterpret_cast<SegmentPlan*>(static_cast<uint8_t*>(workspace) + plan.off_plans);
     a.flags = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + plan.off_flags);
     a.flag_words = plan.segments * plan.lists;
     a.geom = geom;
@@ -907,6 +1033,7 @@ int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const
     a.max_tokens = p.max_tokens;
     a.lists = static_cast<uint32_t>(plan.lists);
     a.move_tasks = static_cast<uint32_t>(plan.segments * plan.lists);
+    a.kept_lists = static_cast<int32_t>(p.batch * kept_heads);
     a.kept_heads = static_cast<int32_t>(kept_heads);
     a.num_kv_heads = p.num_kv_heads;
     a.layers = static_cast<uint32_t>(layers);
@@ -917,8 +1044,8 @@ int launch_kv_compact(const pplb200_attn_params& p, const CacheGeom& geom, const
     a.rows_per_seg = plan.rows_per_seg;
     a.segments = static_cast<int32_t>(plan.segments);
     // each kernel starts while the one before it drains, and waits for it before it reads or writes anything
-    launch_dependent(kv_compact_end_kernel, dim3(static_cast<unsigned>(p.batch * kept_heads)), dim3(kEndThreads), 0, stream, a);
-    const int rc = check_launch("kv_compact_end_kernel");
+    launch_dependent(kv_compact_scan_kernel, dim3(static_cast<unsigned>(a.kept_lists)), dim3(kScanThreads), 0, stream, a);
+    const int rc = check_launch("kv_compact_scan_kernel");
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }

@@ -153,7 +153,7 @@ int launch_kv_evict_select(const pplb200_attn_params& p, const CacheGeom& geom, 
 struct CompactPlan {
     int32_t heads_per_cta, rows_per_seg;
     int64_t lists, segments;
-    uint64_t off_ends, off_flags, bytes;
+    uint64_t off_ends, off_tops, off_plans, off_flags, bytes;
 };
 int make_compact_plan(const pplb200_attn_params& p, int64_t kept_heads, int64_t max_kept, int64_t layers,
                       CompactPlan* plan);

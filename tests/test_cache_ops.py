@@ -457,3 +457,99 @@ def test_compact_ends_a_list_at_its_first_negative_entry(gpu, pkg, layout, page,
         assert op.device_status() == 0
         for g, x in zip(got, want):
             assert np.array_equal(g.cpu().numpy(), x)
+
+
+# ---- lists with entries that break the rules -------------------------------------------------------------
+
+def entries_that_move(kept, base, n):
+    """(index, position) of a list's entries that count: in range, and above every entry in range before."""
+    out, top = [], -1
+    for i, p in enumerate(kept):
+        if p < 0:
+            break
+        if i <= p < n - base and p > top:
+            out.append((i, p))
+            top = p
+    return out
+
+
+def skipping_reference(hc, kept, base, layers):
+    cache, scale, weight = hc.cache.copy(), hc.scale.copy(), hc.weight.copy()
+    for b in range(len(hc.lens)):
+        for g in range(hc.heads):
+            mine = kept[b, g if kept.shape[1] > 1 else 0]
+            end = int(np.argmax(mine < 0)) if (mine < 0).any() else len(mine)
+            pairs = np.array(entries_that_move(mine, base[b], hc.lens[b]), dtype=np.int64).reshape(-1, 2)
+            src, dst = hc.rows(b, base[b] + pairs[:, 1]), hc.rows(b, base[b] + pairs[:, 0])
+            for layer in range(layers):
+                for which in range(2):
+                    if hc.layout == 0:
+                        cache[dst, layer, which, g] = hc.cache[src, layer, which, g]
+                        scale[dst, layer, which, g] = hc.scale[src, layer, which, g]
+                    else:
+                        cache[layer, which, g, dst] = hc.cache[layer, which, g, src]
+                        scale[layer, which, g, dst] = hc.scale[layer, which, g, src]
+                weight[layer, g, dst] = hc.weight[layer, g, src]
+                weight[layer, g, hc.rows(b, np.arange(base[b] + end, hc.lens[b]))] = 0
+    return cache, scale, weight
+
+
+def spoil(rng, kept, where, kind):
+    """Entries that break the rules at the indices `where` of a shifted list."""
+    for i in where:
+        kept[i] = {"huge": 1 << 40, "low": 0, "same": kept[i - 1] if i else 1 << 33,
+                   "over": int(rng.integers(0, len(kept))), "most": np.iinfo(np.int64).max}[kind]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["huge", "low", "same", "over", "most"])
+@pytest.mark.parametrize("drop", [1, 70, 200])
+@pytest.mark.parametrize("per_head", [True, False])
+def test_compact_skips_bad_entries_of_long_lists(gpu, pkg, kind, drop, per_head):
+    """Every segment's destinations are others' sources, and entries break the rules at the beginnings, at the ends and in
+    the middle of segments: these alone are skipped, and the rows of the others move as they would without them."""
+    from ppl_nn_b200 import capi, ops
+    rng = np.random.default_rng(drop + per_head)
+    lens, base = [3000, 517, 2900, 140], np.array([0, 5, 0, 1], dtype=np.int64)
+    hc = HostCache(rng, lens, 8, 64, 0, 0, 2)
+    kept = np.full((len(lens), 8 if per_head else 1, max(lens)), -1, dtype=np.int64)
+    for b, n in enumerate(lens):
+        for g in range(kept.shape[1]):
+            count = max(0, n - int(base[b]) - drop)
+            kept[b, g, :count] = np.arange(drop, drop + count)
+            at = [i for i in (64, 63, 8, 200, 128 + g, 256, 255, 1000, 1024 + g) if i < count]
+            spoil(rng, kept[b, g, :count], at, kind)
+    want = skipping_reference(hc, kept, base, 2)
+    op = ops.KeyValueCacheCompact(ops.KeyValueCacheParam(**hc.param()))
+    for _ in range(5):
+        got = [dev(hc.cache), dev(hc.scale), dev(hc.weight)]
+        op.forward(dev(kept), dev(hc.starts), dev(base), dev(np.array(lens)), hc.max_len, got[0], got[1], weight=got[2],
+                   num_layers=2)
+        assert op.device_status() == capi.DEV_KEPT_INVALID
+        for g, x in zip(got, want):
+            assert np.array_equal(g.cpu().numpy(), x)
+
+
+def wait_range(tops, seg, rows):
+    """The earlier segments that the kernel of the moves waits for, as it finds them."""
+    below = lambda a, x: int(np.searchsorted(a, x, side="left"))  # noqa: E731
+    return below(tops[1:seg + 1], seg * rows), below(tops[:seg], seg * rows + rows - 1) - 1
+
+
+@pytest.mark.parametrize("rows", [8, 16, 32, 64])
+def test_segments_wait_for_all_whose_rows_they_overwrite(rows):
+    """The rule by which a segment finds the earlier ones to wait for, on lists with anything in them."""
+    rng = np.random.default_rng(rows)
+    for trial in range(60):
+        n, width = int(rng.integers(1, 900)), int(rng.integers(1, 700))
+        kept = np.sort(rng.integers(0, n, size=width)) if trial % 2 else np.arange(width) + int(rng.integers(0, 90))
+        bad = rng.random(width) < rng.choice([0, 0.02, 0.3])
+        kept = np.where(bad, rng.choice([0, 5, n - 1, n + 3, 1 << 40], size=width), kept)
+        moves = entries_that_move(kept, 0, n)
+        in_range = np.array([p if i <= p < n else -1 for i, p in enumerate(kept)])
+        segments = -(-width // rows)
+        tops = np.array([max(in_range[:e * rows], default=-1) for e in range(segments)])
+        for seg in range(segments):
+            lo, hi = wait_range(tops, seg, rows)
+            need = {i // rows for i, p in moves if i // rows < seg and seg * rows <= p < (seg + 1) * rows}
+            assert all(lo <= e <= hi for e in need) and hi < seg
