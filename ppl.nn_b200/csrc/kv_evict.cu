@@ -30,8 +30,8 @@
 // so those are found by bisection.  Persistent CTAs draw their segments from a counter in an order in which a list's
 // earlier segments come first.  Nobody waits before it has raised the flags of the segments it has begun, so the lowest
 // flag not yet up always belongs to a CTA that can go on.
-// Measured: 16 sequences of up to 16384 positions, 2048 kept per kv head, weights too (176 MB): 49 us behind 6 for the
-// lists, 58 a call (3.0 TB/s); 4 of up to 131072, paged, 16001 kept (347 MB): 103 behind 9, 115 a call (3.0 TB/s); the
+// Measured: 16 sequences of up to 16384 positions, 2048 kept per kv head, weights too (176 MB): 47 us behind 6 for the
+// lists, 55 a call (3.2 TB/s); 4 of up to 131072, paged, 16001 kept (347 MB): 101 behind 9, 112 a call (3.1 TB/s); the
 // accepted paths of 32 sequences in 32 layers (26 MB): 7 us behind 4, 19 a call.  Scattered rows of 128 + 32 bytes are read
 // in whole sectors but not in whole DRAM bursts.
 #include <type_traits>
@@ -521,18 +521,18 @@ constexpr int kCompactCtas = 8;       // per SM: 160 KB on their way
 constexpr int kSegmentRows = 64;      // rows x heads of a segment
 constexpr int kClearRows = 8192;      // weights zeroed by a CTA
 
-// Flags order reads before other CTAs' writes, and nothing else.  When a segment raises its flag its sources have
-// arrived in its shared memory (the asynchronous copies have completed and the CTA has met at a barrier), so no later
-// write can reach them, and nothing it wrote is read by whoever sees the flag.  A relaxed store and relaxed loads do: a
-// fence ahead of the store would wait for the stores of every CTA on the SM (measured 4 to 7 us per segment).
+// A flag orders a segment's reads before other CTAs' writes.  When it is raised the sources have arrived in shared memory
+// (the asynchronous copies have completed and the CTA has met at a barrier); the release hands that on, and whoever
+// acquires the flag meets at a barrier of its own before anyone there writes.  Measured against relaxed accesses, which
+// leave the order to the machine: 55 against 58 us and 112 against 115 us (the calls of the header).
 __device__ __forceinline__ void raise_flag(uint32_t* flag) {
-    asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(flag), "r"(1u) : "memory");
+    asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(flag), "r"(1u) : "memory");
 }
 __device__ __forceinline__ bool wait_flag(const uint32_t* flag) {
     long long t0 = 0;
     for (;;) {
         uint32_t v;
-        asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
         if (v != 0u) {
             return true;
         }
