@@ -24,8 +24,8 @@
 //
 // Roundings: a key rounded to fp16 costs 1e-3 of the output's magnitude where keys have outlying channels, and 3e-3 where
 // several positions compete for a row (against 2e-4 for the fp16 output itself), so K is split into fp16(k) and the exact
-// remainder, two tiles whose products with Q meet in one accumulator.  Weights and values are rounded to fp16, by 2^-12 of
-// each and independently, which averages out; scores, maxima, sums and outputs are held in fp32.
+// remainder, two tiles whose products with Q meet in one accumulator.  Weights and values are rounded to fp16, by up to 2^-11 of
+// each and independently, which averages out (weights below 2^-21 of the row's largest by up to 2^-32 of that); scores, maxima, sums and outputs are held in fp32.
 //
 // Measured (8 kv heads of 128), main kernel and whole call: 32 sequences of 256 to 8192 positions, 4 to 64 rows per kv
 // head, 392 MB of cache: 165 and 198 us (with rounded keys 145 and 163); 64 such sequences, 200 to 264 rows: 508 and 602
@@ -54,7 +54,11 @@ constexpr int kTileM = 128;  // rows of an MMA
 constexpr int kBlockN = kTileRows;  // positions of a block
 constexpr int kMinRange = 4;  // blocks: no range is cut finer
 constexpr float kNegBig = -1.0e30f;
-constexpr float kRescaleSlack = 8.0f;
+constexpr float kRescaleSlack = 8.0f;  // how far, in powers of two, a maximum may run ahead of a row's reference
+// A weight is held in fp16 as 2^kLift times its ratio to the reference: at most 2^(7 + 8), and nothing above 2^-32 of the
+// largest vanishes.  (Without the lift 2^-25: behind one token that takes 98 % of a row, the other 131071 would lose a
+// quarter of their part.)  The factor is in numerator and sum alike.
+constexpr float kLift = 7.0f;
 
 template <int DH, int MT>
 struct TTraits {
@@ -673,9 +677,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
                         tmem_wait_st();
                     }
                 }
-                // P = exp2(s * scale - m_ref) as packed fp16; the row sum adds the rounded values that P V uses, in
+                // P = exp2(s * scale - m_ref + kLift) as packed fp16; the row sum adds the rounded values that P V uses, in
                 // four chains (one chain of 64 dependent additions would be as long as the exponentials)
                 const uint32_t t_pb = t_p + (pc & 1) * T::kPCols;
+                const float lift = kLift - m_ref;
                 float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int q = 0; q < kBlockN / 32; ++q) {
@@ -683,7 +688,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_code, const __grid_const
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const float2 x = __ffma2_rn(make_float2(sv[32 * q + 2 * e], sv[32 * q + 2 * e + 1]),
-                                                    make_float2(sc, sc), make_float2(-m_ref, -m_ref));
+                                                    make_float2(sc, sc), make_float2(lift, lift));
                         pk[e] = h2_as_u32(__floats2half2_rn(ex2_approx(x.x), ex2_approx(x.y)));
                         add_half2_to_float(l4[e & 3], pk[e]);
                     }

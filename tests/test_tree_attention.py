@@ -174,3 +174,46 @@ def test_tree_attention_reports_bad_inputs(gpu, pkg):  # noqa: F811
     got, status = run_tree(hc, q, good, start, n, 4, 0)
     assert status & capi.DEV_ROW_OUT_OF_RANGE
     assert np.all(np.abs(got[:5] - want[:5]) <= tol[:5])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("above", [14.0, 17.0, 18.0, 19.0])
+def test_what_stands_behind_a_dominant_token_is_kept(gpu, pkg, above):  # noqa: F811
+    """131071 positions whose scores spread by 1 around a mean, and a first token (a sink) that stands `above` over it, with
+    values near zero: the others hold 10 to 0.1 % of the weight and nearly all of the output.  All the sequences read the
+    same rows, so that most of them are worked on from the sink to the end by one CTA.
+
+    Tolerance: a score is a sum of 2 Dh exact products in fp32 (Dh / 8 instructions, 2^-22 of the products' magnitudes
+    each), an error of the exponent of a weight and of the normaliser; weights, values and the output are rounded to
+    fp16 (2^-11); fp16 holds a weight as 2^7 or more times its ratio to the row's largest, so that below the normal range
+    the rounding, at most 2^-25, is 2^-32 of the largest, in the numerator and in the sum; 2^-16 covers the exponentials
+    and the fp32 sums."""
+    import torch
+    from ppl_nn_b200 import ops
+    rng = np.random.default_rng(int(above))
+    heads, dim, hist, batch, u = 2, 64, 131071, 300, 2.0 ** -11
+    hc = HostCache(rng, [hist + 1], 1, dim)
+    rows = hc.rows(0, np.arange(hist + 1))
+    sign = rng.choice([-1, 1], size=(heads, dim))
+    q = np.broadcast_to(sign, (batch, heads, dim)).astype(np.float16)
+    # uniform codes have a spread of 73.3: 8 * 73.3 * scale / 8 = 1
+    hc.scale[rows, 0, 0] = np.float16(1 / 73.3)
+    hc.cache[rows[0], 0, 0, 0] = np.where(sign[0] == sign[1], 127, 0) * sign[0]  # both heads' sink
+    agree = int((sign[0] == sign[1]).sum())
+    hc.scale[rows[0], 0, 0] = np.float16(above * 8 / (127 * agree))
+    hc.cache[rows, 0, 1] = rng.integers(30, 128, size=(hist + 1, 1, dim))  # values of one sign: nothing cancels
+    hc.scale[rows[0], 0, 1] = np.float16(1e-5)
+    k, v = hc.values(0, 0, 0, rows), hc.values(1, 0, 0, rows)
+    s = (k @ sign.T.astype(np.float64)) / math.sqrt(dim)  # [positions, heads]
+    p = np.exp(s - s.max(0))
+    p /= p.sum(0)
+    want, mag = p.T @ v, p.T @ np.abs(v)
+    off = (dim / 8) * 2.0 ** -22 * np.abs(k).sum(1).max() / math.sqrt(dim)
+    tol = mag * (2 * off + 2 * u + 2.0 ** -16) + u * np.abs(want) + 2 * len(rows) * 2.0 ** -32 * np.abs(v).max()
+    op = ops.TreeAttention(ops.MultiHeadCacheAttentionParam(num_heads=heads, num_kv_heads=1, head_dim=dim, **hc.param()))
+    i64 = lambda x: torch.tensor(x, dtype=torch.int64, device=gpu)  # noqa: E731
+    out = op.forward(dev(q), None, torch.arange(batch + 1, device=gpu), i64([int(hc.starts[0])] * batch), i64([hist] * batch), 1,
+                     hist + 1, dev(hc.cache), dev(hc.scale))
+    assert op.device_status() == 0
+    got = out.cpu().numpy().astype(np.float64)
+    assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
