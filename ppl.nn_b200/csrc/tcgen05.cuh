@@ -1,5 +1,5 @@
 // tcgen05 (5th-generation tensor core) wrappers shared by the attention kernels: TMEM allocation and access, the MMA
-// and its descriptors, and the bounded waits of a CTA whose roles give up together.
+// and its descriptors, and (warp_wait.cuh) the bounded waits of a CTA whose roles give up together.
 #pragma once
 
 #include "common.cuh"
@@ -198,59 +198,6 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
     return done != 0;
 }
 
-// Bounded wait that also gives up as soon as another thread of the CTA has given up.  The common case,
-// a phase that has completed already, costs one test; the polling loop is kept out of line.
-static __device__ __noinline__ bool wait_or_abort_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                                uint32_t* status, uint32_t code) {
-    const long long t0 = clock64();
-    for (uint32_t i = 0;; i += 4) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (PPLB200_PREFILL_WAIT(bar, parity)) {
-                return true;
-            }
-        }
-        if ((i & 255u) == 252u) {
-            if (*abort_flag) {
-                return false;
-            }
-            if (clock64() - t0 > kWaitBudgetCycles) {
-                break;
-            }
-        }
-    }
-    *abort_flag = 1;
-    atomicOr(status, code);
-    return false;
-}
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                              uint32_t* status, uint32_t code) {
-    if (PPLB200_PREFILL_WAIT(bar, parity)) {
-        return true;
-    }
-    return wait_or_abort_slow(bar, parity, abort_flag, status, code);
-}
-
-// The same for a thread that is in no hurry: parked by the hardware instead of polling, so that it leaves the issue
-// slots to the others.
-__device__ __forceinline__ bool wait_or_abort_parked(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                                     uint32_t* status, uint32_t code) {
-    const uint32_t addr = smem_u32(bar);
-    if (mbar_try_wait_hint(addr, parity, PPLB200_WAIT_HINT_NS)) {
-        return true;
-    }
-    const long long t0 = clock64();
-    while (!mbar_try_wait_hint(addr, parity, PPLB200_WAIT_HINT_NS)) {
-        if (*abort_flag) {
-            return false;
-        }
-        if (clock64() - t0 > kWaitBudgetCycles) {
-            *abort_flag = 1;
-            atomicOr(status, code);
-            return false;
-        }
-    }
-    return true;
-}
-
 }  // namespace pplb200
+
+#include "warp_wait.cuh"
