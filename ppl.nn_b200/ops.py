@@ -408,25 +408,28 @@ class _CacheOp(_Base):
 
     def _check_cache(self, cache, scale):
         """(device, kv heads, head_dim, rows) of an INT8 cache with num_layer layers and its scales."""
-        a = self.param
         if scale is None or scale.numel() == 0:
             raise OpError("RC_UNSUPPORTED", "currently only support qunatized cache but scale not found")
         _require_cuda(cache=cache)
         device = cache.get_device()
         _require(device, torch.int8, cache=cache)
         _require(device, torch.float16, scale=scale)
-        shape = cache.shape
-        if len(shape) != 5 or scale.shape != shape[:4] + (shape[4] // 8,):
+        return device, *self._cache_shape(tuple(cache.shape), tuple(scale.shape))
+
+    def _cache_shape(self, shape, scale_shape):
+        """(kv heads, head_dim, rows) of a cache and its scales."""
+        a = self.param
+        if len(shape) != 5 or scale_shape != shape[:4] + (shape[4] // 8,):
             raise OpError("RC_INVALID_VALUE", "cache and scale do not belong together")
         if a.cache_layout == 0:
-            rows, layers, _, heads, dim = shape
+            rows, layers, kv, heads, dim = shape
         elif a.cache_layout == 3:
-            layers, _, heads, rows, dim = shape
+            layers, kv, heads, rows, dim = shape
         else:
             raise OpError("RC_UNSUPPORTED", "currently only support cache_layout == 0 or cache_layout == 3")
-        if layers != a.num_layer:
-            raise OpError("RC_INVALID_VALUE", "cache does not have num_layer layers")
-        return device, heads, dim, rows
+        if layers != a.num_layer or kv != 2:
+            raise OpError("RC_INVALID_VALUE", "cache does not have num_layer layers of K and V")
+        return heads, dim, rows
 
     def _check_weight(self, device, weight, heads, rows) -> None:
         _require(device, torch.float32, weight=weight)

@@ -54,6 +54,25 @@ def test_sizes_that_would_wrap_around_are_refused(pkg, built_lib):
     assert rc == capi.SUCCESS and n > 0x7fffffff * 16 * 8
 
 
+@pytest.mark.parametrize("layout", [0, 3])
+def test_a_cache_without_both_k_and_v_is_refused(pkg, built_lib, layout):
+    """The rows' addresses follow from the attributes: a cache of K alone would be read beyond its end."""
+    from ppl_nn_b200 import ops
+    op = ops.KeyValueCacheCompact(ops.KeyValueCacheParam(num_layer=3, layer_idx=0, quant_bit=8, cache_layout=layout))
+
+    def shapes(rows, layers, kv, heads, dim):
+        lead = (rows, layers, kv, heads) if layout == 0 else (layers, kv, heads, rows)
+        return lead + (dim,), lead + (dim // 8,)
+
+    assert op._cache_shape(*shapes(50, 3, 2, 4, 64)) == (4, 64, 50)
+    for bad in ((50, 3, 1, 4, 64), (50, 3, 3, 4, 64), (50, 2, 2, 4, 64), (50, 3, 0, 4, 64)):
+        with pytest.raises(ops.OpError):
+            op._cache_shape(*shapes(*bad))
+    cache, scale = shapes(50, 3, 2, 4, 64)
+    with pytest.raises(ops.OpError):
+        op._cache_shape(cache, scale[:-1] + (4,))
+
+
 @pytest.mark.gpu
 def test_calls_without_work_leave_no_status(gpu, pkg):  # noqa: F811
     import torch
