@@ -394,7 +394,8 @@ enum {
     PPLB200_DEV_OK = 0,
     PPLB200_DEV_TMA_WAIT_TIMEOUT = 1,  /* a wait for a bulk-tensor copy ran out of iterations    */
     PPLB200_DEV_MMA_WAIT_TIMEOUT = 2,  /* a wait for a tensor-core commit ran out of iterations   */
-    PPLB200_DEV_LENGTH_CLAMPED = 4,    /* a sequence exceeded max_kvlen / max_seqlen and was cut   */
+    PPLB200_DEV_LENGTH_CLAMPED = 4,    /* a sequence exceeded max_kvlen / max_seqlen and was cut, or (operators
+                                          around the cache) its seqstarts or start_pos are out of range  */
     PPLB200_DEV_ROW_OUT_OF_RANGE = 8,  /* cachestarts/start_pos named a row outside [0, max_tokens):
                                           that row was neither read nor written                     */
     PPLB200_DEV_MASK_OUT_OF_RANGE = 16,/* attn_mask has fewer columns than kvstarts needs: the missing

@@ -552,7 +552,7 @@ int launch_dh(const pplb200_attn_params& p, const WeightArgs& a, cudaStream_t st
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    const dim3 spread(grid.x, static_cast<unsigned>((p.max_kvlen + kSpread - 1) / kSpread), grid.z);
+    const dim3 spread(grid.x, static_cast<unsigned>(p.max_kvlen > 0 ? (p.max_kvlen + kSpread - 1) / kSpread : 1), grid.z);
     launch_dependent(rows <= 2    ? attn_weight_spread_kernel<0>
                      : rows <= 4  ? attn_weight_spread_kernel<1>
                      : rows <= 8  ? attn_weight_spread_kernel<2>
@@ -574,7 +574,8 @@ int make_weight_plan(const pplb200_attn_params& p, WeightPlan* plan) {
            p.batch * p.num_kv_heads * ((p.max_kvlen + 2 * plan->chunk - 1) / (2 * plan->chunk)) >= 148 * 4 * 8) {
         plan->chunk *= 2;
     }
-    plan->chunks = (p.max_kvlen + plan->chunk - 1) / plan->chunk;
+    // at least one: lengths that the bounds cut to nothing are still looked at, and reported
+    plan->chunks = p.max_kvlen > 0 ? (p.max_kvlen + plan->chunk - 1) / plan->chunk : 1;
     plan->score_rows = static_cast<int32_t>(rows <= 2 ? rows : (rows + 3) / 4 * 4);
     const uint64_t all_rows = static_cast<uint64_t>(p.total_tokens) * p.num_heads;
     const uint64_t positions = static_cast<uint64_t>(p.batch) * p.num_kv_heads * p.max_kvlen;
@@ -591,9 +592,6 @@ int make_weight_plan(const pplb200_attn_params& p, WeightPlan* plan) {
 int launch_attn_weight(const pplb200_attn_params& p, const CacheGeom& geom, const WeightPlan& plan, const void* query,
                        const int64_t* seqstarts, const int64_t* cachestarts, const int64_t* start_pos,
                        const void* cache, const void* scale, float* weight, void* workspace, cudaStream_t stream) {
-    if (plan.chunks <= 0 || p.max_seqlen <= 0) {
-        return PPLB200_SUCCESS;
-    }
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     WeightArgs a = {};
     a.q = static_cast<const __half*>(query);

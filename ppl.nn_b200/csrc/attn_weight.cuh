@@ -43,17 +43,21 @@ __device__ __forceinline__ Span span_of(const WeightArgs& a, int64_t b) {
     Span s;
     s.tok0 = a.seqstarts[b];
     int64_t n = a.seqstarts[b + 1] - s.tok0;
-    if (s.tok0 < 0 || s.tok0 + n > a.total_tokens) {
+    bool cut = s.tok0 < 0 || n < 0 || n > a.total_tokens - s.tok0;  // not rows of the query: no tokens
+    n = cut ? 0 : n;
+    cut = cut || n > a.max_seqlen;
+    n = n > a.max_seqlen ? a.max_seqlen : n;
+    s.start = a.start_pos[b];
+    if (s.start < 0) {  // no such position: no tokens
+        cut = cut || n > 0;
         n = 0;
     }
-    bool cut = n > a.max_seqlen;
-    n = cut ? a.max_seqlen : (n < 0 ? 0 : n);
-    s.start = a.start_pos[b];
-    int64_t len = s.start < 0 ? 0 : s.start + n;
-    if (len > a.max_kvlen) {
-        len = a.max_kvlen;
-        cut = true;
+    if (s.start > a.max_kvlen - n) {
+        s.start = s.start > a.max_kvlen ? a.max_kvlen : s.start;
+        cut = cut || n > 0;
     }
+    int64_t len = s.start + n;
+    len = len > a.max_kvlen ? a.max_kvlen : len;
     if (cut && threadIdx.x == 0) {
         atomicOr(a.status, kDevLengthClamped);
     }

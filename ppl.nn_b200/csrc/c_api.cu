@@ -769,10 +769,6 @@ int pplb200_tree_attn_forward(const pplb200_attn_params* p, const void* query, c
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    // a batch without room for a block has nothing that would clear the status word
-    if (plan.ranges <= 0) {
-        return clear_status(workspace, static_cast<cudaStream_t>(stream_v));
-    }
     return launch_tree_attn(*p, make_geom(*p), plan, query, parents, seqstarts, cachestarts, start_pos, cache, scale,
                             workspace, attn_output, static_cast<cudaStream_t>(stream_v));
 }

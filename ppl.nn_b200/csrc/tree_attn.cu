@@ -886,6 +886,7 @@ int make_tree_plan(const pplb200_attn_params& p, int sm_count, TreePlan* plan) {
     const double units = static_cast<double>(p.batch) * (p.num_kv_heads / plan->lanes) * row_tiles * blocks;
     const int64_t places = resident / plan->lanes;
     plan->ranges = units > static_cast<double>(places) * kMinRange ? places : (static_cast<int64_t>(units) + kMinRange - 1) / kMinRange;
+    plan->ranges = plan->ranges < 1 ? 1 : plan->ranges;  // lengths that the bounds cut to nothing are still reported
     plan->words = (p.max_seqlen + 63) / 64;
     const uint64_t slot_rows = static_cast<uint64_t>(plan->ranges) * plan->lanes * 2 * tile_rows;
     plan->off_prefix = 256;
@@ -901,9 +902,6 @@ int launch_tree_attn(const pplb200_attn_params& p, const CacheGeom& geom, const 
                      const int64_t* parents, const int64_t* seqstarts, const int64_t* cachestarts,
                      const int64_t* start_pos, const void* cache, const void* scale, void* workspace,
                      void* attn_output, cudaStream_t stream) {
-    if (plan.ranges <= 0) {
-        return PPLB200_SUCCESS;
-    }
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     TreeArgs a = {};
     a.q = static_cast<const __half*>(query);

@@ -100,6 +100,42 @@ def test_calls_without_work_leave_no_status(gpu, pkg):  # noqa: F811
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [[2, 3], [40, 9]])  # kept scores, and scores formed twice
+def test_sequences_that_are_left_out_are_reported(gpu, pkg, n):  # noqa: F811
+    """Rows that are not the query's, starts below zero and bounds that leave nothing: what cannot be served is reported,
+    the others are served."""
+    from ppl_nn_b200 import capi, ops
+    rng = np.random.default_rng(n[0])
+    start = [60, 200]
+    hc = HostCache(rng, [s + m for s, m in zip(start, n)], 2, 64)
+    q = rng.standard_normal((sum(n), 8, 64)).astype(np.float16)
+    parents = sum([draw_parents(rng, m, "tree") for m in n], [])
+    tree, weigh = ops.TreeAttention(attention_param(hc, 8)), ops.AttentionWeight(attention_param(hc, 8))
+    lone = HostCache(rng, [hc.lens[0]], 2, 64)  # the first sequence by itself
+    lone.starts, lone.cache, lone.scale, lone.weight, lone.max_tokens = hc.starts[:1], hc.cache, hc.scale, hc.weight, hc.max_tokens
+    want, tol = weight_reference(lone, q, start[:1], n[:1], 8, 0, True)
+    for seq, first in (([0, n[0], sum(n) + 1], start), ([0, n[0], n[0] - 1], start), ([0, n[0], sum(n)], [60, -1]),
+                       ([0, n[0], sum(n)], [60, -(1 << 62)])):
+        weight = dev(hc.weight)
+        weigh.forward(dev(q), i64(seq), dev(hc.starts), i64(first), max(n), hc.max_len, dev(hc.cache), dev(hc.scale), weight)
+        assert weigh.device_status() == capi.DEV_LENGTH_CLAMPED, (seq, first)
+        assert np.all(np.abs(weight.cpu().numpy() - want) <= tol)
+        tree.forward(dev(q), i64(parents), i64(seq), dev(hc.starts), i64(first), max(n), hc.max_len, dev(hc.cache), dev(hc.scale))
+        assert tree.device_status() == capi.DEV_LENGTH_CLAMPED, (seq, first)
+    for most_n, most_len in ((0, hc.max_len), (max(n), 0), (0, 0)):
+        weight = dev(hc.weight)
+        weigh.forward(dev(q), dev(starts_of(n)), dev(hc.starts), i64(start), most_n, most_len, dev(hc.cache), dev(hc.scale), weight)
+        assert weigh.device_status() == capi.DEV_LENGTH_CLAMPED
+        assert np.array_equal(weight.cpu().numpy(), hc.weight)
+        tree.forward(dev(q), i64(parents), dev(starts_of(n)), dev(hc.starts), i64(start), most_n, most_len, dev(hc.cache), dev(hc.scale))
+        assert tree.device_status() == capi.DEV_LENGTH_CLAMPED
+    # only padding: nothing is left out
+    weigh.forward(dev(q), i64([0, 0, 0]), dev(hc.starts), i64(start), 0, hc.max_len, dev(hc.cache), dev(hc.scale), weight)
+    tree.forward(dev(q), i64(parents), i64([0, 0, 0]), dev(hc.starts), i64(start), 0, hc.max_len, dev(hc.cache), dev(hc.scale))
+    assert weigh.device_status() == 0 and tree.device_status() == 0
+
+
+@pytest.mark.gpu
 def test_wrong_types_and_shapes_are_refused(gpu, pkg):  # noqa: F811
     import torch
     from ppl_nn_b200 import ops
