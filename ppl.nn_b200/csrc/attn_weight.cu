@@ -33,7 +33,8 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kChunk = 512;     // positions of a CTA, at least
-constexpr int kSpread = 2048;   // positions of a CTA of attn_weight_spread_kernel
+constexpr int kSpread = 2048;   // positions of a CTA of attn_weight_spread_kernel, where a grid holds that many CTAs
+constexpr int64_t kMaxChunks = 65535;  // a grid dimension
 constexpr int kStages = 3;      // tiles of a warp's ring
 constexpr float kNegBig = kWeightNegBig;
 
@@ -451,14 +452,14 @@ __global__ void __launch_bounds__(kThreads, RB == 32 ? 3 : RB == 16 ? 4 : RB >= 
 // A thread per position at a time: the weights of the kept scores.  V: how many float4 the rows of a position take; 0: one
 // or two rows.
 template <int V>
-__global__ void __launch_bounds__(256) attn_weight_spread_kernel(const WeightArgs a) {
+__global__ void __launch_bounds__(256) attn_weight_spread_kernel(const WeightArgs a, int32_t spread) {
     grid_launch_dependents();
     grid_dependency_wait();
     __shared__ float2 norm[kScoreRows];
     const int64_t b = blockIdx.z;
     const int head = blockIdx.x;
     const Span s = span_of(a, b);
-    const int32_t first = blockIdx.y * kSpread;
+    const int32_t first = blockIdx.y * spread;
     if (first >= s.len) {
         return;
     }
@@ -487,7 +488,7 @@ __global__ void __launch_bounds__(256) attn_weight_spread_kernel(const WeightArg
         return ex2_approx(fmaf(x, a.scale_log2, -v.x)) * v.y;
     };
     constexpr int kPer = V == 0 ? 8 : (V >= 8 ? 1 : 8 / V);  // positions of a thread whose loads go out together
-    for (int32_t pos0 = first + threadIdx.x; pos0 < first + kSpread && pos0 < s.len; pos0 += kPer * 256) {
+    for (int32_t pos0 = first + threadIdx.x; pos0 < first + spread && pos0 < s.len; pos0 += kPer * 256) {
         float sum[kPer];
         if constexpr (V == 0) {
             float x[kPer][2];
@@ -552,13 +553,17 @@ int launch_dh(const pplb200_attn_params& p, const WeightArgs& a, cudaStream_t st
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    const dim3 spread(grid.x, static_cast<unsigned>(p.max_kvlen > 0 ? (p.max_kvlen + kSpread - 1) / kSpread : 1), grid.z);
+    int64_t share = kSpread;
+    while (share * kMaxChunks < p.max_kvlen) {
+        share *= 2;
+    }
+    const dim3 spread(grid.x, static_cast<unsigned>(p.max_kvlen > 0 ? (p.max_kvlen + share - 1) / share : 1), grid.z);
     launch_dependent(rows <= 2    ? attn_weight_spread_kernel<0>
                      : rows <= 4  ? attn_weight_spread_kernel<1>
                      : rows <= 8  ? attn_weight_spread_kernel<2>
                      : rows <= 16 ? attn_weight_spread_kernel<4>
                                   : attn_weight_spread_kernel<8>,
-                     spread, dim3(256), 0, stream, a);
+                     spread, dim3(256), 0, stream, a, static_cast<int32_t>(share));
     return check_launch("attn_weight_spread_kernel");
 }
 
@@ -586,7 +591,7 @@ int make_weight_plan(const pplb200_attn_params& p, WeightPlan* plan) {
     plan->off_part = plan->off_norm + (all_rows * 8 + 255) / 256 * 256;
     plan->off_score = plan->off_part + (all_rows * plan->chunks * 8 + 255) / 256 * 256;
     plan->bytes = plan->off_score + (kept ? (positions * plan->score_rows * 4 + 255) / 256 * 256 : 0);
-    return plan->chunks > 65535 ? PPLB200_UNSUPPORTED : PPLB200_SUCCESS;  // a grid dimension
+    return plan->chunks > kMaxChunks ? PPLB200_UNSUPPORTED : PPLB200_SUCCESS;
 }
 
 int launch_attn_weight(const pplb200_attn_params& p, const CacheGeom& geom, const WeightPlan& plan, const void* query,

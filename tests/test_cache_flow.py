@@ -136,6 +136,23 @@ def test_sequences_that_are_left_out_are_reported(gpu, pkg, n):  # noqa: F811
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,n,bound", [(2, [1, 1, 1], 140000000)])
+def test_weights_under_roomy_bounds(gpu, pkg, heads, n, bound):  # noqa: F811
+    """Short sequences under a bound that would ask for more CTAs than a grid dimension has."""
+    from ppl_nn_b200 import ops
+    rng = np.random.default_rng(heads)
+    start = [700, 0, 64]
+    hc = HostCache(rng, [s + m for s, m in zip(start, n)], 1 if heads == 8 else 2, 64)
+    q = rng.standard_normal((sum(n), heads, 64)).astype(np.float16)
+    want, tol = weight_reference(hc, q, start, n, heads, 0, True)
+    op = ops.AttentionWeight(attention_param(hc, heads))
+    weight = dev(hc.weight)
+    op.forward(dev(q), dev(starts_of(n)), dev(hc.starts), i64(start), max(n), bound, dev(hc.cache), dev(hc.scale), weight)
+    assert op.device_status() == 0
+    assert np.all(np.abs(weight.cpu().numpy() - want) <= tol)
+
+
+@pytest.mark.gpu
 def test_wrong_types_and_shapes_are_refused(gpu, pkg):  # noqa: F811
     import torch
     from ppl_nn_b200 import ops
