@@ -35,6 +35,10 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kChunk = 512;     // positions of a CTA, at least
 constexpr int kSpread = 2048;   // positions of a CTA of attn_weight_spread_kernel, where a grid holds that many CTAs
 constexpr int64_t kMaxChunks = 65535;  // a grid dimension
+// Scores that would take more than this are formed twice instead: the bounds ask for batch x max_kvlen of them, whatever
+// the lengths are.  (64 sequences of up to 16384 positions, 8 kv heads: 32 rows keep 1 GB and take 480 us, twice formed 785;
+// 4 rows 128 MB and 160 us.  So the limit is high, a fortieth of the memory.)
+constexpr uint64_t kScoreBytes = 4ull << 30;
 constexpr int kStages = 3;      // tiles of a warp's ring
 constexpr float kNegBig = kWeightNegBig;
 
@@ -573,24 +577,25 @@ int make_weight_plan(const pplb200_attn_params& p, WeightPlan* plan) {
     // With kept scores a CTA's start (lengths, rows and queries, each waiting for the one before) is worth longer chunks
     // as long as there are some 8 CTAs for each place on the chip.
     const int64_t rows = p.max_seqlen * (p.num_heads / p.num_kv_heads);
-    const bool kept = rows > 0 && rows <= kScoreRows;
-    plan->chunk = kept ? kChunk : kWindowChunk;
-    while (kept && plan->chunk < 8 * kChunk &&
-           p.batch * p.num_kv_heads * ((p.max_kvlen + 2 * plan->chunk - 1) / (2 * plan->chunk)) >= 148 * 4 * 8) {
-        plan->chunk *= 2;
-    }
-    // at least one: lengths that the bounds cut to nothing are still looked at, and reported
-    plan->chunks = p.max_kvlen > 0 ? (p.max_kvlen + plan->chunk - 1) / plan->chunk : 1;
-    plan->score_rows = static_cast<int32_t>(rows <= 2 ? rows : (rows + 3) / 4 * 4);
+    plan->score_rows = rows > kScoreRows ? 0 : static_cast<int32_t>(rows <= 2 ? rows : (rows + 3) / 4 * 4);
     const uint64_t all_rows = static_cast<uint64_t>(p.total_tokens) * p.num_heads;
     const uint64_t positions = static_cast<uint64_t>(p.batch) * p.num_kv_heads * p.max_kvlen;
     if (positions > 1ull << 50 || all_rows > 1ull << 40) {  // keeps the sizes below from wrapping around
         return PPLB200_UNSUPPORTED;
     }
+    plan->kept = rows <= kScoreRows &&
+                 (positions * plan->score_rows * 4 <= kScoreBytes || p.max_kvlen > kWindowChunk * kMaxChunks);
+    plan->chunk = plan->kept ? kChunk : kWindowChunk;
+    while (plan->kept && plan->chunk < 8 * kChunk &&
+           p.batch * p.num_kv_heads * ((p.max_kvlen + 2 * plan->chunk - 1) / (2 * plan->chunk)) >= 148 * 4 * 8) {
+        plan->chunk *= 2;
+    }
+    // at least one: lengths that the bounds cut to nothing are still looked at, and reported
+    plan->chunks = p.max_kvlen > 0 ? (p.max_kvlen + plan->chunk - 1) / plan->chunk : 1;
     plan->off_norm = 256;  // behind the status word
     plan->off_part = plan->off_norm + (all_rows * 8 + 255) / 256 * 256;
     plan->off_score = plan->off_part + (all_rows * plan->chunks * 8 + 255) / 256 * 256;
-    plan->bytes = plan->off_score + (kept ? (positions * plan->score_rows * 4 + 255) / 256 * 256 : 0);
+    plan->bytes = plan->off_score + (plan->kept ? (positions * plan->score_rows * 4 + 255) / 256 * 256 : 0);
     return plan->chunks > kMaxChunks ? PPLB200_UNSUPPORTED : PPLB200_SUCCESS;
 }
 
@@ -623,7 +628,7 @@ int launch_attn_weight(const pplb200_attn_params& p, const CacheGeom& geom, cons
     a.chunks = static_cast<int32_t>(plan.chunks);
     a.chunk = plan.chunk;
     a.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(p.head_dim));
-    if (p.max_seqlen * a.group > kScoreRows) {
+    if (!plan.kept) {
         return launch_weight_window(p, a, stream);
     }
     return p.head_dim == 128 ? launch_dh<128>(p, a, stream) : launch_dh<64>(p, a, stream);

@@ -138,6 +138,7 @@ int launch_tree_attn(const pplb200_attn_params& p, const CacheGeom& geom, const 
 struct WeightPlan {
     int32_t chunk;   // positions of a chunk
     int64_t chunks;  // chunks per sequence
+    bool kept;           // the scores are kept, not formed twice
     int32_t score_rows;  // kept scores of a position: the query rows per kv head, above 2 a multiple of 4
     uint64_t off_norm, off_part, off_score, bytes;
 };

@@ -135,10 +135,24 @@ def test_sequences_that_are_left_out_are_reported(gpu, pkg, n):  # noqa: F811
     assert weigh.device_status() == 0 and tree.device_status() == 0
 
 
+def test_kept_scores_take_a_bounded_workspace(pkg, built_lib):
+    """64 sequences whose bound is 131072 positions, whatever their lengths: 8.6 GB of scores, which are formed twice."""
+    from ppl_nn_b200 import capi
+    bounds = dict(num_heads=64, num_kv_heads=8, batch=64, total_tokens=256, max_tokens=1 << 20)
+    size = lambda **kw: built_lib.attn_weight_workspace_size(_params(built_lib, capi, **bounds, **kw))  # noqa: E731
+    for max_seqlen in (1, 2, 4):
+        for max_kvlen in (1 << 14, 1 << 17, 1 << 19, 1 << 22):
+            rc, n = size(max_seqlen=max_seqlen, max_kvlen=max_kvlen)
+            parts = 8 * 256 * 64 * (max_kvlen // 512 + 2)  # maxima and sums of the rows' chunks
+            assert rc == capi.SUCCESS and n <= (4 << 30) + parts
+    assert size(max_seqlen=4, max_kvlen=1 << 16)[1] > 4 << 30  # up to the limit they are kept
+
+
 @pytest.mark.gpu
-@pytest.mark.parametrize("heads,n,bound", [(2, [1, 1, 1], 140000000)])
+@pytest.mark.parametrize("heads,n,bound", [(2, [1, 1, 1], 140000000), (8, [4, 1, 3], 12000000)])
 def test_weights_under_roomy_bounds(gpu, pkg, heads, n, bound):  # noqa: F811
-    """Short sequences under a bound that would ask for more CTAs than a grid dimension has."""
+    """Short sequences under a bound that would ask for more CTAs than a grid dimension has, or (32 rows) for more kept
+    scores than there is room for."""
     from ppl_nn_b200 import ops
     rng = np.random.default_rng(heads)
     start = [700, 0, 64]
