@@ -399,12 +399,14 @@ def _require(device: int, dtype: torch.dtype, **tensors) -> None:
 class _CacheOp(_Base):
     """What the operators around the cache share: checks, parameters from the cache's geometry, and a workspace whose
     first word is the device status word.  The workspace is allocated per call, so that calls of one object on two
-    streams, or in two captured graphs, never share one; the last call's is kept for device_status()."""
+    streams, or in two captured graphs, never share one; the last call's, and its stream, are kept for
+    device_status()."""
 
     def __init__(self, param):
         super().__init__()
         self.param = param
         self._workspace: torch.Tensor | None = None
+        self._call_stream = 0
 
     def _check_cache(self, cache, scale):
         """(device, kv heads, head_dim, rows) of an INT8 cache with num_layer layers and its scales."""
@@ -478,17 +480,20 @@ class _CacheOp(_Base):
         elif rc == capi.SUCCESS:
             self._workspace = ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
             # the current stream's handle; a Stream object around it costs 5 us, a fifth of a small call
-            rc = fn(p, *args, ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(device))
+            self._call_stream = torch._C._cuda_getCurrentRawStream(device)
+            rc = fn(p, *args, ws.data_ptr(), nbytes, self._call_stream)
         self._raise(name, rc)
 
     def device_status(self) -> int:
-        """Status word left by the kernels of the last forward (synchronises the stream)."""
+        """Status word left by the kernels of the last forward.  Synchronises its stream, and the current one: a
+        captured forward is replayed there."""
         if self._workspace is None:
             return 0
         with torch.cuda.device(self._workspace.device):
-            rc, s = self.lib.mhca_device_status(_ptr(self._workspace), _stream())
-        self._raise("pplb200_mhca_device_status", rc)
-        return s
+            for stream in dict.fromkeys((self._call_stream, _stream())):
+                rc, s = self.lib.mhca_device_status(_ptr(self._workspace), stream)
+                self._raise("pplb200_mhca_device_status", rc)
+        return s  # the last reading: both streams are done by then
 
 
 class TreeAttention(_CacheOp):

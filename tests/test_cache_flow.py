@@ -444,6 +444,34 @@ def test_steps_on_two_streams_share_the_operators(gpu, pkg):  # noqa: F811
                 assert torch.equal(x, y)
 
 
+@pytest.mark.gpu
+def test_the_status_of_a_call_on_another_stream(gpu, pkg):  # noqa: F811
+    """The status word is read behind the call's own stream, also from elsewhere and before anyone has waited for it."""
+    import torch
+    from ppl_nn_b200 import capi, ops
+    rng = np.random.default_rng(1)
+    hc = HostCache(rng, [40, 90], 2, 64)
+    args = (dev(rng.standard_normal((7, 4, 64)).astype(np.float16)), i64([-1, 0, 9, -1, 0, 1, 2]), i64([0, 3, 7]), dev(hc.starts),
+            i64([37, 86]), 4, 90, dev(hc.cache), dev(hc.scale))
+    tree, side = ops.TreeAttention(attention_param(hc, 4)), torch.cuda.Stream()
+    for fill in (0, 255):  # what the workspace may hold from before
+        with torch.cuda.stream(side):
+            del_me = torch.full((1 << 20,), fill, dtype=torch.uint8, device=gpu)
+            del del_me
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100000000)
+            tree.forward(*args)
+        assert tree.device_status() == capi.DEV_PARENT_INVALID
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tree.forward(*args)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100000000)
+        graph.replay()
+        assert tree.device_status() == capi.DEV_PARENT_INVALID
+
+
 # ---- long caches -------------------------------------------------------------------------------------
 
 @pytest.mark.gpu
