@@ -310,7 +310,7 @@ int pplb200_rope_kv_append_i8g8(const pplb200_rope_params* p, const pplb200_attn
  * Uses batch, max_seqlen (<= 1024), max_kvlen (>= start_pos[b] + seqlen), total_tokens, max_tokens and the cache
  * geometry of the params; is_causal, decoding_batches and phase_mask are not used.  `workspace`:
  * pplb200_tree_attn_workspace_size() bytes, 256-byte aligned (its first word is the status word); attn_output is
- * 32-byte aligned and not query.  No counterpart in the reference.
+ * 32-byte aligned and does not overlap query.  No counterpart in the reference.
  */
 int pplb200_tree_attn_workspace_size(const pplb200_attn_params* p, uint64_t* bytes);
 

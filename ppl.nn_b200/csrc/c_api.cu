@@ -757,8 +757,10 @@ int pplb200_tree_attn_forward(const pplb200_attn_params* p, const void* query, c
     if (rc != PPLB200_SUCCESS) {
         return rc;
     }
-    if (query == attn_output) {
-        return fail(PPLB200_INVALID_VALUE, "attn_output must not be query: other CTAs still read it");
+    const uintptr_t q0 = reinterpret_cast<uintptr_t>(query), o0 = reinterpret_cast<uintptr_t>(attn_output);
+    const uint64_t bytes = static_cast<uint64_t>(p->total_tokens) * p->num_heads * p->head_dim * 2;
+    if ((q0 <= o0 ? o0 - q0 : q0 - o0) < bytes) {
+        return fail(PPLB200_INVALID_VALUE, "attn_output must not overlap query: other CTAs still read it");
     }
     TreePlan plan;
     rc = make_tree_plan(*p, di.sm_count, &plan);

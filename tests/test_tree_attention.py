@@ -217,3 +217,21 @@ def test_what_stands_behind_a_dominant_token_is_kept(gpu, pkg, above):  # noqa: 
     assert op.device_status() == 0
     got = out.cpu().numpy().astype(np.float64)
     assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shift", [0, 1, 6, -1, -6])
+def test_an_output_over_the_query_is_refused(gpu, pkg, shift):  # noqa: F811
+    """Other parts of the call still read what this one would write, also where the two only overlap."""
+    import torch
+    from ppl_nn_b200 import ops
+    hc = HostCache(np.random.default_rng(0), [30], 2, 64)
+    room = torch.zeros(21, 4, 64, dtype=torch.float16, device=gpu)
+    op = ops.TreeAttention(ops.MultiHeadCacheAttentionParam(num_heads=4, num_kv_heads=2, head_dim=64, **hc.param()))
+    i64 = lambda x: torch.tensor(x, dtype=torch.int64, device=gpu)  # noqa: E731
+    args = (None, i64([0, 7]), dev(hc.starts), i64([20]), 7, 30, dev(hc.cache), dev(hc.scale))
+    with pytest.raises(ops.OpError):
+        op.forward(room[7:14], *args, attn_output=room[7 + shift:14 + shift])
+    for beside in (0, 14):
+        op.forward(room[7:14], *args, attn_output=room[beside:beside + 7])
+        assert op.device_status() == 0
