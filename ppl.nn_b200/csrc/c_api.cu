@@ -713,6 +713,11 @@ static int validate_tree(const pplb200_attn_params* p) {
     if (p->max_seqlen * (p->num_heads / p->num_kv_heads) > 0x7fffff) {
         return fail(PPLB200_UNSUPPORTED, "more than 2^23 query rows of a kv head in a sequence");
     }
+    // a (sequence, kv head)'s blocks of 64 positions x 128 or 256 query rows are counted in 32 bits
+    const int64_t rows = p->max_seqlen * (p->num_heads / p->num_kv_heads);
+    if ((rows + 127) / 128 * ((p->max_kvlen + 63) / 64) > 0x7fffffff) {
+        return fail(PPLB200_UNSUPPORTED, "more than 2^31 blocks of 64 positions and 128 query rows in a sequence");
+    }
     return PPLB200_SUCCESS;
 }
 

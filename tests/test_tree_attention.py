@@ -40,6 +40,19 @@ def test_arguments_are_refused(built_lib, pkg, kw, expect):
     assert _tree_call(built_lib, _params(built_lib, capi, batch=0, total_tokens=0), q=None, out=None) == capi.SUCCESS
 
 
+def test_more_blocks_than_32_bits_count_are_refused(built_lib, pkg):
+    """Blocks of a (sequence, kv head): 64 positions x 128 query rows."""
+    from ppl_nn_b200 import capi
+    for heads, max_seqlen, max_kvlen, expect in (
+            (4096, 1024, 1 << 23, "RC_UNSUPPORTED"),  # 2^15 x 2^17
+            (4096, 1024, (1 << 22) - 64, "RC_SUCCESS"), (8, 1024, 0x7fff0000, "RC_SUCCESS")):
+        p = _params(built_lib, capi, num_heads=heads, num_kv_heads=1, max_seqlen=max_seqlen, max_kvlen=max_kvlen)
+        rc, _ = built_lib.tree_attn_workspace_size(p)
+        assert built_lib.status_str(rc) == expect
+        if expect != "RC_SUCCESS":
+            assert built_lib.status_str(_tree_call(built_lib, p)) == expect
+
+
 def draw_parents(rng, n, kind):
     if kind == "chain":
         return list(range(-1, n - 1))
