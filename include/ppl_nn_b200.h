@@ -397,7 +397,8 @@ enum {
     PPLB200_DEV_LENGTH_CLAMPED = 4,    /* a sequence exceeded max_kvlen / max_seqlen and was cut, or (operators
                                           around the cache) its seqstarts or start_pos are out of range  */
     PPLB200_DEV_ROW_OUT_OF_RANGE = 8,  /* cachestarts/start_pos named a row outside [0, max_tokens):
-                                          that row was neither read nor written                     */
+                                          that row was neither read nor written (attention counts it as a
+                                          key and a value of zeros, i.e. with a score of 0)          */
     PPLB200_DEV_MASK_OUT_OF_RANGE = 16,/* attn_mask has fewer columns than kvstarts needs: the missing
                                           entries were read as 0                                    */
     PPLB200_DEV_KEPT_INVALID = 32,     /* a kept list is not strictly ascending or names a position outside

@@ -658,6 +658,56 @@ def test_keys_of_a_tree_are_not_rounded(gpu, pkg, heads, kv_heads, dim, n):  # n
     assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
 
 
+class OutsideCache(HostCache):
+    """A cache some of whose positions name rows outside it: keys and values of zeros, without a weight of their own."""
+
+    def values(self, which, layer, head, rows):
+        inside = (rows >= 0) & (rows < self.max_tokens)
+        out = np.zeros((len(rows), self.dim))
+        out[inside] = super().values(which, layer, head, rows[inside])
+        return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [[1, 1], [4, 2], [40, 9]])  # 2, 8 and 80 query rows
+@pytest.mark.parametrize("layout,page,where", [(0, 0, "beyond"), (3, 0, "before"), (0, 16, "beyond"), (3, 64, "before"), (0, 48, "beyond")])
+def test_rows_outside_the_cache_count_as_zeros(gpu, pkg, n, layout, page, where):  # noqa: F811
+    """Reported, and read as zeros, as decode and prefill read them: with a score of 0."""
+    from ppl_nn_b200 import capi, ops
+    rng = np.random.default_rng(page + n[0])
+    start, heads = [150, 333], 4
+    hc = OutsideCache(rng, [s + m for s, m in zip(start, n)], 2, 64, layout, page)
+    while page and (hc.starts == hc.max_tokens - page).any():  # the last page is to be nobody's
+        hc = OutsideCache(rng, [s + m for s, m in zip(start, n)], 2, 64, layout, page)
+    hc.scale[:] = 0.002  # scores of a few tenths: the rows outside weigh as much as the others
+    if page:
+        hc.starts[1, 2] = hc.max_tokens + 5 if where == "beyond" else -page
+        hc.starts[0, 1] = hc.max_tokens - 16 if page > 16 else 1 << 40  # a page that ends outside, where it is long enough
+    else:
+        hc.starts[1] = hc.max_tokens - 200 if where == "beyond" else -7
+    q = rng.standard_normal((sum(n), heads, 64)).astype(np.float16)
+    args = (dev(starts_of(n)), dev(hc.starts), i64(start), max(n), hc.max_len, dev(hc.cache), dev(hc.scale))
+    parents = sum([draw_parents(rng, m, "tree") for m in n], [])
+    rows = hc.rows
+    if where == "before" and not page:  # no position of a sequence that starts before the cache has a row
+        hc.rows = lambda b, p: rows(b, p) if b == 0 else np.full(len(p), -1)
+    tree = ops.TreeAttention(attention_param(hc, heads))
+    got = tree.forward(dev(q), i64(parents), *args).cpu().numpy()
+    assert tree.device_status() == capi.DEV_ROW_OUT_OF_RANGE
+    want, tol = tree_reference(hc, q, parents, start, n, heads, 0)
+    assert np.all(np.abs(got - want) <= tol)
+    # the reference of the weights adds to the row of each position: those outside go behind the cache
+    named, held = hc.rows, hc.weight
+    hc.weight = np.concatenate([held, np.zeros((1, 2, 1 << 10), dtype=np.float32)], axis=-1)
+    hc.rows = lambda b, p: np.where((named(b, p) >= 0) & (named(b, p) < hc.max_tokens), named(b, p), hc.max_tokens + np.asarray(p))
+    want, tol = weight_reference(hc, q, start, n, heads, 0, True)
+    weight, weigh = dev(held), ops.AttentionWeight(attention_param(hc, heads))
+    weigh.forward(dev(q), *args, weight)
+    assert weigh.device_status() == capi.DEV_ROW_OUT_OF_RANGE
+    want, tol = want[..., :hc.max_tokens], tol[..., :hc.max_tokens]
+    assert np.all(np.abs(weight.cpu().numpy() - want) <= tol)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("n", [[3, 1], [40, 9]])
 def test_tokens_behind_the_last_sequence_are_padding(gpu, pkg, n):  # noqa: F811
