@@ -554,6 +554,50 @@ def test_select_of_long_lists(gpu, pkg, kind, n):  # noqa: F811
     assert torch.equal(got[0, 0].cpu(), torch.from_numpy(want))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["signs", "zeros", "few numbers", "infinities", "denormal", "negative", "nan at the cut", "all nan"])
+@pytest.mark.parametrize("layout,page", [(0, 0), (3, 48)])
+def test_select_of_long_lists_of_special_weights(gpu, pkg, kind, layout, page):  # noqa: F811
+    """The bracket of the sample compares the weights themselves, the lists their keys: signs, zeros of both signs (which
+    are equal), denormal numbers, infinities and NaN (below every number), with the cut on either side of them."""
+    from ppl_nn_b200 import ops
+    rng = np.random.default_rng(len(kind) + page)
+    n, sink, recent = 70001, 4, 300
+    hc = HostCache(rng, [n, 40000], 1, 64, layout, page)
+    for b, m in enumerate(hc.lens):
+        w = rng.standard_normal(m).astype(np.float32)
+        pick = rng.random(m)
+        if kind == "zeros":  # a third positive, the cut among the zeros of both signs
+            w = np.where(pick < 0.33, np.abs(w), np.where(pick < 0.6, 0.0, -0.0)).astype(np.float32)
+        elif kind == "few numbers":
+            w[pick < 0.9] = np.nan
+        elif kind == "infinities":
+            w[pick < 0.3], w[pick > 0.7] = np.inf, -np.inf
+        elif kind == "denormal":
+            w = (w * 1e-40).astype(np.float32)
+        elif kind == "negative":
+            w = -np.abs(w)
+            w[pick < 0.2] = -0.0
+        elif kind == "nan at the cut":
+            w[pick < 0.5] = np.nan
+            w[pick > 0.9] = np.inf
+        elif kind == "all nan":
+            w[:] = np.nan
+        hc.weight[0, 0, hc.rows(b, np.arange(m))] = w
+    op = ops.KeyValueCacheEvict(ops.KeyValueCacheEvictParam(**hc.param(), sink=sink, recent=recent))
+    for budget in (sink + recent + 1, 6000, 20000, 30304, 39000):
+        kept = op.forward(dev(hc.weight), dev(hc.starts), i64(hc.lens), i64([budget, budget - 7]), n, budget).cpu().numpy()
+        assert op.device_status() == 0
+        for b, m in enumerate(hc.lens):
+            k = budget - 7 * b
+            w = hc.weight[0, 0, hc.rows(b, np.arange(m))].astype(np.float64)
+            s, r = min(sink, k - min(recent, k)), min(recent, k)
+            cand = np.arange(s, m - r)
+            order = cand[np.lexsort((cand, -np.where(np.isnan(w), 0, w)[cand], np.isnan(w)[cand]))][:k - r - s]
+            want = np.sort(np.concatenate([np.arange(s), order, np.arange(m - r, m)]))
+            assert np.array_equal(kept[b, 0, :k], want) and (kept[b, 0, k:] == -1).all()
+
+
 # ---- forms of the weights and of the tree --------------------------------------------------------------
 
 MORE_WEIGHT_CASES = [

@@ -553,3 +553,30 @@ def test_segments_wait_for_all_whose_rows_they_overwrite(rows):
             lo, hi = wait_range(tops, seg, rows)
             need = {i // rows for i, p in moves if i // rows < seg and seg * rows <= p < (seg + 1) * rows}
             assert all(lo <= e <= hi for e in need) and hi < seg
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,per_head,n", [(8, False, 21001), (2, False, 40100), (1, True, 70100)])  # 8, 32 and 64 rows a segment
+@pytest.mark.parametrize("kind", [None, "huge", "over"])
+def test_compact_of_lists_with_many_segments(gpu, pkg, heads, per_head, n, kind):
+    """More than 1024 segments: the scan of the lists works through them in several steps."""
+    from ppl_nn_b200 import capi, ops
+    rng = np.random.default_rng(n)
+    hc = HostCache(rng, [n, 900], heads, 64)
+    base = np.array([3, 0], dtype=np.int64)
+    kept = np.full((2, heads if per_head else 1, n), -1, dtype=np.int64)
+    for b, m in enumerate(hc.lens):
+        count = m - int(base[b]) - 70
+        for g in range(kept.shape[1]):
+            kept[b, g, :count] = np.arange(70, 70 + count)
+            kept[b, g, count + 1:] = 5  # stale
+            if kind:
+                spoil(rng, kept[b, g, :count], [i for i in (64, 8191, 8192, 16384, 32768, 65536, 65599) if i < count], kind)
+    want = skipping_reference(hc, kept, base, 1)
+    op = ops.KeyValueCacheCompact(ops.KeyValueCacheParam(**hc.param()))
+    for _ in range(3):
+        got = [dev(hc.cache), dev(hc.scale), dev(hc.weight)]
+        op.forward(dev(kept), dev(hc.starts), dev(base), dev(np.array(hc.lens)), hc.max_len, got[0], got[1], weight=got[2])
+        assert op.device_status() == (capi.DEV_KEPT_INVALID if kind else 0)
+        for g, x in zip(got, want):
+            assert np.array_equal(g.cpu().numpy(), x)
