@@ -22,7 +22,10 @@
 // 92 % of a copy's rate), 155 us with the spread kernel, whose traffic is 4 + 4 + 8 bytes a position against 160.  With
 // split keys, bound by their instructions, it was 190.  64 sequences of up to 16384 positions, 8 kv heads (739 MB): 4 rows
 // 160, 8 rows 185, 16 rows 255, 32 rows 480 us; attn_window.cu takes 785 us for up to 32 rows and 839 for 128, the kept
-// scores of more than 32 rows would be twice the bytes of K and more.  Chunks of 512 positions waste a CTA's start, so
+// scores of more than 32 rows would be twice the bytes of K and more.  The score kernel of 4
+// and 8 rows is bound by its instructions (2.7 a cycle, DRAM 54 %), that of 16 and 32 rows by latency (113 and 168 registers
+// leave 23 and 18 % of an SM's warps; tensor pipe 33 and 40 %), and 32 rows have 256 bytes of scores written and read
+// against 160 of K.  At Dh 128 the forms for 4 and for 32 rows spill a little (24 and 68 bytes).  Chunks of 512 positions waste a CTA's start, so
 // they grow to 4096 while the chip stays full.
 #include "attn_weight.cuh"
 

@@ -15,11 +15,11 @@
 // memory adds the four warps up.
 // The order of every sum is fixed.
 //
-// Measured: 4 sequences of 8192 to 32768 positions, 8 kv heads of 128, 116 to 128 rows: statistics 68 us, weights 80 us,
-// 163 us in all; with warp-level products (mma.sync, 32 rows at a time) 408 us.  For up to 32 rows attn_weight.cu is the
-// faster one (figures there).  Bound by neither pipe: a block takes a CTA 2150 cycles for the statistics and 2600 for the
-// weights, the converters work 1500 of them, the tensor pipe is busy 40 % and 25 %; 760 CTAs on 296 places leave the third
-// wave partly empty, but with chunks of 512 or 2048 positions the two passes take longer (196 and 208 us against 180).
+// Measured: 4 sequences of 8192 to 32768 positions, 8 kv heads of 128, 116 to 128 rows: statistics 68 us, join 4, weights
+// 84 (each kernel by itself), 159 to 164 a call; with warp-level products (mma.sync, 32 rows at a time) 408 us.  For up to
+// 32 rows attn_weight.cu is the faster one (figures there).  Bound by no pipe: tensor 39 % and 31 %, DRAM 22 % and 18 %, 2.3
+// and 2.1 instructions a cycle; 760 CTAs on 296 places leave the third wave partly empty, but chunks of 512 or 2048
+// positions took longer (tried on an earlier form, whose two passes together took 196 and 208 us against 180).
 #include "attn_weight.cuh"
 #include "kv_tiles.cuh"
 #include "ragged.cuh"

@@ -31,9 +31,10 @@
 // earlier segments come first.  Nobody waits before it has raised the flags of the segments it has begun, so the lowest
 // flag not yet up always belongs to a CTA that can go on.
 // Measured: 16 sequences of up to 16384 positions, 2048 kept per kv head, weights too (176 MB): 47 us behind 6 for the
-// lists, 55 a call (3.2 TB/s); 4 of up to 131072, paged, 16001 kept (347 MB): 101 behind 9, 112 a call (3.1 TB/s); the
-// accepted paths of 32 sequences in 32 layers (26 MB): 7 us behind 4, 19 a call.  Scattered rows of 128 + 32 bytes are read
-// in whole sectors but not in whole DRAM bursts.
+// lists, 55 a call (3.2 TB/s); 4 of up to 131072, paged, 16001 kept (347 MB): 100 behind 9, 112 a call (3.1 TB/s); the
+// accepted paths of 32 sequences in 32 layers (26 MB): 7 us behind 4, 19 a call.  DRAM is 43 to 46 % busy, about the bytes
+// that have to move; the first stall is the barrier: a CTA begins no copy of its next segment before the stores of this
+// one are on their way.
 #include <type_traits>
 
 #include "common.cuh"

@@ -24,19 +24,24 @@
 //
 // Roundings: a key rounded to fp16 costs 1e-3 of the output's magnitude where keys have outlying channels, and 3e-3 where
 // several positions compete for a row (against 2e-4 for the fp16 output itself), so K is split into fp16(k) and the exact
-// remainder, two tiles whose products with Q meet in one accumulator.  Weights and values are rounded to fp16, by up to 2^-11 of
-// each and independently, which averages out (weights below 2^-21 of the row's largest by up to 2^-32 of that); scores, maxima, sums and outputs are held in fp32.
+// remainder, two tiles whose products with Q meet in one accumulator.  Weights and values are rounded to fp16, by up to
+// 2^-11 of each and independently, which averages out (weights below 2^-21 of the row's largest by up to 2^-32 of that);
+// scores, maxima, sums and outputs are held in fp32.
 //
-// Measured (8 kv heads of 128), main kernel and whole call: 32 sequences of 256 to 8192 positions, 4 to 64 rows per kv
-// head, 392 MB of cache: 165 and 198 us (with rounded keys 145 and 163); 64 such sequences, 200 to 264 rows: 508 and 602
-// us (445 and 515), 537 and 637 with one stage of tiles; 4 of up to 131072, paged, 228 to 256 rows: 650 and 712 us (470
-// and 549).  What bounds it: the converters, the MMAs' reads of shared memory and the softmax are about as long as one
-// another (at MT = 1 and with rounded keys a block took a CTA 3300 cycles, of which the converters worked 2600, the MMA
-// warp waited 1050 for tiles and the softmax 790 for scores; tensor pipe 31 %, DRAM 36 %).  More converter warps do not
-// pay at 96 registers a thread: with rounded keys, converters apart for K and V and double-buffered scores the three calls
-// took 177, 565 and 574 us.  MT = 2 against MT = 1 for 256 rows: K and V are fetched and converted once for both tiles.
+// Measured (8 kv heads of 128): 32 sequences of 256 to 8192 positions, 4 to 64 rows per kv head, 392 MB of cache: 167 us
+// for the main kernel by itself, 3 for the plan, 13 for the merge, 193 to 199 a call; 64 such sequences, 200 to 264 rows:
+// 493, 3 and 23, 601 to 615 a call; 4 of up to 131072, paged, 228 to 256 rows: 617, 3 and 20, 706 to 719 a call.  The
+// kernels by themselves run at 1965 MHz; calls one behind the other draw the card's 1000 W and run at about 1690, which is
+// what the calls take beyond the sum.  (Keys rounded to fp16: 163, 515 and 549 a call.)
+// What bounds it: tensor pipe 39 % with one tile and 50 % with two, DRAM 30 % and 22 %, 1.9 and 2.1 instructions a cycle:
+// the converters, the MMAs' reads of shared memory and the softmax are about as long as one another.  With one tile the 96
+// registers that two CTAs an SM leave a thread are just short (56 bytes spilled); with two there are 128.  More converter
+// warps were tried with one tile and with rounded keys only, where they did not pay: converters apart for K and V and
+// double-buffered scores took 177, 565 and 574 us.  MT = 2 against MT = 1 for 256 rows: K and V are fetched and converted
+// once for both tiles; what lies between 129 and 199 rows, and batches of which only some sequences have that many, were
+// not measured apart.
 //
-// Waits on mbarriers are bounded and give up together (see tcgen05.cuh).
+// Waits on mbarriers are bounded and give up together (see warp_wait.cuh).
 #include <cub/block/block_scan.cuh>
 
 #include "common.cuh"
