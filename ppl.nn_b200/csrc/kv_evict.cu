@@ -575,8 +575,8 @@ __device__ __forceinline__ int32_t count_below(const int32_t* tops, int32_t coun
 }
 
 // A CTA per kept list: where it ends, and the plans of its segments.  Behind the first negative entry there may be
-// anything, and a list may be out of order, so the entries are looked at one and all: a bisection would have to trust
-// them.  (What stands behind the end enters the maxima of segments that have nothing to move.)  Clears the status word,
+// anything, and a list may be out of order, so the entries up to there are looked at one and all: a bisection would have
+// to trust them.  (What stands behind the end enters the maxima of segments that have nothing to move.)  Clears the status word,
 // the ticket and the flags on the way, so that the call needs no other launch before the moving one.
 __global__ void __launch_bounds__(kScanThreads) kv_compact_scan_kernel(const CompactArgs a) {
     __shared__ int32_t s_end, s_bad, warp_top[kScanThreads / 32], seg_top[kScanThreads];
@@ -602,7 +602,9 @@ __global__ void __launch_bounds__(kScanThreads) kv_compact_scan_kernel(const Com
     int64_t n = a.kvlens[b];
     n = n > a.max_kvlen ? a.max_kvlen : n;
     constexpr int kUnroll = 8;  // entries of a thread whose loads go out together; a warp's 256 are neighbours
-    for (int64_t i0 = warp * (32 * kUnroll) + lane; i0 - lane < a.max_kept; i0 += kUnroll * kScanThreads) {
+    bool ended = false;
+    for (int64_t step = 0; step < a.max_kept && !ended; step += kUnroll * kScanThreads) {
+        const int64_t i0 = step + warp * (32 * kUnroll) + lane;
         int64_t p[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
@@ -617,6 +619,7 @@ __global__ void __launch_bounds__(kScanThreads) kv_compact_scan_kernel(const Com
             const int32_t left = __shfl_up_sync(0xffffffffu, top[u], 1);
             if (i < a.max_kept) {
                 if (p[u] < 0) {
+                    ended = true;
                     atomicMin(&s_end, static_cast<int32_t>(i));
                 } else if (top[u] <= (lane > 0 ? left : last)) {  // as long as all count, the one before is the highest
                     atomicMin(&s_bad, static_cast<int32_t>(i));
@@ -649,18 +652,18 @@ __global__ void __launch_bounds__(kScanThreads) kv_compact_scan_kernel(const Com
                 }
             }
         }
+        ended = __syncthreads_or(ended);
     }
-    __syncthreads();
-    const int32_t end = s_end;
+    const int32_t end = s_end, used = (end + rows - 1) >> shift;  // segments with entries
     const bool orderly = s_bad >= end;
     if (tid == 0) {
         a.ends[blockIdx.x] = make_int2(end, orderly);
     }
     // each segment's own maximum -> the maximum of those before it
     int32_t carry = -1;
-    for (int32_t e0 = 0; e0 < a.segments; e0 += kScanThreads) {
+    for (int32_t e0 = 0; e0 < used; e0 += kScanThreads) {
         const int32_t e = e0 + tid;
-        const int32_t top = warp_max_scan(e < a.segments ? tops[e] : -1, lane);
+        const int32_t top = warp_max_scan(e < used ? tops[e] : -1, lane);
         __syncthreads();
         if (lane == 31) {
             warp_top[warp] = top;
@@ -670,7 +673,7 @@ __global__ void __launch_bounds__(kScanThreads) kv_compact_scan_kernel(const Com
         int32_t before = __shfl_sync(0xffffffffu, all, warp > 0 ? warp - 1 : 0);  // of the warps before
         before = warp > 0 && before > carry ? before : carry;
         const int32_t mine = __shfl_up_sync(0xffffffffu, top, 1);
-        if (e < a.segments) {
+        if (e < used) {
             tops[e] = lane > 0 && mine > before ? mine : before;
         }
         const int32_t most = __shfl_sync(0xffffffffu, all, 31);
@@ -696,7 +699,7 @@ __global__ void __launch_bounds__(kScanThreads) kv_compact_scan_kernel(const Com
         return;
     }
     __syncthreads();
-    for (int32_t e = warp; e < a.segments; e += kScanThreads / 32) {  // a warp per segment
+    for (int32_t e = warp; e < used; e += kScanThreads / 32) {  // a warp per segment
         const int64_t first = static_cast<int64_t>(e) * rows;
         int32_t before = tops[e];
         for (int32_t j = lane; j - lane < rows; j += 32) {
