@@ -348,7 +348,7 @@ int pplb200_attn_weight_accumulate(const pplb200_attn_params* p, const void* que
  *   weight   [num_layer, num_kv_heads, max_tokens] fp32 as above (layer layer_idx is read)
  *   kvlens   [batch], budgets [batch] int64
  *   kept     [batch, num_kv_heads, max_budget] int64: the kept positions in ascending order, then -1
- * A budget above max_budget, or a length above max_kvlen, is cut to it (a cut length is reported as
+ * A budget above max_budget, or a length above max_kvlen, is cut to it, negative ones to 0 (a cut length is reported as
  * PPLB200_DEV_LENGTH_CLAMPED).  Uses batch, max_kvlen, max_tokens, num_kv_heads and the cache geometry.
  * `workspace`: pplb200_kv_evict_workspace_size() bytes, 256-byte aligned (its first word is the status word).
  * No counterpart in the reference.
@@ -371,8 +371,9 @@ int pplb200_kv_evict_select(const pplb200_attn_params* p, const float* weight, c
  * Positions behind the kept ones keep their codes and scales; the caller's lengths become base[b] + entries.  Two
  * sequences of a call must not share rows that either of them moves.  An entry that is below its own index, outside
  * its sequence, or not above every entry before it that is neither, is skipped and reported
- * (PPLB200_DEV_KEPT_INVALID); the others move as they would without it.  `workspace`: pplb200_kv_compact_workspace_size() bytes, 256-byte aligned
- * (its first word is the status word).  No counterpart in the reference.
+ * (PPLB200_DEV_KEPT_INVALID); the others move as they would without it.  `workspace`:
+ * pplb200_kv_compact_workspace_size() bytes, 256-byte aligned (its first word is the status word).  No counterpart in the
+ * reference.
  */
 int pplb200_kv_compact_workspace_size(const pplb200_attn_params* p, int64_t kept_heads, int64_t max_kept,
                                       int64_t layers, uint64_t* bytes);

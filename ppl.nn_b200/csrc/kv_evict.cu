@@ -182,13 +182,12 @@ __global__ void __launch_bounds__(NT) kv_evict_select_kernel(const SelectArgs a)
     const int64_t b = blockIdx.y;
     const int head = blockIdx.x;
     int64_t n64 = a.kvlens[b], k64 = a.budgets[b];
-    if (n64 > a.max_kvlen) {
+    if (n64 > a.max_kvlen || n64 < 0) {
         if (tid == 0) {
             atomicOr(a.status, kDevLengthClamped);
         }
-        n64 = a.max_kvlen;
+        n64 = n64 < 0 ? 0 : a.max_kvlen;
     }
-    n64 = n64 < 0 ? 0 : n64;
     k64 = k64 > a.max_budget ? a.max_budget : k64;
     k64 = k64 > n64 ? n64 : (k64 < 0 ? 0 : k64);
     const int64_t r = a.recent < k64 ? a.recent : k64;

@@ -328,6 +328,20 @@ def test_evict_select_long_list_and_cut_length(gpu, pkg):
     assert list(kept[0, 0].cpu().numpy()) == select_reference(w, 5000, 2000, 4, 1000)
 
 
+@pytest.mark.gpu
+def test_evict_select_reports_negative_lengths(gpu, pkg):
+    from ppl_nn_b200 import capi, ops
+    rng = np.random.default_rng(6)
+    hc = HostCache(rng, [50, 3000], 2, 64)
+    op = ops.KeyValueCacheEvict(ops.KeyValueCacheEvictParam(**hc.param(), sink=1, recent=2))
+    for most in (50, 3000):  # short and long lists
+        kept = op.forward(dev(hc.weight), dev(hc.starts), dev(np.array([-1, most])), dev(np.array([7, 9])), most, 9).cpu().numpy()
+        assert op.device_status() == capi.DEV_LENGTH_CLAMPED
+        assert (kept[0] == -1).all()
+        for g in range(2):
+            assert list(kept[1, g]) == select_reference(hc.weight[0, g, hc.rows(1, np.arange(most))], most, 9, 1, 2)
+
+
 # ---- compaction ------------------------------------------------------------------------------------
 
 def compact_reference(hc, kept, base, first_layer, layers, with_weight, lens=None):
