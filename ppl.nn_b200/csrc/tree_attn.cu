@@ -208,7 +208,8 @@ __global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(const TreeArgs 
     }
     bad = __syncthreads_or(bad);
     if (tid == 0) {
-        const bool cut = n != s.n || a.start_pos[b] != s.start || s.start + n > a.max_kvlen;
+        // (a sequence without tokens, as in a padded batch, has nothing to cut, wherever it starts)
+        const bool cut = n != 0 && (n != s.n || a.start_pos[b] != s.start || s.start + n > a.max_kvlen);
         a.flags[b] = (cut ? kDevLengthClamped : 0u) | (bad ? kDevParentInvalid : 0u);
     }
     for (int32_t i = tid; i < s.n; i += kPlanThreads) {

@@ -129,6 +129,18 @@ def test_sequences_that_are_left_out_are_reported(gpu, pkg, n):  # noqa: F811
         assert np.array_equal(weight.cpu().numpy(), hc.weight)
         tree.forward(dev(q), i64(parents), dev(starts_of(n)), dev(hc.starts), i64(start), most_n, most_len, dev(hc.cache), dev(hc.scale))
         assert tree.device_status() == capi.DEV_LENGTH_CLAMPED
+    # a sequence without tokens, wherever it starts: nothing is left out
+    for seq in ([0, n[0], n[0]], [0, 0, n[1]]):
+        for far in (-1, 1 << 40):
+            first = [far if seq[b] == seq[b + 1] else start[b] for b in range(2)]
+            weight = dev(hc.weight)
+            weigh.forward(dev(q), i64(seq), dev(hc.starts), i64(first), max(n), hc.max_len, dev(hc.cache), dev(hc.scale), weight)
+            tree.forward(dev(q), i64(parents), i64(seq), dev(hc.starts), i64(first), max(n), hc.max_len, dev(hc.cache), dev(hc.scale))
+            assert weigh.device_status() == 0, (seq, far)
+            # (the second sequence's tokens are the first ones here: their parents are other's, and reported)
+            assert tree.device_status() in ((0,) if seq[1] else (0, capi.DEV_PARENT_INVALID)), (seq, far)
+            if seq[1]:
+                assert np.all(np.abs(weight.cpu().numpy() - want) <= tol)
     # only padding: nothing is left out
     weigh.forward(dev(q), i64([0, 0, 0]), dev(hc.starts), i64(start), 0, hc.max_len, dev(hc.cache), dev(hc.scale), weight)
     tree.forward(dev(q), i64(parents), i64([0, 0, 0]), dev(hc.starts), i64(start), 0, hc.max_len, dev(hc.cache), dev(hc.scale))
