@@ -306,7 +306,9 @@ int pplb200_rope_kv_append_i8g8(const pplb200_rope_params* p, const pplb200_attn
  *           before it (parent < i); -1: a child of the history.  Null: every token is the child of the one before it
  *           (a single drafted chain).  A parent that breaks the rule counts as -1 (PPLB200_DEV_PARENT_INVALID).
  *   query, attn_output [total_tokens, num_heads, head_dim] fp16; keys and values are the cache's codes times scales,
- *           scores scaled by 1 / sqrt(head_dim).  The accepted path is kept with pplb200_kv_compact.
+ *           scores scaled by 1 / sqrt(head_dim).  The accepted path is kept with pplb200_kv_compact.  What a token
+ *           does not see does not matter, but for a V scale of a drafted token that is not finite: it reaches every
+ *           query of its sequence and kv head (0 * inf).
  * Uses batch, max_seqlen (<= 1024), max_kvlen (>= start_pos[b] + seqlen), total_tokens, max_tokens and the cache
  * geometry of the params; is_causal, decoding_batches and phase_mask are not used.  `workspace`:
  * pplb200_tree_attn_workspace_size() bytes, 256-byte aligned (its first word is the status word); attn_output is
